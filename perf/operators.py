@@ -438,7 +438,8 @@ def _run_own(st):
         r = llmt.policy_loss(st["logp"], st["old"], st["adv"], st["offsets"],
                              ref_logp=st.get("ref"), entropy=st.get("entropy"),
                              mask=st.get("mask"), clip_low=c["low"], clip_high=c["high"],
-                             kl_coef=c["kl"], entropy_coef=c["ent"], mean=c["mean"])
+                             kl_coef=c["kl"], entropy_coef=c["ent"], mean=c["mean"],
+                             per_sequence=c["per_sequence"])
         out = dict(loss=r.loss, stats=r.stats, dlogp=r.dlogp)
         if "entropy" in st:
             out["dentropy"] = r.dentropy
