@@ -368,6 +368,89 @@ int llmt_attention_block_bwd(const void* q_raw, const void* k_raw, const void* v
                              float* dq_raw, float* dk_raw, float* dv,
                              int B, int S, int nq, int nkv, float theta, float eps, void* stream);
 
+/* ---- tuning on preferences and rewards: operators on the caller's logits ----
+ * No counterpart in the reference, whose only loss is the cross entropy.  They
+ * allocate nothing: what they need beyond their outputs is the caller's
+ * workspace (16-byte aligned, at least the bytes that the *_workspace function
+ * gives for the same sizes; it may be NULL where that is 0), so a call can be
+ * captured into a HIP graph.  A workspace belongs to one call at a time: two
+ * streams, or two graphs that may run at once, take one each.  Results do not
+ * depend on the workspace's contents and repeat bit for bit. */
+
+enum { LLMT_F32 = 0, LLMT_F16 = 1, LLMT_BF16 = 2 };
+
+/* Log-probabilities of target tokens.  logits [rows, V] of `dtype`, ld
+ * elements from row to row (ld >= V; any alignment of whole elements), scaled
+ * by inv_temp > 0 before the softmax:
+ *   x = logits * inv_temp,  m = max x,  l = ln sum exp(x - m)
+ *   logp[i] = x[target] - m - l,  stats[i] = (m, l),
+ *   entropy[i] = -sum p ln p (may be NULL).
+ * A row whose target is outside [0, V) (padding, a prompt token) is not read:
+ * its outputs are 0.  Logits of -inf have probability 0; a row of nothing but
+ * -inf gives logp -inf, stats (-inf, 0), entropy 0.  A NaN or +inf makes the
+ * outputs of its own row NaN.  rows may be 0. */
+size_t llmt_token_logprobs_workspace(int rows, int V, int dtype);
+int llmt_token_logprobs(const void* logits, int dtype, long long ld, const int* targets, int rows,
+                        int V, float inv_temp, float* logp, float* stats, float* entropy,
+                        void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradient: with p = exp(x - m - l) from the forward's stats,
+ *   dlogits[j] = inv_temp (dlogp (1[j = target] - p_j)
+ *                          - dentropy p_j (ln p_j + entropy)),
+ * of the logits' type, rounded once.  dentropy may be NULL (entropy is then
+ * not read).  Rows without a target, rows of nothing but -inf, and rows whose
+ * dlogp and dentropy are both 0 are written as zeros and not read.  dlogits
+ * may be logits itself (with ldd = ld); any other overlap is refused.  In fp16 a
+ * probability times a small dlogp underflows: pass dlogp times a loss scale. */
+int llmt_token_logprobs_bwd(const void* logits, int dtype, long long ld, const int* targets,
+                            const float* stats, const float* entropy, const float* dlogp,
+                            const float* dentropy, int rows, int V, float inv_temp, void* dlogits,
+                            long long ldd, void* stream);
+
+/* Preference loss on n pairs of sequences.  Sequence s is tokens offsets[s] ..
+ * offsets[s + 1] - 1 of the T (offsets int32 [2 n + 1], ascending); pair i
+ * prefers sequence 2 i to sequence 2 i + 1.  logp, and ref_logp of the frozen
+ * reference model (may be NULL: none), fp32 [T]; mask (bytes [T], may be NULL)
+ * leaves tokens out.  With r = beta * sum over the kept tokens of
+ * (logp - ref_logp), divided by their number with `average` (0 without any):
+ *   z = r[2 i] - r[2 i + 1] - margin
+ *   losses[i] = (1 - label_smoothing) f(z) + label_smoothing f(-z)
+ * f: ln(1 + exp(-z)) (sigmoid), max(0, 1 - z) (hinge), (z - 1/2)^2 (square:
+ * beta^2 times the identity-preference loss).  loss [1] is the mean of losses
+ * [n], rewards [2 n] are r, dlogp [T] (may be NULL) the gradient of the mean:
+ * 0 at tokens left out and at tokens of no sequence. */
+enum { LLMT_PREF_SIGMOID = 0, LLMT_PREF_HINGE = 1, LLMT_PREF_SQUARE = 2 };
+typedef struct {
+    int kind, average;
+    float beta, label_smoothing, margin;
+} llmt_pref_params;
+int llmt_preference_loss(const float* logp, const float* ref_logp, const unsigned char* mask,
+                         const int* offsets, int T, int n, const llmt_pref_params* params,
+                         float* loss, float* losses, float* rewards, float* dlogp, void* stream);
+
+/* Clipped policy loss with a KL term over the tokens of n sequences (offsets
+ * int32 [n + 1] as above).  Per kept token, with A its advantage (fp32 [T], or
+ * [n] with adv_per_sequence), ratio = exp(logp - old_logp) (old_logp NULL: the
+ * policy that sampled is this one, ratio 1) and d = ref_logp - logp:
+ *   policy = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *   kl     = exp(d) - d - 1                       (0 with ref_logp NULL)
+ *   l      = policy + kl_coef kl - entropy_coef entropy   (entropy may be NULL)
+ * loss [1] is the mean of l over all kept tokens (LLMT_MEAN_TOKEN), or the
+ * mean over the n sequences of their kept tokens' means, a sequence without
+ * any counting as 0 (LLMT_MEAN_SEQUENCE).  stats [3]: policy, kl and the share
+ * of clipped tokens, averaged the same way.  dlogp, dentropy [T] (may be NULL):
+ * the gradient of loss, 0 at tokens left out and at tokens of no sequence. */
+enum { LLMT_MEAN_TOKEN = 0, LLMT_MEAN_SEQUENCE = 1 };
+typedef struct {
+    int mean, adv_per_sequence;
+    float clip_low, clip_high, kl_coef, entropy_coef;
+} llmt_policy_params;
+size_t llmt_policy_loss_workspace(int T, int n);
+int llmt_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
+                     const float* advantages, const float* entropy, const unsigned char* mask,
+                     const int* offsets, int T, int n, const llmt_policy_params* params,
+                     float* loss, float* stats, float* dlogp, float* dentropy, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

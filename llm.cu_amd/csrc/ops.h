@@ -370,4 +370,60 @@ hipError_t adamw(float* p, const float* g, float* m, float* v, long long n, cons
 hipError_t lora_init(float* p, float* m, float* v, long long n, unsigned long long seed,
                      float a_std, float b_std, const AdamShadow& sh, hipStream_t st);
 
+// ---------------------------------------------------------------- tuning losses
+// Element types of caller-supplied logits (LLMT_F32, LLMT_F16, LLMT_BF16).
+enum { kF32 = 0, kF16 = 1, kBF16 = 2 };
+struct LogprobArgs {
+  const void* logits;  // [rows, ld] of `dtype`
+  long long ld;
+  int dtype;
+  const int* targets;
+  int rows, V;
+  float it;            // inverse temperature
+  float* logp;         // forward outputs
+  float* stats;        // [rows, 2]: max, ln sum exp(x - max)
+  float* entropy;      // NULL, or [rows] (an input of the backward)
+  const float* dlogp;  // backward
+  const float* dentropy;
+  void* dlogits;       // [rows, ldd] of `dtype`; may be the logits themselves
+  long long ldd;
+};
+size_t logprob_workspace(int rows, int V, int dtype);
+hipError_t logprob_fwd(const LogprobArgs& a, void* workspace, hipStream_t st);
+hipError_t logprob_bwd(const LogprobArgs& a, hipStream_t st);
+
+struct PrefArgs {
+  const float* logp;
+  const float* ref;            // NULL: no reference
+  const unsigned char* mask;   // NULL: every token counts
+  const int* offsets;          // [2 n + 1]
+  int T, n, kind, average;
+  double beta, margin, smooth;
+  float* losses;               // [n]
+  float* rewards;              // [2 n]
+  float* mean;                 // [1]
+  float* dlogp;                // NULL, or [T]
+};
+hipError_t preference_loss(const PrefArgs& a, hipStream_t st);
+
+struct PolicyArgs {
+  const float* logp;
+  const float* old;            // NULL: the ratio is 1
+  const float* ref;            // NULL: no KL term
+  const float* adv;            // [T], or [n] with adv_per_seq
+  const float* entropy;        // NULL: no bonus
+  const unsigned char* mask;
+  const int* offsets;          // [n + 1]
+  int T, n, adv_per_seq, seq_mean;
+  double clip_low, clip_high, kl_coef, ent_coef;
+  float* loss;                 // [1]
+  float* stats;                // [3]: policy term, KL, clipped fraction
+  float* dlogp;                // NULL, or [T]
+  float* dentropy;             // NULL, or [T]
+  int* counts;                 // workspace
+  double* parts;
+};
+size_t policy_workspace(int T, int n);
+hipError_t policy_loss(PolicyArgs a, void* workspace, hipStream_t st);
+
 }  // namespace llmt

@@ -11,6 +11,7 @@ import ctypes as C
 import os
 import re
 from pathlib import Path
+from typing import NamedTuple
 
 HERE = Path(__file__).resolve().parent
 PKG = HERE.parent
@@ -24,6 +25,7 @@ LIB_PATH = PKG / "libllmt.so"
 HEADER = ROOT / "include" / "llmt.h"
 
 vp, i32, f32, sz, u64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_uint64
+i64 = C.c_longlong
 fp = C.POINTER(C.c_float)
 
 LLMT_OK, LLMT_ERR_ARG, LLMT_ERR_HIP, LLMT_ERR_IO, LLMT_ERR_STATE = 0, -1, -2, -3, -4
@@ -45,6 +47,16 @@ class HParams(C.Structure):
     _fields_ = [(n, f32) for n in ("lr", "beta1", "beta2", "eps", "wd")]
 
 
+class PrefParams(C.Structure):
+    _fields_ = [("kind", i32), ("average", i32)] + \
+               [(n, f32) for n in ("beta", "label_smoothing", "margin")]
+
+
+class PolicyParams(C.Structure):
+    _fields_ = [("mean", i32), ("adv_per_sequence", i32)] + \
+               [(n, f32) for n in ("clip_low", "clip_high", "kl_coef", "entropy_coef")]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     "llmt_last_error": (C.c_char_p, []),
@@ -58,6 +70,14 @@ _PROTOS = {
     "llmt_attention_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp]),
     "llmt_attention_block_bwd": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32,
                                        f32, f32, vp]),
+    "llmt_token_logprobs_workspace": (sz, [i32, i32, i32]),
+    "llmt_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, f32, vp, vp, vp, vp, sz, vp]),
+    "llmt_token_logprobs_bwd": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, i32, i32, f32, vp, i64,
+                                      vp]),
+    "llmt_preference_loss": (i32, [vp, vp, vp, vp, i32, i32, C.POINTER(PrefParams), vp, vp, vp,
+                                   vp, vp]),
+    "llmt_policy_loss_workspace": (sz, [i32, i32]),
+    "llmt_policy_loss": (i32, [vp] * 7 + [i32, i32, C.POINTER(PolicyParams)] + [vp] * 5 + [sz, vp]),
     "llmt_ctx_create": (i32, [C.POINTER(Dims), i32, i32, i32, vp, C.POINTER(vp)]),
     "llmt_ctx_destroy": (i32, [vp]),
     "llmt_ctx_device_bytes": (sz, [vp]),
@@ -189,6 +209,209 @@ def cross_entropy(logits, targets, seq_len, want_dlogits=True, stream=None):
     check(lib().llmt_cross_entropy(ptr(logits), ptr(targets), rows, V, seq_len, ptr(dl), ptr(lr),
                                    ptr(lm), stream_ptr(stream)))
     return lm, lr, dl
+
+
+# ------------------------------------------------------------------ preferences and rewards
+
+class _On:
+    """The device of the given tensors and a stream on it, for one call: the
+    outputs and the workspace are allocated there, and the inputs are kept from
+    reuse until the stream has passed the call.  `stream` None is the device's
+    current stream."""
+
+    def __init__(self, stream, **tensors):
+        import torch
+        self.inputs = [t for t in tensors.values() if t is not None]
+        for name, t in tensors.items():
+            if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda):
+                raise LlmtError(f"{name} must be a device tensor")
+        self.device = self.inputs[0].device
+        for name, t in tensors.items():
+            if t is not None and t.device != self.device:
+                raise LlmtError(f"{name} is on {t.device}, not on {self.device}")
+        if stream is not None and stream.device != self.device:
+            raise LlmtError(f"the stream is on {stream.device}, the tensors on {self.device}")
+        self.stream = stream
+        self.ctx = None
+        if stream is not None:
+            self.ctx = torch.cuda.stream(stream)
+        elif self.device.index != torch.cuda.current_device():
+            self.ctx = torch.cuda.device(self.device)
+
+    def __enter__(self):
+        import torch
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        self.ptr = C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        return self
+
+    def __exit__(self, *exc):
+        import torch
+        if self.stream is not None and not torch.cuda.is_current_stream_capturing():
+            for t in self.inputs:
+                t.record_stream(self.stream)
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
+
+    def empty(self, *shape, dtype=None):
+        import torch
+        return torch.empty(shape, dtype=dtype or torch.float32, device=self.device)
+
+
+def _expect(name, t, dtype, *shape):
+    """t is a contiguous tensor of this type and shape (None: any length)."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise LlmtError(f"{name} must be {dtype} (got {t.dtype})")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise LlmtError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    if not t.is_contiguous():
+        raise LlmtError(f"{name} must be contiguous")
+
+
+def _logits_dtype(name, t):
+    """The library's code for the type of a [rows, V] tensor with unit column stride."""
+    import torch
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    if code is None:
+        raise LlmtError(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
+    if t.dim() != 2 or t.shape[1] < 1 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise LlmtError(f"{name} must be [rows, V] with V >= 1 and a column stride of 1")
+    return code
+
+
+def _ld(t):
+    """Elements from row to row (a single row's stride is of no account)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _byte_mask(mask, T):
+    import torch
+    if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
+        raise LlmtError(f"mask must be bool or uint8 (got {mask.dtype})")
+    _expect("mask", mask, None if mask is None else mask.dtype, T)
+
+
+def token_logprobs(logits, targets, temperature=1.0, want_entropy=False, stream=None):
+    """Log-probabilities of targets int32 [rows] under softmax(logits /
+    temperature), logits [rows, V] fp32, fp16 or bf16 (rows may be strided):
+    (logp [rows], stats [rows, 2] for token_logprobs_bwd, entropy [rows] or
+    None), fp32.  Rows whose target is outside [0, V) are skipped (zeros)."""
+    import torch
+    with _On(stream, logits=logits, targets=targets) as on:
+        dt = _logits_dtype("logits", logits)
+        rows, V = logits.shape
+        _expect("targets", targets, torch.int32, rows)
+        logp, stats = on.empty(rows), on.empty(rows, 2)
+        ent = on.empty(rows) if want_entropy else None
+        need = lib().llmt_token_logprobs_workspace(rows, V, dt)
+        ws = on.empty(need, dtype=torch.uint8) if need else None
+        check(lib().llmt_token_logprobs(ptr(logits), dt, _ld(logits), ptr(targets), rows, V,
+                                        1.0 / temperature, ptr(logp), ptr(stats), ptr(ent),
+                                        ptr(ws), need, on.ptr))
+    return logp, stats, ent
+
+
+def token_logprobs_bwd(logits, targets, stats, dlogp, entropy=None, dentropy=None,
+                       temperature=1.0, out=None, stream=None):
+    """The gradient of the logits from those of token_logprobs' logp and,
+    where given, its entropy; in the logits' type.  out may be the logits
+    themselves (they are overwritten)."""
+    import torch
+    with _On(stream, logits=logits, targets=targets, stats=stats, dlogp=dlogp, entropy=entropy,
+             dentropy=dentropy, out=out) as on:
+        dt = _logits_dtype("logits", logits)
+        rows, V = logits.shape
+        _expect("targets", targets, torch.int32, rows)
+        _expect("stats", stats, torch.float32, rows, 2)
+        for name, t in (("dlogp", dlogp), ("entropy", entropy), ("dentropy", dentropy)):
+            _expect(name, t, torch.float32, rows)
+        if out is None:
+            out = on.empty(rows, V, dtype=logits.dtype)
+        elif out.shape != logits.shape or _logits_dtype("out", out) != dt:
+            raise LlmtError("out must have the logits' shape and type")
+        check(lib().llmt_token_logprobs_bwd(ptr(logits), dt, _ld(logits), ptr(targets), ptr(stats),
+                                            ptr(entropy), ptr(dlogp), ptr(dentropy), rows, V,
+                                            1.0 / temperature, ptr(out), _ld(out), on.ptr))
+    return out
+
+
+PREF_LOSSES = {"sigmoid": 0, "hinge": 1, "square": 2}
+MEANS = {"token": 0, "sequence": 1}
+
+
+def preference_loss(logp, ref_logp, offsets, loss="sigmoid", beta=0.1, label_smoothing=0.0,
+                    margin=0.0, average=False, mask=None, want_grad=True, stream=None):
+    """Preference loss of n pairs of sequences (llmt_preference_loss): pair i
+    prefers sequence 2 i to 2 i + 1, sequence s being tokens offsets[s] ..
+    offsets[s + 1] - 1 of logp and ref_logp (may be None), fp32 [T]; offsets
+    int32 [2 n + 1]; mask bool [T] keeps tokens.  Returns (mean loss [1],
+    losses [n], rewards [2 n], dlogp [T] or None)."""
+    import torch
+    if loss not in PREF_LOSSES:
+        raise LlmtError(f"loss must be one of {sorted(PREF_LOSSES)} (got {loss!r})")
+    with _On(stream, logp=logp, ref_logp=ref_logp, offsets=offsets, mask=mask) as on:
+        T = logp.shape[0] if logp.dim() == 1 else -1
+        _expect("logp", logp, torch.float32, None)
+        _expect("ref_logp", ref_logp, torch.float32, T)
+        _expect("offsets", offsets, torch.int32, None)
+        _byte_mask(mask, T)
+        n = offsets.shape[0] // 2
+        if n < 1 or offsets.shape[0] != 2 * n + 1:
+            raise LlmtError(f"offsets must be [2 n + 1] with n >= 1 (got {list(offsets.shape)})")
+        mean, losses, rewards = on.empty(1), on.empty(n), on.empty(2 * n)
+        dlogp = on.empty(T) if want_grad else None
+        p = PrefParams(PREF_LOSSES[loss], int(average), beta, label_smoothing, margin)
+        check(lib().llmt_preference_loss(ptr(logp), ptr(ref_logp), ptr(mask), ptr(offsets), T, n,
+                                         C.byref(p), ptr(mean), ptr(losses), ptr(rewards),
+                                         ptr(dlogp), on.ptr))
+    return mean, losses, rewards, dlogp
+
+
+class PolicyLoss(NamedTuple):
+    """loss [1], stats [3] (policy term, KL, share of clipped tokens), and the
+    gradients of loss by logp and by entropy [T] (None where not wanted)."""
+    loss: object
+    stats: object
+    dlogp: object
+    dentropy: object
+
+
+def policy_loss(logp, old_logp, advantages, offsets, ref_logp=None, entropy=None, mask=None,
+                clip_low=0.2, clip_high=0.2, kl_coef=0.0, entropy_coef=0.0, mean="token",
+                per_sequence=False, want_grad=True, stream=None):
+    """Clipped policy loss with a KL term (llmt_policy_loss) over n sequences,
+    sequence s being tokens offsets[s] .. offsets[s + 1] - 1 of the fp32 [T]
+    arrays; advantages [T], or [n] with per_sequence.  old_logp None: ratio 1;
+    ref_logp None: no KL term.  Returns a PolicyLoss."""
+    import torch
+    if mean not in MEANS:
+        raise LlmtError(f"mean must be one of {sorted(MEANS)} (got {mean!r})")
+    with _On(stream, logp=logp, old_logp=old_logp, advantages=advantages, offsets=offsets,
+             ref_logp=ref_logp, entropy=entropy, mask=mask) as on:
+        T = logp.shape[0] if logp.dim() == 1 else -1
+        _expect("logp", logp, torch.float32, None)
+        for name, t in (("old_logp", old_logp), ("ref_logp", ref_logp), ("entropy", entropy)):
+            _expect(name, t, torch.float32, T)
+        _expect("offsets", offsets, torch.int32, None)
+        _byte_mask(mask, T)
+        n = offsets.shape[0] - 1
+        if n < 1:
+            raise LlmtError("offsets must be [n + 1] with n >= 1")
+        _expect("advantages", advantages, torch.float32, n if per_sequence else T)
+        loss, stats = on.empty(1), on.empty(3)
+        dlogp = on.empty(T) if want_grad else None
+        dent = on.empty(T) if want_grad and entropy is not None else None
+        need = lib().llmt_policy_loss_workspace(T, n)
+        ws = on.empty(need, dtype=torch.uint8)
+        p = PolicyParams(MEANS[mean], int(per_sequence), clip_low, clip_high, kl_coef, entropy_coef)
+        check(lib().llmt_policy_loss(ptr(logp), ptr(old_logp), ptr(ref_logp), ptr(advantages),
+                                     ptr(entropy), ptr(mask), ptr(offsets), T, n, C.byref(p),
+                                     ptr(loss), ptr(stats), ptr(dlogp), ptr(dent), ptr(ws), need,
+                                     on.ptr))
+    return PolicyLoss(loss, stats, dlogp, dent)
 
 
 # ------------------------------------------------------------------ training context
