@@ -451,6 +451,41 @@ int llmt_policy_loss(const float* logp, const float* old_logp, const float* ref_
                      float* loss, float* stats, float* dlogp, float* dentropy, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* ---- orthogonalised updates (no counterpart in the reference) ----
+ * Newton-Schulz orthogonalisation of fp32 matrices whose short side is at most
+ * 64 (adapters: their rank): X0 = X / (|X|_F + eps), then `steps` times
+ * X <- 3.4445 X - 4.7750 (X X^T) X + 2.0315 (X X^T)^2 X (of the transpose for a
+ * tall X), in fp64, rounded once.  A zero matrix gives zeros; a NaN or an
+ * infinity makes its own matrix NaN.  count matrices [rows, cols], stride_x
+ * elements from one to the next and ldx from row to row; out likewise, and may
+ * be x itself with the same strides (any other overlap of the two is refused).  The
+ * matrices of one argument must not overlap one another.  1 <= steps <= 20. */
+size_t llmt_orthogonalize_workspace(int count, int rows, int cols);
+int llmt_orthogonalize(const float* x, long long stride_x, long long ldx, float* out,
+                       long long stride_out, long long ldo, int count, int rows, int cols,
+                       int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Muon on an arena of `layers` layers of nmat (<= 8) matrices, [rows_host[j],
+ * cols_host[j]] each (host arrays), one behind another without gaps; p, g, m
+ * fp32 arenas of that layout that do not overlap:
+ *   m <- momentum m + g;   u = nesterov ? g + momentum m : m
+ *   p <- p (1 - lr wd) - lr s orthogonalised(u)
+ * with s = 0.2 sqrt(max(rows, cols)) (LLMT_MUON_SCALE_RMS: updates of AdamW's
+ * size) or sqrt(max(1, rows / cols)) (LLMT_MUON_SCALE_SHAPE). */
+enum { LLMT_MUON_SCALE_RMS = 0, LLMT_MUON_SCALE_SHAPE = 1 };
+typedef struct {
+    float lr, momentum, wd, eps;
+    int steps, nesterov, scale;
+} llmt_muon_params;
+size_t llmt_muon_update_workspace(int layers, int nmat, const int* rows_host, const int* cols_host);
+int llmt_muon_update(float* p, const float* g, float* m, int layers, int nmat,
+                     const int* rows_host, const int* cols_host, const llmt_muon_params* params,
+                     void* workspace, size_t workspace_bytes, void* stream);
+/* Muon over a context's whole adapter arena from its GRAD arena (the M arena
+ * holds the momentum, V is not used), in place of llmt_adamw; one host
+ * synchronisation. */
+int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params);
+
 #ifdef __cplusplus
 }
 #endif

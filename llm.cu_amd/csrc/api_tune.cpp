@@ -1,12 +1,14 @@
-// api_tune.cpp — C ABI of the operators for tuning on preferences and rewards:
-// token log-probabilities, the preference and policy losses.  Every entry
-// point validates its arguments on the host before any launch and allocates
-// nothing.
+// api_tune.cpp — C ABI of the operators for tuning on preferences and rewards
+// (token log-probabilities, the preference and policy losses) and of the
+// orthogonalised updates.  Every entry point validates its arguments on the
+// host before any launch; the standalone ones allocate nothing.
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/llmt.h"
-#include "ops.h"
+#include "ctx.h"
 
 using namespace llmt;
 
@@ -35,6 +37,68 @@ static int check_logits(const char* fn, const void* logits, int dtype, long long
   TRY_ARG(inv_temp > 0.f && isfinite(inv_temp), "%s: inv_temp must be positive and finite", fn);
   TRY_ARG(rows == 0 || (logits && targets), "%s: NULL argument", fn);
   TRY_ARG(aligned(logits, esize(dtype)) && aligned(targets, 4), "%s: misaligned argument", fn);
+  return LLMT_OK;
+}
+
+// Whether na floats at a and nb floats at b do not meet.
+static bool apart(const void* a, long long na, const void* b, long long nb) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  return a0 + (size_t)na * 4 <= b0 || b0 + (size_t)nb * 4 <= a0;
+}
+
+// Matrices of one call, and the long side of one: grids and indexes stay
+// within 31 bits.
+constexpr int kMaxMatrices = 1 << 20, kMaxLong = 1 << 30;
+
+static NsMat ns_matrix(int rows, int cols) {
+  NsMat m{};
+  m.tall = rows > cols;
+  m.r = std::min(rows, cols);
+  m.n = std::max(rows, cols);
+  m.ld_in = m.ld_out = cols;
+  m.lr = 0.f;
+  return m;
+}
+
+// The layout of an arena of layers x nmat matrices.
+static int muon_layout(const char* fn, int layers, int nmat, const int* rows, const int* cols,
+                       NsArgs& a) {
+  TRY_ARG(layers >= 1 && nmat >= 1 && nmat <= kNsMats && rows && cols,
+          "%s: layers=%d nmat=%d (1 to %d matrices a layer)", fn, layers, nmat, kNsMats);
+  TRY_ARG(layers <= kMaxMatrices / kNsMats, "%s: %d layers, at most %d", fn, layers,
+          kMaxMatrices / kNsMats);
+  a.layers = layers;
+  a.nmat = nmat;
+  long long off = 0;
+  for (int j = 0; j < nmat; ++j) {
+    TRY_ARG(rows[j] >= 1 && cols[j] >= 1 && std::min(rows[j], cols[j]) <= kNsMaxShort &&
+                std::max(rows[j], cols[j]) <= kMaxLong,
+            "%s: matrix %d is %d x %d (short side 1 to %d)", fn, j, rows[j], cols[j], kNsMaxShort);
+    a.mat[j] = ns_matrix(rows[j], cols[j]);
+    a.mat[j].off = off;
+    off += (long long)rows[j] * cols[j];
+  }
+  a.in_stride = a.out_stride = off;
+  return LLMT_OK;
+}
+
+static int muon_params(const char* fn, const llmt_muon_params* p, NsArgs& a) {
+  TRY_ARG(p, "%s: NULL params", fn);
+  TRY_ARG(isfinite(p->lr) && p->momentum >= 0.f && p->momentum < 1.f && isfinite(p->wd) &&
+              p->eps > 0.f && isfinite(p->eps) && p->steps >= 1 && p->steps <= 20,
+          "%s: momentum in [0, 1), eps positive, steps in [1, 20], finite lr and wd", fn);
+  TRY_ARG(p->scale == LLMT_MUON_SCALE_RMS || p->scale == LLMT_MUON_SCALE_SHAPE, "%s: scale %d", fn,
+          p->scale);
+  a.mu = p->momentum;
+  a.nesterov = p->nesterov != 0;
+  a.steps = p->steps;
+  a.eps = p->eps;
+  a.decay = (float)(1.0 - (double)p->lr * p->wd);
+  for (int j = 0; j < a.nmat; ++j) {
+    const double r = a.mat[j].r, n = a.mat[j].n;
+    const double s = p->scale == LLMT_MUON_SCALE_RMS ? 0.2 * sqrt(n) : a.mat[j].tall ? sqrt(n / r) : 1.0;
+    a.mat[j].lr = (float)(p->lr * s);
+  }
   return LLMT_OK;
 }
 
@@ -194,6 +258,123 @@ int llmt_policy_loss(const float* logp, const float* old_logp, const float* ref_
   a.dlogp = dlogp;
   a.dentropy = dentropy;
   return done(policy_loss(a, workspace, (hipStream_t)stream));
+}
+
+size_t llmt_orthogonalize_workspace(int count, int rows, int cols) {
+  if (count < 1 || count > kMaxMatrices || rows < 1 || cols < 1 ||
+      std::min(rows, cols) > kNsMaxShort || std::max(rows, cols) > kMaxLong)
+    return 0;
+  NsArgs a{};
+  a.layers = count;
+  a.nmat = 1;
+  a.mat[0] = ns_matrix(rows, cols);
+  return ns_workspace(a);
+}
+
+int llmt_orthogonalize(const float* x, long long stride_x, long long ldx, float* out,
+                       long long stride_out, long long ldo, int count, int rows, int cols,
+                       int steps, float eps, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  set_error("");
+  TRY_ARG(count >= 0 && rows >= 1 && cols >= 1, "llmt_orthogonalize: count=%d rows=%d cols=%d",
+          count, rows, cols);
+  TRY_ARG(std::min(rows, cols) <= kNsMaxShort && std::max(rows, cols) <= kMaxLong,
+          "llmt_orthogonalize: %d x %d: the short side is at most %d", rows, cols, kNsMaxShort);
+  TRY_ARG(count <= kMaxMatrices, "llmt_orthogonalize: %d matrices, at most %d", count, kMaxMatrices);
+  TRY_ARG(steps >= 1 && steps <= 20 && eps > 0.f && isfinite(eps),
+          "llmt_orthogonalize: steps in [1, 20], eps positive");
+  const long long span_x = (long long)(rows - 1) * ldx + cols;
+  const long long span_o = (long long)(rows - 1) * ldo + cols;
+  TRY_ARG(ldx >= cols && ldo >= cols &&
+              (count <= 1 || (stride_x >= span_x && stride_out >= span_o)),
+          "llmt_orthogonalize: ldx=%lld ldo=%lld stride_x=%lld stride_out=%lld", ldx, ldo, stride_x,
+          stride_out);
+  if (count == 0) return LLMT_OK;
+  TRY_ARG(x && out, "llmt_orthogonalize: NULL argument");
+  TRY_ARG(aligned(x, 4) && aligned(out, 4), "llmt_orthogonalize: misaligned argument");
+  if (x == out)
+    TRY_ARG(ldx == ldo && (count == 1 || stride_x == stride_out),
+            "llmt_orthogonalize: in place with other strides");
+  else
+    TRY_ARG(apart(x, (count - 1) * stride_x + span_x, out, (count - 1) * stride_out + span_o),
+            "llmt_orthogonalize: out overlaps x");
+  NsArgs a{};
+  a.x = x;
+  a.out = out;
+  a.in_stride = stride_x;
+  a.out_stride = stride_out;
+  a.layers = count;
+  a.nmat = 1;
+  a.mat[0] = ns_matrix(rows, cols);
+  a.mat[0].ld_in = ldx;
+  a.mat[0].ld_out = ldo;
+  a.steps = steps;
+  a.eps = eps;
+  const size_t need = ns_workspace(a);
+  TRY_ARG(workspace && workspace_bytes >= need && aligned(workspace, 16),
+          "llmt_orthogonalize: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace ? workspace_bytes : 0, need);
+  return done(newton_schulz(a, workspace, (hipStream_t)stream));
+}
+
+size_t llmt_muon_update_workspace(int layers, int nmat, const int* rows_host,
+                                  const int* cols_host) {
+  NsArgs a{};
+  return muon_layout("", layers, nmat, rows_host, cols_host, a) == LLMT_OK ? ns_workspace(a) : 0;
+}
+
+int llmt_muon_update(float* p, const float* g, float* m, int layers, int nmat,
+                     const int* rows_host, const int* cols_host, const llmt_muon_params* params,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("");
+  NsArgs a{};
+  int rc = muon_layout("llmt_muon_update", layers, nmat, rows_host, cols_host, a);
+  if (rc) return rc;
+  if ((rc = muon_params("llmt_muon_update", params, a))) return rc;
+  TRY_ARG(p && g && m, "llmt_muon_update: NULL argument");
+  TRY_ARG(aligned(p, 4) && aligned(g, 4) && aligned(m, 4), "llmt_muon_update: misaligned argument");
+  const long long n = a.in_stride * layers;
+  TRY_ARG(apart(p, n, g, n) && apart(p, n, m, n) && apart(g, n, m, n),
+          "llmt_muon_update: p, g and m overlap");
+  const size_t need = ns_workspace(a);
+  TRY_ARG(workspace && workspace_bytes >= need && aligned(workspace, 16),
+          "llmt_muon_update: workspace of %zu bytes, %zu needed (16-byte aligned)",
+          workspace ? workspace_bytes : 0, need);
+  a.x = g;
+  a.m = m;
+  a.out = p;
+  return done(newton_schulz(a, workspace, (hipStream_t)stream));
+}
+
+int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params) {
+  set_error("");
+  Ctx* c = reinterpret_cast<Ctx*>(ctx);
+  TRY_ARG(c, "llmt_muon: NULL ctx");
+  // a layer of the arena: q, k, v, o; A [rank, in] then B [out, rank]
+  const int q = c->Q, kv = c->KV, h = c->H;
+  const int in[4] = {h, h, h, q}, out[4] = {q, kv, kv, h};
+  int rows[8], cols[8];
+  for (int j = 0; j < 4; ++j) {
+    rows[2 * j] = cols[2 * j + 1] = kRank;
+    cols[2 * j] = in[j];
+    rows[2 * j + 1] = out[j];
+  }
+  NsArgs a{};
+  int rc = muon_layout("llmt_muon", c->L, 8, rows, cols, a);
+  if (rc) return rc;
+  if ((rc = muon_params("llmt_muon", params, a))) return rc;
+  TRY_ARG((size_t)a.in_stride == c->lora_per_layer, "llmt_muon: the arena's layout");
+  if (!c->muon_ws) {
+    c->muon_ws = c->alloc(ns_workspace(a));
+    if (!c->muon_ws) return LLMT_ERR_HIP;
+  }
+  a.x = c->lora_g;
+  a.m = c->lora_m;
+  a.out = c->lora_p;
+  hipError_t e = newton_schulz(a, c->muon_ws, c->st);
+  if (e == hipSuccess) e = c->refresh_shadows();
+  if (e == hipSuccess) e = hipStreamSynchronize(c->st);
+  return done(e);
 }
 
 }  // extern "C"

@@ -129,6 +129,7 @@ struct Ctx {
   // A_q | A_k | A_v transposed, [L][H][3 R] (the LoRA dx term's MFMA operand
   // in the attention norm's backward)
   _Float16* shadow_at = nullptr;
+  void* muon_ws = nullptr;  // llmt_muon's workspace, allocated by its first call
   AdamHp* hp_dev = nullptr;
   AdamHp* host_hp = nullptr;
 

@@ -426,4 +426,30 @@ struct PolicyArgs {
 size_t policy_workspace(int T, int n);
 hipError_t policy_loss(PolicyArgs a, void* workspace, hipStream_t st);
 
+// ---------------------------------------------------------------- orthogonalised updates
+// One matrix of a layer: element (s, k), s on its short side (r <= kNsMaxShort),
+// k on its long side (n), at off + s ld + k, or off + k ld + s of a tall one.
+constexpr int kNsMaxShort = 64;
+constexpr int kNsMats = 8;
+struct NsMat {
+  long long off, ld_in, ld_out;
+  int r, n, tall;
+  float lr;            // MUON: learning rate times the matrix's scale
+};
+struct NsArgs {
+  const float* x;      // the update, or with m the gradient
+  float* m;            // NULL (orthogonalise), or the momentum (Muon)
+  float* out;          // the result, or the parameters
+  long long in_stride, out_stride;  // layer to layer
+  int layers, nmat, steps, nesterov;
+  float mu, decay;
+  double eps;
+  NsMat mat[kNsMats];
+  int splits;          // filled by newton_schulz
+  double* gram;
+  double* proj;
+};
+size_t ns_workspace(const NsArgs& a);
+hipError_t newton_schulz(const NsArgs& a, void* workspace, hipStream_t st);
+
 }  // namespace llmt

@@ -57,6 +57,11 @@ class PolicyParams(C.Structure):
                [(n, f32) for n in ("clip_low", "clip_high", "kl_coef", "entropy_coef")]
 
 
+class MuonParams(C.Structure):
+    _fields_ = [(n, f32) for n in ("lr", "momentum", "wd", "eps")] + \
+               [(n, i32) for n in ("steps", "nesterov", "scale")]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     "llmt_last_error": (C.c_char_p, []),
@@ -78,6 +83,12 @@ _PROTOS = {
                                    vp, vp]),
     "llmt_policy_loss_workspace": (sz, [i32, i32]),
     "llmt_policy_loss": (i32, [vp] * 7 + [i32, i32, C.POINTER(PolicyParams)] + [vp] * 5 + [sz, vp]),
+    "llmt_orthogonalize_workspace": (sz, [i32, i32, i32]),
+    "llmt_orthogonalize": (i32, [vp, i64, i64, vp, i64, i64, i32, i32, i32, i32, f32, vp, sz, vp]),
+    "llmt_muon_update_workspace": (sz, [i32, i32, C.POINTER(i32), C.POINTER(i32)]),
+    "llmt_muon_update": (i32, [vp, vp, vp, i32, i32, C.POINTER(i32), C.POINTER(i32),
+                               C.POINTER(MuonParams), vp, sz, vp]),
+    "llmt_muon": (i32, [vp, C.POINTER(MuonParams)]),
     "llmt_ctx_create": (i32, [C.POINTER(Dims), i32, i32, i32, vp, C.POINTER(vp)]),
     "llmt_ctx_destroy": (i32, [vp]),
     "llmt_ctx_device_bytes": (sz, [vp]),
@@ -414,6 +425,67 @@ def policy_loss(logp, old_logp, advantages, offsets, ref_logp=None, entropy=None
     return PolicyLoss(loss, stats, dlogp, dent)
 
 
+# ------------------------------------------------------------------ orthogonalised updates
+
+def orthogonalize(x, steps=5, eps=1e-7, out=None, stream=None):
+    """Newton-Schulz orthogonalisation (llmt_orthogonalize) of a matrix [rows,
+    cols] or a stack [count, rows, cols], fp32, the short side at most 64; rows
+    may be strided.  out may be x itself."""
+    import torch
+    with _On(stream, x=x, out=out) as on:
+        if x.dtype != torch.float32 or x.dim() not in (2, 3) or 0 in x.shape[-2:]:
+            raise LlmtError("x must be float32 [rows, cols] or [count, rows, cols]")
+        if out is None:
+            out = on.empty(*x.shape)
+        elif out.shape != x.shape or out.dtype != torch.float32:
+            raise LlmtError("out must have x's shape and type")
+        rows, cols = x.shape[-2:]
+        count = x.shape[0] if x.dim() == 3 else 1
+
+        def strides(name, t):  # of one row or one matrix the stride is of no account
+            if cols > 1 and t.stride(-1) != 1:
+                raise LlmtError(f"{name} must have a column stride of 1")
+            ld = t.stride(-2) if rows > 1 else cols
+            return (t.stride(0) if count > 1 else rows * ld), ld
+
+        (sx, ldx), (so, ldo) = strides("x", x), strides("out", out)
+        need = lib().llmt_orthogonalize_workspace(count, rows, cols)
+        ws = on.empty(need, dtype=torch.uint8)
+        check(lib().llmt_orthogonalize(ptr(x), sx, ldx, ptr(out), so, ldo, count, rows, cols,
+                                       steps, eps, ptr(ws), need, on.ptr))
+    return out
+
+
+MUON_SCALES = {"rms": 0, "shape": 1}
+
+
+def muon_hparams(lr=2e-3, momentum=0.95, wd=0.01, eps=1e-7, steps=5, nesterov=True,
+                 scale="rms") -> MuonParams:
+    """Muon's hyper-parameters (llmt_muon_update)."""
+    if scale not in MUON_SCALES:
+        raise LlmtError(f"scale must be one of {sorted(MUON_SCALES)} (got {scale!r})")
+    return MuonParams(lr, momentum, wd, eps, steps, int(nesterov), MUON_SCALES[scale])
+
+
+def muon_update(p, g, m, shapes, hp: MuonParams, stream=None):
+    """One Muon step in place on flat fp32 arenas p and m from the gradients g:
+    layers of the matrices `shapes` [(rows, cols), ..] one behind another."""
+    import torch
+    with _On(stream, p=p, g=g, m=m) as on:
+        n = p.shape[0] if p.dim() == 1 else -1
+        for name, t in (("p", p), ("g", g), ("m", m)):
+            _expect(name, t, torch.float32, n if n >= 0 else None)
+        per = sum(r * c for r, c in shapes)
+        if per < 1 or n < 1 or n % per:
+            raise LlmtError(f"the arena's {n} elements are not whole layers of {per}")
+        k = len(shapes)
+        rows, cols = (i32 * k)(*(s[0] for s in shapes)), (i32 * k)(*(s[1] for s in shapes))
+        need = lib().llmt_muon_update_workspace(n // per, k, rows, cols)
+        ws = on.empty(need, dtype=torch.uint8)
+        check(lib().llmt_muon_update(ptr(p), ptr(g), ptr(m), n // per, k, rows, cols, C.byref(hp),
+                                     ptr(ws), need, on.ptr))
+
+
 # ------------------------------------------------------------------ training context
 
 PROFILE_CATEGORIES = ("gemm_fwd", "gemm_bwd", "gemm_lm_head", "attention", "row_epilogues",
@@ -576,6 +648,10 @@ class Context:
             __cuda_array_interface__ = {"shape": (rows, V), "typestr": "<f4",
                                         "data": (addr, False), "version": 3, "strides": None}
         return torch.as_tensor(_View(), device="cuda").clone()
+
+    def muon(self, hp: MuonParams):
+        """One Muon step over the adapters from the GRAD arena (llmt_muon)."""
+        check(lib().llmt_muon(self.h, C.byref(hp)))
 
     def head_ce(self, hidden16, targets, want_dlogits=False):
         """C1 on the context's tied embedding: (loss, dlogits or None, dhidden)."""

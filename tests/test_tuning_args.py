@@ -92,11 +92,60 @@ def test_policy_refusals(bad):
     assert llmt.lib().llmt_last_error().decode().startswith("llmt_policy_loss:")
 
 
+def ortho(x=A(1), sx=800, ldx=100, out=A(2), so=800, ldo=100, count=2, rows=8, cols=100, steps=5,
+          eps=1e-7, ws=A(8), need=1 << 20):
+    return llmt.lib().llmt_orthogonalize(x, sx, ldx, out, so, ldo, count, rows, cols, steps, eps, ws,
+                                         need, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(count=-1), dict(count=2 ** 21), dict(rows=0), dict(cols=0, ldx=0, ldo=0),
+    dict(rows=65, sx=6500, so=6500), dict(ldx=99), dict(ldo=99), dict(sx=799), dict(so=799),
+    dict(steps=0), dict(steps=21), dict(eps=0.0), dict(eps=math.nan), dict(x=None), dict(out=None),
+    dict(x=C.c_void_p(0x100002)), dict(ws=None), dict(need=100), dict(ws=C.c_void_p(0x800004)),
+    dict(out=A(1), so=801), dict(out=A(1), ldo=101, so=900), dict(out=C.c_void_p(0x100004)),
+    dict(out=C.c_void_p(0x100000 + 4 * 1599)), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldo=2 ** 31,
+                                                    sx=2 ** 36, so=2 ** 36)])
+def test_orthogonalize_refusals(bad):
+    assert ortho(**bad) == ARG
+    assert llmt.lib().llmt_last_error().decode().startswith("llmt_orthogonalize:")
+
+
+def muon(p=A(1), g=A(2), m=A(3), layers=2, shapes=((8, 100), (50, 8)), nmat=None,
+         params=(0.01, 0.9, 0.0, 1e-7, 5, 1, 0), ws=A(8), need=1 << 20):
+    k = len(shapes)
+    rows, cols = (C.c_int * k)(*(s[0] for s in shapes)), (C.c_int * k)(*(s[1] for s in shapes))
+    hp = None if params is None else C.byref(llmt.MuonParams(*params))
+    return llmt.lib().llmt_muon_update(p, g, m, layers, k if nmat is None else nmat, rows, cols, hp,
+                                       ws, need, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(p=None), dict(g=None), dict(m=None), dict(layers=0), dict(layers=2 ** 20), dict(nmat=0),
+    dict(nmat=9), dict(shapes=((65, 65),)), dict(shapes=((0, 5),)), dict(params=None),
+    dict(params=(math.nan, 0.9, 0.0, 1e-7, 5, 1, 0)), dict(params=(0.01, 1.0, 0.0, 1e-7, 5, 1, 0)),
+    dict(params=(0.01, -0.1, 0.0, 1e-7, 5, 1, 0)), dict(params=(0.01, 0.9, math.inf, 1e-7, 5, 1, 0)),
+    dict(params=(0.01, 0.9, 0.0, 0.0, 5, 1, 0)), dict(params=(0.01, 0.9, 0.0, 1e-7, 0, 1, 0)),
+    dict(params=(0.01, 0.9, 0.0, 1e-7, 5, 1, 2)), dict(g=A(1)), dict(m=C.c_void_p(0x200004)),
+    dict(p=C.c_void_p(0x300000 - 4 * 2399)), dict(ws=None), dict(need=64),
+    dict(m=C.c_void_p(0x300002))])
+def test_muon_refusals(bad):
+    assert muon(**bad) == ARG
+    assert llmt.lib().llmt_last_error().decode().startswith("llmt_muon_update:")
+
+
+def test_context_muon_refuses_null():
+    assert llmt.lib().llmt_muon(None, None) == ARG
+
+
 def test_workspace_sizes():
     L = llmt.lib()
     assert L.llmt_policy_loss_workspace(-1, 2) == 0 and L.llmt_policy_loss_workspace(5, 0) == 0
     assert L.llmt_policy_loss_workspace(2 ** 31 - 1, 2 ** 29) < 2 ** 33
     assert L.llmt_token_logprobs_workspace(0, 100, 0) == 0
+    assert L.llmt_orthogonalize_workspace(1, 65, 65) == 0 and L.llmt_orthogonalize_workspace(0, 4, 4) == 0
+    assert L.llmt_orthogonalize_workspace(1, 16, 2048) > 0
+    assert L.llmt_muon_update_workspace(1, 9, None, None) == 0
 
 
 def test_the_binding_refuses_host_tensors():
@@ -106,6 +155,8 @@ def test_the_binding_refuses_host_tensors():
                  lambda: llmt.token_logprobs_bwd(x, t, x, x[:, 0]),
                  lambda: llmt.preference_loss(x[0], None, off),
                  lambda: llmt.policy_loss(x[0], None, x[0], off),
+                 lambda: llmt.orthogonalize(x),
+                 lambda: llmt.muon_update(x[0], x[1], x[1], [(2, 4)], llmt.muon_hparams()),
                  lambda: llmt.token_logprobs([1.0], t)):
         with pytest.raises(llmt.LlmtError, match="must be a device tensor"):
             call()
@@ -113,3 +164,5 @@ def test_the_binding_refuses_host_tensors():
         llmt.preference_loss(x[0], None, off, loss="dpo")
     with pytest.raises(llmt.LlmtError, match="mean must be one of"):
         llmt.policy_loss(x[0], None, x[0], off, mean="sum")
+    with pytest.raises(llmt.LlmtError, match="scale must be one of"):
+        llmt.muon_hparams(scale="spectral")
