@@ -225,49 +225,56 @@ def cross_entropy(logits, targets, seq_len, want_dlogits=True, stream=None):
 # ------------------------------------------------------------------ preferences and rewards
 
 class _On:
-    """The device of the given tensors and a stream on it, for one call: the
-    outputs and the workspace are allocated there, and the inputs are kept from
-    reuse until the stream has passed the call.  `stream` None is the device's
-    current stream."""
+    """The device of a call's tensors and its stream, where the outputs and the
+    workspace are allocated.  `stream` None is the device's current stream;
+    otherwise the inputs are kept from reuse until the stream has passed the
+    call.  `raw` is the stream's address."""
 
-    def __init__(self, stream, **tensors):
+    __slots__ = ("inputs", "stream", "ctx", "raw")
+
+    def __init__(self, names, tensors, stream):
         import torch
-        self.inputs = [t for t in tensors.values() if t is not None]
-        for name, t in tensors.items():
-            if t is not None and not (isinstance(t, torch.Tensor) and t.is_cuda):
-                raise LlmtError(f"{name} must be a device tensor")
-        self.device = self.inputs[0].device
-        for name, t in tensors.items():
-            if t is not None and t.device != self.device:
-                raise LlmtError(f"{name} is on {t.device}, not on {self.device}")
-        if stream is not None and stream.device != self.device:
-            raise LlmtError(f"the stream is on {stream.device}, the tensors on {self.device}")
-        self.stream = stream
-        self.ctx = None
+        index = -1
+        for t in tensors:
+            if t is not None:
+                at = t.get_device() if isinstance(t, torch.Tensor) else -1
+                if at < 0 or (index >= 0 and at != index):
+                    name = names.split()[[t is u for u in tensors].index(True)]
+                    raise LlmtError(f"{name} must be a device tensor" if at < 0 else
+                                    f"{name} is on device {at}, other tensors on {index}")
+                index = at
+        self.stream, self.ctx = stream, None
         if stream is not None:
+            if stream.device_index != index:
+                raise LlmtError(f"the stream is on {stream.device}, the tensors on device {index}")
+            self.inputs = tensors
             self.ctx = torch.cuda.stream(stream)
-        elif self.device.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(self.device)
+            self.raw = stream.cuda_stream
+        else:
+            if torch._C._cuda_getDevice() != index:
+                self.ctx = torch.cuda.device(index)
+            self.raw = torch._C._cuda_getCurrentRawStream(index)
 
     def __enter__(self):
-        import torch
         if self.ctx is not None:
             self.ctx.__enter__()
-        self.ptr = C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
         return self
 
     def __exit__(self, *exc):
-        import torch
-        if self.stream is not None and not torch.cuda.is_current_stream_capturing():
-            for t in self.inputs:
-                t.record_stream(self.stream)
         if self.ctx is not None:
+            if self.stream is not None:
+                import torch
+                if not torch.cuda.is_current_stream_capturing():
+                    for t in self.inputs:
+                        if t is not None:
+                            t.record_stream(self.stream)
             self.ctx.__exit__(*exc)
         return False
 
-    def empty(self, *shape, dtype=None):
-        import torch
-        return torch.empty(shape, dtype=dtype or torch.float32, device=self.device)
+
+def _at(t):
+    """The address of a tensor's first element, or None."""
+    return None if t is None else t.data_ptr()
 
 
 def _expect(name, t, dtype, *shape):
@@ -276,7 +283,8 @@ def _expect(name, t, dtype, *shape):
         return
     if t.dtype != dtype:
         raise LlmtError(f"{name} must be {dtype} (got {t.dtype})")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    if t.shape != shape and (t.dim() != len(shape) or
+                             any(n is not None and n != m for n, m in zip(shape, t.shape))):
         raise LlmtError(f"{name} must be {list(shape)} (got {list(t.shape)})")
     if not t.is_contiguous():
         raise LlmtError(f"{name} must be contiguous")
@@ -311,17 +319,19 @@ def token_logprobs(logits, targets, temperature=1.0, want_entropy=False, stream=
     (logp [rows], stats [rows, 2] for token_logprobs_bwd, entropy [rows] or
     None), fp32.  Rows whose target is outside [0, V) are skipped (zeros)."""
     import torch
-    with _On(stream, logits=logits, targets=targets) as on:
+    with _On("logits targets", (logits, targets), stream) as on:
         dt = _logits_dtype("logits", logits)
         rows, V = logits.shape
         _expect("targets", targets, torch.int32, rows)
-        logp, stats = on.empty(rows), on.empty(rows, 2)
-        ent = on.empty(rows) if want_entropy else None
-        need = lib().llmt_token_logprobs_workspace(rows, V, dt)
-        ws = on.empty(need, dtype=torch.uint8) if need else None
-        check(lib().llmt_token_logprobs(ptr(logits), dt, _ld(logits), ptr(targets), rows, V,
-                                        1.0 / temperature, ptr(logp), ptr(stats), ptr(ent),
-                                        ptr(ws), need, on.ptr))
+        logp = logits.new_empty(rows, dtype=torch.float32)
+        stats = logits.new_empty((rows, 2), dtype=torch.float32)
+        ent = torch.empty_like(logp) if want_entropy else None
+        L = lib()
+        need = L.llmt_token_logprobs_workspace(rows, V, dt)
+        ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_token_logprobs(logits.data_ptr(), dt, _ld(logits), targets.data_ptr(), rows, V,
+                                    1.0 / temperature, logp.data_ptr(), stats.data_ptr(), _at(ent),
+                                    _at(ws), need, on.raw))
     return logp, stats, ent
 
 
@@ -331,21 +341,23 @@ def token_logprobs_bwd(logits, targets, stats, dlogp, entropy=None, dentropy=Non
     where given, its entropy; in the logits' type.  out may be the logits
     themselves (they are overwritten)."""
     import torch
-    with _On(stream, logits=logits, targets=targets, stats=stats, dlogp=dlogp, entropy=entropy,
-             dentropy=dentropy, out=out) as on:
+    with _On("logits targets stats dlogp entropy dentropy out",
+             (logits, targets, stats, dlogp, entropy, dentropy, out), stream) as on:
         dt = _logits_dtype("logits", logits)
         rows, V = logits.shape
         _expect("targets", targets, torch.int32, rows)
         _expect("stats", stats, torch.float32, rows, 2)
-        for name, t in (("dlogp", dlogp), ("entropy", entropy), ("dentropy", dentropy)):
-            _expect(name, t, torch.float32, rows)
+        _expect("dlogp", dlogp, torch.float32, rows)
+        _expect("entropy", entropy, torch.float32, rows)
+        _expect("dentropy", dentropy, torch.float32, rows)
         if out is None:
-            out = on.empty(rows, V, dtype=logits.dtype)
+            out = logits.new_empty((rows, V))
         elif out.shape != logits.shape or _logits_dtype("out", out) != dt:
             raise LlmtError("out must have the logits' shape and type")
-        check(lib().llmt_token_logprobs_bwd(ptr(logits), dt, _ld(logits), ptr(targets), ptr(stats),
-                                            ptr(entropy), ptr(dlogp), ptr(dentropy), rows, V,
-                                            1.0 / temperature, ptr(out), _ld(out), on.ptr))
+        check(lib().llmt_token_logprobs_bwd(logits.data_ptr(), dt, _ld(logits), targets.data_ptr(),
+                                            stats.data_ptr(), _at(entropy), dlogp.data_ptr(),
+                                            _at(dentropy), rows, V, 1.0 / temperature,
+                                            out.data_ptr(), _ld(out), on.raw))
     return out
 
 
@@ -361,23 +373,24 @@ def preference_loss(logp, ref_logp, offsets, loss="sigmoid", beta=0.1, label_smo
     int32 [2 n + 1]; mask bool [T] keeps tokens.  Returns (mean loss [1],
     losses [n], rewards [2 n], dlogp [T] or None)."""
     import torch
-    if loss not in PREF_LOSSES:
+    kind = PREF_LOSSES.get(loss)
+    if kind is None:
         raise LlmtError(f"loss must be one of {sorted(PREF_LOSSES)} (got {loss!r})")
-    with _On(stream, logp=logp, ref_logp=ref_logp, offsets=offsets, mask=mask) as on:
-        T = logp.shape[0] if logp.dim() == 1 else -1
+    with _On("logp ref_logp offsets mask", (logp, ref_logp, offsets, mask), stream) as on:
         _expect("logp", logp, torch.float32, None)
+        T = logp.shape[0]
         _expect("ref_logp", ref_logp, torch.float32, T)
         _expect("offsets", offsets, torch.int32, None)
         _byte_mask(mask, T)
         n = offsets.shape[0] // 2
         if n < 1 or offsets.shape[0] != 2 * n + 1:
             raise LlmtError(f"offsets must be [2 n + 1] with n >= 1 (got {list(offsets.shape)})")
-        mean, losses, rewards = on.empty(1), on.empty(n), on.empty(2 * n)
-        dlogp = on.empty(T) if want_grad else None
-        p = PrefParams(PREF_LOSSES[loss], int(average), beta, label_smoothing, margin)
-        check(lib().llmt_preference_loss(ptr(logp), ptr(ref_logp), ptr(mask), ptr(offsets), T, n,
-                                         C.byref(p), ptr(mean), ptr(losses), ptr(rewards),
-                                         ptr(dlogp), on.ptr))
+        mean, losses, rewards = logp.new_empty(3 * n + 1).split_with_sizes((1, n, 2 * n))
+        dlogp = torch.empty_like(logp) if want_grad else None
+        p = PrefParams(kind, average, beta, label_smoothing, margin)
+        check(lib().llmt_preference_loss(logp.data_ptr(), _at(ref_logp), _at(mask),
+                                         offsets.data_ptr(), T, n, p, mean.data_ptr(),
+                                         losses.data_ptr(), rewards.data_ptr(), _at(dlogp), on.raw))
     return mean, losses, rewards, dlogp
 
 
@@ -398,30 +411,33 @@ def policy_loss(logp, old_logp, advantages, offsets, ref_logp=None, entropy=None
     arrays; advantages [T], or [n] with per_sequence.  old_logp None: ratio 1;
     ref_logp None: no KL term.  Returns a PolicyLoss."""
     import torch
-    if mean not in MEANS:
+    kind = MEANS.get(mean)
+    if kind is None:
         raise LlmtError(f"mean must be one of {sorted(MEANS)} (got {mean!r})")
-    with _On(stream, logp=logp, old_logp=old_logp, advantages=advantages, offsets=offsets,
-             ref_logp=ref_logp, entropy=entropy, mask=mask) as on:
-        T = logp.shape[0] if logp.dim() == 1 else -1
+    with _On("logp old_logp advantages offsets ref_logp entropy mask",
+             (logp, old_logp, advantages, offsets, ref_logp, entropy, mask), stream) as on:
         _expect("logp", logp, torch.float32, None)
-        for name, t in (("old_logp", old_logp), ("ref_logp", ref_logp), ("entropy", entropy)):
-            _expect(name, t, torch.float32, T)
+        T = logp.shape[0]
+        _expect("old_logp", old_logp, torch.float32, T)
+        _expect("ref_logp", ref_logp, torch.float32, T)
+        _expect("entropy", entropy, torch.float32, T)
         _expect("offsets", offsets, torch.int32, None)
         _byte_mask(mask, T)
         n = offsets.shape[0] - 1
         if n < 1:
             raise LlmtError("offsets must be [n + 1] with n >= 1")
         _expect("advantages", advantages, torch.float32, n if per_sequence else T)
-        loss, stats = on.empty(1), on.empty(3)
-        dlogp = on.empty(T) if want_grad else None
-        dent = on.empty(T) if want_grad and entropy is not None else None
-        need = lib().llmt_policy_loss_workspace(T, n)
-        ws = on.empty(need, dtype=torch.uint8)
-        p = PolicyParams(MEANS[mean], int(per_sequence), clip_low, clip_high, kl_coef, entropy_coef)
-        check(lib().llmt_policy_loss(ptr(logp), ptr(old_logp), ptr(ref_logp), ptr(advantages),
-                                     ptr(entropy), ptr(mask), ptr(offsets), T, n, C.byref(p),
-                                     ptr(loss), ptr(stats), ptr(dlogp), ptr(dent), ptr(ws), need,
-                                     on.ptr))
+        L = lib()
+        need = L.llmt_policy_loss_workspace(T, n)
+        ws = logp.new_empty(need, dtype=torch.uint8) if need else None
+        loss, stats = logp.new_empty(4).split_with_sizes((1, 3))
+        dlogp = torch.empty_like(logp) if want_grad else None
+        dent = torch.empty_like(logp) if want_grad and entropy is not None else None
+        p = PolicyParams(kind, per_sequence, clip_low, clip_high, kl_coef, entropy_coef)
+        check(L.llmt_policy_loss(logp.data_ptr(), _at(old_logp), _at(ref_logp),
+                                 advantages.data_ptr(), _at(entropy), _at(mask), offsets.data_ptr(),
+                                 T, n, p, loss.data_ptr(), stats.data_ptr(), _at(dlogp), _at(dent),
+                                 _at(ws), need, on.raw))
     return PolicyLoss(loss, stats, dlogp, dent)
 
 
@@ -432,11 +448,11 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None, stream=None):
     cols] or a stack [count, rows, cols], fp32, the short side at most 64; rows
     may be strided.  out may be x itself."""
     import torch
-    with _On(stream, x=x, out=out) as on:
+    with _On("x out", (x, out), stream) as on:
         if x.dtype != torch.float32 or x.dim() not in (2, 3) or 0 in x.shape[-2:]:
             raise LlmtError("x must be float32 [rows, cols] or [count, rows, cols]")
         if out is None:
-            out = on.empty(*x.shape)
+            out = x.new_empty(x.shape)
         elif out.shape != x.shape or out.dtype != torch.float32:
             raise LlmtError("out must have x's shape and type")
         rows, cols = x.shape[-2:]
@@ -449,10 +465,11 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None, stream=None):
             return (t.stride(0) if count > 1 else rows * ld), ld
 
         (sx, ldx), (so, ldo) = strides("x", x), strides("out", out)
-        need = lib().llmt_orthogonalize_workspace(count, rows, cols)
-        ws = on.empty(need, dtype=torch.uint8)
-        check(lib().llmt_orthogonalize(ptr(x), sx, ldx, ptr(out), so, ldo, count, rows, cols,
-                                       steps, eps, ptr(ws), need, on.ptr))
+        L = lib()
+        need = L.llmt_orthogonalize_workspace(count, rows, cols)
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_orthogonalize(x.data_ptr(), sx, ldx, out.data_ptr(), so, ldo, count, rows,
+                                   cols, steps, eps, _at(ws), need, on.raw))
     return out
 
 
@@ -471,19 +488,22 @@ def muon_update(p, g, m, shapes, hp: MuonParams, stream=None):
     """One Muon step in place on flat fp32 arenas p and m from the gradients g:
     layers of the matrices `shapes` [(rows, cols), ..] one behind another."""
     import torch
-    with _On(stream, p=p, g=g, m=m) as on:
-        n = p.shape[0] if p.dim() == 1 else -1
-        for name, t in (("p", p), ("g", g), ("m", m)):
-            _expect(name, t, torch.float32, n if n >= 0 else None)
+    with _On("p g m", (p, g, m), stream) as on:
+        _expect("p", p, torch.float32, None)
+        n = p.shape[0]
+        _expect("g", g, torch.float32, n)
+        _expect("m", m, torch.float32, n)
         per = sum(r * c for r, c in shapes)
         if per < 1 or n < 1 or n % per:
             raise LlmtError(f"the arena's {n} elements are not whole layers of {per}")
         k = len(shapes)
-        rows, cols = (i32 * k)(*(s[0] for s in shapes)), (i32 * k)(*(s[1] for s in shapes))
-        need = lib().llmt_muon_update_workspace(n // per, k, rows, cols)
-        ws = on.empty(need, dtype=torch.uint8)
-        check(lib().llmt_muon_update(ptr(p), ptr(g), ptr(m), n // per, k, rows, cols, C.byref(hp),
-                                     ptr(ws), need, on.ptr))
+        rows, cols = zip(*shapes)
+        rows, cols = (i32 * k)(*rows), (i32 * k)(*cols)
+        L = lib()
+        need = L.llmt_muon_update_workspace(n // per, k, rows, cols)
+        ws = p.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_muon_update(p.data_ptr(), g.data_ptr(), m.data_ptr(), n // per, k, rows, cols,
+                                 hp, _at(ws), need, on.raw))
 
 
 # ------------------------------------------------------------------ training context
