@@ -311,7 +311,7 @@ int llmt_orthogonalize(const float* x, long long stride_x, long long ldx, float*
   a.steps = steps;
   a.eps = eps;
   const size_t need = ns_workspace(a);
-  TRY_ARG(workspace && workspace_bytes >= need && aligned(workspace, 16),
+  TRY_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
           "llmt_orthogonalize: workspace of %zu bytes, %zu needed (16-byte aligned)",
           workspace ? workspace_bytes : 0, need);
   return done(newton_schulz(a, workspace, (hipStream_t)stream));
@@ -337,7 +337,7 @@ int llmt_muon_update(float* p, const float* g, float* m, int layers, int nmat,
   TRY_ARG(apart(p, n, g, n) && apart(p, n, m, n) && apart(g, n, m, n),
           "llmt_muon_update: p, g and m overlap");
   const size_t need = ns_workspace(a);
-  TRY_ARG(workspace && workspace_bytes >= need && aligned(workspace, 16),
+  TRY_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
           "llmt_muon_update: workspace of %zu bytes, %zu needed (16-byte aligned)",
           workspace ? workspace_bytes : 0, need);
   a.x = g;
@@ -364,8 +364,9 @@ int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params) {
   if (rc) return rc;
   if ((rc = muon_params("llmt_muon", params, a))) return rc;
   TRY_ARG((size_t)a.in_stride == c->lora_per_layer, "llmt_muon: the arena's layout");
-  if (!c->muon_ws) {
-    c->muon_ws = c->alloc(ns_workspace(a));
+  const size_t need = ns_workspace(a);
+  if (need && !c->muon_ws) {
+    c->muon_ws = c->alloc(need);
     if (!c->muon_ws) return LLMT_ERR_HIP;
   }
   a.x = c->lora_g;

@@ -92,7 +92,8 @@ def test_policy_refusals(bad):
     assert llmt.lib().llmt_last_error().decode().startswith("llmt_policy_loss:")
 
 
-def ortho(x=A(1), sx=800, ldx=100, out=A(2), so=800, ldo=100, count=2, rows=8, cols=100, steps=5,
+# short sides above 16: these take a workspace
+def ortho(x=A(1), sx=2000, ldx=100, out=A(2), so=2000, ldo=100, count=2, rows=20, cols=100, steps=5,
           eps=1e-7, ws=A(8), need=1 << 20):
     return llmt.lib().llmt_orthogonalize(x, sx, ldx, out, so, ldo, count, rows, cols, steps, eps, ws,
                                          need, None)
@@ -100,18 +101,18 @@ def ortho(x=A(1), sx=800, ldx=100, out=A(2), so=800, ldo=100, count=2, rows=8, c
 
 @pytest.mark.parametrize("bad", [
     dict(count=-1), dict(count=2 ** 21), dict(rows=0), dict(cols=0, ldx=0, ldo=0),
-    dict(rows=65, sx=6500, so=6500), dict(ldx=99), dict(ldo=99), dict(sx=799), dict(so=799),
+    dict(rows=65, sx=6500, so=6500), dict(ldx=99), dict(ldo=99), dict(sx=1999), dict(so=1999),
     dict(steps=0), dict(steps=21), dict(eps=0.0), dict(eps=math.nan), dict(x=None), dict(out=None),
     dict(x=C.c_void_p(0x100002)), dict(ws=None), dict(need=100), dict(ws=C.c_void_p(0x800004)),
-    dict(out=A(1), so=801), dict(out=A(1), ldo=101, so=900), dict(out=C.c_void_p(0x100004)),
-    dict(out=C.c_void_p(0x100000 + 4 * 1599)), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldo=2 ** 31,
+    dict(out=A(1), so=2001), dict(out=A(1), ldo=101, so=2100), dict(out=C.c_void_p(0x100004)),
+    dict(out=C.c_void_p(0x100000 + 4 * 3999)), dict(cols=2 ** 30 + 1, ldx=2 ** 31, ldo=2 ** 31,
                                                     sx=2 ** 36, so=2 ** 36)])
 def test_orthogonalize_refusals(bad):
     assert ortho(**bad) == ARG
     assert llmt.lib().llmt_last_error().decode().startswith("llmt_orthogonalize:")
 
 
-def muon(p=A(1), g=A(2), m=A(3), layers=2, shapes=((8, 100), (50, 8)), nmat=None,
+def muon(p=A(1), g=A(2), m=A(3), layers=2, shapes=((8, 100), (50, 20)), nmat=None,
          params=(0.01, 0.9, 0.0, 1e-7, 5, 1, 0), ws=A(8), need=1 << 20):
     k = len(shapes)
     rows, cols = (C.c_int * k)(*(s[0] for s in shapes)), (C.c_int * k)(*(s[1] for s in shapes))
@@ -127,7 +128,7 @@ def muon(p=A(1), g=A(2), m=A(3), layers=2, shapes=((8, 100), (50, 8)), nmat=None
     dict(params=(0.01, -0.1, 0.0, 1e-7, 5, 1, 0)), dict(params=(0.01, 0.9, math.inf, 1e-7, 5, 1, 0)),
     dict(params=(0.01, 0.9, 0.0, 0.0, 5, 1, 0)), dict(params=(0.01, 0.9, 0.0, 1e-7, 0, 1, 0)),
     dict(params=(0.01, 0.9, 0.0, 1e-7, 5, 1, 2)), dict(g=A(1)), dict(m=C.c_void_p(0x200004)),
-    dict(p=C.c_void_p(0x300000 - 4 * 2399)), dict(ws=None), dict(need=64),
+    dict(p=C.c_void_p(0x300000 - 4 * 3599)), dict(ws=None), dict(need=64),
     dict(m=C.c_void_p(0x300002))])
 def test_muon_refusals(bad):
     assert muon(**bad) == ARG
@@ -144,7 +145,7 @@ def test_workspace_sizes():
     assert L.llmt_policy_loss_workspace(2 ** 31 - 1, 2 ** 29) < 2 ** 33
     assert L.llmt_token_logprobs_workspace(0, 100, 0) == 0
     assert L.llmt_orthogonalize_workspace(1, 65, 65) == 0 and L.llmt_orthogonalize_workspace(0, 4, 4) == 0
-    assert L.llmt_orthogonalize_workspace(1, 16, 2048) > 0
+    assert L.llmt_orthogonalize_workspace(1, 17, 2048) > 0
     assert L.llmt_muon_update_workspace(1, 9, None, None) == 0
 
 
