@@ -81,8 +81,9 @@ struct Stage {
 
 // A lane's pieces of a stage: piece i's place in LDS (its first element, and
 // `step` to the next), its offset from the stage's first element in memory,
-// and where the matrix ends.  A stage that is whole (all of KW, the short side
-// all of 16 NT) takes plain 16-byte accesses; the others ask for every piece.
+// and where the matrix ends.  A stage of all KW elements takes plain 16-byte
+// accesses where the short side is all of 16 NT, 16-byte ones or none where it
+// is whole pieces; the others count elements.
 template <int NT>
 struct Lane {
   static constexpr int PC = Stage<NT>::PC, LD = Stage<NT>::LD, KW = Stage<NT>::KW;
@@ -105,30 +106,32 @@ struct Lane {
   __device__ __forceinline__ int lds(int i) const { return kk(i) * LD + sh(i); }
   // Offset of the stage at k from the matrix's start.
   __device__ __forceinline__ long long base(int k) const { return tall ? k * ld : k; }
-  __device__ __forceinline__ bool whole(int k, int k1) const { return k + KW <= k1 && r == 16 * NT; }
   // Elements of piece i of the stage at k.
   __device__ __forceinline__ int have(int i, int k, int k1) const {
     return tall ? (k + kk(i) < k1 ? r - sh(i) : 0) : (sh(i) < r ? k1 - (k + kk(i)) : 0);
   }
-  __device__ __forceinline__ void load(floatx4 (&x)[PC], const float* p, int k, int k1) const {
-    p += base(k);
-    if (whole(k, k1)) {
+  // f(i, elements) for every piece of the stage at k.
+  template <typename F>
+  __device__ __forceinline__ void pieces(int k, int k1, F&& f) const {
+    const bool all = k + KW <= k1;
+    if (all && r == 16 * NT) {
 #pragma unroll
-      for (int i = 0; i < PC; ++i) x[i] = load4(p + at(i), 4);
+      for (int i = 0; i < PC; ++i) f(i, 4);
+    } else if (all && r % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < PC; ++i) f(i, sh(i) < r ? 4 : 0);
     } else {
 #pragma unroll
-      for (int i = 0; i < PC; ++i) x[i] = load4(p + at(i), have(i, k, k1));
+      for (int i = 0; i < PC; ++i) f(i, have(i, k, k1));
     }
+  }
+  __device__ __forceinline__ void load(floatx4 (&x)[PC], const float* p, int k, int k1) const {
+    p += base(k);
+    pieces(k, k1, [&](int i, int n) { x[i] = load4(p + at(i), n); });
   }
   __device__ __forceinline__ void store(float* p, const floatx4 (&x)[PC], int k, int k1) const {
     p += base(k);
-    if (whole(k, k1)) {
-#pragma unroll
-      for (int i = 0; i < PC; ++i) store4(p + at(i), x[i], 4);
-    } else {
-#pragma unroll
-      for (int i = 0; i < PC; ++i) store4(p + at(i), x[i], have(i, k, k1));
-    }
+    pieces(k, k1, [&](int i, int n) { store4(p + at(i), x[i], n); });
   }
   __device__ __forceinline__ void put(float (*S)[LD], const floatx4 (&x)[PC]) const {
 #pragma unroll
@@ -428,7 +431,7 @@ __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a)
 // itself (2 us, during which its first loads arrive), which is less than the
 // launch that it saves.
 template <int NT, bool MUON>
-__global__ __launch_bounds__(NTH) void ns_apply_kernel(const NsArgs a) {
+__global__ __launch_bounds__(NTH, 2) void ns_apply_kernel(const NsArgs a) {
   constexpr int KW = Stage<NT>::KW, LD = Stage<NT>::LD, PC = Stage<NT>::PC;
   __shared__ float S_[NW][KW][LD];
   const int mat = blockIdx.x / a.splits, split = blockIdx.x - mat * a.splits;
