@@ -238,12 +238,13 @@ class _On:
         for t in tensors:
             if t is not None:
                 at = t.get_device() if isinstance(t, torch.Tensor) else -1
-                if at < 0 or (index >= 0 and at != index):
-                    name = names.split()[[t is u for u in tensors].index(True)]
-                    raise LlmtError(f"{name} must be a device tensor" if at < 0 else
-                                    f"{name} is on device {at}, other tensors on {index}")
-                index = at
-        self.stream, self.ctx = stream, None
+                if at != index or at < 0:
+                    if index >= 0 or at < 0:
+                        name = names.split()[[t is u for u in tensors].index(True)]
+                        raise LlmtError(f"{name} must be a device tensor" if at < 0 else
+                                        f"{name} is on device {at}, other tensors on {index}")
+                    index = at
+        self.stream = stream
         if stream is not None:
             if stream.device_index != index:
                 raise LlmtError(f"the stream is on {stream.device}, the tensors on device {index}")
@@ -251,8 +252,7 @@ class _On:
             self.ctx = torch.cuda.stream(stream)
             self.raw = stream.cuda_stream
         else:
-            if torch._C._cuda_getDevice() != index:
-                self.ctx = torch.cuda.device(index)
+            self.ctx = None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
             self.raw = torch._C._cuda_getCurrentRawStream(index)
 
     def __enter__(self):
@@ -278,16 +278,15 @@ def _at(t):
 
 
 def _expect(name, t, dtype, *shape):
-    """t is a contiguous tensor of this type and shape (None: any length)."""
-    if t is None:
+    """t, where given, is a contiguous tensor of this type and shape (None: any length)."""
+    if t is None or (t.dtype is dtype and t.is_contiguous() and
+                     (t.shape == shape or (shape == (None,) and t.dim() == 1))):
         return
     if t.dtype != dtype:
         raise LlmtError(f"{name} must be {dtype} (got {t.dtype})")
-    if t.shape != shape and (t.dim() != len(shape) or
-                             any(n is not None and n != m for n, m in zip(shape, t.shape))):
-        raise LlmtError(f"{name} must be {list(shape)} (got {list(t.shape)})")
     if not t.is_contiguous():
         raise LlmtError(f"{name} must be contiguous")
+    raise LlmtError(f"{name} must be {list(shape)} (got {list(t.shape)})")
 
 
 def _logits_dtype(name, t):
@@ -308,9 +307,8 @@ def _ld(t):
 
 def _byte_mask(mask, T):
     import torch
-    if mask is not None and mask.dtype not in (torch.bool, torch.uint8):
-        raise LlmtError(f"mask must be bool or uint8 (got {mask.dtype})")
-    _expect("mask", mask, None if mask is None else mask.dtype, T)
+    if mask is not None:
+        _expect("mask", mask, torch.uint8 if mask.dtype is torch.uint8 else torch.bool, T)
 
 
 def token_logprobs(logits, targets, temperature=1.0, want_entropy=False, stream=None):
@@ -430,7 +428,7 @@ def policy_loss(logp, old_logp, advantages, offsets, ref_logp=None, entropy=None
         L = lib()
         need = L.llmt_policy_loss_workspace(T, n)
         ws = logp.new_empty(need, dtype=torch.uint8) if need else None
-        loss, stats = logp.new_empty(4).split_with_sizes((1, 3))
+        loss, stats = logp.new_empty(1), logp.new_empty(3)
         dlogp = torch.empty_like(logp) if want_grad else None
         dent = torch.empty_like(logp) if want_grad and entropy is not None else None
         p = PolicyParams(kind, per_sequence, clip_low, clip_high, kl_coef, entropy_coef)

@@ -71,7 +71,8 @@ def test_preference_refusals(bad):
     assert llmt.lib().llmt_last_error().decode().startswith("llmt_preference_loss:")
 
 
-def policy(logp=A(1), old=A(2), ref=None, adv=A(3), ent=None, mask=None, off=A(4), T=10, n=2,
+# enough tokens for a workspace
+def policy(logp=A(1), old=A(2), ref=None, adv=A(3), ent=None, mask=None, off=A(4), T=50000, n=2,
            params=(0, 0, 0.2, 0.2, 0.0, 0.0), loss=A(5), stats=A(6), d=A(7), de=None, ws=A(8),
            need=1 << 20):
     p = None if params is None else C.byref(llmt.PolicyParams(*params))
