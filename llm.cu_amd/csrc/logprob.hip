@@ -49,15 +49,18 @@ struct Piece<__bf16> {
 
 // The statistics are kept in base 2: with y = logits * c, c = it log2 e,
 // (m, s, u) are the largest y, sum 2^(y - m) and sum 2^(y - m) (y - m), each
-// y - m one fma.  16-bit logits are bound by the VALU as much as by HBM, and
-// this is the fewest instructions an element.  The rounding of m is a common
-// offset, taken out once a row (finish).  The empty set is (-inf, 0, 0).
+// y - m one fma; x is the largest logit itself.  16-bit logits are bound by the VALU as much as by HBM, and
+// this is the fewest instructions an element.  The roundings of m and c are
+// common to a row's terms; finish takes them out of its m, and the rounding of
+// c leaves 2^-24 of each y - m.  The empty set is (-inf, 0, 0), -inf.
 struct Stat {
-  float m, s, u;
+  float m, s, u, x;
 };
+__device__ __forceinline__ Stat empty_stat() { return {-INFINITY, 0.f, 0.f, -INFINITY}; }
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
 template <bool ENT>
-__device__ __forceinline__ void merge(Stat& a, float m2, float s2, float u2) {
+__device__ __forceinline__ void merge(Stat& a, const Stat& b) {
+  const float m2 = b.m, s2 = b.s, u2 = b.u;
   const float mn = fmaxf(a.m, m2), ref = finite_ref(mn);
   const float d1 = a.m - ref, d2 = m2 - ref;
   const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
@@ -69,6 +72,7 @@ __device__ __forceinline__ void merge(Stat& a, float m2, float s2, float u2) {
   }
   a.s = a.s * f1 + s2 * f2;
   a.m = mn;
+  a.x = fmaxf(a.x, b.x);
 }
 
 // Adds NV logits to a thread's statistics: one rescale.
@@ -90,15 +94,16 @@ __device__ __forceinline__ void add(Stat& a, const float (&x)[NV], float c) {
   if constexpr (ENT) a.u = fmaf(f, fmaf(a.s, fmaxf(d, kFar), a.u), u);
   a.s = fmaf(a.s, f, s);
   a.m = m;
+  a.x = fmaxf(a.x, mx);
 }
 
 template <bool ENT>
 __device__ __forceinline__ Stat wave_merge(Stat a) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(a.m, o, 64), s2 = __shfl_xor(a.s, o, 64);
-    const float u2 = ENT ? __shfl_xor(a.u, o, 64) : 0.f;
-    merge<ENT>(a, m2, s2, u2);
+    const Stat b = {__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64),
+                    ENT ? __shfl_xor(a.u, o, 64) : 0.f, __shfl_xor(a.x, o, 64)};
+    merge<ENT>(a, b);
   }
   return a;
 }
@@ -145,8 +150,9 @@ __device__ __forceinline__ void finish(const Stat& a, float xt, float it, long l
     if constexpr (ENT) entropy[row] = 0.f;
     return;
   }
-  const double mn = (double)a.m * 0.6931471805599453;
-  const float m = (float)mn, ls = logf(a.s), l = ls + (float)(mn - m);
+  // the offset m of the sums in natural units, by the c that they took
+  const double mn = (double)a.m * ((double)it / (double)(it * kLog2e));
+  const float m = a.x * it, ls = logf(a.s), l = ls + (float)(mn - m);
   logp[row] = fmaf(xt, it, -m) - l;
   stats[row] = make_float2(m, l);
   if constexpr (ENT) entropy[row] = fmaf(-0.69314718f, a.u / a.s, ls);
@@ -168,7 +174,7 @@ __device__ __forceinline__ Stat block_merge(Stat a, Stat* part) {
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
   __syncthreads();
   if (threadIdx.x == 0)
-    for (int w = 1; w < NTH / 64; ++w) merge<ENT>(a, part[w].m, part[w].s, part[w].u);
+    for (int w = 1; w < NTH / 64; ++w) merge<ENT>(a, part[w]);
   return a;
 }
 
@@ -188,7 +194,7 @@ __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ 
       continue;
     }
     const T* x = logits + row * ld;
-    Stat a{-INFINITY, 0.f, 0.f};
+    Stat a = empty_stat();
     scan<ENT>(a, x, 0, V, threadIdx.x, NTH, it * kLog2e);
     a = block_merge<ENT>(a, part);
     if (threadIdx.x == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
@@ -213,7 +219,7 @@ __global__ __launch_bounds__(NTH) void logprob_wave_kernel(const T* __restrict__
       continue;
     }
     const T* x = logits + row * ld;
-    Stat a{-INFINITY, 0.f, 0.f};
+    Stat a = empty_stat();
     scan<ENT>(a, x, 0, V, lane, 64, it * kLog2e);
     a = wave_merge<ENT>(a);
     if (lane == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
@@ -233,10 +239,10 @@ __global__ __launch_bounds__(NTH) void logprob_part_kernel(const T* __restrict__
   const int t = targets[row];
   if (t < 0 || t >= V) return;
   const int j0 = (int)min((long long)ch * width, (long long)V), j1 = min(V - j0, width) + j0;
-  Stat a{-INFINITY, 0.f, 0.f};
+  Stat a = empty_stat();
   scan<ENT>(a, logits + row * ld, j0, j1, threadIdx.x, NTH, it * kLog2e);
   a = block_merge<ENT>(a, part);
-  if (threadIdx.x == 0) parts[blockIdx.x] = make_float4(a.m, a.s, a.u, 0.f);
+  if (threadIdx.x == 0) parts[blockIdx.x] = make_float4(a.m, a.s, a.u, a.x);
 }
 
 template <bool ENT, typename T>
@@ -254,10 +260,10 @@ __global__ __launch_bounds__(64) void logprob_merge_kernel(const T* __restrict__
     return;
   }
   const float xt = (float)logits[row * ld + t];
-  Stat a{-INFINITY, 0.f, 0.f};
+  Stat a = empty_stat();
   for (int c = threadIdx.x; c < chunks; c += 64) {
     const float4 p = parts[(long long)row * chunks + c];
-    merge<ENT>(a, p.x, p.y, p.z);
+    merge<ENT>(a, Stat{p.x, p.y, p.z, p.w});
   }
   a = wave_merge<ENT>(a);
   if (threadIdx.x == 0) finish<ENT>(a, xt, it, row, logp, stats, entropy);

@@ -508,10 +508,14 @@ __global__ __launch_bounds__(NTH) void policy_final_kernel(const PolicyArgs a, i
 
 // Workgroups whose partial sums the final kernel adds: tiles of the tokens, or
 // groups of sequences.
-constexpr int kSeqWg = 2048;     // eight workgroups a CU
-constexpr int kShortSeq = 512;   // tokens a sequence on average up to which a wave takes it
+constexpr int kSeqWg = 2048;  // eight workgroups a CU
 bool one_workgroup(int T, int n) { return T <= kOneTokens && n <= kOneSeqs; }
-bool wave_a_sequence(int T, int n) { return T / n <= kShortSeq; }
+// A wave takes a sequence where it is one step of it (256 tokens on average:
+// 2000 x 65 8.3 us, 17 with a workgroup each), or two and the sequences are
+// more than the workgroups that the registers let run at once (2000 x 260:
+// 11.2 and 17.9; 500 x 260: 9.5 and 8.5).
+constexpr int kSeqResident = 768;
+bool wave_a_sequence(int T, int n) { return T / n <= (n > kSeqResident ? 512 : 256); }
 int policy_grid(int T, int n, int seq_mean) {
   if (!seq_mean) return (int)(((long long)T + kTile - 1) / kTile);
   const int per = wave_a_sequence(T, n) ? NTH / 64 : 1;
@@ -521,26 +525,29 @@ size_t counts_bytes() { return kCountWg * sizeof(int); }
 
 }  // namespace
 
+// Few and short pairs: one workgroup, a wave a pair, no second launch, which
+// costs the caller 3 us (8 x 26 tokens 5.7 us, 6.3 in two; 16 x 390: 9.0 and
+// 6.4; 16 x 1040 would be 12.9 and 7.3).  Else a workgroup a pair while all can
+// run at once (500 x 390: 6.9 us, 8.0 with a wave each), a wave a pair beyond
+// (2048 x 390: 9.3, 12.0 with a workgroup each; 2048 x 910: 12.2 and 14.1), and
+// twice the threads for long ones (100 x 2600: 7.8 and 9.2).
 hipError_t preference_loss(const PrefArgs& a, hipStream_t st) {
-  const int mean_len = a.T / a.n;  // tokens a pair
-  auto go = [&](auto waves, auto block, unsigned grid) {
+  constexpr int kResident = 1024;
+  const int len = a.T / a.n;  // tokens a pair on average
+  auto go = [&](auto waves, auto block, int wgs) {
     constexpr int W = decltype(waves)::value, B = decltype(block)::value;
+    const int grid = std::min(wgs, 1 << 16);
     hipLaunchKernelGGL((pref_kernel<W, B>), dim3(grid), dim3(B), 0, st, a);
+    return grid;
   };
   using std::integral_constant;
-  unsigned grid = 1;
-  if (a.n <= 64 && mean_len <= 1024) {
-    go(integral_constant<int, 1>(), integral_constant<int, 1024>(), 1);
-  } else if (mean_len <= 512) {
-    grid = (unsigned)std::min((a.n + 3) / 4, 1 << 16);
-    go(integral_constant<int, 1>(), integral_constant<int, 256>(), grid);
-  } else if (mean_len <= 4096) {
-    grid = (unsigned)std::min(a.n, 1 << 16);
-    go(integral_constant<int, 4>(), integral_constant<int, 256>(), grid);
-  } else {
-    grid = (unsigned)std::min(a.n, 1 << 16);
-    go(integral_constant<int, 8>(), integral_constant<int, 512>(), grid);
-  }
+  const int grid = a.n <= 16 && len <= 512
+                       ? go(integral_constant<int, 1>(), integral_constant<int, 1024>(), 1)
+                   : a.n > kResident && len <= 1024
+                       ? go(integral_constant<int, 1>(), integral_constant<int, 256>(), (a.n + 3) / 4)
+                   : len <= 2048
+                       ? go(integral_constant<int, 4>(), integral_constant<int, 256>(), a.n)
+                       : go(integral_constant<int, 8>(), integral_constant<int, 512>(), a.n);
   LLMT_LAUNCH_CHECK();
   if (grid > 1) {
     hipLaunchKernelGGL(pref_mean_kernel, dim3(1), dim3(kMeanThreads), 0, st, a.losses, a.n, a.mean);
