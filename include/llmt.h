@@ -406,6 +406,18 @@ int llmt_token_logprobs_bwd(const void* logits, int dtype, long long ld, const i
                             const float* dentropy, int rows, int V, float inv_temp, void* dlogits,
                             long long ldd, void* stream);
 
+/* The same through a context's model: a forward that gives the log-probability
+ * of every target, logp [batch * seq_len] (0 where the target is outside
+ * [0, V): prompts, padding, the last position of a window), and the backward
+ * of any function of them from dlogp, its gradient: the adapter gradients go
+ * to the GRAD arena (overwritten), for llmt_adamw or llmt_muon.  The backward
+ * takes the stashes of the last forward and fails with LLMT_ERR_STATE if that
+ * was not llmt_forward_logprobs'; it may be called more than once.  tokens,
+ * targets, batch as in llmt_step; one host synchronisation each. */
+int llmt_forward_logprobs(llmt_ctx* ctx, const int* tokens, const int* targets, int batch,
+                          float* logp);
+int llmt_backward_logprobs(llmt_ctx* ctx, const float* dlogp);
+
 /* Preference loss on n pairs of sequences.  Sequence s is tokens offsets[s] ..
  * offsets[s + 1] - 1 of the T (offsets int32 [2 n + 1], ascending); pair i
  * prefers sequence 2 i to sequence 2 i + 1.  logp, and ref_logp of the frozen

@@ -156,7 +156,7 @@ int llmt_layer_forward(llmt_ctx* ctx, int layer, const float* x, float* y, int b
   const int T = batch * c->S;
   Stash& s = c->stash[layer];
   Layer& w = c->layers[layer];
-  c->pad_batch = 0;  // rows a later step may pad are written here
+  c->pad_batch = c->logp_batch = 0;  // rows a later step may pad are written here
   TRY_HIP(copy_norm(x, w.attn_norm, c->dims.eps, c->H, T, s.x_in, s.xn, c->st));
   TRY_HIP(c->layer_fwd(layer, batch, w.attn_norm, y, c->xf16));
   TRY_HIP(hipStreamSynchronize(c->st));
@@ -169,7 +169,7 @@ int llmt_layer_backward(llmt_ctx* ctx, int layer, const float* dy, float* dx, in
   TRY_ARG(c && dy && dx && layer >= 0 && layer < c->L, "llmt_layer_backward: bad arguments");
   TRY_ARG(batch >= 1 && batch <= c->maxB && (batch * c->S) % 16 == 0, "batch");
   const int T = batch * c->S;
-  c->pad_batch = 0;
+  c->pad_batch = c->logp_batch = 0;
   // g16 feeds the layer's down dX, which takes int8 weights' scale from it
   TRY_HIP(grad_rows(dy, c->H, T, c->d_res, c->g16, c->rinv, c->layers[layer].wdT.kscale, c->st));
   TRY_HIP(c->layer_bwd(layer, batch));
@@ -244,7 +244,7 @@ int llmt_head_ce(llmt_ctx* ctx, const void* hidden16, const int* targets, int ba
   TRY_ARG(c->embed_ready, "embedding not set");
   TRY_ARG(batch >= 1 && batch <= c->maxB && (batch * c->S) % 16 == 0, "batch");
   const int T = batch * c->S;
-  c->pad_batch = 0;
+  c->pad_batch = c->logp_batch = 0;
   int rc = head_ce_packed(c->st, (const _Float16*)hidden16, c->Eh, c->EhT, targets, T, c->S, c->H,
                           c->V, c->logits, c->grad16, c->ce_stats, c->lse_rows, c->loss_rows,
                           c->loss_dev, dlogits, dhidden, c->part, c->part_elems);

@@ -141,6 +141,8 @@ struct Ctx {
   _Float16* grad16 = nullptr;
   float2* ce_stats = nullptr;  // [Tmax, ce_stats_per_row(V)]: CE chunk or logits-tile pairs
   float* lse_rows = nullptr;   // [Tmax]
+  float2* logp_stats = nullptr;  // [Tmax]: llmt_forward_logprobs' softmax statistics
+  int logp_batch = 0;            // > 0: the stashes are that call's, of this batch
   int head_tiles = 0;          // > 0: the last forward's logits GEMM wrote its tile pairs
   float* loss_rows = nullptr;
   float* loss_dev = nullptr;
@@ -241,9 +243,10 @@ struct Ctx {
   hipError_t forward(const int* tok, int B, float* logits_out);
   // Fused CE over lg (NULL: the context's logits): loss, grad16, optional fp32 dlogits.
   hipError_t ce(const float* lg, const int* tgt, int B, float* dlogits_out);
-  hipError_t head_bwd(int B);
+  // row_factor: per-row factors of grad16 (NULL: the mean cross entropy's).
+  hipError_t head_bwd(int B, const float* row_factor = nullptr);
   hipError_t layer_bwd(int l, int B);
-  hipError_t backward(int B, int accumulate);
+  hipError_t backward(int B, int accumulate, const float* row_factor = nullptr);
   hipError_t optimizer();
   hipError_t refresh_shadows();
   // tok / tgt: device token and target ids read in place (default: tok_buf, tgt_buf)

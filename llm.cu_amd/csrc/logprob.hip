@@ -279,12 +279,18 @@ constexpr int kBwdPieces = sizeof(T) == 4 ? 1 : 2;
 // against 13.4 us).  NT: gradients beyond the 256 MB last-level cache are
 // stored nontemporal (1000 x 151936 fp32: 194 us, 201 without), smaller ones
 // stay there for the next kernel.
-template <bool ENT, bool NT, typename T>
+// TO: the type written.  With `factor` the rows are written for dlogp = -1
+// times kGradLogitScale (the lm_head dX GEMM's operand) and factor[row] gets
+// what they lack of the gradient, -dlogp; rows from `rows` to `factor_rows`
+// get a factor of 0.
+template <bool ENT, bool NT, typename T, typename TO = T>
 __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const T* logits, long long ld, const int* __restrict__ targets,
     const float2* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ dlogp, const float* __restrict__ dentropy, int rows, int V, float it,
-    int chunks, T* dlogits, long long ldd) {
+    int chunks, TO* dlogits, long long ldd, float* __restrict__ factor, int factor_rows) {
+  typedef typename Piece<T>::V Vec;
+  typedef TO VecO __attribute__((ext_vector_type(Piece<T>::N), aligned(sizeof(TO))));
   constexpr int N = Piece<T>::N, BU = kBwdPieces<T>, WAVES = NTH / 64;
   const long long items = (long long)rows * chunks;
   const int lane = threadIdx.x & 63;
@@ -293,7 +299,12 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
        w += (long long)gridDim.x * WAVES) {
     const int row = (int)(w / chunks), ch = (int)(w - (long long)row * chunks);
     const int t = targets[row];
-    const float g = dlogp[row] * it, h = ENT ? dentropy[row] * it : 0.f;
+    float g = dlogp[row] * it;
+    if (factor) {
+      if (ch == 0 && lane == 0) factor[row] = t < 0 || t >= V ? 0.f : -g;
+      g = g == 0.f ? 0.f : -kGradLogitScale;
+    }
+    const float h = ENT ? dentropy[row] * it : 0.f;
     const float2 st = stats[row];
     const bool zero = t < 0 || t >= V || (g == 0.f && h == 0.f) ||
                       (st.x == -INFINITY && st.y == 0.f);
@@ -301,7 +312,7 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const long long start = (long long)ch * (BU * N * 64);
     const int j0 = (int)start, j1 = (int)min((long long)V, start + BU * N * 64);
     const T* x = logits + row * ld;
-    T* d = dlogits + row * ldd;
+    TO* d = dlogits + row * ldd;
     auto log_p = [&](float xv) {
       const float z = fmaf(xv, it, -st.x) - st.y;
       // exp is 0 far below, and 0 * z has to stay 0
@@ -316,32 +327,35 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
       return ENT ? fmaf(-h * p, z + entropy[row], dg) : dg;
     };
     const int np = (j1 - j0) / N;
-    typename Piece<T>::V v[BU];
+    Vec v[BU];
     if (!zero)
 #pragma unroll
       for (int u = 0; u < BU; ++u)
         if (lane + u * 64 < np)
-          v[u] = *reinterpret_cast<const typename Piece<T>::V*>(x + j0 + N * (lane + u * 64));
+          v[u] = *reinterpret_cast<const Vec*>(x + j0 + N * (lane + u * 64));
 #pragma unroll
     for (int u = 0; u < BU; ++u) {
       const int k = lane + u * 64;
       if (k < np) {
         const int j = j0 + N * k;
-        typename Piece<T>::V o;
+        VecO o;
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = zero ? (T)0.f : (T)value((float)v[u][e]);
+        for (int e = 0; e < N; ++e) o[e] = zero ? (TO)0.f : (TO)value((float)v[u][e]);
         if (!zero && (unsigned)(t - j) < (unsigned)N)
 #pragma unroll
           for (int e = 0; e < N; ++e)
-            if (t == j + e) o[e] = (T)at_target((float)v[u][e]);
-        auto* to = reinterpret_cast<typename Piece<T>::V*>(d + j);
+            if (t == j + e) o[e] = (TO)at_target((float)v[u][e]);
+        auto* to = reinterpret_cast<VecO*>(d + j);
         if constexpr (NT) __builtin_nontemporal_store(o, to);
         else *to = o;
       }
     }
     const int j = j0 + N * np + lane;
-    if (j < j1) d[j] = zero ? (T)0.f : (T)(j == t ? at_target((float)x[j]) : value((float)x[j]));
+    if (j < j1) d[j] = zero ? (TO)0.f : (TO)(j == t ? at_target((float)x[j]) : value((float)x[j]));
   }
+  if (factor)
+    for (int r = rows + blockIdx.x * NTH + threadIdx.x; r < factor_rows; r += gridDim.x * NTH)
+      factor[r] = 0.f;
 }
 
 }  // namespace
@@ -419,7 +433,8 @@ static hipError_t launch_bwd(const LogprobArgs& a, hipStream_t st) {
   const long long wgs = ((long long)a.rows * chunks + NTH / 64 - 1) / (NTH / 64);
   hipLaunchKernelGGL((logprob_bwd_kernel<ENT, NT, T>), dim3(std::min(wgs, 1ll << 22)), dim3(NTH), 0,
                      st, (const T*)a.logits, a.ld, a.targets, (const float2*)a.stats, a.entropy,
-                     a.dlogp, a.dentropy, a.rows, a.V, a.it, chunks, (T*)a.dlogits, a.ldd);
+                     a.dlogp, a.dentropy, a.rows, a.V, a.it, chunks, (T*)a.dlogits, a.ldd,
+                     (float*)nullptr, 0);
   LLMT_LAUNCH_CHECK();
   return hipSuccess;
 }
@@ -431,6 +446,64 @@ hipError_t logprob_bwd(const LogprobArgs& a, hipStream_t st) {
       return a.dentropy ? launch_bwd<true, true, T>(a, st) : launch_bwd<false, true, T>(a, st);
     return a.dentropy ? launch_bwd<true, false, T>(a, st) : launch_bwd<false, false, T>(a, st);
   });
+}
+
+// ------------------------------------------------------------------ in a context
+
+namespace {
+// A wave a row: the (max, sum exp(x - max)) pairs of the logits GEMM's column
+// tiles, in a fixed order, into the row's statistics.
+__global__ __launch_bounds__(64) void logprob_pairs_kernel(const float2* __restrict__ pairs,
+                                                           int ntiles,
+                                                           const float* __restrict__ logits,
+                                                           const int* __restrict__ targets, int V,
+                                                           float* __restrict__ logp,
+                                                           float2* __restrict__ stats) {
+  const int row = blockIdx.x, t = targets[row];
+  if (t < 0 || t >= V) {
+    if (threadIdx.x == 0) no_target<false>(row, logp, stats, nullptr);
+    return;
+  }
+  const float xt = logits[(long long)row * V + t];
+  float m = -INFINITY, s = 0.f;
+  for (int i = threadIdx.x; i < ntiles; i += 64) {
+    const float2 p = pairs[(long long)row * ntiles + i];
+    softmax_merge(m, s, p.x, p.y);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+    softmax_merge(m, s, m2, s2);
+  }
+  if (threadIdx.x == 0) {
+    const float l = logf(s);
+    logp[row] = (xt - m) - l;
+    stats[row] = make_float2(m, l);
+  }
+}
+}  // namespace
+
+hipError_t logprob_from_pairs(const float2* pairs, int ntiles, const float* logits,
+                              const int* targets, int rows, int V, float* logp, float2* stats,
+                              hipStream_t st) {
+  hipLaunchKernelGGL(logprob_pairs_kernel, dim3(rows), dim3(64), 0, st, pairs, ntiles, logits,
+                     targets, V, logp, stats);
+  LLMT_LAUNCH_CHECK();
+  return hipSuccess;
+}
+
+hipError_t logprob_grad16(const float* logits, const int* targets, const float2* stats,
+                          const float* dlogp, int rows, int V, _Float16* grad16, float* factor,
+                          int factor_rows, hipStream_t st) {
+  constexpr int per = kBwdPieces<float> * Piece<float>::N * 64;
+  const int chunks = (V + per - 1) / per;
+  const long long wgs = ((long long)rows * chunks + NTH / 64 - 1) / (NTH / 64);
+  hipLaunchKernelGGL((logprob_bwd_kernel<false, false, float, _Float16>),
+                     dim3(std::min(wgs, 1ll << 22)), dim3(NTH), 0, st, logits, (long long)V,
+                     targets, stats, (const float*)nullptr, dlogp, (const float*)nullptr, rows, V,
+                     1.0f, chunks, grad16, (long long)V, factor, factor_rows);
+  LLMT_LAUNCH_CHECK();
+  return hipSuccess;
 }
 
 }  // namespace llmt

@@ -392,6 +392,17 @@ size_t logprob_workspace(int rows, int V, int dtype);
 hipError_t logprob_fwd(const LogprobArgs& a, void* workspace, hipStream_t st);
 hipError_t logprob_bwd(const LogprobArgs& a, hipStream_t st);
 
+// The same in a training context: logp and stats from the softmax pairs of
+// the logits GEMM's column tiles, and the lm_head dX GEMM's fp16 operand
+// grad16 = (p - onehot) * kGradLogitScale with the row factors -dlogp that it
+// lacks (0 for rows without a target and for rows .. factor_rows - 1).
+hipError_t logprob_from_pairs(const float2* pairs, int ntiles, const float* logits,
+                              const int* targets, int rows, int V, float* logp, float2* stats,
+                              hipStream_t st);
+hipError_t logprob_grad16(const float* logits, const int* targets, const float2* stats,
+                          const float* dlogp, int rows, int V, _Float16* grad16, float* factor,
+                          int factor_rows, hipStream_t st);
+
 struct PrefArgs {
   const float* logp;
   const float* ref;            // NULL: no reference

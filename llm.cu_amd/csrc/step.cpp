@@ -288,6 +288,7 @@ hipError_t Ctx::layer_fwd(int l, int B, const float* next_w, float* x_out, _Floa
 
 hipError_t Ctx::forward(const int* tok, int B, float* logits_out) {
   const int T = rows(B);
+  logp_batch = 0;
   {
     // the token gather fills the B * S real rows (the pad rows stay zero)
     const int nt = B * S;
@@ -374,7 +375,7 @@ AttnArgs Ctx::attn_args(const Stash& s) const {
 // lm_head dX over the vocabulary (from the fp16 grad16 = (p - onehot) * 2^14)
 // and the final RMSNorm backward: leaves the residual-stream gradient in
 // d_res and its fp16 operand in g16 / rinv.
-hipError_t Ctx::head_bwd(int B) {
+hipError_t Ctx::head_bwd(int B, const float* row_factor) {
   const int T = rows(B);
   const float eps = dims.eps;
   const int n_valid = B * (S - 1);
@@ -384,8 +385,8 @@ hipError_t Ctx::head_bwd(int B) {
   LLMT_HIP_TRY(gemm(CAT_GEMM_HEAD, grad16, V, sh_, 1, T, V, nullptr, 0, &go));
   NormBwdArgs nb{};
   nb.in = row_in(go);
-  nb.rinv_in = nullptr;
-  nb.gscale = 1.0f / (kGradLogitScale * (float)n_valid);
+  nb.rinv_in = row_factor;
+  nb.gscale = 1.0f / (kGradLogitScale * (row_factor ? 1.0f : (float)n_valid));
   nb.dh_out = nullptr;
   nb.x = x_final;
   nb.w = final_norm;
@@ -541,8 +542,8 @@ hipError_t Ctx::lora_grads(int l0, int nl, int B, int accumulate) {
   }, 0, per_layer * nl);
 }
 
-hipError_t Ctx::backward(int B, int accumulate) {
-  LLMT_HIP_TRY(head_bwd(B));
+hipError_t Ctx::backward(int B, int accumulate, const float* row_factor) {
+  LLMT_HIP_TRY(head_bwd(B, row_factor));
   for (int l = L - 1; l >= 0; --l) LLMT_HIP_TRY(layer_bwd(l, B));
   // every layer's adapter gradients in one launch
   LLMT_HIP_TRY(lora_grads(0, L, B, accumulate));
@@ -746,6 +747,7 @@ static bool graph_inputs(Ctx* c, const int* tokens, const int* targets) {
 // loss read-back, so a step is one graph launch and one wait.
 static int run_step(Ctx* c, int batch, int with_adam, float* loss_host,
                     const int* tokens = nullptr, const int* targets = nullptr) {
+  c->logp_batch = 0;  // a replayed graph does not pass through Ctx::forward
   TRY_HIP(c->clear_pad_rows(batch));
   if (c->use_graph && !c->recording) {
     if (!c->graph_exec || c->graph_batch != batch || c->graph_adam != with_adam ||
@@ -808,6 +810,41 @@ int llmt_forward_backward(llmt_ctx* ctx, const int* tokens, const int* targets, 
   if (graph_inputs(c, tokens, targets)) return run_step(c, batch, 0, loss_host, tokens, targets);
   if ((rc = stage_inputs(c, tokens, targets, batch))) return rc;
   return run_step(c, batch, 0, loss_host);
+}
+
+int llmt_forward_logprobs(llmt_ctx* ctx, const int* tokens, const int* targets, int batch,
+                          float* logp) {
+  set_error("");
+  Ctx* c = C_(ctx);
+  int rc = check_tokens(c, tokens, targets, batch);
+  if (rc) return rc;
+  TRY_ARG(logp, "llmt_forward_logprobs: NULL logp");
+  if ((rc = stage_inputs(c, tokens, targets, batch))) return rc;
+  TRY_HIP(c->clear_pad_rows(batch));
+  TRY_HIP(c->forward(c->tok_buf, batch, nullptr));
+  const int n = batch * c->S;
+  TRY_HIP(logprob_from_pairs(c->ce_stats, c->head_tiles, c->logits, c->tgt_buf, n, c->V, logp,
+                             c->logp_stats, c->st));
+  TRY_HIP(hipStreamSynchronize(c->st));
+  c->logp_batch = batch;
+  return LLMT_OK;
+}
+
+int llmt_backward_logprobs(llmt_ctx* ctx, const float* dlogp) {
+  set_error("");
+  Ctx* c = C_(ctx);
+  TRY_ARG(c && dlogp, "llmt_backward_logprobs: NULL argument");
+  const int batch = c->logp_batch;
+  if (!batch) {
+    set_error("llmt_backward_logprobs: the context's last forward is not llmt_forward_logprobs'");
+    return LLMT_ERR_STATE;
+  }
+  // lse_rows: the cross entropy's own row buffer, free here
+  TRY_HIP(logprob_grad16(c->logits, c->tgt_buf, c->logp_stats, dlogp, batch * c->S, c->V, c->grad16,
+                         c->lse_rows, c->rows(batch), c->st));
+  TRY_HIP(c->backward(batch, 0, c->lse_rows));
+  TRY_HIP(hipStreamSynchronize(c->st));
+  return LLMT_OK;
 }
 
 int llmt_adamw(llmt_ctx* ctx, const llmt_hparams* hp, int step) {

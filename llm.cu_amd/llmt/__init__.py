@@ -79,6 +79,8 @@ _PROTOS = {
     "llmt_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, f32, vp, vp, vp, vp, sz, vp]),
     "llmt_token_logprobs_bwd": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, i32, i32, f32, vp, i64,
                                       vp]),
+    "llmt_forward_logprobs": (i32, [vp, vp, vp, i32, vp]),
+    "llmt_backward_logprobs": (i32, [vp, vp]),
     "llmt_preference_loss": (i32, [vp, vp, vp, vp, i32, i32, C.POINTER(PrefParams), vp, vp, vp,
                                    vp, vp]),
     "llmt_policy_loss_workspace": (sz, [i32, i32]),
@@ -523,6 +525,7 @@ class Context:
         self.dims = dims
         self.max_batch = max_batch
         self.seq_len = seq_len
+        self.logp_rows = 0  # of the last forward_logprobs
         h = vp()
         sp = None if stream is None else C.c_void_p(stream.cuda_stream)
         check(lib().llmt_ctx_create(C.byref(dims), max_batch, seq_len, 1 if int8 else 0, sp,
@@ -666,6 +669,26 @@ class Context:
             __cuda_array_interface__ = {"shape": (rows, V), "typestr": "<f4",
                                         "data": (addr, False), "version": 3, "strides": None}
         return torch.as_tensor(_View(), device="cuda").clone()
+
+    def forward_logprobs(self, tokens, targets):
+        """The forward's log-probability of every target, fp32 [B * seq_len]
+        (0 where the target is outside [0, V)); backward_logprobs then takes
+        the gradient of any function of them (llmt_forward_logprobs)."""
+        import torch
+        B = self._check_tokens(tokens, targets)
+        logp = torch.empty(B * self.seq_len, dtype=torch.float32, device=tokens.device)
+        check(lib().llmt_forward_logprobs(self.h, ptr(tokens), ptr(targets), B, ptr(logp)))
+        self.logp_rows = B * self.seq_len
+        return logp
+
+    def backward_logprobs(self, dlogp):
+        """Adapter gradients into the GRAD arena from the gradient of the last
+        forward_logprobs' result (llmt_backward_logprobs)."""
+        import torch
+        if not (isinstance(dlogp, torch.Tensor) and dlogp.is_cuda):
+            raise LlmtError("dlogp must be a device tensor")
+        _expect("dlogp", dlogp, torch.float32, self.logp_rows)
+        check(lib().llmt_backward_logprobs(self.h, ptr(dlogp)))
 
     def muon(self, hp: MuonParams):
         """One Muon step over the adapters from the GRAD arena (llmt_muon)."""
