@@ -13,8 +13,8 @@
 //
 // Both are bound by HBM: the forward reads the logits once, the backward
 // reads them and writes their gradient.  4096 x 151936 fp32, a quarter of the
-// rows without a target: forward 323 us, 5.8 TB/s.  1000 x 151936 fp32:
-// backward 194 us, 6.3 TB/s (a plain copy 4.8-5.1).
+// rows without a target: forward 283 us, 6.6 TB/s.  1000 x 151936 fp32:
+// backward 194-225 us by box, 5.4-6.3 TB/s (a plain copy 4.8-5.1).
 #include <algorithm>
 
 #include "ops.h"
@@ -108,19 +108,23 @@ __device__ __forceinline__ Stat wave_merge(Stat a) {
   return a;
 }
 
-// A thread's share of columns [j0, j1) of a row, `nth` threads a row.
-template <bool ENT, typename T>
+// A thread's share of columns [j0, j1) of a row, `nth` threads a row, 16 logits
+// at a time (16-bit logits: 2000 x 16000 12.2 us, 12.6 with 32 at a time).
+template <bool ENT, bool NT, typename T>
 __device__ __forceinline__ void scan(Stat& a, const T* row, int j0, int j1, int tid, int nth,
                                      float c) {
-  constexpr int N = Piece<T>::N, U = 4;
+  constexpr int N = Piece<T>::N, U = 16 / N;
   typedef typename Piece<T>::V Vec;
   const int np = (j1 - j0) / N;
   int k = tid;
   for (; k + (U - 1) * nth < np; k += U * nth) {
     Vec v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      v[u] = *reinterpret_cast<const Vec*>(row + j0 + (long long)N * (k + u * nth));
+    for (int u = 0; u < U; ++u) {
+      auto* p = reinterpret_cast<const Vec*>(row + j0 + (long long)N * (k + u * nth));
+      if constexpr (NT) v[u] = __builtin_nontemporal_load(p);
+      else v[u] = *p;
+    }
     float x[U * N];
 #pragma unroll
     for (int i = 0; i < U * N; ++i) x[i] = (float)v[i / N][i % N];
@@ -179,7 +183,7 @@ __device__ __forceinline__ Stat block_merge(Stat a, Stat* part) {
 }
 
 // A workgroup a row.
-template <bool ENT, typename T>
+template <bool ENT, bool NT, typename T>
 __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ logits,
                                                           long long ld,
                                                           const int* __restrict__ targets, int rows,
@@ -195,7 +199,7 @@ __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ 
     }
     const T* x = logits + row * ld;
     Stat a = empty_stat();
-    scan<ENT>(a, x, 0, V, threadIdx.x, NTH, it * kLog2e);
+    scan<ENT, NT>(a, x, 0, V, threadIdx.x, NTH, it * kLog2e);
     a = block_merge<ENT>(a, part);
     if (threadIdx.x == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
     __syncthreads();
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ 
 }
 
 // A wave a row, for short ones.
-template <bool ENT, typename T>
+template <bool ENT, bool NT, typename T>
 __global__ __launch_bounds__(NTH) void logprob_wave_kernel(const T* __restrict__ logits,
                                                            long long ld,
                                                            const int* __restrict__ targets,
@@ -220,7 +224,7 @@ __global__ __launch_bounds__(NTH) void logprob_wave_kernel(const T* __restrict__
     }
     const T* x = logits + row * ld;
     Stat a = empty_stat();
-    scan<ENT>(a, x, 0, V, lane, 64, it * kLog2e);
+    scan<ENT, NT>(a, x, 0, V, lane, 64, it * kLog2e);
     a = wave_merge<ENT>(a);
     if (lane == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
   }
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(NTH) void logprob_part_kernel(const T* __restrict__
   if (t < 0 || t >= V) return;
   const int j0 = (int)min((long long)ch * width, (long long)V), j1 = min(V - j0, width) + j0;
   Stat a = empty_stat();
-  scan<ENT>(a, logits + row * ld, j0, j1, threadIdx.x, NTH, it * kLog2e);
+  scan<ENT, false>(a, logits + row * ld, j0, j1, threadIdx.x, NTH, it * kLog2e);
   a = block_merge<ENT>(a, part);
   if (threadIdx.x == 0) parts[blockIdx.x] = make_float4(a.m, a.s, a.u, a.x);
 }
@@ -393,7 +397,15 @@ static hipError_t with_type(int dtype, F&& f) {
   }
 }
 
-template <bool ENT, typename T>
+// Logits beyond the 256 MB last-level cache stream past it (4096 x 151936 fp32,
+// a quarter of the rows skipped: 283 us nontemporal, 321 not; 1000 x 151936 with
+// the backward behind it 290 and 303); smaller ones stay for the backward
+// (256 x 151936 with it 79 us, 90 nontemporal).
+static bool beyond_cache(const LogprobArgs& a, size_t esize) {
+  return (double)a.rows * a.V * esize > 256.0 * (1 << 20);
+}
+
+template <bool ENT, bool NT, typename T>
 static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st) {
   const T* x = (const T*)a.logits;
   float2* stats = (float2*)a.stats;
@@ -407,11 +419,11 @@ static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st
     hipLaunchKernelGGL((logprob_merge_kernel<ENT, T>), dim3(a.rows), dim3(64), 0, st, x, a.ld,
                        a.targets, a.V, a.it, chunks, parts, a.logp, stats, a.entropy);
   } else if (a.V <= kWaveV) {
-    hipLaunchKernelGGL((logprob_wave_kernel<ENT, T>),
+    hipLaunchKernelGGL((logprob_wave_kernel<ENT, NT, T>),
                        dim3(std::min((a.rows + NTH / 64 - 1) / (NTH / 64), 1 << 20)), dim3(NTH), 0,
                        st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
   } else {
-    hipLaunchKernelGGL((logprob_row_kernel<ENT, T>), dim3(std::min(a.rows, 1 << 20)), dim3(NTH), 0,
+    hipLaunchKernelGGL((logprob_row_kernel<ENT, NT, T>), dim3(std::min(a.rows, 1 << 20)), dim3(NTH), 0,
                        st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
   }
   LLMT_LAUNCH_CHECK();
@@ -421,8 +433,10 @@ static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st
 hipError_t logprob_fwd(const LogprobArgs& a, void* workspace, hipStream_t st) {
   return with_type(a.dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    return a.entropy ? launch_fwd<true, T>(a, (float4*)workspace, st)
-                     : launch_fwd<false, T>(a, (float4*)workspace, st);
+    float4* ws = (float4*)workspace;
+    if (beyond_cache(a, sizeof(T)))
+      return a.entropy ? launch_fwd<true, true, T>(a, ws, st) : launch_fwd<false, true, T>(a, ws, st);
+    return a.entropy ? launch_fwd<true, false, T>(a, ws, st) : launch_fwd<false, false, T>(a, ws, st);
   });
 }
 
@@ -442,7 +456,7 @@ static hipError_t launch_bwd(const LogprobArgs& a, hipStream_t st) {
 hipError_t logprob_bwd(const LogprobArgs& a, hipStream_t st) {
   return with_type(a.dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    if ((double)a.rows * a.V * sizeof(T) > 256.0 * (1 << 20))
+    if (beyond_cache(a, sizeof(T)))
       return a.dentropy ? launch_bwd<true, true, T>(a, st) : launch_bwd<false, true, T>(a, st);
     return a.dentropy ? launch_bwd<true, false, T>(a, st) : launch_bwd<false, false, T>(a, st);
   });
