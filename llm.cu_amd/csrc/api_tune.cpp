@@ -26,14 +26,22 @@ static int done(hipError_t e) {
 
 static bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
 
+// Matrices of one call, the long side of one (also a vocabulary), and a row or
+// matrix stride: grids and indexes stay within 31 bits, offsets within 62.
+constexpr int kMaxMatrices = 1 << 20, kMaxLong = 1 << 30;
+constexpr long long kMaxStride = 1ll << 40;
+static bool strides_fit(long long rows, long long ld) {
+  return ld <= kMaxStride && (double)rows * (double)ld <= 1e18;
+}
+
 static size_t esize(int dtype) { return dtype == LLMT_F32 ? 4 : 2; }
 
 // The checks that the log-probabilities' two directions share.
 static int check_logits(const char* fn, const void* logits, int dtype, long long ld,
                         const int* targets, int rows, int V, float inv_temp) {
   TRY_ARG(dtype == LLMT_F32 || dtype == LLMT_F16 || dtype == LLMT_BF16, "%s: dtype %d", fn, dtype);
-  TRY_ARG(rows >= 0 && V >= 1 && ld >= V, "%s: rows=%d V=%d ld=%lld (rows >= 0, V >= 1, ld >= V)",
-          fn, rows, V, ld);
+  TRY_ARG(rows >= 0 && V >= 1 && V <= kMaxLong && ld >= V && strides_fit(rows, ld),
+          "%s: rows=%d V=%d ld=%lld (rows >= 0, V in [1, 2^30], ld >= V)", fn, rows, V, ld);
   TRY_ARG(inv_temp > 0.f && isfinite(inv_temp), "%s: inv_temp must be positive and finite", fn);
   TRY_ARG(rows == 0 || (logits && targets), "%s: NULL argument", fn);
   TRY_ARG(aligned(logits, esize(dtype)) && aligned(targets, 4), "%s: misaligned argument", fn);
@@ -45,10 +53,6 @@ static bool apart(const void* a, long long na, const void* b, long long nb) {
   const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
   return a0 + (size_t)na * 4 <= b0 || b0 + (size_t)nb * 4 <= a0;
 }
-
-// Matrices of one call, and the long side of one: grids and indexes stay
-// within 31 bits.
-constexpr int kMaxMatrices = 1 << 20, kMaxLong = 1 << 30;
 
 static NsMat ns_matrix(int rows, int cols) {
   NsMat m{};
@@ -144,7 +148,7 @@ int llmt_token_logprobs_bwd(const void* logits, int dtype, long long ld, const i
   const int rc =
       check_logits("llmt_token_logprobs_bwd", logits, dtype, ld, targets, rows, V, inv_temp);
   if (rc) return rc;
-  TRY_ARG(ldd >= V, "llmt_token_logprobs_bwd: ldd=%lld < V=%d", ldd, V);
+  TRY_ARG(ldd >= V && strides_fit(rows, ldd), "llmt_token_logprobs_bwd: ldd=%lld, V=%d", ldd, V);
   if (rows == 0) return LLMT_OK;
   TRY_ARG(stats && dlogp && dlogits && (!dentropy || entropy),
           "llmt_token_logprobs_bwd: NULL argument (dentropy needs entropy)");
@@ -283,9 +287,11 @@ int llmt_orthogonalize(const float* x, long long stride_x, long long ldx, float*
   TRY_ARG(count <= kMaxMatrices, "llmt_orthogonalize: %d matrices, at most %d", count, kMaxMatrices);
   TRY_ARG(steps >= 1 && steps <= 20 && eps > 0.f && isfinite(eps),
           "llmt_orthogonalize: steps in [1, 20], eps positive");
-  const long long span_x = (long long)(rows - 1) * ldx + cols;
-  const long long span_o = (long long)(rows - 1) * ldo + cols;
-  TRY_ARG(ldx >= cols && ldo >= cols &&
+  const bool bounded = strides_fit(rows, ldx) && strides_fit(rows, ldo) &&
+                       stride_x <= kMaxStride && stride_out <= kMaxStride;
+  const long long span_x = bounded ? (long long)(rows - 1) * ldx + cols : 0;
+  const long long span_o = bounded ? (long long)(rows - 1) * ldo + cols : 0;
+  TRY_ARG(bounded && ldx >= cols && ldo >= cols &&
               (count <= 1 || (stride_x >= span_x && stride_out >= span_o)),
           "llmt_orthogonalize: ldx=%lld ldo=%lld stride_x=%lld stride_out=%lld", ldx, ldo, stride_x,
           stride_out);

@@ -14,7 +14,7 @@
 // Both are bound by HBM: the forward reads the logits once, the backward
 // reads them and writes their gradient.  4096 x 151936 fp32, a quarter of the
 // rows without a target: forward 283 us, 6.6 TB/s.  1000 x 151936 fp32:
-// backward 194-225 us by box, 5.4-6.3 TB/s (a plain copy 4.8-5.1).
+// backward 194 us, 6.3 TB/s (a plain copy 4.8-5.1).
 #include <algorithm>
 
 #include "ops.h"
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ 
                                                           float2* __restrict__ stats,
                                                           float* __restrict__ entropy) {
   __shared__ Stat part[NTH / 64];
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const int t = targets[row];
     if (t < 0 || t >= V) {
       if (threadIdx.x == 0) no_target<ENT>(row, logp, stats, entropy);
@@ -283,11 +283,11 @@ constexpr int kBwdPieces = sizeof(T) == 4 ? 1 : 2;
 // against 13.4 us).  NT: gradients beyond the 256 MB last-level cache are
 // stored nontemporal (1000 x 151936 fp32: 194 us, 201 without), smaller ones
 // stay there for the next kernel.
-// TO: the type written.  With `factor` the rows are written for dlogp = -1
-// times kGradLogitScale (the lm_head dX GEMM's operand) and factor[row] gets
+// TO: the type written.  FACTOR: the rows are written for dlogp = -1 times
+// kGradLogitScale (the lm_head dX GEMM's operand) and factor[row] gets
 // what they lack of the gradient, -dlogp; rows from `rows` to `factor_rows`
 // get a factor of 0.
-template <bool ENT, bool NT, typename T, typename TO = T>
+template <bool ENT, bool NT, typename T, typename TO = T, bool FACTOR = false>
 __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const T* logits, long long ld, const int* __restrict__ targets,
     const float2* __restrict__ stats, const float* __restrict__ entropy,
@@ -304,7 +304,7 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const int row = (int)(w / chunks), ch = (int)(w - (long long)row * chunks);
     const int t = targets[row];
     float g = dlogp[row] * it;
-    if (factor) {
+    if constexpr (FACTOR) {
       if (ch == 0 && lane == 0) factor[row] = t < 0 || t >= V ? 0.f : -g;
       g = g == 0.f ? 0.f : -kGradLogitScale;
     }
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const int j = j0 + N * np + lane;
     if (j < j1) d[j] = zero ? (TO)0.f : (TO)(j == t ? at_target((float)x[j]) : value((float)x[j]));
   }
-  if (factor)
+  if constexpr (FACTOR)
     for (int r = rows + blockIdx.x * NTH + threadIdx.x; r < factor_rows; r += gridDim.x * NTH)
       factor[r] = 0.f;
 }
@@ -412,7 +412,7 @@ static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st
   const int chunks = fwd_chunks(a.rows, a.V, a.dtype);
   if (chunks > 1) {
     constexpr int N = Piece<T>::N;  // chunks start at whole pieces
-    const int width = ((a.V + chunks - 1) / chunks + N - 1) / N * N;
+    const int width = (int)(((long long)a.V + chunks - 1) / chunks + N - 1) / N * N;
     hipLaunchKernelGGL((logprob_part_kernel<ENT, T>), dim3(a.rows * chunks), dim3(NTH), 0, st, x,
                        a.ld, a.targets, a.V, a.it, chunks, width, parts);
     LLMT_LAUNCH_CHECK();
@@ -420,7 +420,7 @@ static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st
                        a.targets, a.V, a.it, chunks, parts, a.logp, stats, a.entropy);
   } else if (a.V <= kWaveV) {
     hipLaunchKernelGGL((logprob_wave_kernel<ENT, NT, T>),
-                       dim3(std::min((a.rows + NTH / 64 - 1) / (NTH / 64), 1 << 20)), dim3(NTH), 0,
+                       dim3(std::min(((long long)a.rows + NTH / 64 - 1) / (NTH / 64), 1ll << 20)), dim3(NTH), 0,
                        st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
   } else {
     hipLaunchKernelGGL((logprob_row_kernel<ENT, NT, T>), dim3(std::min(a.rows, 1 << 20)), dim3(NTH), 0,
@@ -512,7 +512,7 @@ hipError_t logprob_grad16(const float* logits, const int* targets, const float2*
   constexpr int per = kBwdPieces<float> * Piece<float>::N * 64;
   const int chunks = (V + per - 1) / per;
   const long long wgs = ((long long)rows * chunks + NTH / 64 - 1) / (NTH / 64);
-  hipLaunchKernelGGL((logprob_bwd_kernel<false, false, float, _Float16>),
+  hipLaunchKernelGGL((logprob_bwd_kernel<false, false, float, _Float16, true>),
                      dim3(std::min(wgs, 1ll << 22)), dim3(NTH), 0, st, logits, (long long)V,
                      targets, stats, (const float*)nullptr, dlogp, (const float*)nullptr, rows, V,
                      1.0f, chunks, grad16, (long long)V, factor, factor_rows);

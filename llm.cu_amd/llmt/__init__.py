@@ -302,6 +302,12 @@ def _logits_dtype(name, t):
     return code
 
 
+def _inverse(temperature):
+    if not temperature > 0:
+        raise LlmtError(f"temperature must be positive (got {temperature})")
+    return 1.0 / temperature
+
+
 def _ld(t):
     """Elements from row to row (a single row's stride is of no account)."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -330,7 +336,7 @@ def token_logprobs(logits, targets, temperature=1.0, want_entropy=False, stream=
         need = L.llmt_token_logprobs_workspace(rows, V, dt)
         ws = logits.new_empty(need, dtype=torch.uint8) if need else None
         check(L.llmt_token_logprobs(logits.data_ptr(), dt, _ld(logits), targets.data_ptr(), rows, V,
-                                    1.0 / temperature, logp.data_ptr(), stats.data_ptr(), _at(ent),
+                                    _inverse(temperature), logp.data_ptr(), stats.data_ptr(), _at(ent),
                                     _at(ws), need, on.raw))
     return logp, stats, ent
 
@@ -356,7 +362,7 @@ def token_logprobs_bwd(logits, targets, stats, dlogp, entropy=None, dentropy=Non
             raise LlmtError("out must have the logits' shape and type")
         check(lib().llmt_token_logprobs_bwd(logits.data_ptr(), dt, _ld(logits), targets.data_ptr(),
                                             stats.data_ptr(), _at(entropy), dlogp.data_ptr(),
-                                            _at(dentropy), rows, V, 1.0 / temperature,
+                                            _at(dentropy), rows, V, _inverse(temperature),
                                             out.data_ptr(), _ld(out), on.raw))
     return out
 

@@ -269,6 +269,9 @@ def test_the_binding_refuses_wrong_types_and_shapes(dev):
     off, v = torch.tensor([0, 2, 4], dtype=torch.int32, device=dev), torch.zeros(4, device=dev)
     st = torch.zeros(4, 2, device=dev)
     for call in (lambda: llmt.token_logprobs(x.double(), t),
+                 lambda: llmt.token_logprobs(x, t, temperature=0.0),
+                 lambda: llmt.token_logprobs(x, t, temperature=-1.0),
+                 lambda: llmt.token_logprobs(x, t, temperature=float("nan")),
                  lambda: llmt.token_logprobs(x.t(), t),
                  lambda: llmt.token_logprobs(x, t.long()),
                  lambda: llmt.token_logprobs(x, t[:3]),
@@ -290,3 +293,38 @@ def test_the_binding_refuses_wrong_types_and_shapes(dev):
                  lambda: llmt.policy_loss(v, v, v, off, mask=t)):
         with pytest.raises(llmt.LlmtError):
             call()
+
+
+def test_two_streams_at_once(dev):
+    """Calls that run beside one another on two streams share nothing."""
+    g = torch.Generator().manual_seed(13)
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    data = []
+    for k in range(2):
+        off, T = ragged(g, 40, 700)
+        data.append(dict(off=off.to(dev), lp=-torch.rand(T, generator=g).to(dev),
+                         old=-torch.rand(T, generator=g).to(dev),
+                         mask=(torch.rand(T, generator=g) < 0.5).to(dev),
+                         x=torch.randn(5, 60000, generator=g).to(dev),
+                         t=torch.randint(0, 60000, (5,), generator=g, dtype=torch.int32).to(dev),
+                         u=torch.randn(3, 30, 500, generator=g).to(dev)))
+
+    def all_of(d, stream):
+        p = llmt.policy_loss(d["lp"], d["old"], d["old"], d["off"], ref_logp=d["old"],
+                             mask=d["mask"], kl_coef=0.1, stream=stream)
+        q = llmt.preference_loss(d["lp"], d["old"], d["off"], mask=d["mask"], stream=stream)
+        lp, st, _ = llmt.token_logprobs(d["x"], d["t"], stream=stream)
+        return (p.loss, p.stats, p.dlogp, *q, lp, st,
+                llmt.token_logprobs_bwd(d["x"], d["t"], st, lp, stream=stream),
+                llmt.orthogonalize(d["u"], stream=stream))
+
+    want = [all_of(d, None) for d in data]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            got[k].append(all_of(data[k], sides[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[k]))

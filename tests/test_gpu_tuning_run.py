@@ -135,7 +135,9 @@ def test_context_order_of_calls(dev):
             ctx.set_graph(graph)
             for other in (lambda: ctx.forward_backward(tok, tgt),
                           lambda: ctx.step(tok, tgt, llmt.hparams(), 1),
-                          lambda: ctx.layer_forward(0, x, B)):
+                          lambda: ctx.layer_forward(0, x, B),
+                          lambda: ctx.layer_backward(0, x, B),
+                          lambda: ctx.head_ce(x.half(), tgt.reshape(-1))):
                 ctx.forward_logprobs(tok, tgt)
                 ctx.backward_logprobs(d)
                 other()

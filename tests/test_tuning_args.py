@@ -20,6 +20,7 @@ def logprobs(logits=A(1), dtype=0, ld=100, targets=A(2), rows=4, V=100, it=1.0, 
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=3), dict(dtype=-1), dict(ld=99), dict(rows=-1), dict(V=0, ld=0), dict(it=0.0),
+    dict(V=2 ** 30 + 1, ld=2 ** 31), dict(ld=2 ** 41), dict(rows=2 ** 31 - 1, ld=2 ** 39),
     dict(it=-1.0), dict(it=math.inf), dict(it=math.nan), dict(logits=None), dict(targets=None),
     dict(logp=None), dict(stats=None), dict(logits=C.c_void_p(0x100002)),
     dict(logits=C.c_void_p(0x100001), dtype=1), dict(stats=C.c_void_p(0x400004)),
@@ -40,7 +41,7 @@ def bwd(logits=A(1), dtype=0, ld=100, targets=A(2), stats=A(3), ent=None, dlogp=
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=7), dict(ld=99), dict(ldd=99), dict(rows=-2), dict(it=0.0), dict(stats=None),
+    dict(dtype=7), dict(ld=99), dict(ldd=99), dict(ldd=2 ** 62), dict(rows=-2), dict(it=0.0), dict(stats=None),
     dict(dlogp=None), dict(out=None), dict(dent=A(6)), dict(out=C.c_void_p(0x500002)),
     dict(dlogp=C.c_void_p(0x400002)), dict(dent=C.c_void_p(0x600002), ent=A(7)),
     # in place with another row stride, and overlaps that are not in place
@@ -103,6 +104,7 @@ def ortho(x=A(1), sx=2000, ldx=100, out=A(2), so=2000, ldo=100, count=2, rows=20
 @pytest.mark.parametrize("bad", [
     dict(count=-1), dict(count=2 ** 21), dict(rows=0), dict(cols=0, ldx=0, ldo=0),
     dict(rows=65, sx=6500, so=6500), dict(ldx=99), dict(ldo=99), dict(sx=1999), dict(so=1999),
+    dict(ldx=2 ** 62), dict(ldo=2 ** 60), dict(sx=2 ** 50), dict(so=-5), dict(ldx=-100),
     dict(steps=0), dict(steps=21), dict(eps=0.0), dict(eps=math.nan), dict(x=None), dict(out=None),
     dict(x=C.c_void_p(0x100002)), dict(ws=None), dict(need=100), dict(ws=C.c_void_p(0x800004)),
     dict(out=A(1), so=2001), dict(out=A(1), ldo=101, so=2100), dict(out=C.c_void_p(0x100004)),
