@@ -108,12 +108,12 @@ __device__ __forceinline__ Stat wave_merge(Stat a) {
   return a;
 }
 
-// A thread's share of columns [j0, j1) of a row, `nth` threads a row, 16 logits
-// at a time (16-bit logits: 2000 x 16000 12.2 us, 12.6 with 32 at a time).
-template <bool ENT, bool NT, typename T>
+// A thread's share of columns [j0, j1) of a row, `nth` threads a row, BATCH
+// logits at a time.
+template <bool ENT, bool NT, int BATCH = 16, typename T>
 __device__ __forceinline__ void scan(Stat& a, const T* row, int j0, int j1, int tid, int nth,
                                      float c) {
-  constexpr int N = Piece<T>::N, U = 16 / N;
+  constexpr int N = Piece<T>::N, U = BATCH / N;
   typedef typename Piece<T>::V Vec;
   const int np = (j1 - j0) / N;
   int k = tid;
@@ -172,25 +172,25 @@ __device__ __forceinline__ void no_target(long long row, float* logp, float2* st
 }
 
 // The block's statistics, in thread 0.  Contains a barrier.
-template <bool ENT>
+template <bool ENT, int BLOCK>
 __device__ __forceinline__ Stat block_merge(Stat a, Stat* part) {
   a = wave_merge<ENT>(a);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
   __syncthreads();
   if (threadIdx.x == 0)
-    for (int w = 1; w < NTH / 64; ++w) merge<ENT>(a, part[w]);
+    for (int w = 1; w < BLOCK / 64; ++w) merge<ENT>(a, part[w]);
   return a;
 }
 
-// A workgroup a row.
-template <bool ENT, bool NT, typename T>
-__global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ logits,
+// A workgroup of BLOCK threads a row, BATCH logits at a time.
+template <bool ENT, bool NT, int BLOCK, int BATCH, typename T>
+__global__ __launch_bounds__(BLOCK) void logprob_row_kernel(const T* __restrict__ logits,
                                                           long long ld,
                                                           const int* __restrict__ targets, int rows,
                                                           int V, float it, float* __restrict__ logp,
                                                           float2* __restrict__ stats,
                                                           float* __restrict__ entropy) {
-  __shared__ Stat part[NTH / 64];
+  __shared__ Stat part[BLOCK / 64];
   for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
     const int t = targets[row];
     if (t < 0 || t >= V) {
@@ -199,8 +199,8 @@ __global__ __launch_bounds__(NTH) void logprob_row_kernel(const T* __restrict__ 
     }
     const T* x = logits + row * ld;
     Stat a = empty_stat();
-    scan<ENT, NT>(a, x, 0, V, threadIdx.x, NTH, it * kLog2e);
-    a = block_merge<ENT>(a, part);
+    scan<ENT, NT, BATCH>(a, x, 0, V, threadIdx.x, BLOCK, it * kLog2e);
+    a = block_merge<ENT, BLOCK>(a, part);
     if (threadIdx.x == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
     __syncthreads();
   }
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(NTH) void logprob_part_kernel(const T* __restrict__
   const int j0 = (int)min((long long)ch * width, (long long)V), j1 = min(V - j0, width) + j0;
   Stat a = empty_stat();
   scan<ENT, false>(a, logits + row * ld, j0, j1, threadIdx.x, NTH, it * kLog2e);
-  a = block_merge<ENT>(a, part);
+  a = block_merge<ENT, NTH>(a, part);
   if (threadIdx.x == 0) parts[blockIdx.x] = make_float4(a.m, a.s, a.u, a.x);
 }
 
@@ -369,18 +369,23 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
 // 14.6 and 15.4) or the workgroups ahead (300 x 3000: 3.9 against 4.5).
 constexpr int kWaveV = 2048;
 
-// Fewer rows than the chip has CUs (256) are split into chunks, as many as
-// make four workgroups a CU and at least one batch of loads a thread, and
-// merged by a second launch.  The launch is worth 120 KB off a workgroup's
-// share: 1 x 151936 fp32 5.8 us, 15.9 in one workgroup; 1 x 32000 fp32 (110
-// KB) 5.7 and 5.2; 1 x 64000 bf16 (117 KB) 5.7 and 6.3.  From 256 rows on it is
-// never faster (450 x 100000 fp32: 29.9 against 27.5).
-constexpr int kCus = 256, kSplitBytes = 120000;
+// Fewer rows than the chip has CUs (256) take the wide workgroups: a row is
+// one CU's and the latency of its loads (1 x 151936 fp32 9.6 us, 15.9 with 256
+// threads and 16 logits at a time; 128 x 50257 5.8 and 8.0).  From there on
+// the narrow ones, which share CUs, stream better (8192 x 4000: 25.2 and 29.6).
+//
+// Rows too long for one CU are split into chunks, as many as make four
+// workgroups a CU and at least one batch of loads a thread, and merged by a
+// second launch, which costs a caller 3.5 us: worth 192 K logits off a
+// workgroup's share (one row: 151936 split 5.8 us in a graph, 14.0 a call from
+// Python, unsplit 9.6 and 10.2; 262144 bf16 a call and its wait 25 and 31), up
+// to half a row a CU (200 x 262144 bf16: split 20.6, unsplit 17.9).
+constexpr int kCus = 256, kSplitLogits = 192 << 10;
 static int fwd_chunks(int rows, int V, int dtype) {
-  if (V <= kWaveV || rows >= kCus) return 1;
-  const long long es = dtype == kF32 ? 4 : 2, batch = NTH * 4 * (16 / es);
+  if (rows > kCus / 2) return 1;
+  const long long batch = NTH * 4 * (dtype == kF32 ? 4 : 8);
   const long long chunks = std::min((V + batch - 1) / batch, (long long)(4 * kCus / rows));
-  return V * es * (chunks - 1) >= kSplitBytes * chunks ? (int)chunks : 1;
+  return V * (chunks - 1) >= kSplitLogits * chunks ? (int)chunks : 1;
 }
 
 size_t logprob_workspace(int rows, int V, int dtype) {
@@ -422,9 +427,13 @@ static hipError_t launch_fwd(const LogprobArgs& a, float4* parts, hipStream_t st
     hipLaunchKernelGGL((logprob_wave_kernel<ENT, NT, T>),
                        dim3(std::min(((long long)a.rows + NTH / 64 - 1) / (NTH / 64), 1ll << 20)), dim3(NTH), 0,
                        st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
+  } else if (a.rows < kCus) {
+    hipLaunchKernelGGL((logprob_row_kernel<ENT, NT, 512, 32, T>), dim3(a.rows), dim3(512), 0, st, x,
+                       a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
   } else {
-    hipLaunchKernelGGL((logprob_row_kernel<ENT, NT, T>), dim3(std::min(a.rows, 1 << 20)), dim3(NTH), 0,
-                       st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats, a.entropy);
+    hipLaunchKernelGGL((logprob_row_kernel<ENT, NT, NTH, 16, T>), dim3(std::min(a.rows, 1 << 20)),
+                       dim3(NTH), 0, st, x, a.ld, a.targets, a.rows, a.V, a.it, a.logp, stats,
+                       a.entropy);
   }
   LLMT_LAUNCH_CHECK();
   return hipSuccess;
