@@ -370,8 +370,8 @@ __device__ __forceinline__ doublex4 product(const double* m1, const double* m2, 
 // ws.proj[matrix][tile row][tile col][v][lane].
 template <int NT>
 __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a) {
-  __shared__ double sG[NT * NT * 256], sB[NT * NT * 256], sP[NT * NT * 256];
-  __shared__ double tr[NT];
+  constexpr int M = NT * NT * 256;
+  __shared__ double sG[M], sY[M], sB[M], sP[M], tr[NT];
   const int mat = blockIdx.x;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, q = lane >> 4, c = lane & 15;
   int i = 0, j = w;  // wave w's tile
@@ -405,24 +405,23 @@ __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a)
   __syncthreads();
   doublex4 B = kB * G + kC * product<NT>(sG, sG, i, j, lane);
   doublex4 P = kA * I + B;
+  put(sB, B);
+  __syncthreads();
+  // three barriers a step: a buffer is written a barrier after its last reader
   for (int step = 1; step < a.steps; ++step) {
-    put(sB, B);
-    put(sP, P);
-    __syncthreads();
     const doublex4 Y = kA * G + product<NT>(sB, sG, i, j, lane);  // p(G) G
+    if (step > 1) P = kA * P + product<NT>(sB, sP, i, j, lane);
+    put(sY, Y);
     __syncthreads();
-    put(sG, Y);
-    __syncthreads();
-    G = kA * Y + product<NT>(sB, sG, i, j, lane);
-    __syncthreads();
+    G = kA * Y + product<NT>(sB, sY, i, j, lane);
     put(sG, G);
+    put(sP, P);
     __syncthreads();
     B = kB * G + kC * product<NT>(sG, sG, i, j, lane);
     put(sB, B);
     __syncthreads();
-    P = kA * P + product<NT>(sB, sP, i, j, lane);
-    __syncthreads();
   }
+  if (a.steps > 1) P = kA * P + product<NT>(sB, sP, i, j, lane);
   put(a.proj + (long long)mat * NT * NT * 256, P * inv);
 }
 

@@ -156,7 +156,7 @@ def test_strided_rows_and_offset_views(dev, dtype):
     assert (buf[:, :3] == 9).all() and (buf[:, 1004:] == 9).all()
 
 
-@pytest.mark.parametrize("V", [100, 9000, 151936])
+@pytest.mark.parametrize("V", [100, 9000, 151936, 230000])
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_masked_logits(dev, dtype, V):
     """Logits of -inf and of the type's lowest value: probability 0, gradient 0; a row of
@@ -237,7 +237,7 @@ def test_offsets_past_32_bits(dev):
     assert torch.equal(view, want)
 
 
-@pytest.mark.parametrize("rows,V", [(3, 151936), (300, 5000), (40, 500)])
+@pytest.mark.parametrize("rows,V", [(3, 151936), (300, 5000), (40, 500), (5, 230001)])
 def test_same_bits_on_a_side_stream_and_in_a_graph(dev, rows, V):
     g, x, t = problem(rows, V, torch.float32, seed=8)
     xd, td, dl = x.to(dev), t.to(dev), torch.randn(rows, generator=g).to(dev)
