@@ -9,13 +9,19 @@
 //   X_k = P_k X0,  P <- p(G) P,  G <- p(G)^2 G,
 // so the matrix is read once for G0 = U U^T / (|U| + eps)^2 (|U|^2 is its
 // trace) and once for the product P U, and the iteration itself is r x r.
-// That trades 2 steps (4 r^2 n + 2 r^3) flops and as many passes for two.
+// That trades steps x (4 r^2 n + 2 r^3) flops in as many passes over the matrix
+// for 4 r^2 n + 8 steps r^3 in two.
 //
 // G holds the squares of the singular values, and a small one is amplified by
 // up to 3.4445^2 a step: in fp32 the rounding of G (2^-24 of the largest
 // square) would come out of five steps 2e5 times larger.  G, the iteration
 // and the product are therefore fp64 on v_mfma_f64_16x16x4 (inputs are exact
 // there), rounded once to fp32.
+//
+// Bound by HBM where the short side is 16 and matrices are many (the 28-layer
+// Muon step, 128 MB: 26.7 us, 4.8 TB/s, a copy's rate), by the fp64 matrix rate
+// above (28 x 12288 x 64: 4.5 GFLOP, gram 38 us, iteration 43, product 56), by
+// launches and memory round trips for few matrices (1 x 16 x 2048: 10.5 us).
 //
 // All matrices of the iteration are symmetric and commute.  A lane of an f64
 // MFMA result holds rows 4 v + l / 16 (v = 0..3) of column l % 16; read by
@@ -562,7 +568,9 @@ __global__ __launch_bounds__(FTH) void ns_fused_kernel(const NsArgs a) {
   }
 }
 
-constexpr int kTargetWg = 512;  // workgroups of the gram and apply launches
+// Workgroups of the gram and apply launches: two a CU (28 x 12288 x 64: 137 us,
+// 145 with one a CU, 151 with four).
+constexpr int kTargetWg = 512;
 
 // k ranges a matrix, in groups of a stage a wave.
 int splits_for(const NsArgs& a, int nt) {
@@ -584,12 +592,13 @@ size_t class_bytes(const NsArgs& a, int nt) {
 
 // The matrices of `all` whose short side takes nt tiles of 16; 0: those that
 // the one-workgroup kernel takes, which the others then leave out.  It is one
-// launch, but one CU's fp64 rate a matrix: short sides of 16 and long ones of
-// up to 1024 take it at any count (1 x 16 x 512: 9.2 us, 11.7 in two launches;
-// 1 x 16 x 1024: 12.8 and 12.3), longer ones from kFusedMats on (2048: 19.9 and
-// 12.1 for one, 22 for 128, 23.0 and 31.5 for 224; Muon, 64 matrices 25.9 and
-// 18.9, 128 27.1 and 27.9, 224 30.9 and 42).  All matrices of a call that fit
-// go one way.
+// launch, but one CU's fp64 rate and memory lanes a matrix: long sides of up to
+// 1024 take it at any count (in a graph, 1 x 16 x 512: 8.7 us, 10.2 in two
+// launches; 1 x 16 x 1024: 11.5 and 10.6, level with the second launch's cost
+// to a caller), longer ones from kFusedMats matrices on (2048: 17.1 and 10.5
+// for one, 19.1 and 18.1 for 128, 20.6 and 26.3 for 224; Muon, 64 matrices 21.7
+// and 17.4, 128 23.4 and 25.1, 224 27.7 and 37).  All matrices of a call that
+// fit go one way.
 constexpr int kFusedLong = 1024, kFusedMats = 112;
 NsArgs class_of(const NsArgs& all, int nt) {
   auto fits = [](const NsMat& m) { return m.r <= 16 && fused_lds(m.n) <= kLdsBytes; };

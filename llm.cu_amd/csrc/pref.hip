@@ -13,7 +13,9 @@
 // and exp(d) - d - 1 of a small d all lose what matters in fp32, and at 12 to
 // 25 bytes a token the kernels stay bound by memory round trips and launches:
 // loads are issued before anything waits, four tokens a thread, and small
-// inputs take one launch.  Every sum has a fixed order.
+// inputs take one launch.  Every sum has a fixed order.  Preference loss, 4
+// pairs of 390 tokens 5.8 us, 2048 pairs of 910 (16.8 MB) 12; policy loss, 8 x
+// 130 tokens 6.9 us, 512 x 1170 (17 MB) 12, in a graph.
 #include <algorithm>
 
 #include "../../include/llmt.h"
