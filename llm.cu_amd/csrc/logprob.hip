@@ -370,7 +370,7 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
 constexpr int kWaveV = 2048;
 
 // Fewer rows than the chip has CUs (256) take the wide workgroups: a row is
-// one CU's and the latency of its loads (1 x 151936 fp32 9.6 us, 15.9 with 256
+// one CU's loads and exponentials (1 x 151936 fp32 9.6 us, 15.9 with 256
 // threads and 16 logits at a time; 128 x 50257 5.8 and 8.0).  From there on
 // the narrow ones, which share CUs, stream better (8192 x 4000: 25.2 and 29.6).
 //

@@ -4,8 +4,8 @@ the CPU oracle's model with float64 losses; and through the reference-compatible
 
 Bars: the step's own, a loss within 1e-3 and every adapter gradient within 1e-2 relative
 L2 of the fp32 oracle."""
+import copy
 import ctypes as C
-import math
 
 import pytest
 import torch
@@ -14,6 +14,7 @@ import torch.nn.functional as F
 import llmt
 from helpers import SMALL, grad_errors, rel_l2, small_problem, upload_model
 from oracle import lora_step as ref
+from oracle.configs import quantize_model_int8
 
 pytestmark = pytest.mark.gpu
 
@@ -95,7 +96,8 @@ def test_context_backward_of_any_function(dev, batch, seq_len):
         ctx.close()
 
 
-def test_context_backward_equals_the_cross_entropy_step(dev):
+@pytest.mark.parametrize("weights", ["f16", "i8", "untied"])
+def test_context_backward_equals_the_cross_entropy_step(dev, weights):
     """dlogp = -1 / n on the rows with a target is the mean cross entropy: the same gradient
     as llmt_forward_backward up to fp16 roundings that fall to the other side.  Where the two
     sides' values differ by a relative d, one in d / 2^-10 rounds to another neighbour, a step
@@ -105,7 +107,22 @@ def test_context_backward_equals_the_cross_entropy_step(dev):
     Q/K/V operand), and the fp32 differences before them are 1e-6: 16 x 2^-11."""
     W, ad, tok, tgt = small_problem()
     B, S = tok.shape
-    ctx = context(dev, W, ad, B, S)
+    if weights == "i8":
+        W, qs = quantize_model_int8(copy.deepcopy(W))
+        ctx = llmt.Context(llmt.make_dims(SMALL), B, S, int8=True)
+        f = lambda t: t.float().to(dev).contiguous()
+        for l, lw in enumerate(W.layers):
+            q = [qs[(l, n)] for n in ("wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down")]
+            ctx.set_layer_i8(l, [torch.from_numpy(a).to(dev) for a, _ in q],
+                             [torch.from_numpy(b).to(dev) for _, b in q], f(lw.attn_norm),
+                             f(lw.ffn_norm), f(lw.q_norm), f(lw.k_norm))
+        ctx.set_embed_f16(W.embed.half().to(dev), f(W.final_norm))
+        ctx.lora_set("param", llmt.flatten_adapters(ad).to(dev))
+    else:
+        ctx = context(dev, W, ad, B, S)
+    if weights == "untied":
+        g = torch.Generator().manual_seed(4)
+        ctx.set_lm_head_f16((torch.randn(SMALL.vocab, SMALL.hidden, generator=g) * 0.02).half().to(dev))
     try:
         loss = ctx.forward_backward(tok.to(dev), tgt.to(dev))
         want = ctx.lora_get("grad")
