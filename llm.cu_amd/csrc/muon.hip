@@ -20,7 +20,7 @@
 //
 // Bound by HBM where the short side is 16 and matrices are many (the 28-layer
 // Muon step, 128 MB: 26.7 us, 4.8 TB/s, a copy's rate), by the fp64 matrix rate
-// above (28 x 12288 x 64: 4.5 GFLOP, gram 38 us, iteration 43, product 56), by
+// above (28 x 12288 x 64: 4.5 GFLOP, gram 34 us, iteration 42, product 55), by
 // launches and memory round trips for few matrices (1 x 16 x 2048: 10.5 us).
 //
 // All matrices of the iteration are symmetric and commute.  A lane of an f64
@@ -208,9 +208,9 @@ __device__ __forceinline__ void gram_stage(float (*S)[Stage<NT>::LD], doublex4 (
 }
 
 // The stage times P, in its place, rounded.
-template <int NT>
+template <int NT, typename TP>
 __device__ __forceinline__ void apply_stage(float (*S)[Stage<NT>::LD],
-                                            const doublex4 (&P)[NT][NT], int q, int c) {
+                                            const TP& P, int q, int c) {
 #pragma unroll
   for (int k = 0; k < Stage<NT>::KW; k += 16) {
     doublex4 acc[NT];
@@ -222,7 +222,7 @@ __device__ __forceinline__ void apply_stage(float (*S)[Stage<NT>::LD],
       for (int v = 0; v < 4; ++v) {
         const double u = S[k + c][16 * i + 4 * v + q];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j] = mfma64(u, P[i][j][v], acc[j]);
+        for (int j = 0; j < NT; ++j) acc[j] = mfma64(u, P(i, j, v), acc[j]);
       }
     wave_fence();
 #pragma unroll
@@ -259,7 +259,7 @@ __device__ __forceinline__ void k_range(int n, int splits, int b, int& k0, int& 
 
 // G partials of one k range of a matrix: ws.gram[matrix][split][tile][v][lane].
 template <int NT, bool MUON>
-__global__ __launch_bounds__(NTH) void ns_gram_kernel(const NsArgs a) {
+__global__ __launch_bounds__(NTH, 2) void ns_gram_kernel(const NsArgs a) {
   constexpr int KW = Stage<NT>::KW, LD = Stage<NT>::LD;
   __shared__ float S_[NW][KW][LD];
   __shared__ double red[ntri(NT)][256];
@@ -434,7 +434,8 @@ __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a)
 // P U of one k range of a matrix, and with MUON the parameters' update by it
 // (the momentum is already updated).  NT = 1: every workgroup iterates by
 // itself (2 us, during which its first loads arrive), which is less than the
-// launch that it saves.
+// launch that it saves.  Else P is read from LDS as it is used: in registers it
+// left one or two waves a SIMD (28 layers at rank 64: 218 us, 259 so).
 template <int NT, bool MUON>
 __global__ __launch_bounds__(NTH, 2) void ns_apply_kernel(const NsArgs a) {
   constexpr int KW = Stage<NT>::KW, LD = Stage<NT>::LD, PC = Stage<NT>::PC;
@@ -460,9 +461,9 @@ __global__ __launch_bounds__(NTH, 2) void ns_apply_kernel(const NsArgs a) {
     load(k);
     if constexpr (MUON) lo.load(p, a.out + out0, k, k1);
   }
-  doublex4 P[NT][NT];
+  __shared__ double red[NT * NT * 256];  // P; NT = 1: first the sum over the splits
+  doublex4 P1;
   if constexpr (NT == 1) {
-    __shared__ double red[256];  // the sum over the splits, then P
     red[threadIdx.x] = sum_splits(a.gram + (long long)mat * a.splits * 256 + threadIdx.x, a.splits,
                                   256);
     __syncthreads();
@@ -476,16 +477,16 @@ __global__ __launch_bounds__(NTH, 2) void ns_apply_kernel(const NsArgs a) {
     }
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 4; ++v) P[0][0][v] = red[64 * v + lane];
+    for (int v = 0; v < 4; ++v) P1[v] = red[64 * v + lane];
   } else {
     const double* proj = a.proj + (long long)mat * NT * NT * 256;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) P[i][j][v] = proj[(i * NT + j) * 256 + 64 * v + lane];
+    for (int i = 0; i < NT * NT; ++i) red[256 * i + threadIdx.x] = proj[256 * i + threadIdx.x];
+    __syncthreads();
   }
+  auto P = [&](int i, int j, int v) {
+    return NT == 1 ? P1[v] : red[(i * NT + j) * 256 + 64 * v + lane];
+  };
   for (; k < k1; k += KW * NW) {
     wave_fence();
     if constexpr (MUON)
@@ -556,9 +557,10 @@ __global__ __launch_bounds__(FTH) void ns_fused_kernel(const NsArgs a) {
     for (int v = 0; v < 4; ++v) red[64 * v + lane] = P[v];
   }
   __syncthreads();
-  doublex4 P[1][1];
+  doublex4 P1;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) P[0][0][v] = red[64 * v + lane];
+  for (int v = 0; v < 4; ++v) P1[v] = red[64 * v + lane];
+  auto P = [&](int, int, int v) { return P1[v]; };
   for (; k < mt.n; k += FKW * FW) {
     apply_stage<1>(S + k, P, q, c);
     wave_fence();
@@ -568,8 +570,8 @@ __global__ __launch_bounds__(FTH) void ns_fused_kernel(const NsArgs a) {
   }
 }
 
-// Workgroups of the gram and apply launches: two a CU (28 x 12288 x 64: 137 us,
-// 145 with one a CU, 151 with four).
+// Workgroups of the gram and apply launches: two a CU (28 x 12288 x 64: 130 us,
+// 134 with one a CU, 139 with four; 20 x 4096 x 32: 30.4, 30.7, 33.6).
 constexpr int kTargetWg = 512;
 
 // k ranges a matrix, in groups of a stage a wave.
