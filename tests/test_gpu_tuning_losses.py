@@ -190,6 +190,13 @@ def test_policy_loss(dev, n, S, per_seq, use_old, use_ref, use_ent, use_mask, me
         assert p.dentropy is None
 
 
+@pytest.mark.parametrize("n,S", [(120, 1000), (140, 2000)])
+def test_policy_loss_of_many_masked_tokens(dev, n, S):
+    """About 60000 and 140000 tokens: the kept ones are counted by every workgroup, and by
+    a launch of their own."""
+    test_policy_loss(dev, n, S, False, True, True, True, True, "token")
+
+
 def test_policy_gradient_against_differences(dev):
     """As for the preference loss: 2^-24 rounded values over steps of 2^-6 (away from the
     clip borders, where the loss has a corner)."""
