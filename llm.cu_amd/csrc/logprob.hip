@@ -26,6 +26,19 @@ namespace {
 constexpr int NTH = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kFar = -1e4f;  // exp of it is 0
+constexpr float kLeast = -0x1p30f;
+
+// Rows whose largest x is beyond 2^29 (all of a row masked with a large finite
+// value, say): there an fma's x - m keeps the rounding of m, which is more
+// than such logits can differ by without differing altogether.  Their x are
+// rounded before m is subtracted, as m itself was.
+constexpr float kFarRow = 0x1p29f;
+__device__ __forceinline__ bool far_row(float m) { return fabsf(m) > kFarRow && fabsf(m) < INFINITY; }
+__device__ __forceinline__ float far_diff(float logit, float it, float m) {
+#pragma clang fp contract(off)
+  const float x = logit * it;
+  return x - m;
+}
 
 // 16-byte pieces at any alignment of the element: gfx950 takes unaligned
 // global accesses, so rows of an odd length need no peeling.
@@ -49,27 +62,24 @@ struct Piece<__bf16> {
 
 // The statistics are kept in base 2: with y = logits * c, c = it log2 e,
 // (m, s, u) are the largest y, sum 2^(y - m) and sum 2^(y - m) (y - m), each
-// y - m one fma; x is the largest logit itself.  16-bit logits are bound by the VALU as much as by HBM, and
-// this is the fewest instructions an element.  The roundings of m and c are
-// common to a row's terms; finish takes them out of its m, and the rounding of
-// c leaves 2^-24 of each y - m.  The empty set is (-inf, 0, 0), -inf.
+// y - m one fma; x is the largest logit itself.  16-bit logits are bound by the
+// VALU as much as by HBM, and this is the fewest instructions an element.  The
+// roundings of m and c are common to a row's terms; finish takes them out of
+// its m, and the rounding of c leaves 2^-24 of each y - m.  m starts at kLeast
+// and only rises: logits below it (-inf, finite masks) add nothing, every m is
+// finite, and where m >= kLeast the rounding of m moves an exponent by at most
+// 64.  The empty set is (kLeast, 0, 0), -inf.
 struct Stat {
   float m, s, u, x;
 };
-__device__ __forceinline__ Stat empty_stat() { return {-INFINITY, 0.f, 0.f, -INFINITY}; }
-__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ Stat empty_stat() { return {kLeast, 0.f, 0.f, -INFINITY}; }
 template <bool ENT>
 __device__ __forceinline__ void merge(Stat& a, const Stat& b) {
   const float m2 = b.m, s2 = b.s, u2 = b.u;
-  const float mn = fmaxf(a.m, m2), ref = finite_ref(mn);
-  const float d1 = a.m - ref, d2 = m2 - ref;
+  const float mn = fmaxf(a.m, m2);
+  const float d1 = a.m - mn, d2 = m2 - mn;
   const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
-  if constexpr (ENT) {
-    // far below, the factor is 0 and s d has to stay finite (a mask of the
-    // type's lowest value, or an empty side's d = -inf)
-    const float e1 = fmaxf(d1, kFar), e2 = fmaxf(d2, kFar);
-    a.u = f1 * fmaf(a.s, e1, a.u) + f2 * fmaf(s2, e2, u2);
-  }
+  if constexpr (ENT) a.u = f1 * fmaf(a.s, d1, a.u) + f2 * fmaf(s2, d2, u2);
   a.s = a.s * f1 + s2 * f2;
   a.m = mn;
   a.x = fmaxf(a.x, b.x);
@@ -81,17 +91,17 @@ __device__ __forceinline__ void add(Stat& a, const float (&x)[NV], float c) {
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < NV; ++i) mx = fmaxf(mx, x[i]);
-  const float m = fmaxf(a.m, mx * c), ref = finite_ref(m);
-  const float d = a.m - ref, f = __builtin_amdgcn_exp2f(d);
+  const float m = fmaxf(a.m, mx * c);
+  const float d = a.m - m, f = __builtin_amdgcn_exp2f(d);
   float s = 0.f, u = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const float z = fmaf(x[i], c, -ref);
+    const float z = fmaf(x[i], c, -m);
     const float e = __builtin_amdgcn_exp2f(z);
     s += e;
     if constexpr (ENT) u = fmaf(e, fmaxf(z, kFar), u);  // a logit of -inf adds nothing
   }
-  if constexpr (ENT) a.u = fmaf(f, fmaf(a.s, fmaxf(d, kFar), a.u), u);
+  if constexpr (ENT) a.u = fmaf(f, fmaf(a.s, d, a.u), u);
   a.s = fmaf(a.s, f, s);
   a.m = m;
   a.x = fmaxf(a.x, mx);
@@ -109,10 +119,11 @@ __device__ __forceinline__ Stat wave_merge(Stat a) {
 }
 
 // A thread's share of columns [j0, j1) of a row, `nth` threads a row, BATCH
-// logits at a time.
-template <bool ENT, bool NT, int BATCH = 16, typename T>
+// logits at a time.  FAR: of what far_diff makes of them.
+template <bool ENT, bool NT, int BATCH = 16, bool FAR = false, typename T>
 __device__ __forceinline__ void scan(Stat& a, const T* row, int j0, int j1, int tid, int nth,
-                                     float c) {
+                                     float c, float it = 1.f, float m = 0.f) {
+  auto of = [&](T v) { return FAR ? far_diff((float)v, it, m) : (float)v; };
   constexpr int N = Piece<T>::N, U = BATCH / N;
   typedef typename Piece<T>::V Vec;
   const int np = (j1 - j0) / N;
@@ -127,37 +138,51 @@ __device__ __forceinline__ void scan(Stat& a, const T* row, int j0, int j1, int 
     }
     float x[U * N];
 #pragma unroll
-    for (int i = 0; i < U * N; ++i) x[i] = (float)v[i / N][i % N];
+    for (int i = 0; i < U * N; ++i) x[i] = of(v[i / N][i % N]);
     add<ENT, U * N>(a, x, c);
   }
   for (; k < np; k += nth) {
     const Vec v = *reinterpret_cast<const Vec*>(row + j0 + (long long)N * k);
     float x[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = (float)v[e];
+    for (int e = 0; e < N; ++e) x[e] = of(v[e]);
     add<ENT, N>(a, x, c);
   }
   const int j = j0 + N * np + tid;
   if (j < j1) {
-    const float x[1] = {(float)row[j]};
+    const float x[1] = {of(row[j])};
     add<ENT, 1>(a, x, c);
   }
 }
 
-// The row's outputs from its statistics (one thread).
-template <bool ENT>
-__device__ __forceinline__ void finish(const Stat& a, float xt, float it, long long row, float* logp,
-                                       float2* stats, float* entropy) {
-  if (a.m == -INFINITY && a.s == 0.f) {  // every logit is -inf: nothing has any probability
+// The row's outputs from its statistics; all lanes of a wave, with the same `a`.
+template <bool ENT, typename T>
+__device__ __forceinline__ void finish(Stat a, const T* x, int t, int V, float it, long long row,
+                                       float* logp, float2* stats, float* entropy) {
+  const int lane = threadIdx.x & 63;
+  const float m = a.x * it, xt = (float)x[t];
+  const bool far = far_row(m);
+  if (far) {
+    a = empty_stat();
+    scan<ENT, false, Piece<T>::N, true>(a, x, 0, V, lane, 64, kLog2e, it, m);
+    a = wave_merge<ENT>(a);
+  }
+  if (lane) return;
+  if (m == -INFINITY && a.s == 0.f) {  // every x is -inf: nothing has any probability
     logp[row] = -INFINITY;
     stats[row] = make_float2(-INFINITY, 0.f);
     if constexpr (ENT) entropy[row] = 0.f;
     return;
   }
-  // the offset m of the sums in natural units, by the c that they took
-  const double mn = (double)a.m * ((double)it / (double)(it * kLog2e));
-  const float m = a.x * it, ls = logf(a.s), l = ls + (float)(mn - m);
-  logp[row] = fmaf(xt, it, -m) - l;
+  const float ls = logf(a.s);
+  float l = ls;
+  if (far) {
+    logp[row] = far_diff(xt, it, m) - l;
+  } else {
+    // the offset a.m of the sums in natural units, by the c that they took
+    l += (float)((double)a.m * ((double)it / (double)(it * kLog2e)) - m);
+    logp[row] = fmaf(xt, it, -m) - l;
+  }
   stats[row] = make_float2(m, l);
   if constexpr (ENT) entropy[row] = fmaf(-0.69314718f, a.u / a.s, ls);
 }
@@ -171,13 +196,13 @@ __device__ __forceinline__ void no_target(long long row, float* logp, float2* st
   if constexpr (ENT) entropy[row] = 0.f;
 }
 
-// The block's statistics, in thread 0.  Contains a barrier.
+// The block's statistics, in its first wave.  Contains a barrier.
 template <bool ENT, int BLOCK>
 __device__ __forceinline__ Stat block_merge(Stat a, Stat* part) {
   a = wave_merge<ENT>(a);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = a;
   __syncthreads();
-  if (threadIdx.x == 0)
+  if (threadIdx.x < 64)
     for (int w = 1; w < BLOCK / 64; ++w) merge<ENT>(a, part[w]);
   return a;
 }
@@ -201,7 +226,7 @@ __global__ __launch_bounds__(BLOCK) void logprob_row_kernel(const T* __restrict_
     Stat a = empty_stat();
     scan<ENT, NT, BATCH>(a, x, 0, V, threadIdx.x, BLOCK, it * kLog2e);
     a = block_merge<ENT, BLOCK>(a, part);
-    if (threadIdx.x == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
+    if (threadIdx.x < 64) finish<ENT>(a, x, t, V, it, row, logp, stats, entropy);
     __syncthreads();
   }
 }
@@ -226,7 +251,7 @@ __global__ __launch_bounds__(NTH) void logprob_wave_kernel(const T* __restrict__
     Stat a = empty_stat();
     scan<ENT, NT>(a, x, 0, V, lane, 64, it * kLog2e);
     a = wave_merge<ENT>(a);
-    if (lane == 0) finish<ENT>(a, (float)x[t], it, row, logp, stats, entropy);
+    finish<ENT>(a, x, t, V, it, row, logp, stats, entropy);
   }
 }
 
@@ -263,14 +288,13 @@ __global__ __launch_bounds__(64) void logprob_merge_kernel(const T* __restrict__
     if (threadIdx.x == 0) no_target<ENT>(row, logp, stats, entropy);
     return;
   }
-  const float xt = (float)logits[row * ld + t];
   Stat a = empty_stat();
   for (int c = threadIdx.x; c < chunks; c += 64) {
     const float4 p = parts[(long long)row * chunks + c];
     merge<ENT>(a, Stat{p.x, p.y, p.z, p.w});
   }
   a = wave_merge<ENT>(a);
-  if (threadIdx.x == 0) finish<ENT>(a, xt, it, row, logp, stats, entropy);
+  finish<ENT>(a, logits + row * ld, t, V, it, row, logp, stats, entropy);
 }
 
 // 16-byte pieces a lane of the backward: fp32 logits stream best with one
@@ -317,19 +341,24 @@ __global__ __launch_bounds__(NTH) void logprob_bwd_kernel(
     const int j0 = (int)start, j1 = (int)min((long long)V, start + BU * N * 64);
     const T* x = logits + row * ld;
     TO* d = dlogits + row * ldd;
-    auto log_p = [&](float xv) {
-      const float z = fmaf(xv, it, -st.x) - st.y;
-      // exp is 0 far below, and 0 * z has to stay 0
-      return ENT && z < kFar ? kFar : z;
+    // exp is 0 far below, and 0 * z has to stay 0
+    auto log_p = [&](float diff) { return ENT && diff - st.y < kFar ? kFar : diff - st.y; };
+    auto value_of = [&](float z) {
+      return __builtin_amdgcn_exp2f(z * kLog2e) * (ENT ? fmaf(-h, z, gh) : gh);
     };
-    auto value = [&](float xv) {
-      const float z = log_p(xv), p = __builtin_amdgcn_exp2f(z * kLog2e);
-      return p * (ENT ? fmaf(-h, z, gh) : gh);
-    };
-    auto at_target = [&](float xv) {  // g (1 - p) without the cancellation
-      const float z = log_p(xv), p = __builtin_amdgcn_exp2f(z * kLog2e), dg = -g * expm1f(z);
+    auto target_of = [&](float z) {  // g (1 - p) without the cancellation
+      const float p = __builtin_amdgcn_exp2f(z * kLog2e), dg = -g * expm1f(z);
       return ENT ? fmaf(-h * p, z + entropy[row], dg) : dg;
     };
+    auto value = [&](float xv) { return value_of(log_p(fmaf(xv, it, -st.x))); };
+    auto at_target = [&](float xv) { return target_of(log_p(fmaf(xv, it, -st.x))); };
+    if (!FACTOR && !zero && far_row(st.x)) {
+      for (int j = j0 + lane; j < j1; j += 64) {
+        const float z = log_p(far_diff((float)x[j], it, st.x));
+        d[j] = (TO)(j == t ? target_of(z) : value_of(z));
+      }
+      continue;
+    }
     const int np = (j1 - j0) / N;
     Vec v[BU];
     if (!zero)

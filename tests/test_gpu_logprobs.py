@@ -186,6 +186,66 @@ def test_masked_logits(dev, dtype, V):
         assert (d[masked] == 0).all()
 
 
+@pytest.mark.parametrize("mask", [-1e4, -2e8, -1e9, -1e10, -3e12, -1e20, -1e30, -3e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows,V", [(4, 1500), (4, 30000), (4, 230000), (300, 4001)])
+def test_finite_masks(dev, rows, V, dtype, mask):
+    """Masks of large finite values: whole stretches of a row, all of a row but one logit, and
+    all of a row, which leaves its logits equal and every probability 1 / V; logits that are
+    large and positive.  (Sizes where the product with the inverse temperature is off by more
+    than the logits of a softmax differ.)"""
+    g, x, t = problem(rows, V, dtype, seed=11, skip=0.0)
+    x[0, V // 3:] = mask
+    x[1] = mask
+    x[1, V // 2] = 1.0
+    x[2] = mask
+    x[3, :] = -mask
+    x[3, V // 4:] = mask
+    t[0], t[1], t[2], t[3] = 5, V // 2, V - 1, 0
+    dlogp, dent = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    for temperature in (1.0, 0.9, 1.7):
+        if abs(mask) > 2e38 and temperature < 1:
+            continue                      # the scaled logits leave fp32
+        got = llmt.token_logprobs(x.to(dev), t.to(dev), temperature, want_entropy=True)
+        check_forward(x, t, got, temperature)
+        want, lg, ent, _ = forward64(x, t, temperature)
+        assert abs(float(got[0][2]) + math.log(V)) <= 1e-5 and abs(float(got[2][2]) - math.log(V)) <= 1e-4
+        # the gradient by the formula, from probabilities in float64
+        it = float(torch.tensor(1.0 / temperature, dtype=torch.float32))
+        p = lg.exp()
+        lz = torch.where(p > 0, lg, torch.zeros_like(lg))
+        hot = torch.nn.functional.one_hot(t.long(), V).double()
+        for e in (None, dent):
+            d = llmt.token_logprobs_bwd(x.to(dev), t.to(dev), got[1], dlogp.to(dev), got[2],
+                                        None if e is None else e.to(dev), temperature).cpu().double()
+            a = dlogp.double()[:, None] * it
+            ref, size = a * (hot - p), a.abs() * torch.where(hot > 0, (hot - p).abs() + p, p)
+            if e is not None:
+                b = e.double()[:, None] * it
+                ref, size = ref - b * p * (lz + ent[:, None]), size + b.abs() * p * (lz.abs() + ent[:, None])
+            # p and the entropy are off as in the forward; one rounding
+            tol = size * (sum_tol(V) * 4 * (2 + math.log(V)) + (lz.abs() + 4) * 8 * U)
+            tol = tol + (ref.abs() + tol) * torch.finfo(dtype).eps / 2 + SUBNORMAL[dtype]
+            if e is not None:             # H where it all but vanishes: its absolute error
+                tol = tol + b.abs() * p * sum_tol(V) * 2 * (2 + math.log(V))
+            assert ((d - ref).abs() <= tol).all(), float(((d - ref).abs() - tol).max())
+
+
+@pytest.mark.parametrize("V", [100, 9000, 230000])
+def test_scaled_logits_that_leave_fp32(dev, V):
+    """Masks that the inverse temperature takes to -inf are -inf."""
+    g, x, t = problem(3, V, torch.float32, seed=12, skip=0.0)
+    x[0, 50:] = torch.finfo(torch.float32).min
+    t[0] = 3
+    x[1] = torch.finfo(torch.float32).min
+    lp, st, ent = (v.cpu() for v in llmt.token_logprobs(x.to(dev), t.to(dev), 0.5, want_entropy=True))
+    check_forward(x[[0, 2]], t[[0, 2]], tuple(v[[0, 2]] for v in (lp, st, ent)), 0.5)
+    assert lp[1] == -math.inf and st[1].tolist() == [-math.inf, 0.0] and ent[1] == 0
+    one = torch.ones(3, device=dev)
+    d = llmt.token_logprobs_bwd(x.to(dev), t.to(dev), st.to(dev), one, ent.to(dev), one, 0.5).cpu()
+    assert (d[1] == 0).all() and torch.isfinite(d).all() and (d[0, 50:] == 0).all()
+
+
 def test_a_bad_logit_stays_in_its_row(dev):
     g, x, t = problem(6, 20000, torch.float32, seed=4, skip=0.0)
     x[1, 777], x[3, 19999], x[4] = math.nan, math.inf, math.nan
