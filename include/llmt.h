@@ -414,8 +414,9 @@ int llmt_token_logprobs_bwd(const void* logits, int dtype, long long ld, const i
  * of any function of them from dlogp, its gradient: the adapter gradients go
  * to the GRAD arena (overwritten), for llmt_adamw or llmt_muon.  The backward
  * takes the stashes of the last forward and fails with LLMT_ERR_STATE if that
- * was not llmt_forward_logprobs'; it may be called more than once.  tokens,
- * targets, batch as in llmt_step; one host synchronisation each. */
+ * was not llmt_forward_logprobs' or if weights or adapters have been set or
+ * updated since; it may be called more than once.  tokens, targets, batch as
+ * in llmt_step; one host synchronisation each. */
 int llmt_forward_logprobs(llmt_ctx* ctx, const int* tokens, const int* targets, int batch,
                           float* logp);
 int llmt_backward_logprobs(llmt_ctx* ctx, const float* dlogp);

@@ -275,6 +275,7 @@ static hipError_t put_i8(Ctx* c, const int8_t* src, const void* scale, int rows,
 static int put_norms(Ctx* c, Layer& w, const float* attn_norm, const float* ffn_norm,
                      const float* q_norm, const float* k_norm) {
   TRY_ARG(attn_norm && ffn_norm && q_norm && k_norm, "norm weights must be given");
+  c->logp_batch = 0;
   TRY_HIP(hipMemcpyAsync(w.attn_norm, attn_norm, c->H * 4, hipMemcpyDefault, c->st));
   TRY_HIP(hipMemcpyAsync(w.ffn_norm, ffn_norm, c->H * 4, hipMemcpyDefault, c->st));
   TRY_HIP(hipMemcpyAsync(w.q_norm, q_norm, kHeadDim * 4, hipMemcpyDefault, c->st));
@@ -338,6 +339,7 @@ int llmt_set_embed_f16(llmt_ctx* ctx, const void* embed_lm_head, const float* fi
   set_error("");
   Ctx* c = C_(ctx);
   TRY_ARG(c && embed_lm_head && final_norm, "llmt_set_embed_f16: NULL argument");
+  c->logp_batch = 0;
   const _Float16* e = (const _Float16*)embed_lm_head;
   TRY_HIP(pack_f16(e, c->H, 0, c->V, c->H, c->E, c->H, 0, 0, c->st));
   TRY_HIP(pack_f16(e, c->H, 1, c->H, c->V, c->ET, c->V, 0, 0, c->st));
@@ -360,6 +362,7 @@ int llmt_set_lm_head_f16(llmt_ctx* ctx, const void* lm_head) {
   set_error("");
   Ctx* c = C_(ctx);
   TRY_ARG(c && lm_head, "llmt_set_lm_head_f16: NULL argument");
+  c->logp_batch = 0;
   if (!c->head_own) {
     _Float16* eh = c->alloc_n<_Float16>((size_t)c->V * c->H);
     _Float16* eht = eh ? c->alloc_n<_Float16>((size_t)c->V * c->H) : nullptr;

@@ -142,7 +142,8 @@ struct Ctx {
   float2* ce_stats = nullptr;  // [Tmax, ce_stats_per_row(V)]: CE chunk or logits-tile pairs
   float* lse_rows = nullptr;   // [Tmax]
   float2* logp_stats = nullptr;  // [Tmax]: llmt_forward_logprobs' softmax statistics
-  int logp_batch = 0;            // > 0: the stashes are that call's, of this batch
+  int logp_batch = 0;            // > 0: the stashes are that call's, of this batch, and the
+                               // weights and adapters still those that made them
   int head_tiles = 0;          // > 0: the last forward's logits GEMM wrote its tile pairs
   float* loss_rows = nullptr;
   float* loss_dev = nullptr;

@@ -551,6 +551,7 @@ hipError_t Ctx::backward(int B, int accumulate, const float* row_factor) {
 }
 
 hipError_t Ctx::optimizer() {
+  logp_batch = 0;
   float *p = lora_p, *g = lora_g, *m = lora_m, *v = lora_v;
   const long long n = (long long)lora_numel;
   const AdamHp* hp = hp_dev;
@@ -562,6 +563,7 @@ hipError_t Ctx::optimizer() {
 }
 
 hipError_t Ctx::refresh_shadows() {
+  logp_batch = 0;
   LLMT_HIP_TRY(adamw(lora_p, nullptr, nullptr, nullptr, (long long)lora_numel, hp_dev, 0,
                      shadow_desc(), st));
   return hipSuccess;
@@ -679,6 +681,7 @@ int llmt_lora_init(llmt_ctx* ctx, uint64_t seed, float a_std, float b_std) {
   set_error("");
   Ctx* c = C_(ctx);
   TRY_ARG(c, "llmt_lora_init: NULL ctx");
+  c->logp_batch = 0;
   TRY_HIP(lora_init(c->lora_p, c->lora_m, c->lora_v, (long long)c->lora_numel, seed, a_std, b_std,
                     c->shadow_desc(), c->st));
   TRY_HIP(hipMemsetAsync(c->lora_g, 0, c->lora_numel * sizeof(float), c->st));

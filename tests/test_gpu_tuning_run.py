@@ -172,6 +172,32 @@ def test_context_order_of_calls(dev):
         ctx.close()
 
 
+def test_context_refuses_a_backward_through_other_weights(dev):
+    """Weights or adapters that changed after the forward are not those of its stashes."""
+    W, ad, tok, tgt = small_problem()
+    B, S = tok.shape
+    ctx = context(dev, W, ad, B, S)
+    tok, tgt = tok.to(dev), tgt.to(dev)
+    d = torch.zeros(B * S, device=dev)
+    L = llmt.lib()
+    emb, norm = W.embed.half().to(dev), W.final_norm.float().to(dev)
+    try:
+        for other in (lambda: llmt.check(L.llmt_adamw(ctx.h, C.byref(llmt.hparams()), 1)),
+                      lambda: ctx.muon(llmt.muon_hparams()),
+                      lambda: ctx.lora_set("param", llmt.flatten_adapters(ad).to(dev)),
+                      lambda: llmt.check(L.llmt_lora_init(ctx.h, 1, 0.02, 0.0)),
+                      lambda: ctx.set_embed_f16(emb, norm),
+                      lambda: ctx.set_lm_head_f16(emb)):
+            ctx.forward_logprobs(tok, tgt)
+            ctx.backward_logprobs(d)
+            ctx.lora_set("grad", ctx.lora_get("grad"))
+            ctx.backward_logprobs(d)
+            other()
+            assert L.llmt_backward_logprobs(ctx.h, llmt.ptr(d)) == llmt.LLMT_ERR_STATE
+    finally:
+        ctx.close()
+
+
 def test_preference_step(dev):
     """Two pairs of answers: the reference's log-probabilities with the adapters off, the
     policy's with them on, the loss, the backward and two Muon steps."""
