@@ -17,7 +17,6 @@ Kinds (every one through the public `llmt` binding when `own` is true):
 The plain forms compute in 32 bits, and in 64 where 32 lose what matters: the sums over a
 sequence, and the ratios that are compared with the clip borders.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -42,7 +41,6 @@ def f32(x):
     return float(np.float32(x))
 
 
-@functools.cache
 def _llmt():
     root = str(Path(__file__).resolve().parents[1] / "llm.cu_amd")
     if root not in sys.path:
