@@ -224,7 +224,9 @@ int llmt_policy_loss(const float* logp, const float* old_logp, const float* ref_
                      float* stats, float* dlogp, float* dentropy, void* workspace,
                      size_t workspace_bytes, void* stream) {
   set_error("");
-  TRY_ARG(p && offsets && loss && stats && ((logp && advantages) || T == 0),
+  // advantages a sequence are read for every sequence, without tokens too
+  TRY_ARG(p && offsets && loss && stats && (logp || T == 0) &&
+              (advantages || (T == 0 && !p->adv_per_sequence)),
           "llmt_policy_loss: NULL argument");
   TRY_ARG(T >= 0 && n >= 1 && n <= (1 << 29), "llmt_policy_loss: T=%d n=%d", T, n);
   TRY_ARG(p->mean == LLMT_MEAN_TOKEN || p->mean == LLMT_MEAN_SEQUENCE, "llmt_policy_loss: mean %d",
