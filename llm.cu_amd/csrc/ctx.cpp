@@ -274,8 +274,6 @@ static hipError_t put_i8(Ctx* c, const int8_t* src, const void* scale, int rows,
 
 static int put_norms(Ctx* c, Layer& w, const float* attn_norm, const float* ffn_norm,
                      const float* q_norm, const float* k_norm) {
-  TRY_ARG(attn_norm && ffn_norm && q_norm && k_norm, "norm weights must be given");
-  c->logp_batch = 0;
   TRY_HIP(hipMemcpyAsync(w.attn_norm, attn_norm, c->H * 4, hipMemcpyDefault, c->st));
   TRY_HIP(hipMemcpyAsync(w.ffn_norm, ffn_norm, c->H * 4, hipMemcpyDefault, c->st));
   TRY_HIP(hipMemcpyAsync(w.q_norm, q_norm, kHeadDim * 4, hipMemcpyDefault, c->st));
@@ -294,6 +292,8 @@ int llmt_set_layer_f16(llmt_ctx* ctx, int layer, const void* wq, const void* wk,
   TRY_ARG(c && layer >= 0 && layer < c->L, "llmt_set_layer_f16: bad ctx/layer");
   TRY_ARG(c->wfmt == LLMT_WEIGHTS_F16, "context was created for int8 weights");
   TRY_ARG(wq && wk && wv && wo && w_gate && w_up && w_down, "NULL weight");
+  TRY_ARG(attn_norm && ffn_norm && q_norm && k_norm, "norm weights must be given");
+  c->logp_batch = 0;
   Layer& w = c->layers[layer];
   const int H = c->H, Q = c->Q, KV = c->KV, I = c->I;
   TRY_HIP(put_f16(c, wq, Q, H, w.wqkv, 0, w.wqkvT));
@@ -319,6 +319,8 @@ int llmt_set_layer_i8(llmt_ctx* ctx, int layer, const int8_t* const q[7],
   TRY_ARG(c->wfmt == LLMT_WEIGHTS_I8, "context was created for fp16 weights");
   TRY_ARG(q && scale, "NULL weight array");
   for (int i = 0; i < 7; ++i) TRY_ARG(q[i] && scale[i], "NULL weight %d", i);
+  TRY_ARG(attn_norm && ffn_norm && q_norm && k_norm, "norm weights must be given");
+  c->logp_batch = 0;
   Layer& w = c->layers[layer];
   const int H = c->H, Q = c->Q, KV = c->KV, I = c->I;
   TRY_HIP(put_i8(c, q[0], scale[0], Q, H, w.wqkv, 0, w.wqkvT));

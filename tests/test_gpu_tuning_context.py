@@ -1,0 +1,71 @@
+"""GPU: log-probabilities and Muon on a context, where calls meet that do not belong
+together: refused weights, other streams, another optimiser's state."""
+import copy
+import ctypes as C
+
+import pytest
+import torch
+
+import llmt
+from helpers import SMALL, small_problem, upload_model
+from oracle.configs import quantize_model_int8
+
+pytestmark = pytest.mark.gpu
+
+
+def context(dev, W, ad, batch, seq_len, stream=None):
+    ctx = llmt.Context(llmt.make_dims(SMALL), max_batch=batch, seq_len=seq_len, stream=stream)
+    upload_model(ctx, W, dev)
+    ctx.lora_set("param", llmt.flatten_adapters(ad).to(dev))
+    return ctx
+
+
+@pytest.mark.parametrize("weights", ["f16", "i8"])
+def test_layer_setters_and_the_backward(dev, weights):
+    """A setter that refuses its arguments changes nothing; one that takes them ends the
+    stashes of the last forward."""
+    W, ad, tok, tgt = small_problem()
+    B, S = tok.shape
+    tok, tgt = tok.to(dev), tgt.to(dev)
+    L = llmt.lib()
+    f = lambda t: t.float().to(dev).contiguous()
+    norms = [f(t) for t in (W.layers[0].attn_norm, W.layers[0].ffn_norm, W.layers[0].q_norm,
+                            W.layers[0].k_norm)]
+    names = ("wq", "wk", "wv", "wo", "w_gate", "w_up", "w_down")
+    if weights == "i8":
+        W, qs = quantize_model_int8(copy.deepcopy(W))
+        ctx = llmt.Context(llmt.make_dims(SMALL), B, S, int8=True)
+        q = [[torch.from_numpy(qs[(l, n)][0]).to(dev) for n in names] for l in range(2)]
+        s = [[torch.from_numpy(qs[(l, n)][1]).to(dev) for n in names] for l in range(2)]
+
+        def put(l, norms, of=None):
+            of = l if of is None else of
+            arr = lambda ts: (llmt.vp * 7)(*(t.data_ptr() for t in ts))
+            return L.llmt_set_layer_i8(ctx.h, l, arr(q[of]), arr(s[of]), *map(llmt.ptr, norms))
+    else:
+        ctx = llmt.Context(llmt.make_dims(SMALL), B, S)
+        h = [[getattr(lw, n).half().to(dev).contiguous() for n in names] for lw in W.layers]
+
+        def put(l, norms, of=None):
+            return L.llmt_set_layer_f16(ctx.h, l, *map(llmt.ptr, h[l if of is None else of]),
+                                        *map(llmt.ptr, norms))
+    try:
+        assert put(0, norms) == 0 and put(1, norms) == 0
+        ctx.set_embed_f16(W.embed.half().to(dev), f(W.final_norm))
+        ctx.lora_set("param", llmt.flatten_adapters(ad).to(dev))
+        d = torch.linspace(-1, 1, B * S, device=dev)
+        want = ctx.forward_logprobs(tok, tgt)
+        ctx.backward_logprobs(d)
+        grad = ctx.lora_get("grad")
+        for k in range(4):
+            bad = list(norms)
+            bad[k] = None
+            assert put(0, bad, of=1) == llmt.LLMT_ERR_ARG      # the other layer's matrices
+            ctx.backward_logprobs(d)
+            assert torch.equal(ctx.lora_get("grad"), grad)
+            assert torch.equal(ctx.forward_logprobs(tok, tgt), want)
+        assert put(1, norms) == 0
+        assert L.llmt_backward_logprobs(ctx.h, llmt.ptr(d)) == llmt.LLMT_ERR_STATE
+        assert torch.equal(ctx.forward_logprobs(tok, tgt), want)
+    finally:
+        ctx.close()
