@@ -416,7 +416,9 @@ int llmt_token_logprobs_bwd(const void* logits, int dtype, long long ld, const i
  * takes the stashes of the last forward and fails with LLMT_ERR_STATE if that
  * was not llmt_forward_logprobs' or if weights or adapters have been set or
  * updated since; it may be called more than once.  tokens, targets, batch as
- * in llmt_step; one host synchronisation each. */
+ * in llmt_step; one host synchronisation each.  They run on the context's
+ * stream: what other streams write into their inputs has to be finished, or
+ * ordered before that stream, when they are called. */
 int llmt_forward_logprobs(llmt_ctx* ctx, const int* tokens, const int* targets, int batch,
                           float* logp);
 int llmt_backward_logprobs(llmt_ctx* ctx, const float* dlogp);

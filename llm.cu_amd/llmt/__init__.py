@@ -525,9 +525,17 @@ def hparams(lr=3e-4, beta1=0.9, beta2=0.999, eps=1e-8, wd=0.01) -> HParams:
 
 class Context:
     """One llmt_ctx: frozen weights, adapters, stashes and workspaces of the
-    LoRA training step for up to ``max_batch`` sequences of ``seq_len``."""
+    LoRA training step for up to ``max_batch`` sequences of ``seq_len``.
+
+    The library works on ``stream`` (None: one of the context's own, ordered
+    with the legacy default stream).  Calls that take or give tensors first
+    wait for torch's current stream where it is neither of these, and all end
+    with a host synchronisation: tensors are used as they are at the call,
+    whatever stream is current."""
 
     def __init__(self, dims: Dims, max_batch: int, seq_len: int, int8: bool = False, stream=None):
+        import torch
+        self.h = None
         self.dims = dims
         self.max_batch = max_batch
         self.seq_len = seq_len
@@ -537,6 +545,17 @@ class Context:
         check(lib().llmt_ctx_create(C.byref(dims), max_batch, seq_len, 1 if int8 else 0, sp,
                                     C.byref(h)))
         self.h = h
+        # the stream that needs no wait (0: the legacy default stream)
+        self._stream = 0 if stream is None else stream.cuda_stream
+        self._device = torch.cuda.current_device() if stream is None else stream.device_index
+
+    def _follow(self):
+        """Puts the context's stream behind torch's current one."""
+        import torch
+        if torch.cuda.is_initialized():
+            at = torch.cuda.current_stream(self._device)
+            if at.cuda_stream != self._stream:
+                at.synchronize()
 
     def close(self):
         if self.h:
@@ -556,20 +575,24 @@ class Context:
     # -- weights
     def set_layer_f16(self, layer, wq, wk, wv, wo, w_gate, w_up, w_down, attn_norm, ffn_norm,
                       q_norm, k_norm):
+        self._follow()
         check(lib().llmt_set_layer_f16(self.h, layer, *(ptr(t) for t in (
             wq, wk, wv, wo, w_gate, w_up, w_down, attn_norm, ffn_norm, q_norm, k_norm))))
 
     def set_layer_i8(self, layer, qs, scales16, attn_norm, ffn_norm, q_norm, k_norm):
+        self._follow()
         qa = (vp * 7)(*(t.data_ptr() for t in qs))
         sa = (vp * 7)(*(t.data_ptr() for t in scales16))
         check(lib().llmt_set_layer_i8(self.h, layer, qa, sa, ptr(attn_norm), ptr(ffn_norm),
                                       ptr(q_norm), ptr(k_norm)))
 
     def set_embed_f16(self, embed, final_norm):
+        self._follow()
         check(lib().llmt_set_embed_f16(self.h, ptr(embed), ptr(final_norm)))
 
     def set_lm_head_f16(self, lm_head):
         """An untied lm_head [V, H] fp16 (llmt_set_lm_head_f16)."""
+        self._follow()
         check(lib().llmt_set_lm_head_f16(self.h, ptr(lm_head)))
 
     def load_weights_dir(self, path):
@@ -588,11 +611,13 @@ class Context:
         """Copy a flat fp32 tensor (device or host) into an arena."""
         flat = flat.contiguous()
         assert flat.numel() == self.lora_numel and flat.dtype.is_floating_point
+        self._follow()
         check(lib().llmt_lora_copy(self.h, KIND[kind], ptr(flat), 1))
 
     def lora_get(self, kind: str, device="cuda"):
         import torch
         out = torch.empty(self.lora_numel, dtype=torch.float32, device=device)
+        self._follow()
         check(lib().llmt_lora_copy(self.h, KIND[kind], ptr(out), 0))
         return out
 
@@ -639,6 +664,7 @@ class Context:
 
     def step(self, tokens, targets, hp: HParams, step: int) -> float:
         B = self._check_tokens(tokens, targets)
+        self._follow()
         loss = C.c_float()
         check(lib().llmt_step(self.h, ptr(tokens), ptr(targets), B, C.byref(hp), step,
                               C.byref(loss)))
@@ -646,6 +672,7 @@ class Context:
 
     def forward_backward(self, tokens, targets) -> float:
         B = self._check_tokens(tokens, targets)
+        self._follow()
         loss = C.c_float()
         check(lib().llmt_forward_backward(self.h, ptr(tokens), ptr(targets), B, C.byref(loss)))
         return loss.value
@@ -676,13 +703,20 @@ class Context:
                                         "data": (addr, False), "version": 3, "strides": None}
         return torch.as_tensor(_View(), device="cuda").clone()
 
+    def _on_device(self, name, t):
+        if t.get_device() != self._device:
+            raise LlmtError(f"{name} is on device {t.get_device()}, the context on {self._device}")
+
     def forward_logprobs(self, tokens, targets):
         """The forward's log-probability of every target, fp32 [B * seq_len]
         (0 where the target is outside [0, V)); backward_logprobs then takes
         the gradient of any function of them (llmt_forward_logprobs)."""
         import torch
         B = self._check_tokens(tokens, targets)
+        self._on_device("tokens", tokens)
+        self._on_device("targets", targets)
         logp = torch.empty(B * self.seq_len, dtype=torch.float32, device=tokens.device)
+        self._follow()
         check(lib().llmt_forward_logprobs(self.h, ptr(tokens), ptr(targets), B, ptr(logp)))
         self.logp_rows = B * self.seq_len
         return logp
@@ -693,7 +727,9 @@ class Context:
         import torch
         if not (isinstance(dlogp, torch.Tensor) and dlogp.is_cuda):
             raise LlmtError("dlogp must be a device tensor")
+        self._on_device("dlogp", dlogp)
         _expect("dlogp", dlogp, torch.float32, self.logp_rows)
+        self._follow()
         check(lib().llmt_backward_logprobs(self.h, ptr(dlogp)))
 
     def muon(self, hp: MuonParams):
@@ -708,6 +744,7 @@ class Context:
         dl = torch.empty(T, self.dims.vocab, dtype=torch.float32, device=hidden16.device) \
             if want_dlogits else None
         dh = torch.empty(T, self.dims.hidden, dtype=torch.float32, device=hidden16.device)
+        self._follow()
         check(lib().llmt_head_ce(self.h, ptr(hidden16), ptr(targets), T // self.seq_len,
                                  C.byref(loss), ptr(dl), ptr(dh)))
         return loss.value, dl, dh
@@ -715,12 +752,14 @@ class Context:
     def layer_forward(self, layer, x, batch):
         import torch
         y = torch.empty_like(x)
+        self._follow()
         check(lib().llmt_layer_forward(self.h, layer, ptr(x), ptr(y), batch))
         return y
 
     def layer_backward(self, layer, dy, batch):
         import torch
         dx = torch.empty_like(dy)
+        self._follow()
         check(lib().llmt_layer_backward(self.h, layer, ptr(dy), ptr(dx), batch))
         return dx
 
@@ -735,6 +774,7 @@ class Context:
         cats, nl = (C.c_int * mx)(), (C.c_int * mx)()
         us = (C.c_float * mx)()
         fl, by = (C.c_double * mx)(), (C.c_double * mx)()
+        self._follow()
         check(lib().llmt_profile_kernels(self.h, ptr(tokens), ptr(targets),
                                          self._check_tokens(tokens, targets), C.byref(hp), step,
                                          reps, mx, C.byref(ns), names, cats, nl, us, fl, by))

@@ -69,3 +69,60 @@ def test_layer_setters_and_the_backward(dev, weights):
         assert torch.equal(ctx.forward_logprobs(tok, tgt), want)
     finally:
         ctx.close()
+
+
+def busy(seconds=0.03):
+    """Work of about that long on the current stream."""
+    a = torch.zeros(4096, 4096, device="cuda")
+    for _ in range(int(seconds / 1e-3)):
+        torch.mm(a, a, out=torch.empty_like(a))
+
+
+@pytest.mark.parametrize("where", ["side", "given", "same"])
+def test_calls_follow_the_current_stream(dev, where):
+    """A preference step where torch's current stream, the context's or both are a stream
+    that nothing else is ordered with, and inputs are written late: as on the default one."""
+    W, ad, tok, tgt = small_problem()
+    B, S = tok.shape
+    flat = llmt.flatten_adapters(ad).to(dev)
+    tok, tgt = tok.to(dev), tgt.to(dev)
+    offsets = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=dev)
+    ref_lp = torch.full((B * S,), -7.0, device=dev)
+
+    def step(ctx, late):
+        def now(t):                               # t, written as late as its stream gets to it
+            if not late:
+                return t
+            x = torch.zeros_like(t)
+            torch.cuda.current_stream().synchronize()
+            busy()
+            return x.copy_(t)
+
+        ctx.lora_set("param", now(flat))
+        lp = ctx.forward_logprobs(now(tok), now(tgt))
+        if late:
+            busy()
+        d = llmt.preference_loss(lp, ref_lp, offsets, beta=0.5)[3]
+        ctx.backward_logprobs(now(d))
+        grad = ctx.lora_get("grad")
+        logits = ctx.logits(B * S)
+        loss = ctx.forward_backward(now(tok), now(tgt))
+        return lp, d, grad, logits, torch.tensor(loss)
+
+    ctx = context(dev, W, ad, B, S)
+    try:
+        want = step(ctx, False)
+        torch.cuda.synchronize()
+    finally:
+        ctx.close()
+    side = torch.cuda.Stream()
+    ctx = context(dev, W, ad, B, S, stream=None if where == "side" else side)
+    try:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.default_stream() if where == "given" else side):
+            got = step(ctx, True)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    finally:
+        ctx.close()
