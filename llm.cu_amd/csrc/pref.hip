@@ -255,7 +255,7 @@ __device__ __forceinline__ Quad load_quad(const PolicyArgs& a, long long t, int 
   const f4u zero = {0.f, 0.f, 0.f, 0.f};
   Quad x;
   x.lp = load4(a.logp, t, have);
-  x.old = a.old ? load4(a.old, t, have) : x.lp;
+  x.old = a.old ? load4(a.old, t, have) : zero;
   x.ref = a.ref ? load4(a.ref, t, have) : zero;
   x.adv = a.adv_per_seq ? zero : load4(a.adv, t, have);
   x.ent = a.entropy ? load4(a.entropy, t, have) : zero;
@@ -266,7 +266,8 @@ __device__ __forceinline__ Quad load_quad(const PolicyArgs& a, long long t, int 
 // clipped); returns the gradient by its log-probability.
 __device__ __forceinline__ float policy_token(const PolicyArgs& a, const Quad& x, int e,
                                               double adv, double w, double (&v)[4]) {
-  const double lp = x.lp[e], ratio = exp(lp - (double)x.old[e]);
+  // without an old policy the ratio is 1, of a log-probability of -inf too
+  const double lp = x.lp[e], ratio = a.old ? exp(lp - (double)x.old[e]) : lp != lp ? lp : 1.0;
   const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
   const double s1 = ratio * adv, s2 = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
   const bool clip = s1 > s2;

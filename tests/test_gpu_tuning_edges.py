@@ -1,0 +1,51 @@
+"""GPU: the preference and policy losses where a token is impossible, where exponentials
+leave their range, at every kernel's borders and far above its grid, against float64.
+
+The kernels compute in fp64 and round each output once to fp32 (half a step, 2^-24 of
+itself); the mean preference loss is a mean of rounded losses, one more half step."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import llmt
+from test_gpu_tuning_losses import close, f32, ragged
+from test_gpu_tuning_losses import test_policy_loss as check_policy_loss
+
+pytestmark = pytest.mark.gpu
+INF = math.inf
+
+# sequences and their longest length that take one workgroup, tiles of tokens, and a wave
+# or a workgroup a sequence
+SHAPES = [(3, 40), (3000, 5), (40, 700), (800, 300)]
+
+
+def weights(off, keep, mean):
+    """The weight of every token in the two means, in float64."""
+    n = len(off) - 1
+    if mean == "token":
+        return keep.double() / max(1, int(keep.sum()))
+    seq = torch.repeat_interleave(torch.arange(n), (off[1:] - off[:-1]).long())
+    kept = torch.zeros(n, dtype=torch.double).index_add(0, seq, keep.double())
+    return keep.double() / (kept.clamp(min=1)[seq] * n)
+
+
+@pytest.mark.parametrize("mean", ["token", "sequence"])
+@pytest.mark.parametrize("n,S", SHAPES)
+def test_policy_without_an_old_one_at_impossible_tokens(dev, n, S, mean):
+    """old_logp None: the ratio is 1 whatever the log-probability, -inf too; NaN stays NaN."""
+    g = torch.Generator().manual_seed(n + S)
+    off, T = ragged(g, n, S)
+    lp, adv = -torch.rand(T, generator=g), torch.randn(T, generator=g)
+    lp[torch.rand(T, generator=g) < 0.2] = -INF
+    lp[T // 2] = -INF
+    w = weights(off, torch.ones(T, dtype=torch.bool), mean)
+    p = llmt.policy_loss(lp.to(dev), None, adv.to(dev), off.to(dev), mean=mean)
+    want = -(adv.double() * w)
+    close(p.loss, want.sum().reshape(1))
+    close(p.stats, torch.stack([want.sum(), 0 * want[0], 0 * want[0]]))
+    close(p.dlogp, want)
+    lp[T // 2] = math.nan
+    p = llmt.policy_loss(lp.to(dev), None, adv.to(dev), off.to(dev), mean=mean)
+    assert p.loss.isnan() and p.dlogp[T // 2].isnan() and int(p.dlogp.isnan().sum()) == 1
