@@ -262,20 +262,28 @@ __device__ __forceinline__ Quad load_quad(const PolicyArgs& a, long long t, int 
   return x;
 }
 
+// exp(v) and exp(v) - 1 beyond fp64 are its largest number instead: times a
+// factor of 0 (an advantage, the KL's coefficient) they count nothing, times any
+// other they are beyond fp32.  (NaN stays.)
+__device__ __forceinline__ double bounded(double v) {
+  return v > __DBL_MAX__ ? __DBL_MAX__ : v;
+}
+
 // Adds token e of the quad with weight w to the sums (loss, policy term, KL,
 // clipped); returns the gradient by its log-probability.
 __device__ __forceinline__ float policy_token(const PolicyArgs& a, const Quad& x, int e,
                                               double adv, double w, double (&v)[4]) {
   // without an old policy the ratio is 1, of a log-probability of -inf too
-  const double lp = x.lp[e], ratio = a.old ? exp(lp - (double)x.old[e]) : lp != lp ? lp : 1.0;
+  const double lp = x.lp[e];
+  const double ratio = a.old ? bounded(exp(lp - (double)x.old[e])) : lp != lp ? lp : 1.0;
   const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
   const double s1 = ratio * adv, s2 = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
   const bool clip = s1 > s2;
   const double pg = -(clip ? s2 : s1);
   double grad = clip ? 0.0 : -s1, loss = pg, kl = 0.0;
   if (a.ref) {
-    const double d = (double)x.ref[e] - lp, em = expm1(d);
-    kl = em - d;
+    const double d = (double)x.ref[e] - lp, em = bounded(expm1(d));
+    kl = em < __DBL_MAX__ ? bounded(em - d) : em;
     loss += a.kl_coef * kl;
     grad -= a.kl_coef * em;
   }

@@ -49,3 +49,43 @@ def test_policy_without_an_old_one_at_impossible_tokens(dev, n, S, mean):
     lp[T // 2] = math.nan
     p = llmt.policy_loss(lp.to(dev), None, adv.to(dev), off.to(dev), mean=mean)
     assert p.loss.isnan() and p.dlogp[T // 2].isnan() and int(p.dlogp.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("mean", ["token", "sequence"])
+@pytest.mark.parametrize("n,S", SHAPES)
+def test_policy_terms_beyond_exps_range(dev, n, S, mean):
+    """A ratio or a KL that leaves fp64 counts nothing where its factor is 0, and +inf where
+    it is not; a log-probability of -inf has an infinite KL from a finite reference."""
+    g = torch.Generator().manual_seed(n * 3 + S)
+    off, T = ragged(g, n, S)
+    lp = -torch.rand(T, generator=g)
+    old, ref, adv = lp.clone(), lp.clone(), torch.randn(T, generator=g)
+    a, b, c = T // 5, T // 2, T - 1
+    old[a], adv[a] = -2000.0, 0.0                # ratio exp(2000), advantage 0
+    old[b], adv[b] = -INF, 0.0
+    ref[c] = 1000.0
+    ref[0] = -INF
+    w = weights(off, torch.ones(T, dtype=torch.bool), mean)
+    want = -(adv.double() * w)
+    call = lambda **k: llmt.policy_loss(lp.to(dev), old.to(dev), adv.to(dev), off.to(dev), mean=mean, **k)
+    for kl in (None, ref.to(dev)):
+        p = call(ref_logp=kl, kl_coef=0.0)
+        close(p.loss, want.sum().reshape(1))
+        close(p.dlogp, want)
+        assert p.stats[0] == p.loss and p.stats[1] == (0.0 if kl is None else INF)
+    p = call(ref_logp=ref.to(dev), kl_coef=0.05)
+    assert p.loss == INF and p.stats[1] == INF and p.dlogp[c] == -INF
+    fine = torch.ones(T, dtype=torch.bool)
+    fine[[0, c]] = False
+    assert torch.equal(p.dlogp.cpu()[fine], call().dlogp.cpu()[fine])
+    close(p.dlogp[0], want[0] + f32(0.05) * w[0])
+    # an impossible token under a finite reference
+    ref[c], ref[0] = lp[c], lp[0]
+    lp[b], old[b] = -INF, -1.0
+    p = call(ref_logp=ref.to(dev), kl_coef=0.05)
+    assert p.loss == INF and p.stats[1] == INF and p.dlogp[b] == -INF
+    fine = torch.arange(T) != b
+    close(p.dlogp.cpu()[fine], want[fine])
+    adv[a] = -1.0                                 # a weight: the loss has no bound there
+    p = call()
+    assert p.loss == INF and p.dlogp[a] == INF
