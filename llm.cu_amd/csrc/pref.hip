@@ -180,7 +180,7 @@ __global__ __launch_bounds__(BLOCK) void pref_kernel(const PrefArgs a) {
     } else if (a.kind == LLMT_PREF_HINGE) {
       dz = (s - 1.0) * (z < 1.0 ? 1.0 : 0.0) + s * (z > -1.0 ? 1.0 : 0.0);
     } else {
-      dz = (1.0 - s) * (2.0 * z - 1.0) + s * (2.0 * z + 1.0);
+      dz = 2.0 * z - 1.0 + 2.0 * s;
     }
     if (z != z) dz = z;
     if (a.dlogp) {

@@ -89,3 +89,24 @@ def test_policy_terms_beyond_exps_range(dev, n, S, mean):
     adv[a] = -1.0                                 # a weight: the loss has no bound there
     p = call()
     assert p.loss == INF and p.dlogp[a] == INF
+
+
+@pytest.mark.parametrize("smooth", [0.0, 0.25])
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "square"])
+def test_preference_loss_of_an_impossible_answer(dev, kind, smooth):
+    """A chosen or a rejected answer with a log-probability of -inf: the limits of f and f'."""
+    off = torch.arange(7, dtype=torch.int32, device=dev)
+    lp = torch.tensor([-INF, 0.0, 0.0, -INF, -1.0, -2.0], device=dev)
+    mean, losses, rewards, d = llmt.preference_loss(lp, None, off, loss=kind, beta=0.5,
+                                                    label_smoothing=smooth)
+    e = smooth
+    # f' at z = -inf and +inf of (1 - e) f(z) + e f(-z)
+    lo, hi = {"sigmoid": (e - 1, e), "hinge": (e - 1, e), "square": (-INF, INF)}[kind]
+    assert losses[0] == INF and losses[1] == (0.0 if e == 0 and kind != "square" else INF)
+    assert mean == INF and rewards.tolist() == [-INF, 0.0, 0.0, -INF, -0.5, -1.0]
+    want = torch.tensor([lo, -lo, hi, -hi], dtype=torch.double) * 0.5 / 3
+    if kind == "square":
+        assert d.tolist()[:4] == want.tolist()
+    else:
+        close(d[:4], want)
+    assert d[4:].isfinite().all()
