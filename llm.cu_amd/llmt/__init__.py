@@ -313,6 +313,12 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _sizes(names, *sizes):
+    """Sizes that the library takes as int (ctypes would pass on their lower 32 bits)."""
+    if max(sizes) >= 1 << 31:
+        raise LlmtError(f"{names}: {sizes}, each at most 2^31 - 1")
+
+
 def _byte_mask(mask, T):
     import torch
     if mask is not None:
@@ -328,6 +334,7 @@ def token_logprobs(logits, targets, temperature=1.0, want_entropy=False, stream=
     with _On("logits targets", (logits, targets), stream) as on:
         dt = _logits_dtype("logits", logits)
         rows, V = logits.shape
+        _sizes("rows, V", rows, V)
         _expect("targets", targets, torch.int32, rows)
         logp = logits.new_empty(rows, dtype=torch.float32)
         stats = logits.new_empty((rows, 2), dtype=torch.float32)
@@ -351,6 +358,7 @@ def token_logprobs_bwd(logits, targets, stats, dlogp, entropy=None, dentropy=Non
              (logits, targets, stats, dlogp, entropy, dentropy, out), stream) as on:
         dt = _logits_dtype("logits", logits)
         rows, V = logits.shape
+        _sizes("rows, V", rows, V)
         _expect("targets", targets, torch.int32, rows)
         _expect("stats", stats, torch.float32, rows, 2)
         _expect("dlogp", dlogp, torch.float32, rows)
@@ -391,6 +399,7 @@ def preference_loss(logp, ref_logp, offsets, loss="sigmoid", beta=0.1, label_smo
         n = offsets.shape[0] // 2
         if n < 1 or offsets.shape[0] != 2 * n + 1:
             raise LlmtError(f"offsets must be [2 n + 1] with n >= 1 (got {list(offsets.shape)})")
+        _sizes("T, offsets", T, 2 * n + 1)
         mean, losses, rewards = logp.new_empty(3 * n + 1).split_with_sizes((1, n, 2 * n))
         dlogp = torch.empty_like(logp) if want_grad else None
         p = PrefParams(kind, average, beta, label_smoothing, margin)
@@ -432,6 +441,7 @@ def policy_loss(logp, old_logp, advantages, offsets, ref_logp=None, entropy=None
         n = offsets.shape[0] - 1
         if n < 1:
             raise LlmtError("offsets must be [n + 1] with n >= 1")
+        _sizes("T, offsets", T, n + 1)
         _expect("advantages", advantages, torch.float32, n if per_sequence else T)
         L = lib()
         need = L.llmt_policy_loss_workspace(T, n)
@@ -457,12 +467,13 @@ def orthogonalize(x, steps=5, eps=1e-7, out=None, stream=None):
     with _On("x out", (x, out), stream) as on:
         if x.dtype != torch.float32 or x.dim() not in (2, 3) or 0 in x.shape[-2:]:
             raise LlmtError("x must be float32 [rows, cols] or [count, rows, cols]")
+        rows, cols = x.shape[-2:]
+        count = x.shape[0] if x.dim() == 3 else 1
+        _sizes("count, rows, cols", count, rows, cols)
         if out is None:
             out = x.new_empty(x.shape)
         elif out.shape != x.shape or out.dtype != torch.float32:
             raise LlmtError("out must have x's shape and type")
-        rows, cols = x.shape[-2:]
-        count = x.shape[0] if x.dim() == 3 else 1
 
         def strides(name, t):  # of one row or one matrix the stride is of no account
             if cols > 1 and t.stride(-1) != 1:
@@ -504,6 +515,7 @@ def muon_update(p, g, m, shapes, hp: MuonParams, stream=None):
             raise LlmtError(f"the arena's {n} elements are not whole layers of {per}")
         k = len(shapes)
         rows, cols = zip(*shapes)
+        _sizes("layers, rows, cols", n // per, *rows, *cols)
         rows, cols = (i32 * k)(*rows), (i32 * k)(*cols)
         L = lib()
         need = L.llmt_muon_update_workspace(n // per, k, rows, cols)

@@ -110,3 +110,25 @@ def test_preference_loss_of_an_impossible_answer(dev, kind, smooth):
     else:
         close(d[:4], want)
     assert d[4:].isfinite().all()
+
+
+def test_sizes_beyond_32_bits_are_refused(dev):
+    """The library takes sizes of 31 bits; a larger one would arrive as what its lower 32
+    bits say (2^32 + 4 tokens as 4).  Nothing of the tensors is read or written."""
+    N = 2 ** 32 + 4
+    big = torch.empty(N, device=dev)
+    ints = torch.empty(N + 1, dtype=torch.int32, device=dev)
+    few, off = torch.zeros(4, device=dev), torch.tensor([0, 2, 4], dtype=torch.int32, device=dev)
+    rows = big.view(N, 1)
+    for call in (lambda: llmt.token_logprobs(rows, ints[:N]),
+                 lambda: llmt.token_logprobs(big.view(1, N), off[:1]),
+                 lambda: llmt.token_logprobs_bwd(big.view(1, N), off[:1], few[:2].view(1, 2), few[:1]),
+                 lambda: llmt.preference_loss(big, None, off),
+                 lambda: llmt.preference_loss(few, None, ints[:N + 1]),
+                 lambda: llmt.policy_loss(big, None, few[:2], off, per_sequence=True),
+                 lambda: llmt.policy_loss(few, None, few, ints),
+                 lambda: llmt.orthogonalize(rows), lambda: llmt.orthogonalize(big.view(1, 1, N)),
+                 lambda: llmt.orthogonalize(big.view(N, 1, 1)),
+                 lambda: llmt.muon_update(big, big, big, [(1, 1)], llmt.muon_hparams())):
+        with pytest.raises(llmt.LlmtError, match="at most 2"):
+            call()
