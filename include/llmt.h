@@ -251,7 +251,8 @@ int llmt_lora_save(llmt_ctx* ctx, const char* dir, int step);
 int llmt_lora_load(llmt_ctx* ctx, const char* dir, int step);
 /* AdamW moments for resuming a run (no counterpart in the reference, whose
  * driver cannot resume): <dir>/lora_step{N}_adamw.bin holds "LLMTADAM",
- * int32 version 1, int32 step, int64 numel, fp32 m, fp32 v. */
+ * int32 version 1, int32 step, int64 numel, fp32 m, fp32 v.  After llmt_muon the
+ * same file begins with "LLMTMUON": m is Muon's momentum, v unused. */
 int llmt_lora_save_state(llmt_ctx* ctx, const char* dir, int step);
 int llmt_lora_load_state(llmt_ctx* ctx, const char* dir, int step);
 /* Seeded init on the device (the reference draws A with cuRAND, B = 0:
@@ -500,7 +501,9 @@ int llmt_muon_update(float* p, const float* g, float* m, int layers, int nmat,
                      void* workspace, size_t workspace_bytes, void* stream);
 /* Muon over a context's whole adapter arena from its GRAD arena (the M arena
  * holds the momentum, V is not used), in place of llmt_adamw; one host
- * synchronisation. */
+ * synchronisation.  AdamW (llmt_step, llmt_adamw, llmt_profile_kernels) fails
+ * with LLMT_ERR_STATE from then on, until M is set by llmt_lora_copy,
+ * llmt_lora_load_state (of an AdamW state) or llmt_lora_init. */
 int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params);
 
 #ifdef __cplusplus

@@ -380,6 +380,7 @@ int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params) {
   a.x = c->lora_g;
   a.m = c->lora_m;
   a.out = c->lora_p;
+  c->m_is_muon = true;
   hipError_t e = newton_schulz(a, c->muon_ws, c->st);
   if (e == hipSuccess) e = c->refresh_shadows();
   if (e == hipSuccess) e = hipStreamSynchronize(c->st);

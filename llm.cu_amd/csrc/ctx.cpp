@@ -596,8 +596,10 @@ int llmt_lora_load(llmt_ctx* ctx, const char* dir, int step) {
 // AdamW state next to the adapter files: <dir>/lora_step{N}_adamw.bin =
 // "LLMTADAM", int32 version 1, int32 step, int64 numel, fp32 m[numel],
 // fp32 v[numel] (little-endian).  The reference has no resume; this is the
-// state a restart at step N + 1 needs besides the adapters themselves.
-static const char kAdamMagic[8] = {'L', 'L', 'M', 'T', 'A', 'D', 'A', 'M'};
+// state a restart at step N + 1 needs besides the adapters themselves.  With
+// Muon's momentum in the M arena the file begins with "LLMTMUON" (v is unused
+// then), and the context that loads it knows it as that.
+static const char kStateMagic[2][9] = {"LLMTADAM", "LLMTMUON"};
 
 int llmt_lora_save_state(llmt_ctx* ctx, const char* dir, int step) {
   set_error("");
@@ -617,7 +619,7 @@ int llmt_lora_save_state(llmt_ctx* ctx, const char* dir, int step) {
   }
   const int32_t hdr[2] = {1, step};
   const int64_t numel = (int64_t)n;
-  bool ok = fwrite(kAdamMagic, 1, 8, f) == 8 && fwrite(hdr, 4, 2, f) == 2 &&
+  bool ok = fwrite(kStateMagic[c->m_is_muon], 1, 8, f) == 8 && fwrite(hdr, 4, 2, f) == 2 &&
             fwrite(&numel, 8, 1, f) == 1 && fwrite(mv.data(), 4, 2 * n, f) == 2 * n;
   ok = (fclose(f) == 0) && ok;
   if (!ok) {
@@ -643,17 +645,19 @@ int llmt_lora_load_state(llmt_ctx* ctx, const char* dir, int step) {
   int32_t hdr[2];
   int64_t numel = 0;
   std::vector<float> mv(2 * n);
+  auto is = [&](int k) { return memcmp(magic, kStateMagic[k], 8) == 0; };
   const bool ok = fread(magic, 1, 8, f) == 8 && fread(hdr, 4, 2, f) == 2 &&
-                  fread(&numel, 8, 1, f) == 1 && memcmp(magic, kAdamMagic, 8) == 0 &&
+                  fread(&numel, 8, 1, f) == 1 && (is(0) || is(1)) &&
                   hdr[0] == 1 && hdr[1] == step && numel == (int64_t)n &&
                   fread(mv.data(), 4, 2 * n, f) == 2 * n;
   fclose(f);
   if (!ok) {
-    set_error("%s: not an AdamW state of step %d with %zu parameters", path, step, n);
+    set_error("%s: not an AdamW or Muon state of step %d with %zu parameters", path, step, n);
     return LLMT_ERR_IO;
   }
   int rc = llmt_lora_copy(ctx, LLMT_LORA_M, mv.data(), 1);
   if (rc) return rc;
+  c->m_is_muon = is(1);
   return llmt_lora_copy(ctx, LLMT_LORA_V, mv.data() + n, 1);
 }
 

@@ -130,6 +130,7 @@ struct Ctx {
   // in the attention norm's backward)
   _Float16* shadow_at = nullptr;
   void* muon_ws = nullptr;  // llmt_muon's workspace, allocated by its first call
+  bool m_is_muon = false;   // lora_m is Muon's momentum, which AdamW does not take for its own
   AdamHp* hp_dev = nullptr;
   AdamHp* host_hp = nullptr;
 

@@ -669,6 +669,7 @@ int llmt_lora_copy(llmt_ctx* ctx, int kind, float* buf, int to_ctx) {
   const size_t bytes = c->lora_numel * sizeof(float);
   if (to_ctx) {
     TRY_HIP(hipMemcpyAsync(arena[kind], buf, bytes, hipMemcpyDefault, c->st));
+    if (kind == LLMT_LORA_M) c->m_is_muon = false;
     if (kind == LLMT_LORA_PARAM) TRY_HIP(c->refresh_shadows());
   } else {
     TRY_HIP(hipMemcpyAsync(buf, arena[kind], bytes, hipMemcpyDefault, c->st));
@@ -682,6 +683,7 @@ int llmt_lora_init(llmt_ctx* ctx, uint64_t seed, float a_std, float b_std) {
   Ctx* c = C_(ctx);
   TRY_ARG(c, "llmt_lora_init: NULL ctx");
   c->logp_batch = 0;
+  c->m_is_muon = false;
   TRY_HIP(lora_init(c->lora_p, c->lora_m, c->lora_v, (long long)c->lora_numel, seed, a_std, b_std,
                     c->shadow_desc(), c->st));
   TRY_HIP(hipMemsetAsync(c->lora_g, 0, c->lora_numel * sizeof(float), c->st));
@@ -694,6 +696,16 @@ static int check_tokens(Ctx* c, const int* tokens, const int* targets, int batch
   TRY_ARG(batch >= 1 && batch <= c->maxB, "batch %d outside [1, %d]", batch, c->maxB);
   TRY_ARG(c->weights_ready(), "frozen weights not set (llmt_set_layer_* / llmt_set_embed_f16)");
   return LLMT_OK;
+}
+
+// AdamW takes the M and V arenas for its moments: Muon's momentum, a sum of
+// gradients beside a V of zeros, would make its next update hundreds of times
+// too large.
+static int check_adamw(const Ctx* c) {
+  if (!c->m_is_muon) return LLMT_OK;
+  set_error("the M arena holds Muon's momentum, not AdamW's (llmt_lora_copy to M, "
+            "llmt_lora_load_state or llmt_lora_init replaces it)");
+  return LLMT_ERR_STATE;
 }
 
 static int stage_inputs(Ctx* c, const int* tokens, const int* targets, int batch) {
@@ -794,6 +806,7 @@ int llmt_step(llmt_ctx* ctx, const int* tokens, const int* targets, int batch,
   set_error("");
   Ctx* c = C_(ctx);
   int rc = check_tokens(c, tokens, targets, batch);
+  if (!rc) rc = check_adamw(c);
   if (rc) return rc;
   if (graph_inputs(c, tokens, targets)) {
     if ((rc = set_hp_host(c, hp, step))) return rc;
@@ -854,7 +867,8 @@ int llmt_adamw(llmt_ctx* ctx, const llmt_hparams* hp, int step) {
   set_error("");
   Ctx* c = C_(ctx);
   TRY_ARG(c, "NULL ctx");
-  int rc = set_hp(c, hp, step);
+  int rc = check_adamw(c);
+  if (!rc) rc = set_hp(c, hp, step);
   if (rc) return rc;
   TRY_HIP(c->optimizer());
   TRY_HIP(hipStreamSynchronize(c->st));
@@ -924,6 +938,7 @@ int llmt_profile_kernels(llmt_ctx* ctx, const int* tokens, const int* targets, i
   TRY_ARG(nkinds && names && cats && launches && us && flops && bytes && reps >= 1 &&
               max_kinds >= 1,
           "llmt_profile_kernels: outputs, reps, max_kinds");
+  if ((rc = check_adamw(c))) return rc;
   if ((rc = set_hp(c, hp, step))) return rc;
   if ((rc = stage_inputs(c, tokens, targets, batch))) return rc;
   // 1. one eager step, every launch recorded

@@ -643,7 +643,8 @@ class Context:
         check(lib().llmt_lora_load(self.h, str(path).encode(), step))
 
     def lora_save_state(self, path, step: int):
-        """AdamW moments to <path>/lora_step{step}_adamw.bin (for resuming)."""
+        """AdamW moments, or Muon's momentum, to <path>/lora_step{step}_adamw.bin
+        (for resuming with the same optimiser)."""
         check(lib().llmt_lora_save_state(self.h, str(path).encode(), step))
 
     def lora_load_state(self, path, step: int):

@@ -126,3 +126,70 @@ def test_calls_follow_the_current_stream(dev, where):
             assert torch.equal(a, b)
     finally:
         ctx.close()
+
+
+def test_muon_state_is_not_adamws(dev, tmp_path):
+    """Momentum of Muon's in the M arena, stepped there or loaded, is no AdamW state: AdamW
+    refuses until the arena is set anew.  Saved and loaded, Muon continues bit for bit."""
+    W, ad, tok, tgt = small_problem()
+    B, S = tok.shape
+    tok, tgt = tok.to(dev), tgt.to(dev)
+    L, hp, adam = llmt.lib(), llmt.muon_hparams(lr=1e-3), llmt.hparams()
+    flat = llmt.flatten_adapters(ad).to(dev)
+    ctx = context(dev, W, ad, B, S)
+
+    def adamw_refused():
+        before = ctx.lora_get("param"), ctx.lora_get("m")
+        for graph in (False, True):
+            ctx.set_graph(graph)
+            with pytest.raises(llmt.LlmtError, match="Muon"):
+                ctx.step(tok, tgt, adam, 3)
+        ctx.set_graph(False)
+        assert L.llmt_adamw(ctx.h, C.byref(adam), 3) == llmt.LLMT_ERR_STATE
+        with pytest.raises(llmt.LlmtError, match="Muon"):
+            ctx.profile_kernels(tok, tgt, adam, 3, reps=1)
+        assert torch.equal(ctx.lora_get("param"), before[0])
+        assert torch.equal(ctx.lora_get("m"), before[1])
+
+    try:
+        ctx.step(tok, tgt, adam, 1)
+        ctx.lora_save_state(tmp_path, 1)
+        assert (tmp_path / "lora_step1_adamw.bin").read_bytes()[:8] == b"LLMTADAM"
+        m1, p1 = ctx.lora_get("m"), ctx.lora_get("param")
+        ctx.step(tok, tgt, adam, 2)
+        p2 = ctx.lora_get("param")
+        ctx.lora_set("m", torch.zeros_like(m1))
+        ctx.forward_backward(tok, tgt)
+        ctx.muon(hp)
+        adamw_refused()
+        ctx.lora_save_state(tmp_path, 2)
+        m2, pm = ctx.lora_get("m"), ctx.lora_get("param")
+        ctx.forward_backward(tok, tgt)
+        ctx.muon(hp)
+        want = ctx.lora_get("param")
+        # AdamW's state again: its next step as it was
+        ctx.lora_set("param", p1)
+        ctx.lora_load_state(tmp_path, 1)
+        assert torch.equal(ctx.lora_get("m"), m1)
+        ctx.step(tok, tgt, adam, 2)
+        assert torch.equal(ctx.lora_get("param"), p2)
+        # Muon's in a context of its own
+        ctx.close()
+        ctx = context(dev, W, ad, B, S)
+        ctx.lora_set("param", pm)
+        ctx.lora_load_state(tmp_path, 2)
+        assert torch.equal(ctx.lora_get("m"), m2)
+        adamw_refused()
+        ctx.forward_backward(tok, tgt)
+        ctx.muon(hp)
+        assert torch.equal(ctx.lora_get("param"), want)
+        # the arena set anew
+        ctx.lora_set("param", flat)
+        adamw_refused()
+        ctx.lora_set("m", torch.zeros_like(m1))
+        ctx.step(tok, tgt, adam, 1)
+        ctx.muon(hp)
+        ctx.lora_init(1, 0.02, 0.0)
+        ctx.step(tok, tgt, adam, 1)
+    finally:
+        ctx.close()
