@@ -3,6 +3,7 @@ leave their range, at every kernel's borders and far above its grid, against flo
 
 The kernels compute in fp64 and round each output once to fp32 (half a step, 2^-24 of
 itself); the mean preference loss is a mean of rounded losses, one more half step."""
+import ctypes as C
 import math
 
 import pytest
@@ -132,3 +133,94 @@ def test_sizes_beyond_32_bits_are_refused(dev):
                  lambda: llmt.muon_update(big, big, big, [(1, 1)], llmt.muon_hparams())):
         with pytest.raises(llmt.LlmtError, match="at most 2"):
             call()
+
+
+@pytest.mark.parametrize("n,S,per_seq,mean", [
+    (5000, 9, True, "token"),          # more sequences than a workgroup keeps offsets of
+    (10000, 5, True, "sequence"),      # waves of the grid take several sequences each
+    (2500, 1400, False, "sequence"),   # workgroups do
+    (2048, 7, True, "sequence"), (2049, 3, True, "token"), (8191, 1, False, "token"),
+    (8193, 1, False, "sequence")])     # the borders of the single workgroup
+def test_policy_loss_of_many_sequences(dev, n, S, per_seq, mean):
+    check_policy_loss(dev, n, S, per_seq, True, True, True, True, mean)
+
+
+@pytest.mark.parametrize("n,S", [(300_000, 1), (66_000, 550)])
+def test_preference_loss_of_more_pairs_than_workgroups(dev, n, S):
+    """Sequences of S tokens; the sums in float64 on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    lp = -torch.rand(2 * n * S, generator=g, device=dev)
+    off = torch.arange(0, 2 * n * S + 1, S, dtype=torch.int32, device=dev)
+    mean, losses, rewards, d = llmt.preference_loss(lp, None, off, beta=0.1)
+    r = lp.view(2 * n, S).double().sum(1) * f32(0.1)
+    z = r[0::2] - r[1::2]
+    close(rewards, r.cpu(), size=S)
+    close(losses, F.softplus(-z).cpu(), size=S)
+    close(mean, F.softplus(-z).mean().reshape(1).cpu(), size=S, steps=2)
+    dz = -torch.sigmoid(-z) * f32(0.1) / n
+    close(d.view(n, 2, S)[:, 0], dz[:, None].expand(n, S).cpu())
+    close(d.view(n, 2, S)[:, 1], -dz[:, None].expand(n, S).cpu())
+
+
+def guarded(x, fill):
+    """x inside a larger buffer of `fill`: (the buffer, the view of x)."""
+    pad = 97                                      # off 16 bytes, and more than a step of loads
+    buf = torch.full((x.numel() + 2 * pad,), fill, dtype=x.dtype, device=x.device)
+    view = buf[pad:pad + x.numel()]
+    view.copy_(x)
+    return buf, view
+
+
+def unharmed(buf, fill, view):
+    pad = (buf.numel() - view.numel()) // 2
+    return bool((buf[:pad] == fill).all() and (buf[pad + view.numel():] == fill).all())
+
+
+# (T, sequences): each kernel of either loss
+@pytest.mark.parametrize("T,n", [(50, 4), (8001, 4), (30001, 4), (30001, 3000), (90001, 40),
+                                 (90001, 300), (9001, 9000)])
+def test_offsets_of_any_value_stay_in_guarded_arrays(dev, T, n):
+    """Through the C ABI, every array inside a larger one: what is before and behind the
+    outputs stays, what is before and behind the inputs (NaN) is not seen.  Offsets that are
+    ascending but out of [0, T] work as if clamped; any others do no harm."""
+    g = torch.Generator().manual_seed(T + n)
+    L, ptr, f = llmt.lib(), llmt.ptr, torch.float32
+    big = lambda size: torch.randn(size, generator=g).to(dev)
+    inputs = [guarded(-big(T).abs(), math.nan)[1] for _ in range(2)]
+    lp, ref = inputs
+    adv, adv_seq = guarded(big(T), math.nan)[1], guarded(big(n), math.nan)[1]
+    mask = guarded((torch.rand(T, generator=g) < 0.7).to(torch.uint8).to(dev), 1)[1]
+    wild = torch.randint(-2 ** 31, 2 ** 31 - 1, (n + 1,), generator=g, dtype=torch.int64)
+    near = torch.randint(-T // 8, T + T // 8, (n + 1,), generator=g)
+    ascending = near.sort().values
+    ascending[0], ascending[-1] = -2 ** 31, 2 ** 31 - 1
+
+    def run(off):
+        off = guarded(off.to(torch.int32).to(dev), 0)[1]
+        out = []
+        for kind in range(2):
+            outs = [guarded(torch.zeros(k, device=dev), 7.0) for k in (1, n // 2, n, T)]
+            p = llmt.PrefParams(0, kind, 0.1, 0.0, 0.0)
+            llmt.check(L.llmt_preference_loss(ptr(lp), ptr(ref), ptr(mask), ptr(off), T, n // 2,
+                                              C.byref(p), *(ptr(v) for _, v in outs), None))
+            out += outs
+        for mean in range(2):
+            for per_seq in range(2):
+                outs = [guarded(torch.zeros(k, device=dev), 7.0) for k in (1, 3, T)]
+                need = L.llmt_policy_loss_workspace(T, n)
+                room = torch.full((need + 64,), 7, dtype=torch.uint8, device=dev)
+                p = llmt.PolicyParams(mean, per_seq, 0.2, 0.2, 0.1, 0.0)
+                llmt.check(L.llmt_policy_loss(
+                    ptr(lp), ptr(ref), ptr(ref), ptr(adv_seq if per_seq else adv), None, ptr(mask),
+                    ptr(off), T, n, C.byref(p), *(ptr(v) for _, v in outs), None, ptr(room), need,
+                    None))
+                assert (room[need:] == 7).all()
+                out += outs
+        torch.cuda.synchronize()
+        assert all(unharmed(buf, 7.0, v) for buf, v in out)
+        return [v.clone() for _, v in out]
+
+    got, want = run(ascending), run(ascending.clamp(0, T))
+    assert all(torch.equal(a, b) and a.isfinite().all() for a, b in zip(got, want))
+    run(near)
+    run(wild)
