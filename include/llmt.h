@@ -452,6 +452,9 @@ int llmt_preference_loss(const float* logp, const float* ref_logp, const unsigne
  *   policy = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
  *   kl     = exp(d) - d - 1                       (0 with ref_logp NULL)
  *   l      = policy + kl_coef kl - entropy_coef entropy   (entropy may be NULL)
+ * A ratio beyond fp32 counts nothing at an advantage of 0; a logp of -inf has
+ * ratio 0 (1 without old_logp) and a kl of +inf from a finite ref_logp; with
+ * kl_coef 0 the kl, of any size, is only reported in stats.
  * loss [1] is the mean of l over all kept tokens (LLMT_MEAN_TOKEN), or the
  * mean over the n sequences of their kept tokens' means, a sequence without
  * any counting as 0 (LLMT_MEAN_SEQUENCE).  stats [3]: policy, kl and the share

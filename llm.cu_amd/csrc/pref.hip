@@ -255,36 +255,35 @@ __device__ __forceinline__ Quad load_quad(const PolicyArgs& a, long long t, int 
   const f4u zero = {0.f, 0.f, 0.f, 0.f};
   Quad x;
   x.lp = load4(a.logp, t, have);
-  x.old = a.old ? load4(a.old, t, have) : zero;
+  x.old = a.old ? load4(a.old, t, have) : x.lp;
   x.ref = a.ref ? load4(a.ref, t, have) : zero;
   x.adv = a.adv_per_seq ? zero : load4(a.adv, t, have);
   x.ent = a.entropy ? load4(a.entropy, t, have) : zero;
   return x;
 }
 
-// exp(v) and exp(v) - 1 beyond fp64 are its largest number instead: times a
-// factor of 0 (an advantage, the KL's coefficient) they count nothing, times any
-// other they are beyond fp32.  (NaN stays.)
-__device__ __forceinline__ double bounded(double v) {
-  return v > __DBL_MAX__ ? __DBL_MAX__ : v;
-}
-
 // Adds token e of the quad with weight w to the sums (loss, policy term, KL,
-// clipped); returns the gradient by its log-probability.
+// clipped); returns the gradient by its log-probability.  Exponents end at 700:
+// exp of it is 1e304, beyond fp32 times any number but 0, and 0 times 0 (exp's
+// infinity times 0 is NaN).  A NaN stays NaN in the loss.  The guards cost six
+// instructions a token, within the noise of every size; as selects on the results
+// they were 2 to 7% of the call, which these kernels' issue rate bounds.
 __device__ __forceinline__ float policy_token(const PolicyArgs& a, const Quad& x, int e,
                                               double adv, double w, double (&v)[4]) {
-  // without an old policy the ratio is 1, of a log-probability of -inf too
-  const double lp = x.lp[e];
-  const double ratio = a.old ? bounded(exp(lp - (double)x.old[e])) : lp != lp ? lp : 1.0;
+  // -inf less itself is 0: without an old policy the ratio is 1 there too
+  const float lp = __builtin_elementwise_maximum(x.lp[e], -__FLT_MAX__);
+  const float old = __builtin_elementwise_maximum(x.old[e], lp - 700.f);
+  const double ratio = exp((double)lp - (double)old);
   const double lo = 1.0 - a.clip_low, hi = 1.0 + a.clip_high;
   const double s1 = ratio * adv, s2 = (ratio < lo ? lo : ratio > hi ? hi : ratio) * adv;
   const bool clip = s1 > s2;
   const double pg = -(clip ? s2 : s1);
   double grad = clip ? 0.0 : -s1, loss = pg, kl = 0.0;
   if (a.ref) {
-    const double d = (double)x.ref[e] - lp, em = bounded(expm1(d));
-    kl = em < __DBL_MAX__ ? bounded(em - d) : em;
-    loss += a.kl_coef * kl;
+    const double d = (double)x.ref[e] - (double)lp, em = expm1(fmin(d, 700.0));
+    kl = em - d;
+    // with a coefficient of 0 an infinite KL (d = -inf) is only reported
+    loss += a.kl_coef * (a.kl_coef != 0.0 ? kl : em);
     grad -= a.kl_coef * em;
   }
   if (a.entropy) loss -= a.ent_coef * (double)x.ent[e];

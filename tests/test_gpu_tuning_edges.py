@@ -224,3 +224,20 @@ def test_offsets_of_any_value_stay_in_guarded_arrays(dev, T, n):
     assert all(torch.equal(a, b) and a.isfinite().all() for a, b in zip(got, want))
     run(near)
     run(wild)
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e30, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("n,S", SHAPES)
+def test_policy_of_tokens_behind_a_finite_mask(dev, n, S, low):
+    """The same finite log-probability in all three policies, however low: ratio 1, KL 0."""
+    g = torch.Generator().manual_seed(n + 7 * S)
+    off, T = ragged(g, n, S)
+    lp, adv = -torch.rand(T, generator=g), torch.randn(T, generator=g)
+    lp[torch.rand(T, generator=g) < 0.3] = low
+    w = weights(off, torch.ones(T, dtype=torch.bool), "token")
+    x = lp.to(dev)
+    p = llmt.policy_loss(x, x, adv.to(dev), off.to(dev), ref_logp=x, kl_coef=0.5)
+    want = -(adv.double() * w)
+    close(p.loss, want.sum().reshape(1))
+    close(p.dlogp, want)
+    assert p.stats[1] == 0 and p.stats[2] == 0
