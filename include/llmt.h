@@ -390,7 +390,9 @@ enum { LLMT_F32 = 0, LLMT_F16 = 1, LLMT_BF16 = 2 };
  * its outputs are 0.  An x of -inf has probability 0; a row of nothing but
  * -inf gives logp -inf, stats (-inf, 0), entropy 0.  Finite masks of any size
  * are logits like others: a row that they fill is uniform (where |m| exceeds
- * 2^29 each x is rounded to fp32 before m is subtracted).  A NaN or +inf makes
+ * 2^29 each x is rounded to fp32 before m is subtracted); an x beyond fp32's
+ * range is infinite, so masks of its lowest value are -inf at an inv_temp above
+ * 1, and a row of nothing else is one of nothing but -inf.  A NaN or +inf makes
  * the outputs of its own row NaN.  rows may be 0. */
 size_t llmt_token_logprobs_workspace(int rows, int V, int dtype);
 int llmt_token_logprobs(const void* logits, int dtype, long long ld, const int* targets, int rows,

@@ -13,7 +13,8 @@
 //
 // Both are bound by HBM: the forward reads the logits once, the backward
 // reads them and writes their gradient.  4096 x 151936 fp32, a quarter of the
-// rows without a target: forward 283 us, 6.6 TB/s.  1000 x 151936 fp32:
+// rows without a target: forward 283 us in a row, 6.6 TB/s (295 in a graph).  1000
+// x 151936 fp32:
 // backward 194 us, 6.3 TB/s (a plain copy 4.8-5.1).
 #include <algorithm>
 
@@ -405,10 +406,17 @@ constexpr int kWaveV = 2048;
 //
 // Rows too long for one CU are split into chunks, as many as make four
 // workgroups a CU and at least one batch of loads a thread, and merged by a
-// second launch, which costs a caller 3.5 us: worth 192 K logits off a
-// workgroup's share (one row: 151936 split 5.8 us in a graph, 14.0 a call from
-// Python, unsplit 9.6 and 10.2; 262144 bf16 a call and its wait 25 and 31), up
-// to half a row a CU (200 x 262144 bf16: split 20.6, unsplit 17.9).
+// second launch, which costs a caller from Python 4 us: worth 192 K logits off a
+// workgroup's share (one row of 262144 bf16, a call and its wait: split 25 us,
+// unsplit 31), up to half a row a CU (200 x 262144 bf16: split 20.6, unsplit
+// 17.9).  The rule follows such calls.  In a graph a split would be worth it from
+// fewer logits on; 151936, split and unsplit, us:
+//   rows             1          8          32         64         128
+//   fp32 graph    5.9  9.3   6.4  9.7   7.0 10.0  10.6 13.8  16.7 16.9
+//   bf16 graph    5.7  9.4   6.2  9.7   7.0  9.9   7.8  9.9  11.2 11.9
+// while a call in a row is 4 us longer split at each of these sizes, and one with
+// its wait level (fp32, 64 rows: 2.7 us shorter split).  50257 is slower split
+// either way (fp32 graph, 1 and 128 rows: 5.8 and 5.3, 7.9 and 7.0).
 constexpr int kCus = 256, kSplitLogits = 192 << 10;
 static int fwd_chunks(int rows, int V, int dtype) {
   if (rows > kCus / 2) return 1;

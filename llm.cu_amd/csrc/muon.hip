@@ -20,8 +20,8 @@
 //
 // Bound by HBM where the short side is 16 and matrices are many (the 28-layer
 // Muon step, 128 MB: 26.7 us, 4.8 TB/s, a copy's rate), by the fp64 matrix rate
-// above (28 x 12288 x 64: 4.5 GFLOP, gram 34 us, iteration 42, product 55), by
-// launches and memory round trips for few matrices (1 x 16 x 2048: 10.5 us).
+// above (28 x 12288 x 64: 4.5 GFLOP, gram 34 us, iteration 42, product 56), by
+// launches and memory round trips for few matrices (1 x 16 x 2048: 10.3 us).
 //
 // All matrices of the iteration are symmetric and commute.  A lane of an f64
 // MFMA result holds rows 4 v + l / 16 (v = 0..3) of column l % 16; read by
@@ -370,10 +370,11 @@ __device__ __forceinline__ doublex4 product(const double* m1, const double* m2, 
   return x;
 }
 
-// The iteration of one matrix, a wave a tile of the upper triangle (the CU's
-// fp64 rate bounds it, so the lower one is written, not computed): the split
-// partials into G0, then P, scaled for the product with U:
-// ws.proj[matrix][tile row][tile col][v][lane].
+// The iteration of one matrix, a wave a tile of the upper triangle (the lower one
+// is written, not computed): the split partials into G0, then P, scaled for the
+// product with U: ws.proj[matrix][tile row][tile col][v][lane].  Of 42 us at 28
+// matrices of short side 64 the matrix instructions are 18 (22 on the fullest
+// SIMD) and bank conflicts of the transposed tiles 11; the splits are summed before.
 template <int NT>
 __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a) {
   constexpr int M = NT * NT * 256;
@@ -435,7 +436,7 @@ __global__ __launch_bounds__(64 * ntri(NT)) void ns_solve_kernel(const NsArgs a)
 // (the momentum is already updated).  NT = 1: every workgroup iterates by
 // itself (2 us, during which its first loads arrive), which is less than the
 // launch that it saves.  Else P is read from LDS as it is used: in registers it
-// left one or two waves a SIMD (28 layers at rank 64: 218 us, 259 so).
+// left one or two waves a SIMD (28 layers at rank 64: 214 us, 259 so).
 template <int NT, bool MUON>
 __global__ __launch_bounds__(NTH, 2) void ns_apply_kernel(const NsArgs a) {
   constexpr int KW = Stage<NT>::KW, LD = Stage<NT>::LD, PC = Stage<NT>::PC;

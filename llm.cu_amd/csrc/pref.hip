@@ -10,12 +10,14 @@
 //
 // The arithmetic a token takes is done in fp64: a sum over a sequence of
 // thousands of differences, a ratio that is compared with the clip borders
-// and exp(d) - d - 1 of a small d all lose what matters in fp32, and at 12 to
-// 25 bytes a token the kernels stay bound by memory round trips and launches:
-// loads are issued before anything waits, four tokens a thread, and small
-// inputs take one launch.  Every sum has a fixed order.  Preference loss, 4
-// pairs of 390 tokens 5.8 us, 2048 pairs of 910 (16.8 MB) 12; policy loss, 8 x
-// 130 tokens 6.9 us, 512 x 1170 (17 MB) 12, in a graph.
+// and exp(d) - d - 1 of a small d all lose what matters in fp32.  Small inputs
+// are bound by memory round trips and launches: loads are issued before anything
+// waits, four tokens a thread, and they take one launch.  Large ones move 1.4 to
+// 1.6 TB/s in their first kernel, bound by each sequence's steps one after
+// another and, in the policy loss, by the issue of its fp64 exp and expm1.
+// Every sum has a fixed order.  Preference loss, 4 pairs of 417 tokens 5.8 us,
+// 2048 pairs of 797 (14.7 MB) 12; policy loss, 8 x 139 tokens 6.8 us, 512 x 1025
+// (15.2 MB) 12, in a graph.
 #include <algorithm>
 
 #include "../../include/llmt.h"
@@ -406,9 +408,9 @@ __global__ __launch_bounds__(NTH) void policy_count_kernel(const PolicyArgs a) {
 // The mean over the tokens: a tile of the tokens a workgroup, its sums to
 // parts[4 * blockIdx.x].  Of up to kCountHere tokens every workgroup counts the
 // kept ones by itself, the mask's 64 KB at most read from the caches, which costs
-// no more than the launch it saves (both ways, in a graph, tokens half of the
-// largest: 16 x 900 8.5 and 10.3 us, 64 x 700 10.2 and 10.9, 100 x 1000 10.6 and
-// 10.6, 200 x 1000 13.8 and 11.7).
+// no more than the launch it saves (both ways, in a graph: 16 x 522 tokens 8.5
+// and 10.3 us, 64 x 400 10.2 and 10.9, 100 x 576 10.6 and 10.6, 200 x 570 13.8
+// and 11.7).
 constexpr int kCountHere = 65536;
 constexpr int kLdsSeqs = 4096;
 __global__ __launch_bounds__(NTH) void policy_kernel(const PolicyArgs a) {
@@ -543,9 +545,9 @@ __global__ __launch_bounds__(NTH) void policy_final_kernel(const PolicyArgs a, i
 constexpr int kSeqWg = 2048;  // eight workgroups a CU
 bool one_workgroup(int T, int n) { return T <= kOneTokens && n <= kOneSeqs; }
 // A wave takes a sequence where it is one step of it (256 tokens on average:
-// 2000 x 65 8.3 us, 17 with a workgroup each), or two and the sequences are
-// more than the workgroups that the registers let run at once (2000 x 260:
-// 11.2 and 17.9; 500 x 260: 9.5 and 8.5).
+// 2000 x 57 8.4 us, 17 with a workgroup each), or two and the sequences are
+// more than the workgroups that the registers let run at once (2000 x 228:
+// 11.5 and 17.9; 500 x 228: 9.5 and 8.5).
 constexpr int kSeqResident = 768;
 bool wave_a_sequence(int T, int n) { return T / n <= (n > kSeqResident ? 512 : 256); }
 int policy_grid(int T, int n, int seq_mean) {
@@ -558,11 +560,11 @@ size_t counts_bytes() { return kCountWg * sizeof(int); }
 }  // namespace
 
 // Few and short pairs: one workgroup, a wave a pair, no second launch, which
-// costs the caller 3 us (8 x 26 tokens 5.7 us, 6.3 in two; 16 x 390: 9.0 and
-// 6.4; 16 x 1040 would be 12.9 and 7.3).  Else a workgroup a pair while all can
-// run at once (500 x 390: 6.9 us, 8.0 with a wave each), a wave a pair beyond
-// (2048 x 390: 9.3, 12.0 with a workgroup each; 2048 x 910: 12.2 and 14.1), and
-// twice the threads for long ones (100 x 2600: 7.8 and 9.2).
+// costs the caller 3 us (8 x 24 tokens 5.8 us, 6.3 in two; 16 x 345: 9.0 and
+// 6.4; 16 x 919 would be 12.9 and 7.3).  Else a workgroup a pair while all can
+// run at once (500 x 342: 6.9 us, 8.0 with a wave each), a wave a pair beyond
+// (2048 x 342: 9.4, 12.0 with a workgroup each; 2048 x 797: 12.2 and 14.1), and
+// twice the threads for long ones (100 x 2279: 7.8 and 9.2).
 hipError_t preference_loss(const PrefArgs& a, hipStream_t st) {
   constexpr int kResident = 1024;
   const int len = a.T / a.n;  // tokens a pair on average

@@ -384,8 +384,10 @@ def preference_loss(logp, ref_logp, offsets, loss="sigmoid", beta=0.1, label_smo
     """Preference loss of n pairs of sequences (llmt_preference_loss): pair i
     prefers sequence 2 i to 2 i + 1, sequence s being tokens offsets[s] ..
     offsets[s + 1] - 1 of logp and ref_logp (may be None), fp32 [T]; offsets
-    int32 [2 n + 1]; mask bool [T] keeps tokens.  Returns (mean loss [1],
-    losses [n], rewards [2 n], dlogp [T] or None)."""
+    int32 [2 n + 1]; mask bool [T] keeps tokens.  loss "square" is (z - 1/2)^2 of
+    the beta-scaled z: beta^2 times the identity-preference loss, and so is its
+    gradient.  Returns (mean loss [1], losses [n], rewards [2 n], dlogp [T] or
+    None)."""
     import torch
     kind = PREF_LOSSES.get(loss)
     if kind is None:
