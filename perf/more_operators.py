@@ -210,6 +210,8 @@ def prepare(case, seed):
         _prepare_adamw(case, st, g)
     if own:
         st["llmt"] = _llmt()
+        if case["kind"] == "adamw":  # the list that a program makes once
+            st["list"] = st["llmt"].AdamTensors(st["ps"], st["gs"], st["states"], st["copies"])
     return st
 
 
@@ -497,8 +499,7 @@ def _run_own(st):
     if kind == "embed_bwd":
         return llmt.embedding_bwd(st["tok"], st["dout"], st["dw"], scale=st["scale"],
                                   accumulate=st["add"])
-    llmt.adamw_update(st["ps"], st["gs"], st["states"], llmt.hparams(**HP), st["step"],
-                      copies=st["copies"], grad_scale=st["factor"], seed=1)
+    llmt.adamw_update(st["list"], llmt.hparams(**HP), st["step"], grad_scale=st["factor"], seed=1)
     if st["bits"] == 32:
         return _adamw_outputs(st, [st["m"], st["v"]])
     return _adamw_outputs(st, llmt.adamw_moments((st["m"], st["v"], st["me"], st["ve"])))
