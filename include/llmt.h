@@ -511,6 +511,107 @@ int llmt_muon_update(float* p, const float* g, float* m, int layers, int nmat,
  * llmt_lora_load_state (of an AdamW state) or llmt_lora_init. */
 int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params);
 
+/* ---- training all weights on packed sequences (no counterpart in the reference) ----
+ * Attention, embedding and AdamW on the caller's own tensors, for models that
+ * train more than a context's adapters.  As the operators above they run on the
+ * given stream, allocate nothing, repeat bit for bit and can be captured. */
+
+/* Heads of tokens: element (t, h, i), i < head_dim, is p[t token + h head + i]
+ * (strides in elements).  Any layout whose head_dim is contiguous: [T, heads, d],
+ * a part of a fused projection's rows, [heads, T, d].  p is 16-byte aligned, the
+ * strides are multiples of 8, token in [head_dim, 2^23], head in [0, 2^40], for
+ * q, o, dout and dq (group - 1) head at most 2^28.  An output's elements must not
+ * coincide with one another or with another argument's. */
+typedef struct {
+    void* p;
+    long long token, head;
+} llmt_heads;
+
+/* Causal attention with grouped heads over n sequences packed one behind
+ * another.  Sequence s has queries q_offsets[s] .. q_offsets[s + 1] - 1 of the
+ * Tq tokens and keys k_offsets[s] .. k_offsets[s + 1] - 1 of the Tk (device int32
+ * [n + 1], ascending; the same array where a sequence attends to itself).  Its
+ * last query sees all of its keys: with ql queries and kl keys, query t sees keys
+ * 0 .. t + kl - ql, so kl > ql continues a cache (ql = 1: a single new token), and
+ * of ql > kl the first ql - kl queries see none.  Query head h reads KV head
+ * h / (nq / nkv).
+ *   o = softmax(scale q k^T) v,  lse = ln sum exp(scale q k^T)  (fp32 [Tq, nq])
+ * A query without keys, and tokens of no sequence, have o 0 and lse -inf.  dtype
+ * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
+ * fp32, probabilities are rounded to dtype before the second product.
+ * head_dim 64 or 128; Tq nq / nkv and Tk at most 2^30. */
+typedef struct {
+    int dtype, nq, nkv, head_dim;
+    int n, Tq, Tk;
+    float scale;
+    const int* q_offsets;
+    const int* k_offsets;
+} llmt_packed_dims;
+size_t llmt_packed_attention_workspace(const llmt_packed_dims* dims);
+int llmt_packed_attention(const llmt_packed_dims* dims, const llmt_heads* q, const llmt_heads* k,
+                          const llmt_heads* v, const llmt_heads* o, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* Its gradients, in dtype: dq of the queries, dk and dv of the keys (summed over
+ * a group's query heads), from the forward's o and lse and dout = d o.  Queries
+ * without keys, keys without queries and tokens of no sequence get zeros. */
+size_t llmt_packed_attention_bwd_workspace(const llmt_packed_dims* dims);
+int llmt_packed_attention_bwd(const llmt_packed_dims* dims, const llmt_heads* q,
+                              const llmt_heads* k, const llmt_heads* v, const llmt_heads* o,
+                              const float* lse, const llmt_heads* dout, const llmt_heads* dq,
+                              const llmt_heads* dk, const llmt_heads* dv, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Embedding: out[i] = scale weight[tokens[i]], rounded once; zeros where the
+ * token is outside [0, V) (padding).  weight [V, H], ldw elements from row to
+ * row, out [T, H], ldo; LLMT_F32, LLMT_F16 or LLMT_BF16 each.  T, V and H at most
+ * 2^30. */
+int llmt_embedding(const int* tokens, int T, const void* weight, int wdtype, long long ldw, int V,
+                   int H, float scale, void* out, int odtype, long long ldo, void* stream);
+/* Its gradient: dweight[v] = scale sum of dout[i] over tokens[i] = v, or that
+ * added to what dweight holds (accumulate; rows of no token are then not
+ * touched).  Sums are fp32 in the order of the positions, rounded once. */
+size_t llmt_embedding_bwd_workspace(int T, int V, int H);
+int llmt_embedding_bwd(const int* tokens, int T, const void* dout, int ddtype, long long ldd,
+                       float scale, void* dweight, int wdtype, long long ldw, int V, int H,
+                       int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* AdamW over a list of tensors (a host array of `count` descriptors; only the
+ * pointers in it are the device's), as llmt_adamw's formula:
+ *   g' = g grad_scale (one float on the device; NULL: 1)
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + ((1 - beta2) g') g'
+ *   p = p (1 - lr wd) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * and copy, where not NULL, p rounded to copy_dtype (LLMT_F16, LLMT_BF16).  p is
+ * fp32, g any type.  state_bits 32: m and v fp32 [n].  state_bits 8: m and v
+ * bytes [n], m_exp and v_exp a byte for each 256 elements; all zero bytes are
+ * moments of 0.  Under the block's scale 2^(exp - 127), the power of two that
+ * brings its largest magnitude to at most 1.875, an m is sign, 4 exponent and 3
+ * mantissa bits (the 15th binade that of the largest), a v 5 and 3 (the 31st), with
+ * gradual underflow.  They are rounded up with the probability of their
+ * remainder, from a generator's draws of (seed, step, the tensor's place in the
+ * list, element), a v above 0 to at least its smallest code; p is updated from
+ * the moments before that rounding.  A block with a NaN or an infinity (or
+ * beyond 2^127) becomes NaN.  No two written arrays may overlap, nor a written
+ * one a gradient.  hp, step and seed are the call's: a captured call repeats
+ * them. */
+typedef struct {
+    float* p;
+    const void* g;
+    void* m;
+    void* v;
+    unsigned char* m_exp;
+    unsigned char* v_exp;
+    void* copy;
+    long long n;
+    int g_dtype, copy_dtype;
+} llmt_adam_tensor;
+int llmt_adamw_update(const llmt_adam_tensor* tensors_host, int count, int state_bits,
+                      const llmt_hparams* hp, int step, const float* grad_scale, uint64_t seed,
+                      void* stream);
+/* What 8-bit moments of n elements stand for, in fp32. */
+int llmt_adamw_moments(const void* m, const void* v, const unsigned char* m_exp,
+                       const unsigned char* v_exp, long long n, float* m32, float* v32,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -39,11 +39,12 @@ def _sources():
     return sorted(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.cpp")))
 
 
-# Per-file additions.  attn.hip (the attention forward): MFMA results and
+# Per-file additions.  attn.hip, packed_fwd.hip (the attention forwards): MFMA results and
 # accumulators in ordinary VGPRs (its softmax works on every score, so AGPR
 # copies cost VALU slots).  The backward (attn_bwd.hip) keeps its dK/dV
 # accumulators in AGPRs.
-EXTRA = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+EXTRA = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+         "packed_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _compile(src: Path, verbose: bool) -> Path:

@@ -1,0 +1,358 @@
+// api_train.cpp — C ABI of the operators for training all weights on packed
+// sequences: packed attention, embedding, AdamW over a list of tensors.  Every
+// entry point validates its arguments on the host before any launch and
+// allocates nothing on the device.
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <new>
+#include <vector>
+
+#include "../../include/llmt.h"
+#include "ops.h"
+
+using namespace llmt;
+
+#define TRY_ARG(cond, ...)    \
+  do {                        \
+    if (!(cond)) {            \
+      set_error(__VA_ARGS__); \
+      return LLMT_ERR_ARG;    \
+    }                         \
+  } while (0)
+
+static int done(hipError_t e) {
+  return e == hipSuccess ? LLMT_OK : e == hipErrorInvalidValue ? LLMT_ERR_ARG : LLMT_ERR_HIP;
+}
+
+static bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
+static bool known(int dtype) { return dtype == LLMT_F32 || dtype == LLMT_F16 || dtype == LLMT_BF16; }
+static size_t esize(int dtype) { return dtype == LLMT_F32 ? 4 : 2; }
+
+constexpr int kMost = 1 << 30;  // tokens, rows of a group's heads, columns
+constexpr long long kMaxStride = 1ll << 40;
+
+// ---------------------------------------------------------------- packed attention
+
+static bool dims_ok(const llmt_packed_dims* d) {
+  if (!d || (d->dtype != LLMT_F16 && d->dtype != LLMT_BF16)) return false;
+  if (d->head_dim != 64 && d->head_dim != 128) return false;
+  if (d->nkv < 1 || d->nq < d->nkv || d->nq % d->nkv || d->nq > 4096) return false;
+  if (d->n < 1 || d->n > (1 << 24) || d->Tq < 0 || d->Tk < 0 || d->Tk > kMost) return false;
+  const long long rows = (long long)d->Tq * (d->nq / d->nkv);
+  // workgroups: at most one each 16 rows or keys, and one a sequence, for each KV head
+  return rows <= kMost &&
+         (std::max<long long>(rows, d->Tk) / 16 + d->n + 2) * d->nkv < 0x7fffffff &&
+         (long long)d->Tq * d->nq <= 0x7fffffff;
+}
+
+struct View {
+  const char* name;
+  const llmt_heads* h;
+  int T, heads;
+  bool query, written;
+};
+
+static int check_view(const char* fn, const llmt_packed_dims* d, const View& x) {
+  TRY_ARG(x.h, "%s: NULL %s", fn, x.name);
+  if (x.T == 0) return LLMT_OK;
+  const long long t = x.h->token, h = x.h->head, hd = d->head_dim;
+  TRY_ARG(x.h->p && aligned(x.h->p, 16), "%s: %s must be given, 16-byte aligned", fn, x.name);
+  TRY_ARG(t % 8 == 0 && h % 8 == 0 && t >= hd && t <= (1 << 23) && h >= 0 && h <= kMaxStride,
+          "%s: %s has strides %lld (token) and %lld (head): multiples of 8, token in [%lld, 2^23]",
+          fn, x.name, t, h, hd);
+  const long long g = d->nq / d->nkv;
+  TRY_ARG(!x.query || (g - 1) * h <= (1 << 28), "%s: %s has a head stride of %lld over %lld heads",
+          fn, x.name, h, g);
+  TRY_ARG(!x.written || x.heads == 1 || (h >= hd && t >= (x.heads - 1) * h + hd) ||
+              h >= (x.T - 1) * t + hd,
+          "%s: %s overlaps itself (strides %lld, %lld)", fn, x.name, t, h);
+  return LLMT_OK;
+}
+
+// Whether two views have no element in common: apart from one another, or
+// columns of their own in rows of the same stride.
+static bool views_apart(const View& a, const View& b, int hd) {
+  if (a.T == 0 || b.T == 0) return true;
+  auto extent = [&](const View& x) {
+    return ((x.T - 1) * x.h->token + (x.heads - 1) * x.h->head + hd) * 2;
+  };
+  const intptr_t pa = (intptr_t)a.h->p, pb = (intptr_t)b.h->p;
+  if (pa + extent(a) <= pb || pb + extent(b) <= pa) return true;
+  const long long t = a.h->token * 2;
+  const long long wa = ((a.heads - 1) * a.h->head + hd) * 2, wb = ((b.heads - 1) * b.h->head + hd) * 2;
+  if (b.h->token * 2 != t || wa > t || wb > t) return false;
+  const long long delta = (((pb - pa) % t) + t) % t;
+  return delta >= wa && delta + wb <= t;
+}
+
+static int check_packed(const char* fn, const llmt_packed_dims* d, const View* v, int nv,
+                        const float* lse) {
+  TRY_ARG(dims_ok(d), "%s: dtype f16 or bf16, head_dim 64 or 128, nq a multiple of nkv, n in "
+          "[1, 2^24], Tq nq / nkv and Tk at most 2^30", fn);
+  TRY_ARG(d->scale > 0.f && isfinite(d->scale), "%s: scale must be positive and finite", fn);
+  TRY_ARG(d->q_offsets && d->k_offsets && aligned(d->q_offsets, 4) && aligned(d->k_offsets, 4),
+          "%s: offsets must be given, 4-byte aligned", fn);
+  for (int i = 0; i < nv; ++i) {
+    const int rc = check_view(fn, d, v[i]);
+    if (rc) return rc;
+  }
+  TRY_ARG(d->Tq == 0 || (lse && aligned(lse, 4)), "%s: lse must be given, 4-byte aligned", fn);
+  for (int i = 0; i < nv; ++i)
+    for (int k = 0; k < nv; ++k)
+      TRY_ARG(i == k || !v[i].written || views_apart(v[i], v[k], d->head_dim), "%s: %s overlaps %s",
+              fn, v[i].name, v[k].name);
+  return LLMT_OK;
+}
+
+static Heads heads(const llmt_heads* h) { return {h->p, h->token, h->head}; }
+
+static PackArgs pack_args(const llmt_packed_dims* d) {
+  PackArgs a{};
+  a.qoff = d->q_offsets;
+  a.koff = d->k_offsets;
+  a.n = d->n;
+  a.Tq = d->Tq;
+  a.Tk = d->Tk;
+  a.nq = d->nq;
+  a.nkv = d->nkv;
+  a.hd = d->head_dim;
+  a.bf16 = d->dtype == LLMT_BF16;
+  a.scale = d->scale;
+  return a;
+}
+
+static int check_space(const char* fn, size_t need, const void* ws, size_t bytes) {
+  TRY_ARG(need == 0 || (ws && bytes >= need && aligned(ws, 16)),
+          "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", fn, ws ? bytes : 0, need);
+  return LLMT_OK;
+}
+
+// ---------------------------------------------------------------- AdamW
+
+// Whether no written array of the list meets another array of it (gradients may
+// meet one another).  Lists in the order of one arena a kind, the usual case,
+// are seen to be apart in one pass; others are sorted.
+struct Extent {
+  uintptr_t a, b;
+  bool written;
+};
+static bool list_apart(const llmt_adam_tensor* t, int count, int bits) {
+  constexpr int kKinds = 7;
+  auto extent = [&](const llmt_adam_tensor& x, int k) -> Extent {
+    const size_t ms = bits == 8 ? 1 : 4, nb = (size_t)((x.n + 255) / 256);
+    const void* p[kKinds] = {x.p, x.m, x.v, x.copy, bits == 8 ? x.m_exp : nullptr,
+                             bits == 8 ? x.v_exp : nullptr, x.g};
+    const size_t n = (size_t)x.n;
+    const size_t bytes[kKinds] = {n * 4, n * ms, n * ms, n * 2, nb, nb, n * esize(x.g_dtype)};
+    return {(uintptr_t)p[k], p[k] ? (uintptr_t)p[k] + bytes[k] : (uintptr_t)p[k], k < kKinds - 1};
+  };
+  bool ordered = true;
+  Extent all[kKinds];
+  for (int k = 0; k < kKinds && ordered; ++k) {
+    uintptr_t lo = UINTPTR_MAX, hi = 0;
+    for (int i = 0; i < count && ordered; ++i) {
+      const Extent e = extent(t[i], k);
+      if (e.a == e.b) continue;
+      if (e.written && e.a < hi) ordered = false;
+      lo = std::min(lo, e.a);
+      hi = std::max(hi, e.b);
+    }
+    all[k] = {lo, hi, k < kKinds - 1};
+    for (int q = 0; q < k && ordered; ++q)
+      if (all[k].a < all[k].b && all[q].a < all[q].b && all[k].a < all[q].b && all[q].a < all[k].b)
+        ordered = false;
+  }
+  if (ordered) return true;
+  std::vector<Extent> x;
+  x.reserve((size_t)count * kKinds);
+  for (int i = 0; i < count; ++i)
+    for (int k = 0; k < kKinds; ++k) {
+      const Extent e = extent(t[i], k);
+      if (e.a != e.b) x.push_back(e);
+    }
+  std::sort(x.begin(), x.end(), [](const Extent& p, const Extent& q) { return p.a < q.a; });
+  uintptr_t any = 0, written = 0;  // where what began earlier ends
+  for (const Extent& e : x) {
+    if (e.a < (e.written ? any : written)) return false;
+    any = std::max(any, e.b);
+    if (e.written) written = std::max(written, e.b);
+  }
+  return true;
+}
+
+extern "C" {
+
+size_t llmt_packed_attention_workspace(const llmt_packed_dims* dims) {
+  return dims_ok(dims) ? packed_fwd_workspace(pack_args(dims)) : 0;
+}
+
+int llmt_packed_attention(const llmt_packed_dims* d, const llmt_heads* q, const llmt_heads* k,
+                          const llmt_heads* v, const llmt_heads* o, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  set_error("");
+  const char* const fn = "llmt_packed_attention";
+  TRY_ARG(d, "%s: NULL dims", fn);
+  const View views[4] = {{"q", q, d->Tq, d->nq, true, false},
+                         {"k", k, d->Tk, d->nkv, false, false},
+                         {"v", v, d->Tk, d->nkv, false, false},
+                         {"o", o, d->Tq, d->nq, true, true}};
+  int rc = check_packed(fn, d, views, 4, lse);
+  if (rc) return rc;
+  PackArgs a = pack_args(d);
+  if ((rc = check_space(fn, packed_fwd_workspace(a), workspace, workspace_bytes))) return rc;
+  a.q = heads(q);
+  a.k = heads(k);
+  a.v = heads(v);
+  a.o = heads(o);
+  a.lse = lse;
+  return done(packed_fwd(a, workspace, (hipStream_t)stream));
+}
+
+size_t llmt_packed_attention_bwd_workspace(const llmt_packed_dims* dims) {
+  return dims_ok(dims) ? packed_bwd_workspace(pack_args(dims)) : 0;
+}
+
+int llmt_packed_attention_bwd(const llmt_packed_dims* d, const llmt_heads* q, const llmt_heads* k,
+                              const llmt_heads* v, const llmt_heads* o, const float* lse,
+                              const llmt_heads* dout, const llmt_heads* dq, const llmt_heads* dk,
+                              const llmt_heads* dv, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  set_error("");
+  const char* const fn = "llmt_packed_attention_bwd";
+  TRY_ARG(d, "%s: NULL dims", fn);
+  const View views[8] = {{"q", q, d->Tq, d->nq, true, false},
+                         {"k", k, d->Tk, d->nkv, false, false},
+                         {"v", v, d->Tk, d->nkv, false, false},
+                         {"o", o, d->Tq, d->nq, true, false},
+                         {"dout", dout, d->Tq, d->nq, true, false},
+                         {"dq", dq, d->Tq, d->nq, true, true},
+                         {"dk", dk, d->Tk, d->nkv, false, true},
+                         {"dv", dv, d->Tk, d->nkv, false, true}};
+  int rc = check_packed(fn, d, views, 8, lse);
+  if (rc) return rc;
+  PackArgs a = pack_args(d);
+  if ((rc = check_space(fn, packed_bwd_workspace(a), workspace, workspace_bytes))) return rc;
+  a.q = heads(q);
+  a.k = heads(k);
+  a.v = heads(v);
+  a.o = heads(o);
+  a.lse = const_cast<float*>(lse);
+  a.dout = heads(dout);
+  a.dq = heads(dq);
+  a.dk = heads(dk);
+  a.dv = heads(dv);
+  return done(packed_bwd(a, workspace, (hipStream_t)stream));
+}
+
+static int check_embed(const char* fn, const int* tokens, int T, const void* w, int wdtype,
+                       long long ldw, int V, int H, float scale, const void* x, int xdtype,
+                       long long ldx) {
+  TRY_ARG(known(wdtype) && known(xdtype), "%s: dtypes %d and %d", fn, wdtype, xdtype);
+  TRY_ARG(T >= 0 && T <= kMost && V >= 1 && V <= kMost && H >= 1 && H <= kMost,
+          "%s: T=%d V=%d H=%d (at most 2^30)", fn, T, V, H);
+  TRY_ARG(ldw >= H && ldw <= kMaxStride && ldx >= H && ldx <= kMaxStride &&
+              (double)V * ldw <= 1e18 && (double)T * ldx <= 1e18,
+          "%s: row strides %lld and %lld of rows of %d", fn, ldw, ldx, H);
+  TRY_ARG(isfinite(scale), "%s: scale must be finite", fn);
+  TRY_ARG(w && (T == 0 || (tokens && x)), "%s: NULL argument", fn);
+  TRY_ARG(aligned(w, esize(wdtype)) && aligned(x, esize(xdtype)) && aligned(tokens, 4),
+          "%s: misaligned argument", fn);
+  const uintptr_t w0 = (uintptr_t)w, x0 = (uintptr_t)x;
+  TRY_ARG(T == 0 || w0 + ((size_t)(V - 1) * ldw + H) * esize(wdtype) <= x0 ||
+              x0 + ((size_t)(T - 1) * ldx + H) * esize(xdtype) <= w0,
+          "%s: the rows overlap the table", fn);
+  return LLMT_OK;
+}
+
+int llmt_embedding(const int* tokens, int T, const void* weight, int wdtype, long long ldw, int V,
+                   int H, float scale, void* out, int odtype, long long ldo, void* stream) {
+  set_error("");
+  const int rc = check_embed("llmt_embedding", tokens, T, weight, wdtype, ldw, V, H, scale, out,
+                             odtype, ldo);
+  if (rc) return rc;
+  EmbedArgs a{tokens, T, V, H, const_cast<void*>(weight), ldw, wdtype, out, ldo, odtype, scale, 0};
+  return done(embed_fwd(a, (hipStream_t)stream));
+}
+
+size_t llmt_embedding_bwd_workspace(int T, int V, int H) {
+  return T > 0 && T <= kMost && V >= 1 && V <= kMost && H >= 1 && H <= kMost
+             ? embed_bwd_workspace(T, V, H) : 0;
+}
+
+int llmt_embedding_bwd(const int* tokens, int T, const void* dout, int ddtype, long long ldd,
+                       float scale, void* dweight, int wdtype, long long ldw, int V, int H,
+                       int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
+  set_error("");
+  const char* const fn = "llmt_embedding_bwd";
+  int rc = check_embed(fn, tokens, T, dweight, wdtype, ldw, V, H, scale, dout, ddtype, ldd);
+  if (rc) return rc;
+  const size_t need = T > 0 ? embed_bwd_workspace(T, V, H) : 0;
+  if ((rc = check_space(fn, need, workspace, workspace_bytes))) return rc;
+  EmbedArgs a{tokens, T, V, H, dweight, ldw, wdtype, const_cast<void*>(dout), ldd, ddtype, scale,
+              accumulate != 0};
+  return done(embed_bwd(a, workspace, (hipStream_t)stream));
+}
+
+int llmt_adamw_update(const llmt_adam_tensor* t, int count, int state_bits, const llmt_hparams* hp,
+                      int step, const float* grad_scale, uint64_t seed, void* stream) {
+  set_error("");
+  const char* const fn = "llmt_adamw_update";
+  TRY_ARG(count >= 0 && count <= (1 << 20) && (t || count == 0), "%s: %d tensors", fn, count);
+  TRY_ARG(state_bits == 8 || state_bits == 32, "%s: moments of %d bits (8 or 32)", fn, state_bits);
+  TRY_ARG(hp, "%s: NULL hp", fn);
+  TRY_ARG(isfinite(hp->lr) && isfinite(hp->wd) && hp->beta1 >= 0.f && hp->beta1 < 1.f &&
+              hp->beta2 >= 0.f && hp->beta2 < 1.f && hp->eps > 0.f && isfinite(hp->eps) && step >= 1,
+          "%s: betas in [0, 1), eps positive, step from 1 on, finite lr and wd", fn);
+  TRY_ARG(aligned(grad_scale, 4), "%s: misaligned grad_scale", fn);
+  for (int i = 0; i < count; ++i) {
+    const llmt_adam_tensor& x = t[i];
+    TRY_ARG(x.n >= 0 && x.n <= kMaxStride, "%s: tensor %d has %lld elements", fn, i, x.n);
+    TRY_ARG(known(x.g_dtype) && (!x.copy || x.copy_dtype == LLMT_F16 || x.copy_dtype == LLMT_BF16),
+            "%s: tensor %d: gradient dtype %d, copy dtype %d (f16 or bf16)", fn, i, x.g_dtype,
+            x.copy_dtype);
+    if (x.n == 0) continue;
+    TRY_ARG(x.p && x.g && x.m && x.v && (state_bits == 32 || (x.m_exp && x.v_exp)),
+            "%s: tensor %d: NULL argument", fn, i);
+    const size_t ms = state_bits == 8 ? 1 : 4;
+    TRY_ARG(aligned(x.p, 4) && aligned(x.g, esize(x.g_dtype)) && aligned(x.m, ms) &&
+                aligned(x.v, ms) && aligned(x.copy, 2),
+            "%s: tensor %d: misaligned argument", fn, i);
+  }
+  try {
+    TRY_ARG(list_apart(t, count, state_bits), "%s: a written array overlaps another", fn);
+  } catch (const std::bad_alloc&) {
+    TRY_ARG(false, "%s: out of host memory", fn);
+  }
+  static_assert(sizeof(AdamTensor) == sizeof(llmt_adam_tensor), "one layout");
+  AdamStep k{};
+  k.b1 = hp->beta1;
+  k.b2 = hp->beta2;
+  k.c1 = 1.0f - hp->beta1;
+  k.c2 = 1.0f - hp->beta2;
+  k.ib1 = (float)(1.0 / (1.0 - pow((double)hp->beta1, step)));
+  k.ib2 = (float)(1.0 / (1.0 - pow((double)hp->beta2, step)));
+  k.decay = (float)(1.0 - (double)hp->lr * hp->wd);
+  k.lr = hp->lr;
+  k.eps = hp->eps;
+  k.gscale = grad_scale;
+  k.seed = seed;
+  k.step = step;
+  return done(adamw_list(reinterpret_cast<const AdamTensor*>(t), count, state_bits, k,
+                         (hipStream_t)stream));
+}
+
+int llmt_adamw_moments(const void* m, const void* v, const unsigned char* m_exp,
+                       const unsigned char* v_exp, long long n, float* m32, float* v32,
+                       void* stream) {
+  set_error("");
+  const char* const fn = "llmt_adamw_moments";
+  TRY_ARG(n >= 0 && n <= kMaxStride, "%s: n=%lld", fn, n);
+  if (n == 0) return LLMT_OK;
+  TRY_ARG(m && v && m_exp && v_exp && m32 && v32, "%s: NULL argument", fn);
+  TRY_ARG(aligned(m32, 4) && aligned(v32, 4), "%s: misaligned argument", fn);
+  return done(adamw_moments(m, v, m_exp, v_exp, n, m32, v32, (hipStream_t)stream));
+}
+
+}  // extern "C"

@@ -370,6 +370,66 @@ hipError_t adamw(float* p, const float* g, float* m, float* v, long long n, cons
 hipError_t lora_init(float* p, float* m, float* v, long long n, unsigned long long seed,
                      float a_std, float b_std, const AdamShadow& sh, hipStream_t st);
 
+// ---------------------------------------------------------------- packed sequences
+// Heads of tokens: element (t, h, i) at p[t token + h head + i].
+struct Heads {
+  void* p;
+  long long token, head;
+};
+struct PackArgs {
+  Heads q, k, v, o;    // q, o [Tq, nq, hd]; k, v [Tk, nkv, hd]
+  Heads dout, dq, dk, dv;
+  float* lse;          // [Tq, nq]; -inf where a query has no keys
+  const int* qoff;     // [n + 1] each
+  const int* koff;
+  int n, Tq, Tk, nq, nkv, hd, bf16;
+  float scale;
+};
+size_t packed_fwd_workspace(const PackArgs& a);
+hipError_t packed_fwd(const PackArgs& a, void* workspace, hipStream_t st);
+size_t packed_bwd_workspace(const PackArgs& a);
+hipError_t packed_bwd(const PackArgs& a, void* workspace, hipStream_t st);
+
+// Embedding: out[i] = scale * w[tok[i]] (zeros where tok[i] is outside [0, V)).
+struct EmbedArgs {
+  const int* tok;
+  int T, V, H;
+  const void* w;       // [V, ldw]; the backward's dw, written
+  long long ldw;
+  int wtype;
+  void* x;             // [T, ldx]: output rows; the backward's dout, read
+  long long ldx;
+  int xtype;
+  float scale;
+  int add;             // backward: added to what dw holds
+};
+hipError_t embed_fwd(const EmbedArgs& a, hipStream_t st);
+size_t embed_bwd_workspace(int T, int V, int H);
+hipError_t embed_bwd(const EmbedArgs& a, void* workspace, hipStream_t st);
+
+// AdamW over a list of tensors.
+struct AdamTensor {
+  float* p;
+  const void* g;
+  void* m;             // fp32, or a code an element
+  void* v;
+  unsigned char* mexp; // 8-bit moments: an exponent a block of 256
+  unsigned char* vexp;
+  void* copy;          // NULL, or the 16-bit working copy
+  long long n;
+  int gtype, ctype;
+};
+struct AdamStep {
+  float b1, b2, c1, c2, ib1, ib2, decay, lr, eps;
+  const float* gscale; // NULL, or one factor of the gradients on the device
+  unsigned long long seed;  // mixed; of the tensors' draws
+  int step;
+};
+hipError_t adamw_list(const AdamTensor* t, int count, int bits, const AdamStep& k, hipStream_t st);
+hipError_t adamw_moments(const void* m, const void* v, const unsigned char* mexp,
+                         const unsigned char* vexp, long long n, float* m32, float* v32,
+                         hipStream_t st);
+
 // ---------------------------------------------------------------- tuning losses
 // Element types of caller-supplied logits (LLMT_F32, LLMT_F16, LLMT_BF16).
 enum { kF32 = 0, kF16 = 1, kBF16 = 2 };

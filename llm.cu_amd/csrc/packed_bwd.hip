@@ -1,0 +1,403 @@
+// packed_bwd.hip — backward of the packed attention, recomputing the
+// probabilities from q, k and the forward's lse:
+//   P = exp(scale q k^T - lse), dP = dO v^T, dS = P (dP - delta),
+//   delta = rowsum(dO o), dQ = scale dS k, dK = scale dS^T q, dV = P^T dO.
+// Two kinds of workgroups that share no outputs: dQ blocks (rows of one KV
+// head's group, walking their keys) and dK/dV blocks (keys, walking the rows
+// that see them: a sum over the whole group in registers, in a fixed order, no
+// atomics).  Rows, tiles and offsets: packed_attn.h.
+//
+// fp16.  dS spans many binades (a probability of one key in many times a small
+// gradient), so it enters its product times a power of two that belongs to the
+// accumulator's column (a row in dQ, a key in dK) and follows the largest value
+// seen, as a running maximum does; when it changes the column is rescaled,
+// exactly.  bf16 has the range.
+#include <algorithm>
+#include <type_traits>
+
+#include "packed_attn.h"
+
+namespace llmt {
+
+namespace {
+
+// Of each row in the order (KV head, token, head in the group): the base-2 lse,
+// +inf for a row without keys (its probabilities are then 0), and delta.
+struct RowVecs {
+  float* lse2;
+  float* delta;
+};
+__device__ __forceinline__ long long vec_at(const PackArgs& a, int G, int j, long long token) {
+  return ((long long)j * a.Tq + token) * G;
+}
+
+template <class E, int HD>
+__global__ __launch_bounds__(256) void packed_delta_kernel(const PackArgs a, Group gr, RowVecs rv) {
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  constexpr int LR = HD / 8;  // lanes a row
+  const long long R = (long long)a.Tq * a.nq;
+  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  const long long rc = row < R ? row : R - 1;
+  const long long t = rc / a.nq;
+  const int h = (int)(rc - t * a.nq), d = (threadIdx.x % LR) * 8;
+  const T8 x = *reinterpret_cast<const T8*>((const short*)a.dout.p + t * a.dout.token +
+                                            h * a.dout.head + d);
+  const T8 y = *reinterpret_cast<const T8*>((const short*)a.o.p + t * a.o.token + h * a.o.head + d);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s = fmaf((float)x[i], (float)y[i], s);
+  s += dpp16<0xB1>(s);
+  s += dpp16<0x4E>(s);
+  s += dpp16<0x141>(s);
+  if constexpr (LR == 16) s += dpp16<0x140>(s);
+  if (row < R && d == 0) {
+    const int j = h / gr.G;
+    const long long at = vec_at(a, gr.G, j, t) + (h - j * gr.G);
+    const float e = a.lse[rc];
+    rv.lse2[at] = e == -INFINITY ? INFINITY : e * LOG2E;
+    rv.delta[at] = s;
+  }
+}
+
+// The running power of two of an accumulator column.  Returns the factor that
+// brings what has been summed to the new scale.
+struct ColScale {
+  float s = 0x1p100f;
+  __device__ __forceinline__ float follow(float amax) {
+    // amax s in [2^14, 2^15) at most; a maximum of 0 asks for nothing, inf and
+    // NaN keep what is there
+    const int e = __builtin_amdgcn_frexp_expf(amax);
+    const float want = amax > 0.f ? ldexpf(1.0f, min(100, 15 - e)) : s;
+    const float n = fminf(s, want);
+    const float f = n / s;
+    s = n;
+    return f;
+  }
+};
+
+// ---------------------------------------------------------------- dQ
+template <class E, int HD, int NW, int RW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
+  constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+  constexpr bool F = std::is_same_v<E, F16>;
+  __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  Tile x;
+  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+  const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
+  const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
+  const int nkb = (x.kmax + BLK - 1) / BLK;
+  KeyDma<HD, NW, BLK> dk, dv;
+  dk.init(a.k.token, w);
+  dv.init(a.v.token, w);
+  if (nkb > 0) {
+    dk.issue(kbase, a.k.token, 0, x.klen, buf0, w);
+    dv.issue(vbase, a.v.token, 0, x.klen, buf0 + TILE, w);
+  }
+  const int left = x.rows - x.row0 - w * RW * 16;
+  const int wfirst = left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16) + x.shift : -1;
+  const int wlast =
+      left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16 + min(left, RW * 16) - 1) + x.shift : -1;
+  short8v qf[RW][KS], df[RW][KS];
+  int lim[RW], hq[RW];
+  long long at[RW];
+  float lse2[RW], del[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const int i = min(w * RW * 16 + 16 * r + c, x.rows - 1 - x.row0);
+    const int t = gr.div(x.rem + i), h = x.rem + i - t * gr.G;
+    lim[r] = 16 * r + c < left ? x.t0 + t + x.shift : -1;
+    at[r] = x.qstart + x.t0 + t;
+    hq[r] = j * gr.G + h;
+    const short* row = (const short*)a.q.p + at[r] * a.q.token + hq[r] * a.q.head;
+    const short* dor = (const short*)a.dout.p + at[r] * a.dout.token + hq[r] * a.dout.head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
+      df[r][ks] = *reinterpret_cast<const short8v*>(dor + 32 * ks + 8 * g);
+    }
+    const long long vi = vec_at(a, gr.G, j, at[r]) + h;
+    lse2[r] = rv.lse2[vi];
+    del[r] = rv.delta[vi];
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 dqT[RW][DT];
+  ColScale cs[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r)
+#pragma unroll
+    for (int i = 0; i < DT; ++i) dqT[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  auto tile_step = [&](int kb, auto mask_tag, const short* Ks, short* nb) LLMT_INLINE {
+    wait_vm<0>();
+    tile_barrier();
+    if (kb + 1 < nkb) {
+      dk.issue(kbase, a.k.token, (kb + 1) * BLK, x.klen, nb, w);
+      dv.issue(vbase, a.v.token, (kb + 1) * BLK, x.klen, nb + TILE, w);
+    }
+    constexpr bool MASK = decltype(mask_tag)::value;
+    if (MASK && kb * BLK > wlast) return;
+    const short* Vs = Ks + TILE;
+    floatx4 pt[RW][4], dp[RW][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        pt[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+        dp[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const short8v kf = frag_rm<HD>(Ks, mt * 16, ks, lane);
+        const short8v vf = frag_rm<HD>(Vs, mt * 16, ks, lane);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          pt[r][mt] = E::mfma(kf, qf[r][ks], pt[r][mt]);
+          dp[r][mt] = E::mfma(vf, df[r][ks], dp[r][mt]);
+        }
+      }
+    }
+    sched_reads_ahead<8 * KS, 8 * KS * RW, 8, 2 * RW, 2, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      float am = 0.f;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float pv = __builtin_amdgcn_exp2f(fmaf(pt[r][mt][v], sl2, -lse2[r]));
+          if (MASK) pv = kb * BLK + mt * 16 + 4 * g + v <= lim[r] ? pv : 0.f;
+          dp[r][mt][v] = pv * (dp[r][mt][v] - del[r]);
+          if (F) am = fmaxf(am, fabsf(dp[r][mt][v]));
+        }
+      if constexpr (F) {
+        const float f = cs[r].follow(xg_max(am));
+        if (__ballot(f != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < DT; ++i) dqT[r][i] *= f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) dp[r][mt] *= cs[r].s;
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      short8v db[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) db[r] = pair_frag<E>(dp[r][2 * jj], dp[r][2 * jj + 1]);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const short8v kt = frag_tr<HD>(Ks, d * 16, jj, lane);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) dqT[r][d] = E::mfma(kt, db[r], dqT[r][d]);
+      }
+    }
+    sched_reads_ahead<4 * DT, 2 * DT * RW, 8, RW, 2, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // the tiles that every row of the wave sees whole first, without masks
+  const int nfull = left >= RW * 16 ? min((wfirst + 1) / BLK, nkb) : 0;
+  for (int kb = 0; kb < nfull; kb += 2) {
+    tile_step(kb, std::false_type{}, buf0, buf1);
+    if (kb + 1 < nfull) tile_step(kb + 1, std::false_type{}, buf1, buf0);
+  }
+  for (int kb = max(nfull, 0); kb < nkb; ++kb)
+    tile_step(kb, std::true_type{}, (kb & 1) ? buf1 : buf0, (kb & 1) ? buf0 : buf1);
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    if (16 * r + c >= left) continue;
+    const float f = F ? a.scale / cs[r].s : a.scale;
+    short* dq = (short*)a.dq.p + at[r] * a.dq.token + hq[r] * a.dq.head;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<short4v*>(dq + d * 16 + 4 * g) = round4<E>(dqT[r][d] * f);
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+// 64 NW / 4 keys a workgroup, 16 a wave, in registers; the rows that see them
+// pass through LDS in tiles of 64 with their lse and delta.  Row r sees key k
+// where r >= (k - shift) G.
+template <class E, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void packed_dkdv_kernel(const PackArgs a, Group gr, RowVecs rv) {
+  constexpr int KB = NW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+  constexpr bool F = std::is_same_v<E, F16>;
+  constexpr int BUF = 2 * TILE + 2 * BLK * 2;
+  __shared__ __attribute__((aligned(1024))) short buf0[BUF];
+  __shared__ __attribute__((aligned(1024))) short buf1[BUF];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  int blk;
+  const int s = find_tile<KB>(a.koff, a.n, a.Tk, 1, blockIdx.x / a.nkv, &blk);
+  const Span ks = span_of(a.koff, s, a.n, a.Tk);
+  if (blk < 0 || blk >= (ks.len + KB - 1) / KB) return;
+  Span qs = {0, 0};
+  if (s > 0 && s <= a.n) qs = span_of(a.qoff, s, a.n, a.Tq);
+  const int shift = ks.len - qs.len, rows = qs.len * gr.G;
+  const int k0 = blk * KB, kw = k0 + w * 16;
+  const int r0 = min(max(k0 - shift, 0), qs.len) * gr.G;  // the first row that sees a key
+  const int niter = (rows - r0 + BLK - 1) / BLK;
+  // the lane's key, and the first row that sees it
+  const int key = kw + c;
+  const int rmin = key < ks.len ? max(key - shift, 0) * gr.G : 0x7fffffff;
+  const int rfull = kw + 16 <= ks.len ? max(kw + 15 - shift, 0) * gr.G : 0x7fffffff;
+  const short* qbase = (const short*)a.q.p + qs.start * a.q.token + j * gr.G * a.q.head;
+  const short* dbase = (const short*)a.dout.p + qs.start * a.dout.token + j * gr.G * a.dout.head;
+  const long long vbase = vec_at(a, gr.G, j, qs.start);
+  using Dma = RowDma<HD, NW, BLK>;
+  auto issue = [&](int it, short* buf) LLMT_INLINE {
+    const int r = r0 + it * BLK;
+    Dma::go(qbase, a.q.token, a.q.head, gr, r, rows, buf, w);
+    Dma::go(dbase, a.dout.token, a.dout.head, gr, r, rows, buf + TILE, w);
+    float* vec = reinterpret_cast<float*>(buf + 2 * TILE);
+    if (w == 0) dma_vec64(rv.lse2 + vbase, r, rows, vec);
+    if (w == NW - 1) dma_vec64(rv.delta + vbase, r, rows, vec + BLK);
+  };
+  if (niter > 0) issue(0, buf0);
+  const long long tok = ks.start + min(key, ks.len - 1);
+  short8v kf[KS], vf[KS];
+  {
+    const short* kr = (const short*)a.k.p + tok * a.k.token + j * a.k.head;
+    const short* vr = (const short*)a.v.p + tok * a.v.token + j * a.v.head;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      kf[i] = *reinterpret_cast<const short8v*>(kr + 32 * i + 8 * g);
+      vf[i] = *reinterpret_cast<const short8v*>(vr + 32 * i + 8 * g);
+    }
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 dkT[DT], dvT[DT];
+  ColScale cs;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) {
+    dkT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    dvT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto half_tile = [&](int jj, int r, auto mask_tag, const short* Qs, const short* Ds,
+                       const float* lse_s, const float* del_s) LLMT_INLINE {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    floatx4 p[2], ds[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int m0 = (2 * jj + u) * 16;
+      p[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+      ds[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        p[u] = E::mfma(frag_rm<HD>(Qs, m0, i, lane), kf[i], p[u]);
+        ds[u] = E::mfma(frag_rm<HD>(Ds, m0, i, lane), vf[i], ds[u]);
+      }
+    }
+    sched_reads_ahead<4 * KS, 4 * KS, KS == 4 ? 6 : 4, 2, 2, 0>();
+    __builtin_amdgcn_sched_barrier(0);
+    float am = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i0 = (2 * jj + u) * 16 + 4 * g;
+      const floatx4 ls = *reinterpret_cast<const floatx4*>(lse_s + i0);
+      const floatx4 dl = *reinterpret_cast<const floatx4*>(del_s + i0);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float pv = __builtin_amdgcn_exp2f(fmaf(p[u][v], sl2, -ls[v]));
+        if (MASK) pv = r + i0 + v >= rmin && r + i0 + v < rows ? pv : 0.f;
+        ds[u][v] = pv * (ds[u][v] - dl[v]);
+        p[u][v] = F ? pv * (float)(1 << E::PSH) : pv;
+        if (F) am = fmaxf(am, fabsf(ds[u][v]));
+      }
+    }
+    if constexpr (F) {
+      const float f = cs.follow(xg_max(am));
+      if (__ballot(f != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) dkT[i] *= f;
+      }
+      ds[0] *= cs.s;
+      ds[1] *= cs.s;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const short8v pb = pair_frag<E>(p[0], p[1]), db = pair_frag<E>(ds[0], ds[1]);
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      dvT[i] = E::mfma(frag_tr<HD>(Ds, i * 16, jj, lane), pb, dvT[i]);
+      dkT[i] = E::mfma(frag_tr<HD>(Qs, i * 16, jj, lane), db, dkT[i]);
+    }
+    sched_reads_ahead<4 * DT, 2 * DT, 8, 2, 4, 1>();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto tile_step = [&](int it, const short* buf, short* nb) LLMT_INLINE {
+    wait_vm<0>();
+    tile_barrier();
+    if (it + 1 < niter) issue(it + 1, nb);
+    const short* Ds = buf + TILE;
+    const float* lse_s = reinterpret_cast<const float*>(buf + 2 * TILE);
+    const float* del_s = lse_s + BLK;
+    const int r = r0 + it * BLK;
+    if (r >= rfull && r + BLK <= rows) {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+        half_tile(jj, r, std::false_type{}, buf, Ds, lse_s, del_s);
+    } else {
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) half_tile(jj, r, std::true_type{}, buf, Ds, lse_s, del_s);
+    }
+  };
+  for (int it = 0; it < niter; it += 2) {
+    tile_step(it, buf0, buf1);
+    if (it + 1 < niter) tile_step(it + 1, buf1, buf0);
+  }
+  if (key < ks.len) {
+    const float fk = F ? a.scale / cs.s : a.scale;
+    const float fv = 1.0f / (float)(1 << E::PSH);
+    short* dkr = (short*)a.dk.p + tok * a.dk.token + j * a.dk.head;
+    short* dvr = (short*)a.dv.p + tok * a.dv.token + j * a.dv.head;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      *reinterpret_cast<short4v*>(dkr + i * 16 + 4 * g) = round4<E>(dkT[i] * fk);
+      *reinterpret_cast<short4v*>(dvr + i * 16 + 4 * g) = round4<E>(dvT[i] * fv);
+    }
+  }
+}
+
+template <class E, int HD>
+hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
+  const Group gr = group_of(a);
+  const long long R = (long long)a.Tq * a.nq;
+  RowVecs rv = {(float*)ws, (float*)ws + R};
+  if (a.Tq) {
+    constexpr int RB = 256 / (HD / 8);
+    hipLaunchKernelGGL((packed_delta_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)),
+                       dim3(256), 0, st, a, gr, rv);
+    LLMT_LAUNCH_CHECK();
+    const int nt = row_tiles(a, 64);
+    hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), dim3((unsigned)nt * a.nkv), dim3(256), 0, st,
+                       a, gr, nt, rv);
+    LLMT_LAUNCH_CHECK();
+  }
+  if (a.Tk) {
+    hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), dim3((unsigned)key_tiles(a, 64) * a.nkv),
+                       dim3(256), 0, st, a, gr, rv);
+    LLMT_LAUNCH_CHECK();
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t packed_bwd_workspace(const PackArgs& a) { return (size_t)a.Tq * a.nq * 8; }
+
+hipError_t packed_bwd(const PackArgs& a, void* ws, hipStream_t st) {
+  if (a.hd == 128) return a.bf16 ? launch<B16, 128>(a, ws, st) : launch<F16, 128>(a, ws, st);
+  return a.bf16 ? launch<B16, 64>(a, ws, st) : launch<F16, 64>(a, ws, st);
+}
+
+}  // namespace llmt

@@ -1,0 +1,433 @@
+// packed_fwd.hip — forward of the packed attention: o = softmax(scale q k^T) v
+// over the keys that a query may see, and the log of each row's sum of
+// exponentials.  Rows, tiles and offsets: packed_attn.h.
+//
+// Query t of a sequence with ql queries and kl keys sees keys 0 .. t + kl - ql
+// (its own position where the two are equally long); below 0 it sees none, its
+// output is 0 and its lse -inf.  One pass over the keys with the running
+// maximum and sum; the scores never leave registers.
+#include <algorithm>
+
+#include "packed_attn.h"
+
+namespace llmt {
+
+namespace {
+
+// A tile of 16 MT keys of the running softmax for RW 16-row tiles of a wave:
+// st holds raw scores (rows key, column row) and on return probabilities
+// relative to the running maximum, times 2^PSH.  lim: the last key a lane's
+// row sees.
+template <class E, int RW, int DT, bool MASK, int MT>
+__device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[RW], float (&l)[RW],
+                                             floatx4 (&ot)[RW][DT], float sl2, int key0,
+                                             const int (&lim)[RW], int lane) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    float bm = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float s = st[r][mt][v];
+        if (MASK) {
+          s = key0 + mt * 16 + 4 * g + v <= lim[r] ? s : -INFINITY;
+          st[r][mt][v] = s;
+        }
+        bm = fmaxf(bm, s);
+      }
+    bm = xg_max(bm);
+    const float mn = fmaxf(m[r], bm * sl2);  // sl2 > 0: the maximum commutes with the scale
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m[r] - mu);
+    m[r] = mn;
+    const float shift = mu - E::PSH;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        st[r][mt][v] = __builtin_amdgcn_exp2f(fmaf(st[r][mt][v], sl2, -shift));
+    float ps[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      ps[mt] = (st[r][mt][0] + st[r][mt][1]) + (st[r][mt][2] + st[r][mt][3]);
+    if constexpr (MT == 4)
+      l[r] = l[r] * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+    else
+      l[r] = l[r] * alpha + (ps[0] + ps[1]);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) ot[r][dt] *= alpha;
+  }
+}
+
+// Tile by tile, NW waves of 16 RW rows each walk all keys of the workgroup's
+// rows, K and V in LDS tiles of 64 keys, two buffers.
+template <class E, int HD, int NW, int RW>
+__global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, Group gr,
+                                                             int ntiles) {
+  constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+  __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  Tile x;
+  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+
+  const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
+  const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
+  const int nkb = (x.kmax + BLK - 1) / BLK;
+  KeyDma<HD, NW, BLK> dk, dv;
+  dk.init(a.k.token, w);
+  dv.init(a.v.token, w);
+  if (nkb > 0) {
+    dk.issue(kbase, a.k.token, 0, x.klen, buf0, w);
+    dv.issue(vbase, a.v.token, 0, x.klen, buf0 + TILE, w);
+  }
+  const int left = x.rows - x.row0 - w * RW * 16;  // rows from the wave's first on
+  // the last key that the wave's first and last row see
+  const int wfirst = left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16) + x.shift : -1;
+  const int wlast =
+      left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16 + min(left, RW * 16) - 1) + x.shift : -1;
+  short8v qf[RW][KS];
+  int lim[RW];
+  long long at[RW];  // token, and the query head
+  int hq[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const int i = min(w * RW * 16 + 16 * r + c, x.rows - 1 - x.row0);
+    const int t = gr.div(x.rem + i), h = x.rem + i - t * gr.G;
+    const bool ok = 16 * r + c < left;
+    lim[r] = ok ? x.t0 + t + x.shift : -1;
+    at[r] = x.qstart + x.t0 + t;
+    hq[r] = j * gr.G + h;
+    const short* row = (const short*)a.q.p + at[r] * a.q.token + hq[r] * a.q.head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 ot[RW][DT];
+  float m[RW], l[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) ot[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  auto tile = [&](int kb, const short* Ks, short* nb) LLMT_INLINE {
+    wait_vm<0>();
+    tile_barrier();
+    if (kb + 1 < nkb) {
+      dk.issue(kbase, a.k.token, (kb + 1) * BLK, x.klen, nb, w);
+      dv.issue(vbase, a.v.token, (kb + 1) * BLK, x.klen, nb + TILE, w);
+    }
+    if (kb * BLK > wlast) return;  // no row of the wave sees a key of the tile
+    const short* Vs = Ks + TILE;
+    floatx4 st[RW][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) st[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const short8v kf = frag_rm<HD>(Ks, mt * 16, ks, lane);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) st[r][mt] = E::mfma(kf, qf[r][ks], st[r][mt]);
+      }
+    }
+    if (kb * BLK + BLK - 1 <= wfirst && left >= RW * 16)
+      softmax_tile<E, RW, DT, false>(st, m, l, ot, sl2, kb * BLK, lim, lane);
+    else
+      softmax_tile<E, RW, DT, true>(st, m, l, ot, sl2, kb * BLK, lim, lane);
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      short8v pb[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) pb[r] = pair_frag<E>(st[r][2 * jj], st[r][2 * jj + 1]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const short8v vf = frag_tr<HD>(Vs, dt * 16, jj, lane);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r], ot[r][dt]);
+      }
+    }
+  };
+  for (int kb = 0; kb < nkb; kb += 2) {
+    tile(kb, buf0, buf1);
+    if (kb + 1 < nkb) tile(kb + 1, buf1, buf0);
+  }
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const float lr = xg_sum(l[r]);
+    const float inv = lr > 0.f || lr != lr ? 1.0f / lr : 0.f;
+    if (16 * r + c < left) {
+      short* o = (short*)a.o.p + at[r] * a.o.token + hq[r] * a.o.head;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        *reinterpret_cast<short4v*>(o + dt * 16 + 4 * g) = round4<E>(ot[r][dt] * inv);
+      if (g == 0) a.lse[at[r] * a.nq + hq[r]] = (m[r] + (__log2f(lr) - E::PSH)) * LN2;
+    }
+  }
+}
+
+// Few rows: a workgroup takes 16 RW rows and one of nsplit parts of their keys,
+// in 32-key tiles that its four waves take in turn, each through LDS of its own
+// and without a barrier in the loop; the waves' results meet in LDS.  With
+// several parts the result goes to the workspace as (max, sum) and the
+// unnormalised output, for packed_join_kernel.
+constexpr int FS_KEYS = 32;
+struct Parts {
+  int nsplit;
+  float* o;    // [nsplit][Tq nq][hd]
+  float2* ml;  // [nsplit][Tq nq]: base-2 maximum, sum
+};
+
+template <class E, int HD, int RW>
+__global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs a, Group gr,
+                                                                  int ntiles, Parts parts) {
+  constexpr int NW = 4, QB = RW * 16, KS = HD / 32, DT = HD / 16, FT = FS_KEYS * HD;
+  // a wave's K and V tile; later its output, 16 rows x HD fp32 each
+  __shared__ __attribute__((aligned(1024))) short kbuf[NW * FT];
+  __shared__ __attribute__((aligned(1024))) short vbuf[NW * FT];
+  __shared__ float2 ml[NW][QB];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  const int part = blockIdx.y;
+  Tile x;
+  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+  const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
+  const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
+  const int nkt_all = (x.kmax + FS_KEYS - 1) / FS_KEYS;
+  const int per = (nkt_all + parts.nsplit - 1) / parts.nsplit;
+  const int kt0 = part * per + w, nkt = min(nkt_all, (part + 1) * per);
+  short* const Ks = kbuf + w * FT;
+  short* const Vs = vbuf + w * FT;
+  using Dma = KeyDma<HD, 1, FS_KEYS>;
+  Dma dk, dv;
+  dk.init(a.k.token, 0);
+  dv.init(a.v.token, 0);
+  if (kt0 < nkt) {
+    dk.issue(kbase, a.k.token, kt0 * FS_KEYS, x.klen, Ks, 0);
+    dv.issue(vbase, a.v.token, kt0 * FS_KEYS, x.klen, Vs, 0);
+  }
+  const int left = x.rows - x.row0;
+  const int wfirst = x.t0 + x.shift;
+  short8v qf[RW][KS];
+  int lim[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const int i = min(16 * r + c, left - 1);
+    const int t = gr.div(x.rem + i), h = x.rem + i - t * gr.G;
+    lim[r] = 16 * r + c < left ? x.t0 + t + x.shift : -1;
+    const short* row = (const short*)a.q.p + (long long)(x.qstart + x.t0 + t) * a.q.token +
+                       (j * gr.G + h) * a.q.head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 ot[RW][DT];
+  float m[RW], l[RW];
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) ot[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int kt = kt0; kt < nkt; kt += NW) {
+    const bool next = kt + NW < nkt;
+    if (kt != kt0) wait_vm<Dma::CH>();  // this K tile (the V tile may be in flight)
+    else wait_vm<0>();
+    asm volatile("" ::: "memory");
+    floatx4 st[RW][2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) st[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const short8v kf = frag_rm<HD>(Ks, mt * 16, ks, lane);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) st[r][mt] = E::mfma(kf, qf[r][ks], st[r][mt]);
+      }
+    }
+    wait_lds();  // the reads of the K tile have returned
+    asm volatile("" ::: "memory");
+    if (next) dk.issue(kbase, a.k.token, (kt + NW) * FS_KEYS, x.klen, Ks, 0);
+    if (kt * FS_KEYS + FS_KEYS - 1 <= wfirst && left >= QB)
+      softmax_tile<E, RW, DT, false, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
+    else
+      softmax_tile<E, RW, DT, true, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
+    short8v pb[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) pb[r] = pair_frag<E>(st[r][0], st[r][1]);
+    if (next) wait_vm<Dma::CH>();  // this V tile (the next K tile may be in flight)
+    else wait_vm<0>();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const short8v vf = frag_tr<HD>(Vs, dt * 16, 0, lane);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r], ot[r][dt]);
+    }
+    wait_lds();
+    asm volatile("" ::: "memory");
+    if (next) dv.issue(vbase, a.v.token, (kt + NW) * FS_KEYS, x.klen, Vs, 0);
+  }
+
+  // the waves' outputs meet: the first 16 rows where the wave's K tile was, the
+  // second where its V tile was, 16-byte pieces swizzled by the row; wave w then
+  // takes rows 4 w .. 4 w + 3 of each sixteen, 16 lanes a row
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    float* const xo = reinterpret_cast<float*>(r ? vbuf : kbuf) + (w * 16 + c) * HD;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      *reinterpret_cast<floatx4*>(xo + (((4 * dt + g) ^ c) << 2)) = ot[r][dt];
+    const float lw = xg_sum(l[r]);
+    if (g == 0) ml[w][16 * r + c] = make_float2(m[r], lw);
+  }
+  __syncthreads();
+  constexpr int PC = HD / 64;  // 16-byte pieces a lane
+#pragma unroll
+  for (int r = 0; r < RW; ++r) {
+    const float* const xo = reinterpret_cast<const float*>(r ? vbuf : kbuf);
+    const int qi = 4 * w + g, i = 16 * r + qi;
+    float M = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) M = fmaxf(M, ml[u][i].x);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    floatx4 o[PC];
+#pragma unroll
+    for (int e = 0; e < PC; ++e) o[e] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      const float2 p = ml[u][i];
+      const float f = __builtin_amdgcn_exp2f(p.x - mu);
+      L = fmaf(p.y, f, L);
+      const float* row = xo + (u * 16 + qi) * HD;
+#pragma unroll
+      for (int e = 0; e < PC; ++e)
+        o[e] += *reinterpret_cast<const floatx4*>(row + (((PC * c + e) ^ qi) << 2)) * f;
+    }
+    if (i < left) {
+      const int t = gr.div(x.rem + i), h = j * gr.G + x.rem + i - t * gr.G;
+      const long long tok = x.qstart + x.t0 + t;
+      if (parts.nsplit > 1) {
+        const long long at = (long long)part * a.Tq * a.nq + tok * a.nq + h;
+#pragma unroll
+        for (int e = 0; e < PC; ++e)
+          *reinterpret_cast<floatx4*>(parts.o + at * HD + (PC * c + e) * 4) = o[e];
+        if (c == 0) parts.ml[at] = make_float2(M, L);
+      } else {
+        const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
+        short* op = (short*)a.o.p + tok * a.o.token + h * a.o.head;
+#pragma unroll
+        for (int e = 0; e < PC; ++e)
+          *reinterpret_cast<short4v*>(op + (PC * c + e) * 4) = round4<E>(o[e] * inv);
+        if (c == 0) a.lse[tok * a.nq + h] = (M + (__log2f(L) - E::PSH)) * LN2;
+      }
+    }
+  }
+}
+
+// The parts of a row joined in their order: HD / 4 lanes a row.
+template <class E, int HD>
+__global__ __launch_bounds__(256) void packed_join_kernel(const PackArgs a, Parts parts) {
+  constexpr int LR = HD / 4;
+  const long long R = (long long)a.Tq * a.nq;
+  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  if (row >= R) return;
+  const int d = (threadIdx.x % LR) * 4;
+  float M = -INFINITY;
+  for (int s = 0; s < parts.nsplit; ++s) M = fmaxf(M, parts.ml[s * R + row].x);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts.nsplit; ++s) {
+    const float2 p = parts.ml[s * R + row];
+    const float f = __builtin_amdgcn_exp2f(p.x - mu);
+    L = fmaf(p.y, f, L);
+    o += *reinterpret_cast<const floatx4*>(parts.o + (s * R + row) * HD + d) * f;
+  }
+  const long long t = row / a.nq, h = row - t * a.nq;
+  const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
+  *reinterpret_cast<short4v*>((short*)a.o.p + t * a.o.token + h * a.o.head + d) =
+      round4<E>(o * inv);
+  if (d == 0) a.lse[row] = (M + (__log2f(L) - E::PSH)) * LN2;
+}
+
+// The kernel and its split.
+struct FwdPlan {
+  int nw, rw;  // nw 0: packed_fwd_split_kernel
+  int nsplit;
+};
+FwdPlan fwd_plan(const PackArgs& a) {
+  const long long rows = (long long)a.Tq * (a.nq / a.nkv);
+  const long long n = std::min(a.n, a.Tq);
+  if (rows / 128 * a.nkv >= 512) return {4, 2, 1};
+  if (rows / 64 * a.nkv >= 256) return {4, 1, 1};
+  // tiles of 16 rows: at least one a sequence that has queries
+  const long long wgs = std::max<long long>(1, std::max(rows / 16, n) * a.nkv);
+  const long long keys = a.Tk / std::max<long long>(1, n);
+  const long long most = std::min<long long>(64, std::max<long long>(1, keys / 128));
+  return {0, 1, (int)std::min(most, std::max<long long>(1, 768 / wgs))};
+}
+
+template <class E, int HD>
+hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
+  const FwdPlan p = fwd_plan(a);
+  const Group gr = group_of(a);
+  if (p.nw) {
+    const int nt = row_tiles(a, p.nw * p.rw * 16);
+    const dim3 grid((unsigned)nt * a.nkv);
+    if (p.rw == 2)
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt);
+    else
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt);
+    LLMT_LAUNCH_CHECK();
+    return hipSuccess;
+  }
+  Parts parts = {p.nsplit, nullptr, nullptr};
+  const long long R = (long long)a.Tq * a.nq;
+  if (p.nsplit > 1) {
+    parts.o = (float*)ws;
+    parts.ml = (float2*)(parts.o + p.nsplit * R * HD);
+  }
+  const int nt = row_tiles(a, 16 * p.rw);
+  hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1>), dim3((unsigned)nt * a.nkv, p.nsplit),
+                     dim3(256), 0, st, a, gr, nt, parts);
+  LLMT_LAUNCH_CHECK();
+  if (p.nsplit > 1) {
+    constexpr int RB = 256 / (HD / 4);
+    hipLaunchKernelGGL((packed_join_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)), dim3(256),
+                       0, st, a, parts);
+    LLMT_LAUNCH_CHECK();
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+size_t packed_fwd_workspace(const PackArgs& a) {
+  if (a.Tq == 0) return 0;
+  const FwdPlan p = fwd_plan(a);
+  return p.nsplit > 1 ? (size_t)p.nsplit * a.Tq * a.nq * (a.hd * 4 + 8) : 0;
+}
+
+hipError_t packed_fwd(const PackArgs& a, void* ws, hipStream_t st) {
+  if (a.Tq == 0) return hipSuccess;
+  if (a.hd == 128) return a.bf16 ? launch<B16, 128>(a, ws, st) : launch<F16, 128>(a, ws, st);
+  return a.bf16 ? launch<B16, 64>(a, ws, st) : launch<F16, 64>(a, ws, st);
+}
+
+}  // namespace llmt

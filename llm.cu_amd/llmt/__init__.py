@@ -62,6 +62,20 @@ class MuonParams(C.Structure):
                [(n, i32) for n in ("steps", "nesterov", "scale")]
 
 
+class Heads(C.Structure):
+    _fields_ = [("p", vp), ("token", i64), ("head", i64)]
+
+
+class PackedDims(C.Structure):
+    _fields_ = [(n, i32) for n in ("dtype", "nq", "nkv", "head_dim", "n", "Tq", "Tk")] + \
+               [("scale", f32), ("q_offsets", vp), ("k_offsets", vp)]
+
+
+class AdamTensor(C.Structure):
+    _fields_ = [(n, vp) for n in ("p", "g", "m", "v", "m_exp", "v_exp", "copy")] + \
+               [("n", i64), ("g_dtype", i32), ("copy_dtype", i32)]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     "llmt_last_error": (C.c_char_p, []),
@@ -91,6 +105,19 @@ _PROTOS = {
     "llmt_muon_update": (i32, [vp, vp, vp, i32, i32, C.POINTER(i32), C.POINTER(i32),
                                C.POINTER(MuonParams), vp, sz, vp]),
     "llmt_muon": (i32, [vp, C.POINTER(MuonParams)]),
+    "llmt_packed_attention_workspace": (sz, [C.POINTER(PackedDims)]),
+    "llmt_packed_attention": (i32, [C.POINTER(PackedDims)] + [C.POINTER(Heads)] * 4 +
+                              [vp, vp, sz, vp]),
+    "llmt_packed_attention_bwd_workspace": (sz, [C.POINTER(PackedDims)]),
+    "llmt_packed_attention_bwd": (i32, [C.POINTER(PackedDims)] + [C.POINTER(Heads)] * 4 + [vp] +
+                                  [C.POINTER(Heads)] * 4 + [vp, sz, vp]),
+    "llmt_embedding": (i32, [vp, i32, vp, i32, i64, i32, i32, f32, vp, i32, i64, vp]),
+    "llmt_embedding_bwd_workspace": (sz, [i32, i32, i32]),
+    "llmt_embedding_bwd": (i32, [vp, i32, vp, i32, i64, f32, vp, i32, i64, i32, i32, i32, vp, sz,
+                                 vp]),
+    "llmt_adamw_update": (i32, [C.POINTER(AdamTensor), i32, i32, C.POINTER(HParams), i32, vp, u64,
+                                vp]),
+    "llmt_adamw_moments": (i32, [vp, vp, vp, vp, i64, vp, vp, vp]),
     "llmt_ctx_create": (i32, [C.POINTER(Dims), i32, i32, i32, vp, C.POINTER(vp)]),
     "llmt_ctx_destroy": (i32, [vp]),
     "llmt_ctx_device_bytes": (sz, [vp]),
@@ -524,6 +551,270 @@ def muon_update(p, g, m, shapes, hp: MuonParams, stream=None):
         ws = p.new_empty(need, dtype=torch.uint8) if need else None
         check(L.llmt_muon_update(p.data_ptr(), g.data_ptr(), m.data_ptr(), n // per, k, rows, cols,
                                  hp, _at(ws), need, on.raw))
+
+
+# ------------------------------------------------------------------ packed sequences
+
+def _heads(name, t, like=None):
+    """A [T, heads, d] tensor as llmt_heads (the stride of one token or one head is of no
+    account)."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise LlmtError(f"{name} must be [T, heads, head_dim] with a last stride of 1")
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
+        raise LlmtError(f"{name} must be {list(like.shape)} {like.dtype} "
+                        f"(got {list(t.shape)} {t.dtype})")
+    T, heads, d = t.shape
+    token, head = t.stride(0), t.stride(1)
+    if heads < 2:
+        head = d
+    if T < 2:
+        token = (d + 7) // 8 * 8
+    return Heads(t.data_ptr(), token, head)
+
+
+def _packed_dims(q, k, v, q_offsets, k_offsets, scale):
+    import torch
+    dt = {torch.float16: 1, torch.bfloat16: 2}.get(q.dtype)
+    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise LlmtError(f"q, k and v must be float16 or bfloat16 (got {q.dtype}, {k.dtype}, "
+                        f"{v.dtype})")
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise LlmtError("q must be [Tq, nq, head_dim], k and v [Tk, nkv, head_dim]")
+    _expect("q_offsets", q_offsets, torch.int32, None)
+    n = q_offsets.shape[0] - 1
+    _expect("k_offsets", k_offsets, torch.int32, n + 1)
+    if n < 1:
+        raise LlmtError("offsets must be [n + 1] with n >= 1")
+    if k_offsets is None and k.shape[0] != q.shape[0]:
+        raise LlmtError(f"without k_offsets q and k are the same tokens (got {q.shape[0]} and "
+                        f"{k.shape[0]})")
+    d = q.shape[2]
+    _sizes("tokens, heads", n + 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], d)
+    return PackedDims(dt, q.shape[1], k.shape[1], d, n, q.shape[0], k.shape[0],
+                      d ** -0.5 if scale is None else scale, q_offsets.data_ptr(),
+                      (q_offsets if k_offsets is None else k_offsets).data_ptr())
+
+
+def packed_attention(q, k, v, q_offsets, k_offsets=None, scale=None, out=None, stream=None):
+    """Causal attention with grouped heads over packed sequences (llmt_packed_attention): q [Tq,
+    nq, d], k and v [Tk, nkv, d] fp16 or bf16, d 64 or 128, views of any strides with d
+    contiguous; sequence s has queries q_offsets[s] .. q_offsets[s + 1] - 1 and keys k_offsets[s]
+    .. (int32 [n + 1]; None: the queries').  Its last query sees all of its keys.  scale None: 1 /
+    sqrt(d).  Returns (o like q, lse fp32 [Tq, nq]); 0 and -inf where a query has no keys."""
+    import torch
+    with _On("q k v q_offsets k_offsets out", (q, k, v, q_offsets, k_offsets, out), stream) as on:
+        dims = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
+        o = q.new_empty(q.shape) if out is None else out
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+        L = lib()
+        need = L.llmt_packed_attention_workspace(dims)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_packed_attention(dims, _heads("q", q), _heads("k", k), _heads("v", v),
+                                      _heads("out", o, q), lse.data_ptr(), _at(ws), need, on.raw))
+    return o, lse
+
+
+def packed_attention_bwd(q, k, v, o, lse, dout, q_offsets, k_offsets=None, scale=None, out=None,
+                         stream=None):
+    """Gradients (dq, dk, dv) of packed_attention in q's type, from its o and lse and dout, the
+    gradient of o.  out: the three tensors to write, of any strides (parts of a fused
+    projection's gradient)."""
+    import torch
+    dq, dk, dv = (None, None, None) if out is None else out
+    with _On("q k v o lse dout q_offsets k_offsets dq dk dv",
+             (q, k, v, o, lse, dout, q_offsets, k_offsets, dq, dk, dv), stream) as on:
+        dims = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
+        _expect("lse", lse, torch.float32, q.shape[0], q.shape[1])
+        dq = q.new_empty(q.shape) if dq is None else dq
+        dk = k.new_empty(k.shape) if dk is None else dk
+        dv = v.new_empty(v.shape) if dv is None else dv
+        L = lib()
+        need = L.llmt_packed_attention_bwd_workspace(dims)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_packed_attention_bwd(
+            dims, _heads("q", q), _heads("k", k), _heads("v", v), _heads("o", o, q), lse.data_ptr(),
+            _heads("dout", dout, q), _heads("dq", dq, q), _heads("dk", dk, k), _heads("dv", dv, v),
+            _at(ws), need, on.raw))
+    return dq, dk, dv
+
+
+def embedding(tokens, weight, scale=1.0, out_dtype=None, stream=None):
+    """scale weight[tokens] (llmt_embedding): tokens int32 of any shape, weight [V, H] fp32, fp16
+    or bf16 (rows may be strided); zeros where a token is outside [0, V).  out_dtype None: the
+    weight's.  Returns [*tokens.shape, H]."""
+    import torch
+    with _On("tokens weight", (tokens, weight), stream) as on:
+        if tokens.dtype != torch.int32 or not tokens.is_contiguous():
+            raise LlmtError("tokens must be contiguous int32")
+        wd = _logits_dtype("weight", weight)
+        V, H = weight.shape
+        T = tokens.numel()
+        _sizes("tokens, V, H", T, V, H)
+        out = weight.new_empty((*tokens.shape, H), dtype=out_dtype)
+        check(lib().llmt_embedding(tokens.data_ptr(), T, weight.data_ptr(), wd, _ld(weight), V, H,
+                                   scale, out.data_ptr(), _type_code("out_dtype", out.dtype), H,
+                                   on.raw))
+    return out
+
+
+def embedding_bwd(tokens, dout, dweight, scale=1.0, accumulate=False, stream=None):
+    """The table's gradient (llmt_embedding_bwd), written into dweight [V, H] fp32, fp16 or bf16
+    (rows may be strided) or, with accumulate, added to it; tokens int32 of any shape, dout
+    [*tokens.shape, H].  Sums are in the order of the tokens' positions.  Returns dweight."""
+    import torch
+    with _On("tokens dout dweight", (tokens, dout, dweight), stream) as on:
+        if tokens.dtype != torch.int32 or not tokens.is_contiguous():
+            raise LlmtError("tokens must be contiguous int32")
+        wd = _logits_dtype("dweight", dweight)
+        V, H = dweight.shape
+        T = tokens.numel()
+        if dout.shape != (*tokens.shape, H):
+            raise LlmtError(f"dout must be {[*tokens.shape, H]} (got {list(dout.shape)})")
+        ldd = H
+        if not dout.is_contiguous():
+            if dout.dim() != 2 or (H > 1 and dout.stride(1) != 1):
+                raise LlmtError("dout must be contiguous, or [T, H] with a column stride of 1")
+            ldd = _ld(dout)
+        _sizes("tokens, V, H", T, V, H)
+        L = lib()
+        need = L.llmt_embedding_bwd_workspace(T, V, H)
+        ws = dweight.new_empty(need, dtype=torch.uint8) if need else None
+        check(L.llmt_embedding_bwd(tokens.data_ptr(), T, dout.data_ptr(),
+                                   _type_code("dout", dout.dtype), ldd, scale, dweight.data_ptr(), wd,
+                                   _ld(dweight), V, H, int(accumulate), _at(ws), need, on.raw))
+    return dweight
+
+
+def _type_code(name, dtype):
+    import torch
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    if code is None:
+        raise LlmtError(f"{name} must be float32, float16 or bfloat16 (got {dtype})")
+    return code
+
+
+class AdamState(NamedTuple):
+    """Moments of one tensor of n elements: fp32 m and v [n] (m_exp and v_exp None), or 8-bit codes
+    uint8 [n] with a byte for each block of 256 elements."""
+    m: object
+    v: object
+    m_exp: object
+    v_exp: object
+
+
+def adamw_state(p, bits=32) -> AdamState:
+    """Moments of 0 for a tensor p, of 32 or 8 bits."""
+    import torch
+    n = p.numel()
+    if bits == 32:
+        return AdamState(*(torch.zeros(n, dtype=torch.float32, device=p.device) for _ in range(2)),
+                         None, None)
+    if bits != 8:
+        raise LlmtError(f"bits must be 32 or 8 (got {bits})")
+    m, v = (torch.zeros(n, dtype=torch.uint8, device=p.device) for _ in range(2))
+    return AdamState(m, v, *(torch.zeros(-(-n // 256), dtype=torch.uint8, device=p.device)
+                             for _ in range(2)))
+
+
+class AdamTensors:
+    """A list of tensors for adamw_update: parameters fp32, gradients of any type, states (of
+    adamw_state, all of one width) and, where given, 16-bit working copies (or None for some);
+    contiguous, all on one device.  Holds the tensors: a program makes one and keeps it."""
+
+    def __init__(self, params, grads, states, copies=None):
+        import torch
+        k = len(params)
+        copies = [None] * k if copies is None else list(copies)
+        if not (len(grads) == len(states) == len(copies) == k):
+            raise LlmtError(f"{k} params, {len(grads)} grads, {len(states)} states, {len(copies)} "
+                            "copies")
+        self.tensors = []          # of every descriptor, in its order
+        self.table = (AdamTensor * k)()
+        widths = {8 if s[2] is not None else 32 for s in states}
+        if len(widths) > 1:
+            raise LlmtError("states must be all of 32 or all of 8 bits")
+        self.bits = widths.pop() if widths else 32
+        self.device = None
+        for i, (p, g, s, c) in enumerate(zip(params, grads, states, copies)):
+            n = p.numel()
+            code = torch.uint8 if self.bits == 8 else torch.float32
+            nb = -(-n // 256)
+            for name, t, dtype, size in (
+                    ("params", p, torch.float32, n), ("grads", g, None, n), ("states' m", s[0], code, n),
+                    ("states' v", s[1], code, n), ("states' m_exp", s[2], torch.uint8, nb),
+                    ("states' v_exp", s[3], torch.uint8, nb), ("copies", c, None, n)):
+                self._check(f"{name}[{i}]", t, dtype, size, self.bits, name)
+            if c is not None and c.dtype not in (torch.float16, torch.bfloat16):
+                raise LlmtError(f"copies[{i}] must be float16 or bfloat16 (got {c.dtype})")
+            self.table[i] = AdamTensor(
+                p.data_ptr(), g.data_ptr(), s[0].data_ptr(), s[1].data_ptr(), _at(s[2]), _at(s[3]),
+                _at(c), n, _type_code(f"grads[{i}]", g.dtype),
+                0 if c is None else _type_code("copies", c.dtype))
+            self.tensors.append([p, g, *s, c])
+
+    def _check(self, name, t, dtype, size, bits, kind):
+        import torch
+        if t is None:
+            if kind == "copies" or (bits == 32 and kind.endswith("exp")):
+                return
+            raise LlmtError(f"{name} is missing")
+        if not isinstance(t, torch.Tensor) or t.get_device() < 0:
+            raise LlmtError(f"{name} must be a device tensor")
+        if self.device is None:
+            self.device = t.get_device()
+        if t.get_device() != self.device:
+            raise LlmtError(f"{name} is on device {t.get_device()}, other tensors on {self.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise LlmtError(f"{name} must be {dtype} (got {t.dtype})")
+        if t.numel() != size or not t.is_contiguous():
+            raise LlmtError(f"{name} must be contiguous with {size} elements (got {t.numel()})")
+
+    def set_grads(self, grads):
+        """Other gradients for the same parameters."""
+        if len(grads) != len(self.tensors):
+            raise LlmtError(f"{len(grads)} grads for {len(self.tensors)} params")
+        for i, g in enumerate(grads):
+            self._check(f"grads[{i}]", g, None, self.table[i].n, self.bits, "grads")
+            _type_code(f"grads[{i}]", g.dtype)
+        for i, g in enumerate(grads):
+            self.table[i].g = g.data_ptr()
+            self.table[i].g_dtype = _type_code("grads", g.dtype)
+            self.tensors[i][1] = g
+
+
+def adamw_update(tensors: AdamTensors, hp: HParams, step: int, grad_scale=None, seed=0,
+                 stream=None):
+    """One AdamW step in place over all tensors (llmt_adamw_update).  grad_scale fp32 [1] on the
+    device: a factor of the gradients (clipping, a loss scale's inverse).  seed: of the 8-bit
+    moments' rounding; the step's number enters its draws too."""
+    import torch
+    if not tensors.tensors:
+        return
+    first = tensors.tensors[0][0]
+    with _On("params grad_scale", (first, grad_scale), stream) as on:
+        _expect("grad_scale", grad_scale, torch.float32, 1)
+        if stream is not None:
+            on.inputs = [t for row in tensors.tensors for t in row] + [grad_scale]
+        check(lib().llmt_adamw_update(tensors.table, len(tensors.tensors), tensors.bits, hp, step,
+                                      _at(grad_scale), seed & (2 ** 64 - 1), on.raw))
+
+
+def adamw_moments(state, stream=None):
+    """(m, v) in fp32 of a state of adamw_state: its own tensors at 32 bits, what the codes stand
+    for at 8."""
+    import torch
+    m, v, me, ve = state
+    if me is None:
+        return m, v
+    with _On("m v m_exp v_exp", (m, v, me, ve), stream) as on:
+        n = m.numel()
+        for name, t, size in (("m", m, n), ("v", v, n), ("m_exp", me, -(-n // 256)),
+                              ("v_exp", ve, -(-n // 256))):
+            _expect(name, t, torch.uint8, size)
+        m32, v32 = (torch.empty(n, dtype=torch.float32, device=m.device) for _ in range(2))
+        check(lib().llmt_adamw_moments(m.data_ptr(), v.data_ptr(), me.data_ptr(), ve.data_ptr(), n,
+                                       m32.data_ptr(), v32.data_ptr(), on.raw))
+    return m32, v32
 
 
 # ------------------------------------------------------------------ training context
