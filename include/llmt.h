@@ -539,7 +539,7 @@ typedef struct {
  * A query without keys, and tokens of no sequence, have o 0 and lse -inf.  dtype
  * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
  * fp32, probabilities are rounded to dtype before the second product.
- * head_dim 64 or 128; Tq nq / nkv and Tk at most 2^30. */
+ * head_dim 64 or 128; nq at most 64 nkv; Tq nq / nkv and Tk at most 2^30. */
 typedef struct {
     int dtype, nq, nkv, head_dim;
     int n, Tq, Tk;

@@ -38,7 +38,9 @@ constexpr long long kMaxStride = 1ll << 40;
 static bool dims_ok(const llmt_packed_dims* d) {
   if (!d || (d->dtype != LLMT_F16 && d->dtype != LLMT_BF16)) return false;
   if (d->head_dim != 64 && d->head_dim != 128) return false;
-  if (d->nkv < 1 || d->nq < d->nkv || d->nq % d->nkv || d->nq > 4096) return false;
+  if (d->nkv < 1 || d->nq < d->nkv || d->nq % d->nkv || d->nq > 4096 ||
+      d->nq / d->nkv > 64)
+    return false;
   if (d->n < 1 || d->n > (1 << 24) || d->Tq < 0 || d->Tk < 0 || d->Tk > kMost) return false;
   const long long rows = (long long)d->Tq * (d->nq / d->nkv);
   // workgroups: at most one each 16 rows or keys, and one a sequence, for each KV head
@@ -89,7 +91,7 @@ static bool views_apart(const View& a, const View& b, int hd) {
 
 static int check_packed(const char* fn, const llmt_packed_dims* d, const View* v, int nv,
                         const float* lse) {
-  TRY_ARG(dims_ok(d), "%s: dtype f16 or bf16, head_dim 64 or 128, nq a multiple of nkv, n in "
+  TRY_ARG(dims_ok(d), "%s: dtype f16 or bf16, head_dim 64 or 128, nq one to 64 times nkv, n in "
           "[1, 2^24], Tq nq / nkv and Tk at most 2^30", fn);
   TRY_ARG(d->scale > 0.f && isfinite(d->scale), "%s: scale must be positive and finite", fn);
   TRY_ARG(d->q_offsets && d->k_offsets && aligned(d->q_offsets, 4) && aligned(d->k_offsets, 4),

@@ -124,29 +124,41 @@ struct Group {
   }
 };
 
-// Query-side rows (token t, head i of the group at t * token + i * head).
-template <int HD, int NW, int ROWS>
+// Query-side rows (token t, head i of the group at t * token + i * head) in
+// tiles of whole tokens, TR = 64 / G * G rows: a lane's offsets are then the
+// same in every tile.  Tile rows from TR on, and rows past the end, are zeros.
+template <int HD, int NW>
 struct RowDma {
-  static constexpr int P = HD / 8, RPC = 64 / P, CH = ROWS / RPC / NW;
-  // rows r0 .. of the n rows (both counted from src's first token)
-  __device__ static __forceinline__ void go(const short* src, long long token, long long head,
-                                            Group gr, int r0, int n, short* tile, int w) {
+  static constexpr int P = HD / 8, RPC = 64 / P, CH = BLK / RPC / NW;
+  unsigned off[CH];
+  __device__ __forceinline__ void init(long long token, long long head, Group gr, int tr, int w) {
     const int lane = threadIdx.x & 63;
-    const int t0 = r0 / gr.G, rem = r0 - t0 * gr.G;
-    const int left = min(n - r0, ROWS);
-    // the tile's last element: its last row's token at most, the group's last head
-    const int tl = left > 0 ? gr.div(rem + left - 1) : 0;
-    const __amdgpu_buffer_rsrc_t rs =
-        buffer_of(src + (long long)t0 * token,
-                  left > 0 ? (tl * (int)token + (gr.G - 1) * (int)head + HD) * 2 : 0);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int r = RPC * (w + NW * i) + lane / P;
-      const int t = gr.div(rem + r), h = rem + r - t * gr.G;
-      const unsigned off =
-          (unsigned)((t * (int)token + h * (int)head) * 2 + (((lane & (P - 1)) ^ (r & (P - 1))) << 4));
-      buffer_lds16(rs, tile + (w + NW * i) * 512, r < left ? off : 0x80000000u);
+      const int t = gr.div(r), h = r - t * gr.G;
+      off[i] = r < tr ? (unsigned)((t * (int)token + h * (int)head) * 2 +
+                                   (((lane & (P - 1)) ^ (r & (P - 1))) << 4))
+                      : 0x80000000u;
     }
+  }
+  // tokens t0 .. t0 + tokens - 1 of the n tokens at src
+  __device__ __forceinline__ void issue(const short* src, long long token, long long head, Group gr,
+                                        int t0, int n, int tokens, short* tile, int w) const {
+    const int left = min(n - t0, tokens);
+    const __amdgpu_buffer_rsrc_t rs =
+        buffer_of(src + (long long)t0 * token,
+                  left > 0 ? ((left - 1) * (int)token + (gr.G - 1) * (int)head + HD) * 2 : 0);
+    if (left < tokens) {  // heads may lie further apart than tokens: a token past the end inside
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int r = RPC * (w + NW * i) + (int)(threadIdx.x & 63) / P;
+        buffer_lds16(rs, tile + (w + NW * i) * 512, r < left * gr.G ? off[i] : 0x80000000u);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) buffer_lds16(rs, tile + (w + NW * i) * 512, off[i]);
   }
 };
 
@@ -234,15 +246,145 @@ __device__ __forceinline__ int find_tile(const int* off, int n, int T, int per, 
   return lo;
 }
 
+// Longest first.  A workgroup's time follows the number of keys its last row
+// sees (rows that see its first key, in dK/dV), and the sequences' lengths
+// differ: workgroup t takes the t-th tile in falling order of that number, in
+// steps of 64.  Up to kOrdered sequences a wave holds them all, so it finds the
+// step by bisection over the count of tiles above it, then the sequence among
+// those that have tiles of the step (contiguous blocks in each).  More sequences
+// than that are as good in any order: find_tile.
+constexpr int kOrderedRegs = 4, kOrdered = 64 * kOrderedRegs - 2;
+
+__device__ __forceinline__ int wave_isum(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);
+  auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(r[0] + r[1]);
+  r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane((int)(r[0] + r[1]));
+}
+
+__device__ __forceinline__ int wave_max_int(int v) {
+  auto up = [](int x, int y) { return x > y ? x : y; };
+  v = up(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = up(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = up(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  v = up(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+  auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  v = up((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane(up((int)r[0], (int)r[1]));
+}
+
+// Blocks of a sequence with more than x of what they walk (x < 0: all).  ROWS:
+// blocks of QB rows walking keys, the last blocks the longest; else blocks of QB
+// keys walking tokens, the first ones the longest.
+struct SeqLens {
+  int ql, kl;
+};
+template <bool ROWS, int QB>
+__device__ __forceinline__ int blocks_above(SeqLens s, int G, int x) {
+  const int nb = ((ROWS ? s.ql * G : s.kl) + QB - 1) / QB;
+  if (x < 0) return nb;
+  if constexpr (ROWS) {
+    const int y = x - (s.kl - s.ql);  // tokens from y on see more than x keys
+    return y >= s.ql ? 0 : y < 0 ? nb : nb - (int)((unsigned)(y * G) / QB);
+  } else {
+    return s.ql <= x ? 0 : min(nb, max(s.kl - x + QB - 1, 0) / QB);
+  }
+}
+
+// (sequence, block) of the t-th tile; false behind the last.  level and top: its
+// step and the bound of all.
+template <bool ROWS, int QB>
+__device__ __forceinline__ bool nth_longest(const PackArgs& a, int G, int t, int* seq, int* block,
+                                            int* level, int* top) {
+  const int lane = threadIdx.x & 63;
+  SeqLens s[kOrderedRegs];
+  int longest = 0;
+#pragma unroll
+  for (int u = 0; u < kOrderedRegs; ++u) {
+    const int i = 64 * u + lane;
+    s[u] = {0, 0};
+    if (64 * u < a.n + 2 && i < a.n + 2) {
+      const bool in = i > 0 && i <= a.n;
+      // the tokens outside of all sequences walk nothing
+      s[u].ql = ROWS || in ? span_of(a.qoff, i, a.n, a.Tq).len : 0;
+      s[u].kl = !ROWS || in ? span_of(a.koff, i, a.n, a.Tk).len : 0;
+    }
+    longest = max(longest, ROWS ? s[u].kl : s[u].ql);
+  }
+  auto above = [&](int k) {  // tiles above step k: x = -1, 0, 64, 128, ..
+    const int x = k == 0 ? -1 : 64 * (k - 1);
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kOrderedRegs; ++u)
+      if (64 * u < a.n + 2) n += blocks_above<ROWS, QB>(s[u], G, x);
+    return wave_isum(n);
+  };
+  longest = wave_max_int(longest);
+  int lo = 0, hi = (longest + 63) / 64 + 1;  // above(lo) > t >= above(hi)
+  *top = hi;
+  if (above(0) <= t) return false;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (above(mid) > t) lo = mid;
+    else hi = mid;
+  }
+  *level = lo;
+  int r = t - above(hi);
+  const int x0 = lo == 0 ? -1 : 64 * (lo - 1), x1 = 64 * lo;
+#pragma unroll
+  for (int u = 0; u < kOrderedRegs; ++u) {
+    if (64 * u >= a.n + 2) break;
+    const int c0 = blocks_above<ROWS, QB>(s[u], G, x0), c1 = blocks_above<ROWS, QB>(s[u], G, x1);
+    int sum = c0 - c1;  // inclusive sums over the lanes
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(sum, d);
+      sum += lane >= d ? v : 0;
+    }
+    const unsigned long long past = __ballot(sum > r);
+    if (past) {
+      const int l = __ffsll(past) - 1;
+      const int i = r - (sum - (c0 - c1));
+      const int nb = ((ROWS ? s[u].ql * G : s[u].kl) + QB - 1) / QB;
+      *seq = 64 * u + l;
+      *block = __builtin_amdgcn_readlane(ROWS ? nb - c0 + i : c1 + i, l);
+      return true;
+    }
+    r -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;  // (of malformed offsets)
+}
+
+// A wave of a long tile goes before its neighbours': the launch ends with the
+// longest tile.
+__device__ __forceinline__ void set_priority(int level, int top) {
+  if (4 * level >= 3 * top) __builtin_amdgcn_s_setprio(3);
+  else if (2 * level >= top) __builtin_amdgcn_s_setprio(2);
+  else if (4 * level >= top) __builtin_amdgcn_s_setprio(1);
+}
+
 // What a workgroup works on: QB rows from row0 of a sequence, for KV head j.
 struct Tile {
   int qstart, rows, row0, shift, kstart, klen, kmax;
   int t0, rem;  // the first row's token and head in the group
 };
+// ordered: longest first; else in the order of the tokens, from the end.
 template <int QB>
-__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, Tile& x) {
-  int blk;
-  const int s = find_tile<QB>(a.qoff, a.n, a.Tq, gr.G, t, &blk);
+__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, int ntiles, bool ordered,
+                                     Tile& x) {
+  int blk, s;
+  if (ordered) {
+    int level, top;
+    if (!nth_longest<true, QB>(a, gr.G, t, &s, &blk, &level, &top)) return false;
+    set_priority(level, top);
+  } else {
+    s = find_tile<QB>(a.qoff, a.n, a.Tq, gr.G, ntiles - 1 - t, &blk);
+  }
   const Span qs = span_of(a.qoff, s, a.n, a.Tq);
   Span ks = {0, 0};
   if (s > 0 && s <= a.n) ks = span_of(a.koff, s, a.n, a.Tk);
@@ -287,6 +429,11 @@ int row_tiles(const PackArgs& a, int qb) {
   return (int)((long long)a.Tq * (a.nq / a.nkv) / qb) + a.n + 2;
 }
 int key_tiles(const PackArgs& a, int kb) { return a.Tk / kb + a.n + 2; }
+// Whether a launch of nt tiles a KV head goes longest first: where they do not
+// all run at once, and a wave can hold the sequences.
+bool ordered(const PackArgs& a, int nt) {
+  return a.n <= kOrdered && (long long)nt * a.nkv > 512;
+}
 
 }  // namespace
 

@@ -78,7 +78,7 @@ struct ColScale {
 // ---------------------------------------------------------------- dQ
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
+void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowVecs rv) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
@@ -88,7 +88,7 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkb = (x.kmax + BLK - 1) / BLK;
@@ -222,12 +222,14 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
 }
 
 // ---------------------------------------------------------------- dK, dV
-// 64 NW / 4 keys a workgroup, 16 a wave, in registers; the rows that see them
-// pass through LDS in tiles of 64 with their lse and delta.  Row r sees key k
-// where r >= (k - shift) G.
+// 16 NW keys a workgroup, 16 a wave, in registers; the rows that see them pass
+// through LDS in tiles with their lse and delta.  Row r sees key k where
+// r >= (k - shift) G: only the first tiles take a mask.  Rows of zeros (past the
+// end, or past the tile's whole tokens) add nothing by themselves, and keys
+// past the end are not stored.
 template <class E, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dkdv_kernel(const PackArgs a, Group gr, RowVecs rv) {
+void packed_dkdv_kernel(const PackArgs a, Group gr, bool ordered, RowVecs rv) {
   constexpr int KB = NW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   constexpr int BUF = 2 * TILE + 2 * BLK * 2;
@@ -237,34 +239,45 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, RowVecs rv) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
-  int blk;
-  const int s = find_tile<KB>(a.koff, a.n, a.Tk, 1, blockIdx.x / a.nkv, &blk);
+  int blk, s;
+  if (ordered) {
+    int level, top;
+    if (!nth_longest<false, KB>(a, gr.G, blockIdx.x / a.nkv, &s, &blk, &level, &top)) return;
+    set_priority(level, top);
+  } else {
+    s = find_tile<KB>(a.koff, a.n, a.Tk, 1, blockIdx.x / a.nkv, &blk);
+  }
   const Span ks = span_of(a.koff, s, a.n, a.Tk);
   if (blk < 0 || blk >= (ks.len + KB - 1) / KB) return;
   Span qs = {0, 0};
   if (s > 0 && s <= a.n) qs = span_of(a.qoff, s, a.n, a.Tq);
-  const int shift = ks.len - qs.len, rows = qs.len * gr.G;
+  const int shift = ks.len - qs.len;
   const int k0 = blk * KB, kw = k0 + w * 16;
-  const int r0 = min(max(k0 - shift, 0), qs.len) * gr.G;  // the first row that sees a key
-  const int niter = (rows - r0 + BLK - 1) / BLK;
-  // the lane's key, and the first row that sees it
+  const int tokens = 64 / gr.G, tr = tokens * gr.G;   // of a tile
+  const int t0 = min(max(k0 - shift, 0), qs.len);     // the first token that sees a key
+  const int niter = (qs.len - t0 + tokens - 1) / tokens;
+  // tiles with a token that does not see the block's last key
+  const int nmask = min(niter, (max(min(k0 + KB - 1 - shift, qs.len) - t0, 0) + tokens - 1) / tokens);
   const int key = kw + c;
-  const int rmin = key < ks.len ? max(key - shift, 0) * gr.G : 0x7fffffff;
-  const int rfull = kw + 16 <= ks.len ? max(kw + 15 - shift, 0) * gr.G : 0x7fffffff;
+  // the first row, counted from token t0, that sees the lane's key
+  const int rmin = (min(max(key - shift, 0), qs.len) - t0) * gr.G;
   const short* qbase = (const short*)a.q.p + qs.start * a.q.token + j * gr.G * a.q.head;
   const short* dbase = (const short*)a.dout.p + qs.start * a.dout.token + j * gr.G * a.dout.head;
-  const long long vbase = vec_at(a, gr.G, j, qs.start);
-  using Dma = RowDma<HD, NW, BLK>;
+  const long long vbase = vec_at(a, gr.G, j, qs.start + t0);
+  const int rows = (qs.len - t0) * gr.G;
+  RowDma<HD, NW> dq_, dd_;
+  dq_.init(a.q.token, a.q.head, gr, tr, w);
+  dd_.init(a.dout.token, a.dout.head, gr, tr, w);
   auto issue = [&](int it, short* buf) LLMT_INLINE {
-    const int r = r0 + it * BLK;
-    Dma::go(qbase, a.q.token, a.q.head, gr, r, rows, buf, w);
-    Dma::go(dbase, a.dout.token, a.dout.head, gr, r, rows, buf + TILE, w);
+    const int t = t0 + it * tokens;
+    dq_.issue(qbase, a.q.token, a.q.head, gr, t, qs.len, tokens, buf, w);
+    dd_.issue(dbase, a.dout.token, a.dout.head, gr, t, qs.len, tokens, buf + TILE, w);
     float* vec = reinterpret_cast<float*>(buf + 2 * TILE);
-    if (w == 0) dma_vec64(rv.lse2 + vbase, r, rows, vec);
-    if (w == NW - 1) dma_vec64(rv.delta + vbase, r, rows, vec + BLK);
+    if (w == 0) dma_vec64(rv.lse2 + vbase, it * tr, min(rows, (it + 1) * tr), vec);
+    if (w == NW - 1) dma_vec64(rv.delta + vbase, it * tr, min(rows, (it + 1) * tr), vec + BLK);
   };
   if (niter > 0) issue(0, buf0);
-  const long long tok = ks.start + min(key, ks.len - 1);
+  const int tok = ks.start + min(key, ks.len - 1);
   short8v kf[KS], vf[KS];
   {
     const short* kr = (const short*)a.k.p + tok * a.k.token + j * a.k.head;
@@ -283,77 +296,76 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, RowVecs rv) {
     dkT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
     dvT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
-  auto half_tile = [&](int jj, int r, auto mask_tag, const short* Qs, const short* Ds,
-                       const float* lse_s, const float* del_s) LLMT_INLINE {
+  auto tile_step = [&](int it, auto mask_tag, const short* Qs, short* nb) LLMT_INLINE {
     constexpr bool MASK = decltype(mask_tag)::value;
-    floatx4 p[2], ds[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int m0 = (2 * jj + u) * 16;
-      p[u] = floatx4{0.f, 0.f, 0.f, 0.f};
-      ds[u] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        p[u] = E::mfma(frag_rm<HD>(Qs, m0, i, lane), kf[i], p[u]);
-        ds[u] = E::mfma(frag_rm<HD>(Ds, m0, i, lane), vf[i], ds[u]);
-      }
-    }
-    sched_reads_ahead<4 * KS, 4 * KS, KS == 4 ? 6 : 4, 2, 2, 0>();
-    __builtin_amdgcn_sched_barrier(0);
-    float am = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int i0 = (2 * jj + u) * 16 + 4 * g;
-      const floatx4 ls = *reinterpret_cast<const floatx4*>(lse_s + i0);
-      const floatx4 dl = *reinterpret_cast<const floatx4*>(del_s + i0);
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        float pv = __builtin_amdgcn_exp2f(fmaf(p[u][v], sl2, -ls[v]));
-        if (MASK) pv = r + i0 + v >= rmin && r + i0 + v < rows ? pv : 0.f;
-        ds[u][v] = pv * (ds[u][v] - dl[v]);
-        p[u][v] = F ? pv * (float)(1 << E::PSH) : pv;
-        if (F) am = fmaxf(am, fabsf(ds[u][v]));
-      }
-    }
-    if constexpr (F) {
-      const float f = cs.follow(xg_max(am));
-      if (__ballot(f != 1.0f)) {
-#pragma unroll
-        for (int i = 0; i < DT; ++i) dkT[i] *= f;
-      }
-      ds[0] *= cs.s;
-      ds[1] *= cs.s;
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    const short8v pb = pair_frag<E>(p[0], p[1]), db = pair_frag<E>(ds[0], ds[1]);
-#pragma unroll
-    for (int i = 0; i < DT; ++i) {
-      dvT[i] = E::mfma(frag_tr<HD>(Ds, i * 16, jj, lane), pb, dvT[i]);
-      dkT[i] = E::mfma(frag_tr<HD>(Qs, i * 16, jj, lane), db, dkT[i]);
-    }
-    sched_reads_ahead<4 * DT, 2 * DT, 8, 2, 4, 1>();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  auto tile_step = [&](int it, const short* buf, short* nb) LLMT_INLINE {
     wait_vm<0>();
     tile_barrier();
     if (it + 1 < niter) issue(it + 1, nb);
-    const short* Ds = buf + TILE;
-    const float* lse_s = reinterpret_cast<const float*>(buf + 2 * TILE);
+    const short* Ds = Qs + TILE;
+    const float* lse_s = reinterpret_cast<const float*>(Qs + 2 * TILE);
     const float* del_s = lse_s + BLK;
-    const int r = r0 + it * BLK;
-    if (r >= rfull && r + BLK <= rows) {
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj)
-        half_tile(jj, r, std::false_type{}, buf, Ds, lse_s, del_s);
-    } else {
+    for (int jj = 0; jj < 2; ++jj) {
+      floatx4 p[2], ds[2];
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj) half_tile(jj, r, std::true_type{}, buf, Ds, lse_s, del_s);
+      for (int u = 0; u < 2; ++u) {
+        const int m0 = (2 * jj + u) * 16;
+        p[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+        ds[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          p[u] = E::mfma(frag_rm<HD>(Qs, m0, i, lane), kf[i], p[u]);
+          ds[u] = E::mfma(frag_rm<HD>(Ds, m0, i, lane), vf[i], ds[u]);
+        }
+      }
+      sched_reads_ahead<4 * KS, 4 * KS, KS == 4 ? 6 : 4, 2, 2, 0>();
+      __builtin_amdgcn_sched_barrier(0);
+      float am = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i0 = (2 * jj + u) * 16 + 4 * g;
+        const floatx4 ls = *reinterpret_cast<const floatx4*>(lse_s + i0);
+        const floatx4 dl = *reinterpret_cast<const floatx4*>(del_s + i0);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float pv = __builtin_amdgcn_exp2f(fmaf(p[u][v], sl2, -ls[v]));
+          if (MASK) pv = it * tr + i0 + v >= rmin ? pv : 0.f;
+          ds[u][v] = pv * (ds[u][v] - dl[v]);
+          p[u][v] = F ? pv * (float)(1 << E::PSH) : pv;
+          if (F) am = fmaxf(am, fabsf(ds[u][v]));
+        }
+      }
+      if constexpr (F) {
+        const float f = cs.follow(xg_max(am));
+        if (__ballot(f != 1.0f)) {
+#pragma unroll
+          for (int i = 0; i < DT; ++i) dkT[i] *= f;
+        }
+        ds[0] *= cs.s;
+        ds[1] *= cs.s;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const short8v pb = pair_frag<E>(p[0], p[1]), db = pair_frag<E>(ds[0], ds[1]);
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        dvT[i] = E::mfma(frag_tr<HD>(Ds, i * 16, jj, lane), pb, dvT[i]);
+        dkT[i] = E::mfma(frag_tr<HD>(Qs, i * 16, jj, lane), db, dkT[i]);
+      }
+      sched_reads_ahead<4 * DT, 2 * DT, 8, 2, 4, 1>();
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  for (int it = 0; it < niter; it += 2) {
-    tile_step(it, buf0, buf1);
-    if (it + 1 < niter) tile_step(it + 1, buf1, buf0);
+  auto step_rt = [&](int it, auto mask_tag) LLMT_INLINE {
+    tile_step(it, mask_tag, (it & 1) ? buf1 : buf0, (it & 1) ? buf0 : buf1);
+  };
+  int it = 0;
+  for (; it < nmask; ++it) step_rt(it, std::true_type{});
+  // in pairs with statically named buffers: the reads of a tile are then not
+  // made to wait for the next one's DMA
+  if (it < niter && (it & 1)) step_rt(it++, std::false_type{});
+  for (; it < niter; it += 2) {
+    tile_step(it, std::false_type{}, buf0, buf1);
+    if (it + 1 < niter) tile_step(it + 1, std::false_type{}, buf1, buf0);
   }
   if (key < ks.len) {
     const float fk = F ? a.scale / cs.s : a.scale;
@@ -380,12 +392,13 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     LLMT_LAUNCH_CHECK();
     const int nt = row_tiles(a, 64);
     hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), dim3((unsigned)nt * a.nkv), dim3(256), 0, st,
-                       a, gr, nt, rv);
+                       a, gr, nt, ordered(a, nt), rv);
     LLMT_LAUNCH_CHECK();
   }
   if (a.Tk) {
-    hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), dim3((unsigned)key_tiles(a, 64) * a.nkv),
-                       dim3(256), 0, st, a, gr, rv);
+    const int nt = key_tiles(a, 64);
+    hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), dim3((unsigned)nt * a.nkv), dim3(256), 0, st,
+                       a, gr, ordered(a, nt), rv);
     LLMT_LAUNCH_CHECK();
   }
   return hipSuccess;

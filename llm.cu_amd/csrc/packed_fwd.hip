@@ -65,7 +65,7 @@ __device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[R
 // rows, K and V in LDS tiles of 64 keys, two buffers.
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, Group gr,
-                                                             int ntiles) {
+                                                             int ntiles, bool ordered) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
   __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
 
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
@@ -189,7 +189,8 @@ struct Parts {
 
 template <class E, int HD, int RW>
 __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs a, Group gr,
-                                                                  int ntiles, Parts parts) {
+                                                                  int ntiles, bool ordered,
+                                                                  Parts parts) {
   constexpr int NW = 4, QB = RW * 16, KS = HD / 32, DT = HD / 16, FT = FS_KEYS * HD;
   // a wave's K and V tile; later its output, 16 rows x HD fp32 each
   __shared__ __attribute__((aligned(1024))) short kbuf[NW * FT];
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
   const int j = blockIdx.x % a.nkv;
   const int part = blockIdx.y;
   Tile x;
-  if (!find<QB>(a, gr, ntiles - 1 - blockIdx.x / a.nkv, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkt_all = (x.kmax + FS_KEYS - 1) / FS_KEYS;
@@ -391,9 +392,11 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     const int nt = row_tiles(a, p.nw * p.rw * 16);
     const dim3 grid((unsigned)nt * a.nkv);
     if (p.rw == 2)
-      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt);
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt,
+                         ordered(a, nt));
     else
-      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt);
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt,
+                         ordered(a, nt));
     LLMT_LAUNCH_CHECK();
     return hipSuccess;
   }
@@ -405,7 +408,7 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   }
   const int nt = row_tiles(a, 16 * p.rw);
   hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1>), dim3((unsigned)nt * a.nkv, p.nsplit),
-                     dim3(256), 0, st, a, gr, nt, parts);
+                     dim3(256), 0, st, a, gr, nt, ordered(a, nt), parts);
   LLMT_LAUNCH_CHECK();
   if (p.nsplit > 1) {
     constexpr int RB = 256 / (HD / 4);
