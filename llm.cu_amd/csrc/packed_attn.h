@@ -40,10 +40,10 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 // The two element types.  PSH: probabilities enter the second product times
 // 2^PSH.  An fp16 below 2^-14 loses bits, which a probability of one key in
-// many is; times 2^14 the largest, 1, is still in range.
+// many is; times 2^8 the largest, 2^7 in the forward, is still in range.
 struct F16 {
   typedef _Float16 T;
-  static constexpr int PSH = 14;
+  static constexpr int PSH = 8;
   __device__ static __forceinline__ floatx4 mfma(short8v a, short8v b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
                                                   __builtin_bit_cast(half8, b), c, 0, 0, 0);

@@ -7,6 +7,7 @@
 // output is 0 and its lse -inf.  One pass over the keys with the running
 // maximum and sum; the scores never leave registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "packed_attn.h"
 
@@ -61,14 +62,39 @@ __device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[R
   }
 }
 
-// Tile by tile, NW waves of 16 RW rows each walk all keys of the workgroup's
-// rows, K and V in LDS tiles of 64 keys, two buffers.
+// The keys that the wave's rows do not see leave the scores of a tile.
+template <int RW, int MT>
+__device__ __forceinline__ void mask_tile(floatx4 (&st)[RW][MT], int key0, const int (&lim)[RW],
+                                          int g) {
+#pragma unroll
+  for (int r = 0; r < RW; ++r)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        st[r][mt][v] = key0 + mt * 16 + 4 * g + v <= lim[r] ? st[r][mt][v] : -INFINITY;
+}
+
+// NW waves of 16 RW rows each walk all keys of the workgroup's rows, K and V
+// in LDS tiles of 64 keys.  A wave's tiles are a pipeline of two stages in one
+// straight block, so that matrix and vector instructions run side by side: the
+// scores of tile i + 1 beside the exponentials, sums and roundings of tile i,
+// then its output beside the maxima of tile i + 1.
+//
+// The maximum that a row's exponentials refer to follows the running one only
+// when some row of the wave has left it by more than 2^GROW: rescaling the
+// output is then a branch that few tiles take, and what it saves in range is
+// in the types (P stays below 2^GROW, times 2^PSH).
+constexpr float GROW = 7.f;
+
 template <class E, int HD, int NW, int RW>
-__global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, Group gr,
-                                                             int ntiles, bool ordered) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles, bool ordered) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
-  __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
-  __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
+  __shared__ __attribute__((aligned(1024))) short kbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) short kbuf1[TILE];
+  __shared__ __attribute__((aligned(1024))) short vbuf0[TILE];
+  __shared__ __attribute__((aligned(1024))) short vbuf1[TILE];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -82,25 +108,17 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
   KeyDma<HD, NW, BLK> dk, dv;
   dk.init(a.k.token, w);
   dv.init(a.v.token, w);
-  if (nkb > 0) {
-    dk.issue(kbase, a.k.token, 0, x.klen, buf0, w);
-    dv.issue(vbase, a.v.token, 0, x.klen, buf0 + TILE, w);
-  }
+  if (nkb > 0) dk.issue(kbase, a.k.token, 0, x.klen, kbuf0, w);
   const int left = x.rows - x.row0 - w * RW * 16;  // rows from the wave's first on
-  // the last key that the wave's first and last row see
-  const int wfirst = left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16) + x.shift : -1;
-  const int wlast =
-      left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16 + min(left, RW * 16) - 1) + x.shift : -1;
+  const int nfull = (x.t0 + x.shift + 1) / BLK;  // tiles that every row sees whole
   short8v qf[RW][KS];
   int lim[RW];
-  long long at[RW];  // token, and the query head
-  int hq[RW];
+  int at[RW], hq[RW];  // token and query head
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
     const int i = min(w * RW * 16 + 16 * r + c, x.rows - 1 - x.row0);
     const int t = gr.div(x.rem + i), h = x.rem + i - t * gr.G;
-    const bool ok = 16 * r + c < left;
-    lim[r] = ok ? x.t0 + t + x.shift : -1;
+    lim[r] = 16 * r + c < left ? x.t0 + t + x.shift : -1;
     at[r] = x.qstart + x.t0 + t;
     hq[r] = j * gr.G + h;
     const short* row = (const short*)a.q.p + at[r] * a.q.token + hq[r] * a.q.head;
@@ -109,7 +127,7 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
       qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
   }
   const float sl2 = a.scale * LOG2E;
-  floatx4 ot[RW][DT];
+  floatx4 ot[RW][DT], sa[RW][4], sb[RW][4];
   float m[RW], l[RW];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -119,16 +137,7 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
     for (int i = 0; i < DT; ++i) ot[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto tile = [&](int kb, const short* Ks, short* nb) LLMT_INLINE {
-    wait_vm<0>();
-    tile_barrier();
-    if (kb + 1 < nkb) {
-      dk.issue(kbase, a.k.token, (kb + 1) * BLK, x.klen, nb, w);
-      dv.issue(vbase, a.v.token, (kb + 1) * BLK, x.klen, nb + TILE, w);
-    }
-    if (kb * BLK > wlast) return;  // no row of the wave sees a key of the tile
-    const short* Vs = Ks + TILE;
-    floatx4 st[RW][4];
+  auto scores = [&](floatx4 (&st)[RW][4], const short* Ks) LLMT_INLINE {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
@@ -140,26 +149,128 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
         for (int r = 0; r < RW; ++r) st[r][mt] = E::mfma(kf, qf[r][ks], st[r][mt]);
       }
     }
-    if (kb * BLK + BLK - 1 <= wfirst && left >= RW * 16)
-      softmax_tile<E, RW, DT, false>(st, m, l, ot, sl2, kb * BLK, lim, lane);
-    else
-      softmax_tile<E, RW, DT, true>(st, m, l, ot, sl2, kb * BLK, lim, lane);
+  };
+  auto maxima = [&](const floatx4 (&st)[RW][4], float (&bm)[RW]) LLMT_INLINE {
 #pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
-      short8v pb[RW];
+    for (int r = 0; r < RW; ++r) {
+      bm[r] = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < RW; ++r) pb[r] = pair_frag<E>(st[r][2 * jj], st[r][2 * jj + 1]);
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) bm[r] = fmaxf(bm[r], st[r][mt][v]);
+      bm[r] = xg_max(bm[r]) * sl2;  // sl2 > 0: the maximum commutes with the scale
+    }
+  };
+  auto follow = [&](const float (&bm)[RW]) LLMT_INLINE {
+    bool grow = false;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) grow = grow || bm[r] > m[r] + GROW;
+    if (__ballot(grow)) {
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        const float mn = fmaxf(m[r], bm[r]);
+        const float alpha = __builtin_amdgcn_exp2f(m[r] - (mn == -INFINITY ? 0.f : mn));
+        m[r] = mn;
+        l[r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) ot[r][i] *= alpha;
+      }
+    }
+  };
+  // probabilities of the scores st as operands, and their sums
+  auto probs = [&](floatx4 (&st)[RW][4], short8v (&pb)[RW][2]) LLMT_INLINE {
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      const float shift = (m[r] == -INFINITY ? 0.f : m[r]) - E::PSH;
+      float ps[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          st[r][mt][v] = __builtin_amdgcn_exp2f(fmaf(st[r][mt][v], sl2, -shift));
+        ps[mt] = (st[r][mt][0] + st[r][mt][1]) + (st[r][mt][2] + st[r][mt][3]);
+      }
+      l[r] += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      pb[r][0] = pair_frag<E>(st[r][0], st[r][1]);
+      pb[r][1] = pair_frag<E>(st[r][2], st[r][3]);
+    }
+  };
+  auto output = [&](const short8v (&pb)[RW][2], const short* Vs) LLMT_INLINE {
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const short8v vf = frag_tr<HD>(Vs, dt * 16, jj, lane);
 #pragma unroll
-        for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r], ot[r][dt]);
+        for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r][jj], ot[r][dt]);
+      }
+  };
+  // iteration i: K(i + 1) and V(i) have landed, K(i + 2) and V(i + 1) set out
+  auto land = [&](int i, short* K0, short* V1) LLMT_INLINE {
+    wait_vm<0>();
+    tile_barrier();
+    if (i + 2 < nkb) dk.issue(kbase, a.k.token, (i + 2) * BLK, x.klen, K0, w);
+    if (i + 1 < nkb) dv.issue(vbase, a.v.token, (i + 1) * BLK, x.klen, V1, w);
+  };
+  // tile i where tile i + 1 takes no mask
+  auto stage = [&](int i, floatx4 (&st)[RW][4], floatx4 (&nx)[RW][4], short* K0, short* K1,
+                   short* V0, short* V1) LLMT_INLINE {
+    land(i, K0, V1);
+    short8v pb[RW][2];
+    scores(nx, K1);
+    probs(st, pb);
+    float bm[RW];
+    output(pb, V0);
+    maxima(nx, bm);
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int u = 0; u < 2 * KS * RW; ++u) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      if (u % RW == 0 && u < 4 * KS * RW / 2 - 2 * RW) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      if (u >= 2 * KS * RW - 4) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, KS == 4 ? 5 : 10, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, KS == 4 ? 2 : 4, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * DT - 4; ++u) {
+      __builtin_amdgcn_sched_group_barrier(0x008, RW, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4 * RW, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    follow(bm);
+  };
+  if (nkb > 0) {
+    wait_vm<0>();
+    tile_barrier();
+    if (nkb > 1) dk.issue(kbase, a.k.token, BLK, x.klen, kbuf1, w);
+    dv.issue(vbase, a.v.token, 0, x.klen, vbuf0, w);
+    scores(sa, kbuf0);
+    if (nfull < 1) mask_tile<RW, 4>(sa, 0, lim, g);
+    float bm[RW];
+    maxima(sa, bm);
+    follow(bm);
+    // in pairs, so that the buffers are named statically
+    int i = 0;
+    for (; i + 2 < nfull; i += 2) {
+      stage(i, sa, sb, kbuf0, kbuf1, vbuf0, vbuf1);
+      stage(i + 1, sb, sa, kbuf1, kbuf0, vbuf1, vbuf0);
+    }
+    // the rest, masked: i is even
+    for (; i < nkb; ++i) {
+      const bool odd = i & 1;
+      land(i, odd ? kbuf1 : kbuf0, odd ? vbuf0 : vbuf1);
+      short8v pb[RW][2];
+      probs(sa, pb);
+      output(pb, odd ? vbuf1 : vbuf0);
+      if (i + 1 < nkb) {
+        scores(sa, odd ? kbuf0 : kbuf1);
+        mask_tile<RW, 4>(sa, (i + 1) * BLK, lim, g);
+        maxima(sa, bm);
+        follow(bm);
       }
     }
-  };
-  for (int kb = 0; kb < nkb; kb += 2) {
-    tile(kb, buf0, buf1);
-    if (kb + 1 < nkb) tile(kb + 1, buf1, buf0);
   }
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -170,7 +281,7 @@ __global__ __launch_bounds__(NW * 64) void packed_fwd_kernel(const PackArgs a, G
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
         *reinterpret_cast<short4v*>(o + dt * 16 + 4 * g) = round4<E>(ot[r][dt] * inv);
-      if (g == 0) a.lse[at[r] * a.nq + hq[r]] = (m[r] + (__log2f(lr) - E::PSH)) * LN2;
+      if (g == 0) a.lse[(long long)at[r] * a.nq + hq[r]] = (m[r] + (__log2f(lr) - E::PSH)) * LN2;
     }
   }
 }
