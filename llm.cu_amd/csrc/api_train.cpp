@@ -43,9 +43,10 @@ static bool dims_ok(const llmt_packed_dims* d) {
     return false;
   if (d->n < 1 || d->n > (1 << 24) || d->Tq < 0 || d->Tk < 0 || d->Tk > kMost) return false;
   const long long rows = (long long)d->Tq * (d->nq / d->nkv);
-  // workgroups: at most one each 16 rows or keys, and one a sequence, for each KV head
+  // A launch has at most 2^24 workgroups: two each 64 rows or keys, and two a
+  // sequence, for each KV head (one each 16 rows only where those are few).
   return rows <= kMost &&
-         (std::max<long long>(rows, d->Tk) / 16 + d->n + 2) * d->nkv < 0x7fffffff &&
+         (std::max<long long>(rows, d->Tk) / 64 + d->n + 2) * d->nkv * 2 < (1 << 24) &&
          (long long)d->Tq * d->nq <= 0x7fffffff;
 }
 
@@ -92,7 +93,7 @@ static bool views_apart(const View& a, const View& b, int hd) {
 static int check_packed(const char* fn, const llmt_packed_dims* d, const View* v, int nv,
                         const float* lse) {
   TRY_ARG(dims_ok(d), "%s: dtype f16 or bf16, head_dim 64 or 128, nq one to 64 times nkv, n in "
-          "[1, 2^24], Tq nq / nkv and Tk at most 2^30", fn);
+          "[1, 2^24], at most 2^24 workgroups", fn);
   TRY_ARG(d->scale > 0.f && isfinite(d->scale), "%s: scale must be positive and finite", fn);
   TRY_ARG(d->q_offsets && d->k_offsets && aligned(d->q_offsets, 4) && aligned(d->k_offsets, 4),
           "%s: offsets must be given, 4-byte aligned", fn);

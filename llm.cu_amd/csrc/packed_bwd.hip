@@ -21,42 +21,15 @@ namespace llmt {
 
 namespace {
 
-// Of each row in the order (KV head, token, head in the group): the base-2 lse,
-// +inf for a row without keys (its probabilities are then 0), and delta.
+// Of each row in the order (KV head, token, head in the group), written by the dQ
+// blocks: the base-2 lse, +inf for a row without keys (its probabilities are
+// then 0), and delta.
 struct RowVecs {
   float* lse2;
   float* delta;
 };
 __device__ __forceinline__ long long vec_at(const PackArgs& a, int G, int j, long long token) {
   return ((long long)j * a.Tq + token) * G;
-}
-
-template <class E, int HD>
-__global__ __launch_bounds__(256) void packed_delta_kernel(const PackArgs a, Group gr, RowVecs rv) {
-  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
-  constexpr int LR = HD / 8;  // lanes a row
-  const long long R = (long long)a.Tq * a.nq;
-  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
-  const long long rc = row < R ? row : R - 1;
-  const long long t = rc / a.nq;
-  const int h = (int)(rc - t * a.nq), d = (threadIdx.x % LR) * 8;
-  const T8 x = *reinterpret_cast<const T8*>((const short*)a.dout.p + t * a.dout.token +
-                                            h * a.dout.head + d);
-  const T8 y = *reinterpret_cast<const T8*>((const short*)a.o.p + t * a.o.token + h * a.o.head + d);
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s = fmaf((float)x[i], (float)y[i], s);
-  s += dpp16<0xB1>(s);
-  s += dpp16<0x4E>(s);
-  s += dpp16<0x141>(s);
-  if constexpr (LR == 16) s += dpp16<0x140>(s);
-  if (row < R && d == 0) {
-    const int j = h / gr.G;
-    const long long at = vec_at(a, gr.G, j, t) + (h - j * gr.G);
-    const float e = a.lse[rc];
-    rv.lse2[at] = e == -INFINITY ? INFINITY : e * LOG2E;
-    rv.delta[at] = s;
-  }
 }
 
 // The running power of two of an accumulator column.  Returns the factor that
@@ -76,11 +49,14 @@ struct ColScale {
 };
 
 // ---------------------------------------------------------------- dQ
+// 16 NW RW rows a workgroup, 16 RW a wave, against keys in tiles of 64, two
+// halves one after the other.
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowVecs rv) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
   __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
   __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
   const int lane = threadIdx.x & 63;
@@ -92,6 +68,7 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkb = (x.kmax + BLK - 1) / BLK;
+  const int nfull = min(max((x.t0 + x.shift + 1) / BLK, 0), nkb);  // tiles that every row sees whole
   KeyDma<HD, NW, BLK> dk, dv;
   dk.init(a.k.token, w);
   dv.init(a.v.token, w);
@@ -99,13 +76,9 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
     dk.issue(kbase, a.k.token, 0, x.klen, buf0, w);
     dv.issue(vbase, a.v.token, 0, x.klen, buf0 + TILE, w);
   }
-  const int left = x.rows - x.row0 - w * RW * 16;
-  const int wfirst = left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16) + x.shift : -1;
-  const int wlast =
-      left > 0 ? x.t0 + gr.div(x.rem + w * RW * 16 + min(left, RW * 16) - 1) + x.shift : -1;
+  const int left = x.rows - x.row0 - w * RW * 16;  // rows from the wave's first on
   short8v qf[RW][KS], df[RW][KS];
-  int lim[RW], hq[RW];
-  long long at[RW];
+  int lim[RW], at[RW], hq[RW];
   float lse2[RW], del[RW];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -116,14 +89,25 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
     hq[r] = j * gr.G + h;
     const short* row = (const short*)a.q.p + at[r] * a.q.token + hq[r] * a.q.head;
     const short* dor = (const short*)a.dout.p + at[r] * a.dout.token + hq[r] * a.dout.head;
+    const short* orow = (const short*)a.o.p + at[r] * a.o.token + hq[r] * a.o.head;
+    float s = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
       df[r][ks] = *reinterpret_cast<const short8v*>(dor + 32 * ks + 8 * g);
+      const T8 d8 = __builtin_bit_cast(T8, df[r][ks]);
+      const T8 o8 = *reinterpret_cast<const T8*>(orow + 32 * ks + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf((float)d8[e], (float)o8[e], s);
     }
-    const long long vi = vec_at(a, gr.G, j, at[r]) + h;
-    lse2[r] = rv.lse2[vi];
-    del[r] = rv.delta[vi];
+    del[r] = xg_sum(s);
+    const float e = a.lse[(long long)at[r] * a.nq + hq[r]];
+    lse2[r] = e == -INFINITY ? INFINITY : e * LOG2E;
+    if (16 * r + c < left && g == 0) {
+      const long long vi = vec_at(a, gr.G, j, at[r]) + h;
+      rv.lse2[vi] = lse2[r];
+      rv.delta[vi] = del[r];
+    }
   }
   const float sl2 = a.scale * LOG2E;
   floatx4 dqT[RW][DT];
@@ -134,81 +118,78 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
     for (int i = 0; i < DT; ++i) dqT[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   auto tile_step = [&](int kb, auto mask_tag, const short* Ks, short* nb) LLMT_INLINE {
+    constexpr bool MASK = decltype(mask_tag)::value;
     wait_vm<0>();
     tile_barrier();
     if (kb + 1 < nkb) {
       dk.issue(kbase, a.k.token, (kb + 1) * BLK, x.klen, nb, w);
       dv.issue(vbase, a.v.token, (kb + 1) * BLK, x.klen, nb + TILE, w);
     }
-    constexpr bool MASK = decltype(mask_tag)::value;
-    if (MASK && kb * BLK > wlast) return;
     const short* Vs = Ks + TILE;
-    floatx4 pt[RW][4], dp[RW][4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-      for (int r = 0; r < RW; ++r) {
-        pt[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
-        dp[r][mt] = floatx4{0.f, 0.f, 0.f, 0.f};
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const short8v kf = frag_rm<HD>(Ks, mt * 16, ks, lane);
-        const short8v vf = frag_rm<HD>(Vs, mt * 16, ks, lane);
-#pragma unroll
-        for (int r = 0; r < RW; ++r) {
-          pt[r][mt] = E::mfma(kf, qf[r][ks], pt[r][mt]);
-          dp[r][mt] = E::mfma(vf, df[r][ks], dp[r][mt]);
-        }
-      }
-    }
-    sched_reads_ahead<8 * KS, 8 * KS * RW, 8, 2 * RW, 2, 0>();
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int r = 0; r < RW; ++r) {
-      float am = 0.f;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          float pv = __builtin_amdgcn_exp2f(fmaf(pt[r][mt][v], sl2, -lse2[r]));
-          if (MASK) pv = kb * BLK + mt * 16 + 4 * g + v <= lim[r] ? pv : 0.f;
-          dp[r][mt][v] = pv * (dp[r][mt][v] - del[r]);
-          if (F) am = fmaxf(am, fabsf(dp[r][mt][v]));
-        }
-      if constexpr (F) {
-        const float f = cs[r].follow(xg_max(am));
-        if (__ballot(f != 1.0f)) {
-#pragma unroll
-          for (int i = 0; i < DT; ++i) dqT[r][i] *= f;
-        }
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) dp[r][mt] *= cs[r].s;
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
+      floatx4 pt[RW][2], dp[RW][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          pt[r][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+          dp[r][u] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const short8v kf = frag_rm<HD>(Ks, (2 * jj + u) * 16, ks, lane);
+          const short8v vf = frag_rm<HD>(Vs, (2 * jj + u) * 16, ks, lane);
+#pragma unroll
+          for (int r = 0; r < RW; ++r) {
+            pt[r][u] = E::mfma(kf, qf[r][ks], pt[r][u]);
+            dp[r][u] = E::mfma(vf, df[r][ks], dp[r][u]);
+          }
+        }
+      }
+      sched_reads_ahead<4 * KS, 4 * KS * RW, KS == 4 ? 6 : 4, 2 * RW, 2, 0>();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        float am = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            float pv = __builtin_amdgcn_exp2f(fmaf(pt[r][u][v], sl2, -lse2[r]));
+            if (MASK) pv = kb * BLK + (2 * jj + u) * 16 + 4 * g + v <= lim[r] ? pv : 0.f;
+            dp[r][u][v] = pv * (dp[r][u][v] - del[r]);
+            if (F) am = fmaxf(am, fabsf(dp[r][u][v]));
+          }
+        if constexpr (F) {
+          const float f = cs[r].follow(xg_max(am));
+          if (__ballot(f != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < DT; ++i) dqT[r][i] *= f;
+          }
+          dp[r][0] *= cs[r].s;
+          dp[r][1] *= cs[r].s;
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
       short8v db[RW];
 #pragma unroll
-      for (int r = 0; r < RW; ++r) db[r] = pair_frag<E>(dp[r][2 * jj], dp[r][2 * jj + 1]);
+      for (int r = 0; r < RW; ++r) db[r] = pair_frag<E>(dp[r][0], dp[r][1]);
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const short8v kt = frag_tr<HD>(Ks, d * 16, jj, lane);
 #pragma unroll
         for (int r = 0; r < RW; ++r) dqT[r][d] = E::mfma(kt, db[r], dqT[r][d]);
       }
+      sched_reads_ahead<2 * DT, DT * RW, DT == 8 ? 6 : 4, RW, 2, 1>();
+      __builtin_amdgcn_sched_barrier(0);
     }
-    sched_reads_ahead<4 * DT, 2 * DT * RW, 8, RW, 2, 1>();
-    __builtin_amdgcn_sched_barrier(0);
   };
-  // the tiles that every row of the wave sees whole first, without masks
-  const int nfull = left >= RW * 16 ? min((wfirst + 1) / BLK, nkb) : 0;
-  for (int kb = 0; kb < nfull; kb += 2) {
+  for (int kb = 0; kb + 1 < nfull; kb += 2) {
     tile_step(kb, std::false_type{}, buf0, buf1);
-    if (kb + 1 < nfull) tile_step(kb + 1, std::false_type{}, buf1, buf0);
+    tile_step(kb + 1, std::false_type{}, buf1, buf0);
   }
-  for (int kb = max(nfull, 0); kb < nkb; ++kb)
+  for (int kb = nfull & ~1; kb < nkb; ++kb)
     tile_step(kb, std::true_type{}, (kb & 1) ? buf1 : buf0, (kb & 1) ? buf0 : buf1);
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -386,13 +367,17 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   const long long R = (long long)a.Tq * a.nq;
   RowVecs rv = {(float*)ws, (float*)ws + R};
   if (a.Tq) {
-    constexpr int RB = 256 / (HD / 8);
-    hipLaunchKernelGGL((packed_delta_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)),
-                       dim3(256), 0, st, a, gr, rv);
-    LLMT_LAUNCH_CHECK();
-    const int nt = row_tiles(a, 64);
-    hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), dim3((unsigned)nt * a.nkv), dim3(256), 0, st,
-                       a, gr, nt, ordered(a, nt), rv);
+    // 32 rows a wave feed two matrix instructions a fragment; 16 while that
+    // leaves CUs without a workgroup
+    const bool wide = R / a.nkv / 128 * a.nkv >= 256;
+    const int nt = row_tiles(a, wide ? 128 : 64);
+    const dim3 grid((unsigned)nt * a.nkv);
+    if (wide)
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt,
+                         ordered(a, nt), rv);
+    else
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt,
+                         ordered(a, nt), rv);
     LLMT_LAUNCH_CHECK();
   }
   if (a.Tk) {
