@@ -563,8 +563,8 @@ int llmt_packed_attention_bwd(const llmt_packed_dims* dims, const llmt_heads* q,
 
 /* Embedding: out[i] = scale weight[tokens[i]], rounded once; zeros where the
  * token is outside [0, V) (padding).  weight [V, H], ldw elements from row to
- * row, out [T, H], ldo; LLMT_F32, LLMT_F16 or LLMT_BF16 each.  T, V and H at most
- * 2^30. */
+ * row, out [T, H], ldo; LLMT_F32, LLMT_F16 or LLMT_BF16 each.  T at most 2^23, V
+ * 2^30, H 2^20. */
 int llmt_embedding(const int* tokens, int T, const void* weight, int wdtype, long long ldw, int V,
                    int H, float scale, void* out, int odtype, long long ldo, void* stream);
 /* Its gradient: dweight[v] = scale sum of dout[i] over tokens[i] = v, or that

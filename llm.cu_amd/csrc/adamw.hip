@@ -17,11 +17,12 @@
 // collapses.  In bits: y = |x| 2^(127 - e) 2^-112 (m; 2^-96 for v) is the float
 // whose upper 12 bits are the code, and the rounding adds a 16-bit draw below.
 //
-// Memory-bound: 26 bytes an element with fp32 moments, 12 with 8-bit ones (a
-// 16-bit gradient, plus 2 for a copy).  A wave takes blocks of 256 elements, a
-// workgroup 4096 elements of one tensor; the list is cut into launches of
-// kAdamMost descriptors, which travel as kernel arguments.
+// Memory-bound: 26 bytes an element with fp32 moments, 14 with 8-bit ones (a
+// 16-bit gradient, plus 2 for a copy).  A wave takes a block of 256 elements at
+// a time, a workgroup one piece of one tensor.  The list is cut into launches
+// of as many descriptors as travel in 4 KB of kernel arguments.
 #include <algorithm>
+#include <type_traits>
 
 #include "ops.h"
 
@@ -29,24 +30,33 @@ namespace llmt {
 
 namespace {
 
-constexpr int NTH = 256, BLOCK = 256, PER_WG = 4096, PER_WAVE = PER_WG / 4 / BLOCK;
+constexpr int NTH = 256, BLOCK = 256;
+// Elements of a workgroup's piece: U blocks a wave, one after another.
+template <int U>
+constexpr int kPiece = NTH / 64 * BLOCK * U;
 
-struct AdamDev {
+struct AdamDev32 {
   float* p;
   const void* g;
   void* m;
   void* v;
-  unsigned char* mexp;
-  unsigned char* vexp;
   void* copy;
   long long n;
-  int first;         // its first workgroup
-  short gtype, ctype;  // ctype -1: no copy
-  int index, vec;
+  int first;               // its first workgroup
+  unsigned index : 24;     // its place in the list
+  unsigned gtype : 2;
+  unsigned ctype : 2;      // kF32: no copy
+  unsigned vec : 1;        // whole aligned accesses
 };
-constexpr int kAdamMost = 44;
+struct AdamDev8 : AdamDev32 {
+  unsigned char* mexp;
+  unsigned char* vexp;
+};
+template <int BITS>
 struct AdamBatch {
-  AdamDev t[kAdamMost];
+  using Dev = std::conditional_t<BITS == 8, AdamDev8, AdamDev32>;
+  static constexpr int kMost = 3968 / sizeof(Dev);  // 70, and 55 with 8-bit moments
+  Dev t[kMost];
   int count;
 };
 
@@ -152,20 +162,26 @@ __device__ __forceinline__ void moments(const AdamStep& k, float g, float& m, fl
   v = bv + gg;
 }
 
-template <int BITS>
-__global__ __launch_bounds__(NTH) void adamw_list_kernel(const AdamBatch b, const AdamStep k) {
+template <int BITS, int U>
+__global__ __launch_bounds__(NTH) void adamw_list_kernel(const AdamBatch<BITS> b, const AdamStep k) {
   const int lane = threadIdx.x & 63;
-  const int wg = blockIdx.x;
-  // the last tensor that begins at or before this workgroup
-  const unsigned long long le = __ballot(lane < b.count && b.t[min(lane, b.count - 1)].first <= wg);
-  const int ti = __builtin_amdgcn_readfirstlane((int)__popcll(le) - 1);
-  const AdamDev& t = b.t[ti];
+  // a row of workgroups a tensor; or one row of all, in which this workgroup's
+  // tensor is the last that begins at or before it
+  const bool rows = gridDim.y > 1;
+  int ti = rows ? blockIdx.y : 0;
+  for (int hi = rows ? 0 : b.count; hi - ti > 1;) {
+    const int mid = (ti + hi) / 2;
+    if (b.t[mid].first <= (int)blockIdx.x) ti = mid;
+    else hi = mid;
+  }
+  const auto& t = b.t[ti];
+  const int piece = blockIdx.x - (rows ? 0 : t.first);
   const bool vec = t.vec;
   const float gs = k.gscale ? *k.gscale : 1.f;
   const unsigned long long key =
-      BITS == 8 ? mix(k.seed ^ (((unsigned long long)(unsigned)k.step << 32) + (unsigned)t.index)) : 0;
-  const long long base = (long long)(wg - t.first) * PER_WG + (threadIdx.x >> 6) * (PER_WG / 4);
-  for (int u = 0; u < PER_WAVE; ++u) {
+      BITS == 8 ? mix(k.seed ^ (((unsigned long long)(unsigned)k.step << 32) + t.index)) : 0;
+  const long long base = (long long)piece * kPiece<U> + (threadIdx.x >> 6) * (U * BLOCK);
+  for (int u = 0; u < U; ++u) {
     const long long i0 = base + u * BLOCK;
     if (i0 >= t.n) return;
     const long long at = i0 + (vec ? 4 * lane : lane);
@@ -237,71 +253,89 @@ __global__ __launch_bounds__(NTH) void adamw_moments_kernel(const unsigned char*
                                                             const unsigned char* mexp,
                                                             const unsigned char* vexp, long long n,
                                                             float* m32, float* v32, bool vec) {
-  const long long i0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * BLOCK;
-  if (i0 >= n) return;
   const int lane = threadIdx.x & 63;
-  const long long at = i0 + (vec ? 4 * lane : lane);
-  bool ok[4];
+  for (long long i0 = (long long)blockIdx.x * kPiece<1> + (threadIdx.x >> 6) * BLOCK; i0 < n;
+       i0 += (long long)gridDim.x * kPiece<1>) {
+    const long long at = i0 + (vec ? 4 * lane : lane);
+    bool ok[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) ok[e] = at + (vec ? e : 64 * e) < n;
-  unsigned mc[4], vc[4];
-  load4_codes(m + at, vec, ok, mc);
-  load4_codes(v + at, vec, ok, vc);
-  const unsigned me = mexp[i0 / BLOCK], ve = vexp[i0 / BLOCK];
-  float x[4], y[4];
+    for (int e = 0; e < 4; ++e) ok[e] = at + (vec ? e : 64 * e) < n;
+    unsigned mc[4], vc[4];
+    load4_codes(m + at, vec, ok, mc);
+    load4_codes(v + at, vec, ok, vc);
+    const unsigned me = mexp[i0 / BLOCK], ve = vexp[i0 / BLOCK];
+    float x[4], y[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[e] = decode<15>(mc[e], me);
-    y[e] = decode<31>(vc[e], ve);
+    for (int e = 0; e < 4; ++e) {
+      x[e] = decode<15>(mc[e], me);
+      y[e] = decode<31>(vc[e], ve);
+    }
+    store4(m32 + at, vec, ok, x);
+    store4(v32 + at, vec, ok, y);
   }
-  store4(m32 + at, vec, ok, x);
-  store4(v32 + at, vec, ok, y);
 }
 
+constexpr long long kMostWgs = 1 << 24;  // of a launch (2^32 threads)
 bool at4(const void* p, size_t es) { return (uintptr_t)p % (4 * es) == 0; }
 size_t esize(int type) { return type == kF32 ? 4 : 2; }
 
 }  // namespace
 
-hipError_t adamw_list(const AdamTensor* ts, int count, int bits, const AdamStep& k0,
-                      hipStream_t st) {
-  AdamStep k = k0;
-  k.seed = mix(k0.seed);
+template <int BITS, int U>
+static hipError_t launch_list(const AdamTensor* ts, int count, const AdamStep& k, hipStream_t st) {
+  AdamBatch<BITS> b;
   for (int i = 0; i < count;) {
-    AdamBatch b;
+    long long wgs = 0, most = 0;
     b.count = 0;
-    long long wgs = 0;
-    for (; i < count && b.count < kAdamMost; ++i) {
+    for (; i < count && b.count < AdamBatch<BITS>::kMost; ++i) {
       const AdamTensor& t = ts[i];
       if (t.n == 0) continue;
-      const long long w = (t.n + PER_WG - 1) / PER_WG;
-      if (b.count && wgs + w > 0x7fffffff) break;
-      AdamDev& d = b.t[b.count++];
+      const long long w = (t.n + kPiece<U> - 1) / kPiece<U>;
+      if (b.count && wgs + w >= kMostWgs) break;
+      auto& d = b.t[b.count++];
       d.p = t.p;
       d.g = t.g;
       d.m = t.m;
       d.v = t.v;
-      d.mexp = t.mexp;
-      d.vexp = t.vexp;
       d.copy = t.copy;
       d.n = t.n;
       d.first = (int)wgs;
-      d.gtype = (short)t.gtype;
-      d.ctype = (short)(t.copy ? t.ctype : -1);
-      d.index = i;
-      const size_t ms = bits == 8 ? 1 : 4;
+      d.index = (unsigned)i;
+      d.gtype = (unsigned)t.gtype;
+      d.ctype = t.copy ? (unsigned)t.ctype : (unsigned)kF32;
+      const size_t ms = BITS == 8 ? 1 : 4;
       d.vec = at4(t.p, 4) && at4(t.g, esize(t.gtype)) && at4(t.m, ms) && at4(t.v, ms) &&
               (!t.copy || at4(t.copy, 2));
+      if constexpr (BITS == 8) {
+        d.mexp = t.mexp;
+        d.vexp = t.vexp;
+      }
       wgs += w;
+      most = std::max(most, w);
     }
     if (!b.count) break;
-    if (bits == 8)
-      hipLaunchKernelGGL(adamw_list_kernel<8>, dim3((unsigned)wgs), dim3(NTH), 0, st, b, k);
-    else
-      hipLaunchKernelGGL(adamw_list_kernel<32>, dim3((unsigned)wgs), dim3(NTH), 0, st, b, k);
+    // small tensors of like sizes: no search (3.4 us a launch, 5.1 with it);
+    // elsewhere workgroups without work would cost more
+    const bool rows = U == 1 && most * b.count <= 2 * wgs + 1024;
+    const dim3 grid((unsigned)(rows ? most : wgs), rows ? b.count : 1);
+    hipLaunchKernelGGL((adamw_list_kernel<BITS, U>), grid, dim3(NTH), 0, st, b, k);
     LLMT_LAUNCH_CHECK();
   }
   return hipSuccess;
+}
+
+hipError_t adamw_list(const AdamTensor* ts, int count, int bits, const AdamStep& k0,
+                      hipStream_t st) {
+  AdamStep k = k0;
+  k.seed = mix(k0.seed);
+  // few elements: a block a wave, so that none waits for a second (200 tensors
+  // of up to 5000 elements: 13.9 us a call, 24.8 with four)
+  long long n = 0;
+  for (int i = 0; i < count; ++i) n += ts[i].n;
+  const bool few = n <= 2048 * kPiece<1>;
+  if (bits == 8)
+    return few ? launch_list<8, 1>(ts, count, k, st) : launch_list<8, 4>(ts, count, k, st);
+  return few ? launch_list<32, 1>(ts, count, k, st) : launch_list<32, 4>(ts, count, k, st);
 }
 
 hipError_t adamw_moments(const void* m, const void* v, const unsigned char* mexp,
@@ -309,9 +343,9 @@ hipError_t adamw_moments(const void* m, const void* v, const unsigned char* mexp
                          hipStream_t st) {
   if (n == 0) return hipSuccess;
   const bool vec = at4(m, 1) && at4(v, 1) && at4(m32, 4) && at4(v32, 4);
-  hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)((n + 4 * BLOCK - 1) / (4 * BLOCK))),
-                     dim3(NTH), 0, st, (const unsigned char*)m, (const unsigned char*)v, mexp, vexp,
-                     n, m32, v32, vec);
+  const long long wgs = std::min<long long>((n + kPiece<1> - 1) / kPiece<1>, 1 << 23);
+  hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)wgs), dim3(NTH), 0, st,
+                     (const unsigned char*)m, (const unsigned char*)v, mexp, vexp, n, m32, v32, vec);
   LLMT_LAUNCH_CHECK();
   return hipSuccess;
 }

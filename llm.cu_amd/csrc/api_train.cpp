@@ -30,8 +30,9 @@ static bool aligned(const void* p, size_t to) { return (uintptr_t)p % to == 0; }
 static bool known(int dtype) { return dtype == LLMT_F32 || dtype == LLMT_F16 || dtype == LLMT_BF16; }
 static size_t esize(int dtype) { return dtype == LLMT_F32 ? 4 : 2; }
 
-constexpr int kMost = 1 << 30;  // tokens, rows of a group's heads, columns
-constexpr long long kMaxStride = 1ll << 40;
+constexpr int kMost = 1 << 30;  // tokens, rows of a group's heads, a vocabulary
+constexpr int kMaxTokens = 1 << 23, kMaxWidth = 1 << 20;  // of an embedding: its grids
+constexpr long long kMaxStride = 1ll << 40, kMaxElements = 1ll << 35;
 
 // ---------------------------------------------------------------- packed attention
 
@@ -141,46 +142,55 @@ struct Extent {
   uintptr_t a, b;
   bool written;
 };
-static bool list_apart(const llmt_adam_tensor* t, int count, int bits) {
-  constexpr int kKinds = 7;
-  auto extent = [&](const llmt_adam_tensor& x, int k) -> Extent {
-    const size_t ms = bits == 8 ? 1 : 4, nb = (size_t)((x.n + 255) / 256);
-    const void* p[kKinds] = {x.p, x.m, x.v, x.copy, bits == 8 ? x.m_exp : nullptr,
-                             bits == 8 ? x.v_exp : nullptr, x.g};
-    const size_t n = (size_t)x.n;
-    const size_t bytes[kKinds] = {n * 4, n * ms, n * ms, n * 2, nb, nb, n * esize(x.g_dtype)};
-    return {(uintptr_t)p[k], p[k] ? (uintptr_t)p[k] + bytes[k] : (uintptr_t)p[k], k < kKinds - 1};
+constexpr int kKinds = 7;  // p, m, v, copy, the two exponents; the gradient last
+static void extents(const llmt_adam_tensor& x, int bits, Extent (&e)[kKinds]) {
+  const size_t n = (size_t)x.n, nb = (n + 255) / 256, ms = bits == 8 ? n : n * 4;
+  const bool codes = bits == 8;
+  auto put = [&](int k, const void* p, size_t bytes) {
+    e[k] = {(uintptr_t)p, p ? (uintptr_t)p + bytes : 0, k < kKinds - 1};
   };
+  put(0, x.p, n * 4);
+  put(1, x.m, ms);
+  put(2, x.v, ms);
+  put(3, x.copy, n * 2);
+  put(4, codes ? x.m_exp : nullptr, nb);
+  put(5, codes ? x.v_exp : nullptr, nb);
+  put(6, x.g, n * esize(x.g_dtype));
+}
+static bool list_apart(const llmt_adam_tensor* t, int count, int bits) {
+  Extent e[kKinds];
+  uintptr_t lo[kKinds], hi[kKinds];
+  std::fill(lo, lo + kKinds, UINTPTR_MAX);
+  std::fill(hi, hi + kKinds, (uintptr_t)0);
   bool ordered = true;
-  Extent all[kKinds];
-  for (int k = 0; k < kKinds && ordered; ++k) {
-    uintptr_t lo = UINTPTR_MAX, hi = 0;
-    for (int i = 0; i < count && ordered; ++i) {
-      const Extent e = extent(t[i], k);
-      if (e.a == e.b) continue;
-      if (e.written && e.a < hi) ordered = false;
-      lo = std::min(lo, e.a);
-      hi = std::max(hi, e.b);
+  for (int i = 0; i < count && ordered; ++i) {
+    if (t[i].n == 0) continue;
+    extents(t[i], bits, e);
+    for (int k = 0; k < kKinds; ++k) {
+      if (!e[k].a) continue;
+      if (e[k].written && e[k].a < hi[k]) ordered = false;
+      lo[k] = std::min(lo[k], e[k].a);
+      hi[k] = std::max(hi[k], e[k].b);
     }
-    all[k] = {lo, hi, k < kKinds - 1};
-    for (int q = 0; q < k && ordered; ++q)
-      if (all[k].a < all[k].b && all[q].a < all[q].b && all[k].a < all[q].b && all[q].a < all[k].b)
-        ordered = false;
   }
+  for (int k = 0; k < kKinds && ordered; ++k)
+    for (int q = 0; q < k; ++q)
+      if (lo[k] < hi[k] && lo[q] < hi[q] && lo[k] < hi[q] && lo[q] < hi[k]) ordered = false;
   if (ordered) return true;
   std::vector<Extent> x;
   x.reserve((size_t)count * kKinds);
-  for (int i = 0; i < count; ++i)
-    for (int k = 0; k < kKinds; ++k) {
-      const Extent e = extent(t[i], k);
-      if (e.a != e.b) x.push_back(e);
-    }
+  for (int i = 0; i < count; ++i) {
+    if (t[i].n == 0) continue;
+    extents(t[i], bits, e);
+    for (const Extent& k : e)
+      if (k.a) x.push_back(k);
+  }
   std::sort(x.begin(), x.end(), [](const Extent& p, const Extent& q) { return p.a < q.a; });
   uintptr_t any = 0, written = 0;  // where what began earlier ends
-  for (const Extent& e : x) {
-    if (e.a < (e.written ? any : written)) return false;
-    any = std::max(any, e.b);
-    if (e.written) written = std::max(written, e.b);
+  for (const Extent& k : x) {
+    if (k.a < (k.written ? any : written)) return false;
+    any = std::max(any, k.b);
+    if (k.written) written = std::max(written, k.b);
   }
   return true;
 }
@@ -253,8 +263,8 @@ static int check_embed(const char* fn, const int* tokens, int T, const void* w, 
                        long long ldw, int V, int H, float scale, const void* x, int xdtype,
                        long long ldx) {
   TRY_ARG(known(wdtype) && known(xdtype), "%s: dtypes %d and %d", fn, wdtype, xdtype);
-  TRY_ARG(T >= 0 && T <= kMost && V >= 1 && V <= kMost && H >= 1 && H <= kMost,
-          "%s: T=%d V=%d H=%d (at most 2^30)", fn, T, V, H);
+  TRY_ARG(T >= 0 && T <= kMaxTokens && V >= 1 && V <= kMost && H >= 1 && H <= kMaxWidth,
+          "%s: T=%d V=%d H=%d (at most 2^23, 2^30, 2^20)", fn, T, V, H);
   TRY_ARG(ldw >= H && ldw <= kMaxStride && ldx >= H && ldx <= kMaxStride &&
               (double)V * ldw <= 1e18 && (double)T * ldx <= 1e18,
           "%s: row strides %lld and %lld of rows of %d", fn, ldw, ldx, H);
@@ -280,7 +290,7 @@ int llmt_embedding(const int* tokens, int T, const void* weight, int wdtype, lon
 }
 
 size_t llmt_embedding_bwd_workspace(int T, int V, int H) {
-  return T > 0 && T <= kMost && V >= 1 && V <= kMost && H >= 1 && H <= kMost
+  return T > 0 && T <= kMaxTokens && V >= 1 && V <= kMost && H >= 1 && H <= kMaxWidth
              ? embed_bwd_workspace(T, V, H) : 0;
 }
 
@@ -311,7 +321,7 @@ int llmt_adamw_update(const llmt_adam_tensor* t, int count, int state_bits, cons
   TRY_ARG(aligned(grad_scale, 4), "%s: misaligned grad_scale", fn);
   for (int i = 0; i < count; ++i) {
     const llmt_adam_tensor& x = t[i];
-    TRY_ARG(x.n >= 0 && x.n <= kMaxStride, "%s: tensor %d has %lld elements", fn, i, x.n);
+    TRY_ARG(x.n >= 0 && x.n <= kMaxElements, "%s: tensor %d has %lld elements", fn, i, x.n);
     TRY_ARG(known(x.g_dtype) && (!x.copy || x.copy_dtype == LLMT_F16 || x.copy_dtype == LLMT_BF16),
             "%s: tensor %d: gradient dtype %d, copy dtype %d (f16 or bf16)", fn, i, x.g_dtype,
             x.copy_dtype);
@@ -351,7 +361,7 @@ int llmt_adamw_moments(const void* m, const void* v, const unsigned char* m_exp,
                        void* stream) {
   set_error("");
   const char* const fn = "llmt_adamw_moments";
-  TRY_ARG(n >= 0 && n <= kMaxStride, "%s: n=%lld", fn, n);
+  TRY_ARG(n >= 0 && n <= kMaxElements, "%s: n=%lld", fn, n);
   if (n == 0) return LLMT_OK;
   TRY_ARG(m && v && m_exp && v_exp && m32 && v32, "%s: NULL argument", fn);
   TRY_ARG(aligned(m32, 4) && aligned(v32, 4), "%s: misaligned argument", fn);

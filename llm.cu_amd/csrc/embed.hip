@@ -6,7 +6,10 @@
 // is cut into chunks, a group of lanes sums the runs of equal tokens of its
 // chunk in fp32, and a run that spans chunks is joined from their partial sums
 // in order.  No atomics, and a frequent token's rows are shared by as many
-// groups as it has chunks.
+// groups as it has chunks.  Few positions need no sort: a workgroup for each
+// looks whether it is its token's first and gathers the others.  Where the
+// table is written whole, its zeros ride in the sorting launches, which leave
+// the memory idle.
 #include <algorithm>
 
 #include "ops.h"
@@ -100,6 +103,30 @@ __global__ __launch_bounds__(NTH) void embed_kernel(const EmbedArgs a, int lpr) 
   }
 }
 
+// ---------------------------------------------------------------- zeros
+// Rows v0 .. v1 - 1 of the table, by the workgroups from `first` on of a launch.
+struct Zeros {
+  void* w;
+  long long ldw;
+  int v0, v1, H, es, vec;  // es: bytes an element; vec: 16-byte pieces
+  unsigned first;
+};
+__device__ __forceinline__ void zero_rows(const Zeros& z) {
+  const int per = z.vec ? 16 : z.es, n = z.H * z.es / per;  // pieces a row
+  const int lanes = n >= NTH ? NTH : n >= 64 ? 64 : n >= 16 ? 16 : 4;
+  const int groups = NTH / lanes;
+  for (long long v = z.v0 + (long long)(blockIdx.x - z.first) * groups + threadIdx.x / lanes;
+       v < z.v1; v += (long long)(gridDim.x - z.first) * groups) {
+    char* row = (char*)z.w + v * z.ldw * z.es;
+    for (int c = threadIdx.x % lanes; c < n; c += lanes) {
+      if (z.vec) *reinterpret_cast<u32x4*>(row + c * 16ll) = u32x4{0, 0, 0, 0};
+      else if (z.es == 4) *reinterpret_cast<unsigned*>(row + c * 4ll) = 0;
+      else *reinterpret_cast<unsigned short*>(row + c * 2ll) = 0;
+    }
+  }
+}
+__global__ __launch_bounds__(NTH) void embed_zero_kernel(const Zeros z) { zero_rows(z); }
+
 // ---------------------------------------------------------------- sorting
 // Sort key of a position: its token, V where that is outside [0, V).
 __device__ __forceinline__ int key_of(const int* tok, int i, int V) {
@@ -113,7 +140,8 @@ __device__ __forceinline__ int key_of(const int* tok, int i, int V) {
 constexpr int kRankMost = 16384;
 template <int LPI>
 __global__ __launch_bounds__(NTH) void embed_rank_kernel(const int* tok, int T, int V, int* skey,
-                                                         int* spos) {
+                                                         int* spos, const Zeros z) {
+  if (blockIdx.x >= z.first) return zero_rows(z);
   const int sub = threadIdx.x % LPI;
   const int i = blockIdx.x * (NTH / LPI) + threadIdx.x / LPI;
   const int ki = i < T ? key_of(tok, i, V) : V;
@@ -151,14 +179,15 @@ struct SortArgs {
   const int* key;  // NULL on the first pass: the tokens themselves, in order
   const int* pos;
   const int* tok;
-  int T, V, shift, per;
+  int T, V, shift, per, wgs;
   int* hist;  // [workgroups][BINS]
   int* key_out;
   int* pos_out;
 };
 
-__global__ __launch_bounds__(NTH) void embed_count_kernel(const SortArgs a) {
+__global__ __launch_bounds__(NTH) void embed_count_kernel(const SortArgs a, const Zeros z) {
   __shared__ int h[BINS];
+  if (blockIdx.x >= z.first) return zero_rows(z);
   for (int i = threadIdx.x; i < BINS; i += NTH) h[i] = 0;
   __syncthreads();
   const int n = a.per * SORT_WAVES, i0 = blockIdx.x * n;
@@ -170,16 +199,31 @@ __global__ __launch_bounds__(NTH) void embed_count_kernel(const SortArgs a) {
   for (int i = threadIdx.x; i < BINS; i += NTH) a.hist[blockIdx.x * BINS + i] = h[i];
 }
 
-__global__ __launch_bounds__(NTH) void embed_place_kernel(const SortArgs a) {
+__global__ __launch_bounds__(NTH) void embed_place_kernel(const SortArgs a, const Zeros z) {
   __shared__ int at[SORT_WAVES][BINS];  // counts, then the next place
   __shared__ int sums[NTH];
+  if (blockIdx.x >= z.first) return zero_rows(z);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int i = threadIdx.x; i < SORT_WAVES * BINS; i += NTH) (&at[0][0])[i] = 0;
+  const int i0 = (blockIdx.x * SORT_WAVES + w) * a.per;
+  const int end = min(a.T, i0 + a.per);
+  volatile int* mine = at[w];
+  auto key_at = [&](int i) { return i >= end ? 0 : a.key ? a.key[i] : key_of(a.tok, i, a.V); };
+  auto pos_at = [&](int i) { return i >= end ? 0 : a.pos ? a.pos[i] : i; };
+  // the wave's first 256 positions in registers: their loads wait once
+  constexpr int R = 4;
+  int key[R], pos[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    key[r] = key_at(i0 + 64 * r + lane);
+    pos[r] = pos_at(i0 + 64 * r + lane);
+  }
   // a digit's first place: the positions of lower digits, then those of earlier
   // workgroups.  Thread t has digits 2 t and 2 t + 1.
   static_assert(BINS == 2 * NTH, "two digits a thread");
   int before[2] = {0, 0}, total[2] = {0, 0};
-  for (int b = 0; b < (int)gridDim.x; ++b) {
+#pragma unroll 32
+  for (int b = 0; b < a.wgs; ++b) {
     const int2 x = *reinterpret_cast<const int2*>(a.hist + b * BINS + 2 * threadIdx.x);
     if (b < (int)blockIdx.x) {
       before[0] += x.x;
@@ -197,17 +241,16 @@ __global__ __launch_bounds__(NTH) void embed_place_kernel(const SortArgs a) {
     __syncthreads();
   }
   const int lower = sums[threadIdx.x] - total[0] - total[1];
-  const int i0 = (blockIdx.x * SORT_WAVES + w) * a.per;
-  const int end = min(a.T, i0 + a.per);
-  volatile int* mine = at[w];
-  for (int r = i0; r < i0 + a.per; r += 64) {
-    const int i = r + lane;
+  auto count = [&](int i, int k) {
     const bool ok = i < end;
-    const int k = ok ? (a.key ? a.key[i] : key_of(a.tok, i, a.V)) : 0;
     const int d = k >> a.shift & (BINS - 1);
     const unsigned long long m = same_digit(d, ok);
     if (ok && (m & ((1ull << lane) - 1)) == 0) mine[d] = mine[d] + (int)__popcll(m);
-  }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (i0 + 64 * r < end) count(i0 + 64 * r + lane, key[r]);
+  for (int r = i0 + 64 * R; r < end; r += 64) count(r + lane, key_at(r + lane));
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -220,20 +263,22 @@ __global__ __launch_bounds__(NTH) void embed_place_kernel(const SortArgs a) {
     }
   }
   __syncthreads();
-  for (int r = i0; r < i0 + a.per; r += 64) {
-    const int i = r + lane;
+  auto place = [&](int i, int k, int q) {
     const bool ok = i < end;
-    const int k = ok ? (a.key ? a.key[i] : key_of(a.tok, i, a.V)) : 0;
     const int d = k >> a.shift & (BINS - 1);
     const unsigned long long m = same_digit(d, ok), lower_lanes = m & ((1ull << lane) - 1);
     const int first = ok ? mine[d] : 0;
     if (ok) {
       const int p = first + (int)__popcll(lower_lanes);
       a.key_out[p] = k;
-      a.pos_out[p] = a.pos ? a.pos[i] : i;
+      a.pos_out[p] = q;
       if (lower_lanes == 0) mine[d] = first + (int)__popcll(m);
     }
-  }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (i0 + 64 * r < end) place(i0 + 64 * r + lane, key[r], pos[r]);
+  for (int r = i0 + 64 * R; r < end; r += 64) place(r + lane, key_at(r + lane), pos_at(r + lane));
 }
 
 // ---------------------------------------------------------------- sums
@@ -265,36 +310,42 @@ __device__ __forceinline__ void put_row(const SumArgs& a, int v, int c, const fl
   store_n<TW, N>(w, y);
 }
 
-// Chunk k: sorted entries k C ..; lpr lanes a chunk, blockIdx.y: columns.
+// Chunk k: sorted entries k C .. (C up to 32); lpr >= 32 lanes a chunk,
+// blockIdx.y: columns.  A lane holds an entry's token and position, so that the
+// rows' loads, eight at a time, wait for nothing else.
 template <class TX, class TW, int N>
 __global__ __launch_bounds__(NTH) void embed_sum_kernel(const SumArgs a, int lpr) {
   const int k = blockIdx.x * (NTH / lpr) + threadIdx.x / lpr;
   const int c = (blockIdx.y * lpr + threadIdx.x % lpr) * N;
-  if (k >= a.nchunks || c >= a.H) return;
-  const int i0 = k * a.C, end = min(a.T, i0 + a.C);
-  int run = a.skey[i0];
-  bool cont = i0 > 0 && a.skey[i0 - 1] == run;  // from an earlier chunk
+  if (k >= a.nchunks) return;
+  const int i0 = k * a.C, end = min(a.T, i0 + a.C), n = end - i0;
+  const int mine = i0 + min((int)(threadIdx.x % 32), n - 1);
+  const int ekey = a.skey[mine], epos = a.spos[mine];
+  const int before = i0 > 0 ? a.skey[i0 - 1] : -1, behind = end < a.T ? a.skey[end] : -1;
+  const bool on = c < a.H;  // the lanes of a group leave together: they hold its entries
+  int run = __shfl(ekey, 0, 32);
+  bool cont = before == run;  // from an earlier chunk
   float s[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) s[e] = 0.f;
-  for (int i = i0; i < end && run < a.V; i += 4) {
-    int key[4];
-    float x[4][N];
+  for (int i = 0; i < n && run < a.V; i += 8) {
+    int key[8];
+    float x[8][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      key[u] = i + u < end ? a.skey[i + u] : a.V;
-      if (key[u] < a.V) load_n<TX, N>((const TX*)a.x + a.spos[i + u] * a.ldx + c, x[u]);
+    for (int u = 0; u < 8; ++u) {
+      key[u] = i + u < n ? __shfl(ekey, (i + u) & 31, 32) : a.V;
+      const int pos = __shfl(epos, (i + u) & 31, 32);
+      if (on && key[u] < a.V) load_n<TX, N>((const TX*)a.x + pos * a.ldx + c, x[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (i + u >= end) break;
+    for (int u = 0; u < 8; ++u) {
+      if (i + u >= n) break;
       if (key[u] != run) {
-        if (cont) {
-          store_n<float, N>(a.part + (long long)(2 * k) * a.H + c, s);
-          cont = false;
-        } else {
-          put_row<TW, N>(a, run, c, s);
+        if (on) {
+          if (cont) store_n<float, N>(a.part + (long long)(2 * k) * a.H + c, s);
+          else put_row<TW, N>(a, run, c, s);
         }
+        cont = false;
         run = key[u];
 #pragma unroll
         for (int e = 0; e < N; ++e) s[e] = 0.f;
@@ -304,10 +355,10 @@ __global__ __launch_bounds__(NTH) void embed_sum_kernel(const SumArgs a, int lpr
       for (int e = 0; e < N; ++e) s[e] += x[u][e];
     }
   }
-  if (run >= a.V) return;
+  if (run >= a.V || !on) return;
   if (cont)
     store_n<float, N>(a.part + (long long)(2 * k) * a.H + c, s);
-  else if (end < a.T && a.skey[end] == run)
+  else if (behind == run)
     store_n<float, N>(a.part + (long long)(2 * k + 1) * a.H + c, s);
   else
     put_row<TW, N>(a, run, c, s);
@@ -318,42 +369,109 @@ template <class TW, int N>
 __global__ __launch_bounds__(NTH) void embed_join_kernel(const SumArgs a, int lpr) {
   const int k = blockIdx.x * (NTH / lpr) + threadIdx.x / lpr;
   const int c = (blockIdx.y * lpr + threadIdx.x % lpr) * N;
-  if (k >= a.nchunks - 1 || c >= a.H) return;
+  if (k >= a.nchunks - 1) return;
   const int i0 = k * a.C, end = i0 + a.C;
-  const int run = a.skey[end - 1];
-  if (run >= a.V || a.skey[end] != run) return;
-  if (a.skey[i0] == run && i0 > 0 && a.skey[i0 - 1] == run) return;  // begins earlier
+  const int first = a.skey[i0], run = a.skey[end - 1], next = a.skey[end];
+  const int before = i0 > 0 ? a.skey[i0 - 1] : -1;
+  if (run >= a.V || next != run || (first == run && before == run)) return;  // or begins earlier
+  // the chunks that it fills from their start, 32 looked at a time
+  int m = k + 1;
+  for (;;) {
+    const int at = m + (int)(threadIdx.x % 32);
+    const bool in = at < a.nchunks && a.skey[(long long)at * a.C] == run;
+    const unsigned long long b = __ballot(in);
+    const int cnt = __popc((unsigned)(threadIdx.x & 32 ? b >> 32 : b));
+    m += cnt;
+    if (cnt < 32) break;
+  }
+  if (c >= a.H) return;
   float s[N];
   load_n<float, N>(a.part + (long long)(2 * k + 1) * a.H + c, s);
-  for (int m = k + 1; m < a.nchunks; m += 4) {
-    float x[4][N];
-    bool in[4];
+  for (int i = k + 1; i < m; i += 8) {
+    float x[8][N];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      in[u] = m + u < a.nchunks && a.skey[(m + u) * a.C] == run;
-      if (in[u]) load_n<float, N>(a.part + (long long)(2 * (m + u)) * a.H + c, x[u]);
-    }
+    for (int u = 0; u < 8; ++u)
+      if (i + u < m) load_n<float, N>(a.part + (long long)(2 * (i + u)) * a.H + c, x[u]);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (in[u]) {
+    for (int u = 0; u < 8; ++u)
+      if (i + u < m) {
 #pragma unroll
         for (int e = 0; e < N; ++e) s[e] += x[u][e];
       }
-    if (!in[3]) break;
   }
   put_row<TW, N>(a, run, c, s);
 }
 
-// Zeros in every row.
-template <class TW, int N>
-__global__ __launch_bounds__(NTH) void embed_zero_kernel(TW* w, long long ldw, int V, int H,
-                                                         int lpr) {
-  float z[N];
+// Up to kFewMost positions: workgroup (i, columns) of position i.  If no earlier
+// position has its token, the positions that have it are listed in order, each
+// wave sums a quarter of the list, and the quarters are added in order.
+constexpr int kFewMost = 1024;
+template <class TX, class TW, int N>
+__global__ __launch_bounds__(NTH) void embed_few_kernel(const SumArgs a, const int* tok) {
+  __shared__ int list[kFewMost];
+  __shared__ int count[NTH / 64];
+  __shared__ float part[3][64 * N];
+  const int i = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int t = tok[i];
+  if ((unsigned)t >= (unsigned)a.V) return;
+  // wave w looks at positions w P ..
+  constexpr int P = kFewMost / 4, R = P / 64;
+  unsigned long long hit[R];
+  int n = 0;
+  bool earlier = false;
 #pragma unroll
-  for (int e = 0; e < N; ++e) z[e] = 0.f;
-  for (long long v = (long long)blockIdx.x * (NTH / lpr) + threadIdx.x / lpr; v < V;
-       v += (long long)gridDim.x * (NTH / lpr))
-    for (int c = (threadIdx.x % lpr) * N; c < H; c += lpr * N) store_n<TW, N>(w + v * ldw + c, z);
+  for (int r = 0; r < R; ++r) {
+    const int p = w * P + r * 64 + lane;
+    const bool same = p < a.T && tok[p] == t;
+    earlier = earlier || (same && p < i);
+    hit[r] = __ballot(same);
+    n += (int)__popcll(hit[r]);
+  }
+  if (lane == 0) count[w] = n;
+  if (__syncthreads_or(earlier)) return;
+  int at = 0;
+  for (int k = 0; k < w; ++k) at += count[k];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (hit[r] >> lane & 1)
+      list[at + (int)__popcll(hit[r] & ((1ull << lane) - 1))] = w * P + r * 64 + lane;
+    at += (int)__popcll(hit[r]);
+  }
+  __syncthreads();
+  const int total = count[0] + count[1] + count[2] + count[3], per = (total + 3) / 4;
+  const int c = (blockIdx.y * 64 + lane) * N;
+  const bool on = c < a.H;
+  float s[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] = 0.f;
+  for (int k = w * per; on && k < min(total, (w + 1) * per); k += 8) {
+    float x[8][N];
+    const int left = min(total, (w + 1) * per) - k;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (u < left) load_n<TX, N>((const TX*)a.x + list[k + u] * a.ldx + c, x[u]);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (u < left) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += x[u][e];
+      }
+  }
+  if (total == 1) {
+    if (w == 0 && on) put_row<TW, N>(a, t, c, s);
+    return;
+  }
+  if (w > 0) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) part[w - 1][e * 64 + lane] = s[e];
+  }
+  __syncthreads();
+  if (w > 0 || !on) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += part[k][e * 64 + lane];
+  put_row<TW, N>(a, t, c, s);
 }
 
 bool pieces(const void* p, long long ld, int H, size_t es, int N) {
@@ -362,22 +480,30 @@ bool pieces(const void* p, long long ld, int H, size_t es, int N) {
 
 size_t size_of(int type) { return type == kF32 ? 4 : 2; }
 
-int chunk_of(int T) { return T >= 16384 ? 32 : T >= 2048 ? 16 : 4; }
+int chunk_of(int T) { return T >= 16384 ? 32 : T >= 4096 ? 16 : 8; }
 
-// The workspace: sorted keys and positions (twice for the radix passes), its
-// counts, the partial sums.
+// The workspace: sorted keys and positions (twice for the radix passes), the
+// passes' counts, the partial sums.
 struct Space {
   size_t keys, hist, part, total;
 };
-int sort_per(int T) { return T <= 262144 ? 512 : 2048; }
+// Positions a wave of the radix passes: about sqrt(T / 32) workgroups, since
+// every one reads the counts of all of them (32768 positions: a placement takes
+// 20 us with 128 workgroups).
+int sort_per(int T) {
+  int wgs = 16;
+  while (wgs < 256 && (long long)wgs * wgs * 32 < T) wgs += 16;
+  return (T + wgs * 256 - 1) / (wgs * 256) * 64;
+}
+int sort_wgs(int T) { return (T + sort_per(T) * SORT_WAVES - 1) / (sort_per(T) * SORT_WAVES); }
 Space space(int T, int H) {
+  Space s{};
+  if (T <= kFewMost) return s;
   const size_t n = ((size_t)T + 3) & ~(size_t)3;
   const bool radix = T > kRankMost;
-  const int wgs = (T + sort_per(T) * SORT_WAVES - 1) / (sort_per(T) * SORT_WAVES);
-  Space s;
   s.keys = 0;
   s.hist = n * 4 * (radix ? 4 : 2);
-  s.part = s.hist + (radix ? (size_t)wgs * BINS * 4 : 0);
+  s.part = s.hist + (radix ? (size_t)sort_wgs(T) * BINS * 4 : 0);
   const size_t chunks = ((size_t)T + chunk_of(T) - 1) / chunk_of(T);
   s.total = s.part + chunks * 2 * (((size_t)H + 3) & ~(size_t)3) * 4;
   return s;
@@ -410,42 +536,74 @@ hipError_t embed_fwd(const EmbedArgs& a, hipStream_t st) {
   });
 }
 
-size_t embed_bwd_workspace(int T, int V, int H) { return T > 0 ? space(T, H).total : 0; }
+size_t embed_bwd_workspace(int T, int V, int H) { return space(T, H).total; }
 
-hipError_t embed_bwd(const EmbedArgs& a, void* ws, hipStream_t st) {
-  const Space sp = space(std::max(a.T, 1), a.H);
+// Sorted keys and positions, the zeros of the table in the same launches.
+static hipError_t sort_tokens(const EmbedArgs& a, const Space& sp, void* ws, Zeros z, int** key,
+                              int** pos, hipStream_t st) {
   const size_t n = ((size_t)a.T + 3) & ~(size_t)3;
   int* const k0 = (int*)ws;
-  int *key = k0, *pos = k0 + n;
-  if (a.T > kRankMost) {
-    SortArgs s{};
-    s.tok = a.tok;
-    s.T = a.T;
-    s.V = a.V;
-    s.per = sort_per(a.T);
-    s.hist = (int*)((char*)ws + sp.hist);
-    const unsigned wgs = (unsigned)((a.T + s.per * SORT_WAVES - 1) / (s.per * SORT_WAVES));
-    int* buf[2][2] = {{k0, k0 + n}, {k0 + 2 * n, k0 + 3 * n}};
-    int cur = 0;
-    for (s.shift = 0; s.shift == 0 || (s.shift < 31 && (a.V >> s.shift) > 0); s.shift += RB) {
-      s.key_out = buf[cur][0];
-      s.pos_out = buf[cur][1];
-      hipLaunchKernelGGL(embed_count_kernel, dim3(wgs), dim3(NTH), 0, st, s);
-      LLMT_LAUNCH_CHECK();
-      hipLaunchKernelGGL(embed_place_kernel, dim3(wgs), dim3(NTH), 0, st, s);
-      LLMT_LAUNCH_CHECK();
-      s.key = key = s.key_out;
-      s.pos = pos = s.pos_out;
-      cur ^= 1;
-    }
-  } else if (a.T > 0) {
+  const int V = a.V;
+  if (a.T <= kRankMost) {
+    *key = k0;
+    *pos = k0 + n;
+    const int per = a.T <= 8192 ? NTH / 16 : NTH / 8;
+    z.first = (unsigned)((a.T + per - 1) / per);
+    z.v1 = a.add ? 0 : V;
+    const dim3 grid(z.first + (a.add ? 0 : 2048));
     if (a.T <= 8192)
-      hipLaunchKernelGGL(embed_rank_kernel<16>, dim3((unsigned)((a.T + 15) / 16)), dim3(NTH), 0, st,
-                         a.tok, a.T, a.V, key, pos);
+      hipLaunchKernelGGL(embed_rank_kernel<16>, grid, dim3(NTH), 0, st, a.tok, a.T, V, *key, *pos, z);
     else
-      hipLaunchKernelGGL(embed_rank_kernel<8>, dim3((unsigned)((a.T + 31) / 32)), dim3(NTH), 0, st,
-                         a.tok, a.T, a.V, key, pos);
+      hipLaunchKernelGGL(embed_rank_kernel<8>, grid, dim3(NTH), 0, st, a.tok, a.T, V, *key, *pos, z);
     LLMT_LAUNCH_CHECK();
+    return hipSuccess;
+  }
+  SortArgs s{};
+  s.tok = a.tok;
+  s.T = a.T;
+  s.V = V;
+  s.per = sort_per(a.T);
+  s.wgs = sort_wgs(a.T);
+  s.hist = (int*)((char*)ws + sp.hist);
+  int passes = 1;
+  while (passes * RB < 31 && (V >> (passes * RB)) > 0) ++passes;
+  int* buf[2][2] = {{k0, k0 + n}, {k0 + 2 * n, k0 + 3 * n}};
+  z.first = (unsigned)s.wgs;
+  const dim3 grid(z.first + (a.add ? 0 : 2048));
+  for (int p = 0; p < passes; ++p) {
+    s.shift = p * RB;
+    s.key_out = buf[p & 1][0];
+    s.pos_out = buf[p & 1][1];
+    for (int half = 0; half < 2; ++half) {  // a launch's share of the rows
+      z.v0 = (int)((long long)V * (2 * p + half) / (2 * passes));
+      z.v1 = (int)((long long)V * (2 * p + half + 1) / (2 * passes));
+      if (half == 0)
+        hipLaunchKernelGGL(embed_count_kernel, grid, dim3(NTH), 0, st, s, z);
+      else
+        hipLaunchKernelGGL(embed_place_kernel, grid, dim3(NTH), 0, st, s, z);
+      LLMT_LAUNCH_CHECK();
+    }
+    s.key = *key = s.key_out;
+    s.pos = *pos = s.pos_out;
+  }
+  return hipSuccess;
+}
+
+hipError_t embed_bwd(const EmbedArgs& a, void* ws, hipStream_t st) {
+  const Space sp = space(a.T, a.H);
+  const int es = (int)size_of(a.wtype);
+  Zeros z{(void*)a.w, a.ldw, 0, a.V, a.H, es, 0, 0};
+  z.vec = (uintptr_t)a.w % 16 == 0 && a.ldw * es % 16 == 0 && (long long)a.H * es % 16 == 0;
+  int *key = nullptr, *pos = nullptr;
+  if (a.T <= kFewMost) {
+    if (!a.add) {
+      hipLaunchKernelGGL(embed_zero_kernel, dim3(4096), dim3(NTH), 0, st, z);
+      LLMT_LAUNCH_CHECK();
+    }
+    if (a.T == 0) return hipSuccess;
+  } else {
+    const hipError_t e = sort_tokens(a, sp, ws, z, &key, &pos, st);
+    if (e != hipSuccess) return e;
   }
   return with_type(a.wtype, [&](auto* tw) {
     using TW = std::remove_pointer_t<decltype(tw)>;
@@ -453,21 +611,20 @@ hipError_t embed_bwd(const EmbedArgs& a, void* ws, hipStream_t st) {
       using TX = std::remove_pointer_t<decltype(tx)>;
       constexpr int N = Bits<TX>::N;
       const bool vec = pieces(a.w, a.ldw, a.H, sizeof(TW), N) && pieces(a.x, a.ldx, a.H, sizeof(TX), N);
-      const int lpr = lanes_for(a.H, vec ? N : 1), gpb = NTH / lpr;
-      if (!a.add) {
-        const unsigned wgs = (unsigned)std::min<long long>(((long long)a.V + gpb - 1) / gpb, 8192);
-        if (vec)
-          hipLaunchKernelGGL((embed_zero_kernel<TW, N>), dim3(wgs), dim3(NTH), 0, st, (TW*)a.w, a.ldw,
-                             a.V, a.H, lpr);
-        else
-          hipLaunchKernelGGL((embed_zero_kernel<TW, 1>), dim3(wgs), dim3(NTH), 0, st, (TW*)a.w, a.ldw,
-                             a.V, a.H, lpr);
-        LLMT_LAUNCH_CHECK();
-      }
-      if (a.T == 0) return hipSuccess;
       SumArgs s{key, pos, a.T, a.V, a.H, chunk_of(a.T), 0, a.x, a.ldx, (void*)a.w, a.ldw, a.scale,
                 a.add, (float*)((char*)ws + sp.part)};
+      if (a.T <= kFewMost) {
+        const int cols = 64 * (vec ? N : 1);
+        const dim3 grid((unsigned)a.T, (unsigned)((a.H + cols - 1) / cols));
+        if (vec)
+          hipLaunchKernelGGL((embed_few_kernel<TX, TW, N>), grid, dim3(NTH), 0, st, s, a.tok);
+        else
+          hipLaunchKernelGGL((embed_few_kernel<TX, TW, 1>), grid, dim3(NTH), 0, st, s, a.tok);
+        LLMT_LAUNCH_CHECK();
+        return hipSuccess;
+      }
       s.nchunks = (a.T + s.C - 1) / s.C;
+      const int lpr = std::max(32, lanes_for(a.H, vec ? N : 1)), gpb = NTH / lpr;
       const int cols = lpr * (vec ? N : 1);
       const dim3 grid((unsigned)((s.nchunks + gpb - 1) / gpb), (unsigned)((a.H + cols - 1) / cols));
       if (vec) {

@@ -125,11 +125,11 @@ struct Group {
 };
 
 // Query-side rows (token t, head i of the group at t * token + i * head) in
-// tiles of whole tokens, TR = 64 / G * G rows: a lane's offsets are then the
+// tiles of whole tokens, TR = ROWS / G * G rows: a lane's offsets are then the
 // same in every tile.  Tile rows from TR on, and rows past the end, are zeros.
-template <int HD, int NW>
+template <int HD, int NW, int ROWS = BLK>
 struct RowDma {
-  static constexpr int P = HD / 8, RPC = 64 / P, CH = BLK / RPC / NW;
+  static constexpr int P = HD / 8, RPC = 64 / P, CH = ROWS / RPC / NW;
   unsigned off[CH];
   __device__ __forceinline__ void init(long long token, long long head, Group gr, int tr, int w) {
     const int lane = threadIdx.x & 63;
@@ -266,6 +266,16 @@ __device__ __forceinline__ int wave_isum(int v) {
   return __builtin_amdgcn_readfirstlane((int)(r[0] + r[1]));
 }
 
+// Inclusive sums over the lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15: rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31: rows 2, 3
+  return v;
+}
 __device__ __forceinline__ int wave_max_int(int v) {
   auto up = [](int x, int y) { return x > y ? x : y; };
   v = up(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
@@ -282,7 +292,7 @@ __device__ __forceinline__ int wave_max_int(int v) {
 // blocks of QB rows walking keys, the last blocks the longest; else blocks of QB
 // keys walking tokens, the first ones the longest.
 struct SeqLens {
-  int ql, kl;
+  int ql, kl, qstart, kstart;
 };
 template <bool ROWS, int QB>
 __device__ __forceinline__ int blocks_above(SeqLens s, int G, int x) {
@@ -296,23 +306,23 @@ __device__ __forceinline__ int blocks_above(SeqLens s, int G, int x) {
   }
 }
 
-// (sequence, block) of the t-th tile; false behind the last.  level and top: its
-// step and the bound of all.
+// The t-th tile: its sequence's spans and its block in it; false behind the
+// last.  level and top: its step and the bound of all.
 template <bool ROWS, int QB>
-__device__ __forceinline__ bool nth_longest(const PackArgs& a, int G, int t, int* seq, int* block,
-                                            int* level, int* top) {
+__device__ __forceinline__ bool nth_longest(const PackArgs& a, int G, int t, SeqLens* seq,
+                                            int* block, int* level, int* top) {
   const int lane = threadIdx.x & 63;
   SeqLens s[kOrderedRegs];
   int longest = 0;
 #pragma unroll
   for (int u = 0; u < kOrderedRegs; ++u) {
     const int i = 64 * u + lane;
-    s[u] = {0, 0};
+    s[u] = {0, 0, 0, 0};
     if (64 * u < a.n + 2 && i < a.n + 2) {
       const bool in = i > 0 && i <= a.n;
+      const Span q = span_of(a.qoff, i, a.n, a.Tq), k = span_of(a.koff, i, a.n, a.Tk);
       // the tokens outside of all sequences walk nothing
-      s[u].ql = ROWS || in ? span_of(a.qoff, i, a.n, a.Tq).len : 0;
-      s[u].kl = !ROWS || in ? span_of(a.koff, i, a.n, a.Tk).len : 0;
+      s[u] = {ROWS || in ? q.len : 0, !ROWS || in ? k.len : 0, q.start, k.start};
     }
     longest = max(longest, ROWS ? s[u].kl : s[u].ql);
   }
@@ -340,18 +350,14 @@ __device__ __forceinline__ bool nth_longest(const PackArgs& a, int G, int t, int
   for (int u = 0; u < kOrderedRegs; ++u) {
     if (64 * u >= a.n + 2) break;
     const int c0 = blocks_above<ROWS, QB>(s[u], G, x0), c1 = blocks_above<ROWS, QB>(s[u], G, x1);
-    int sum = c0 - c1;  // inclusive sums over the lanes
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int v = __shfl_up(sum, d);
-      sum += lane >= d ? v : 0;
-    }
+    const int sum = wave_scan(c0 - c1);
     const unsigned long long past = __ballot(sum > r);
     if (past) {
       const int l = __ffsll(past) - 1;
       const int i = r - (sum - (c0 - c1));
       const int nb = ((ROWS ? s[u].ql * G : s[u].kl) + QB - 1) / QB;
-      *seq = 64 * u + l;
+      *seq = {__builtin_amdgcn_readlane(s[u].ql, l), __builtin_amdgcn_readlane(s[u].kl, l),
+              __builtin_amdgcn_readlane(s[u].qstart, l), __builtin_amdgcn_readlane(s[u].kstart, l)};
       *block = __builtin_amdgcn_readlane(ROWS ? nb - c0 + i : c1 + i, l);
       return true;
     }
@@ -368,33 +374,67 @@ __device__ __forceinline__ void set_priority(int level, int top) {
   else if (4 * level >= top) __builtin_amdgcn_s_setprio(1);
 }
 
+// The tiles of few rows run at once: any order.  Up to 62 sequences a wave holds
+// them all, and one load finds the t-th tile (numbered as in find_tile) and its
+// spans; false where it lies behind the sequence's end.
+template <bool ROWS, int QB>
+__device__ __forceinline__ bool any_tile(const PackArgs& a, int G, int t, SeqLens* seq, int* block) {
+  const int i = threadIdx.x & 63, last = a.n + 1;
+  const bool in = i > 0 && i < last;
+  Span q = {0, 0}, k = {0, 0};
+  if (i <= last) {
+    if (ROWS || in) q = span_of(a.qoff, i, a.n, a.Tq);
+    if (!ROWS || in) k = span_of(a.koff, i, a.n, a.Tk);
+  }
+  const int first = (int)((ROWS ? (unsigned)q.start * G : (unsigned)k.start) / QB) + i;
+  const int l = max(1, (int)__popcll(__ballot(i <= last && first <= t))) - 1;
+  *seq = {__builtin_amdgcn_readlane(q.len, l), __builtin_amdgcn_readlane(k.len, l),
+          __builtin_amdgcn_readlane(q.start, l), __builtin_amdgcn_readlane(k.start, l)};
+  *block = t - __builtin_amdgcn_readlane(first, l);
+  return true;
+}
+
+// Workgroup t of a launch of nt tiles a KV head: the spans of its sequence and
+// its block in it, which may lie behind the sequence's end (or, with malformed
+// offsets, before it).
+template <bool ROWS, int QB>
+__device__ __forceinline__ bool pick_tile(const PackArgs& a, int G, int t, int nt, SeqLens* seq,
+                                          int* block) {
+  if (nt * a.nkv > 512 && a.n <= kOrdered) {
+    int level, top;
+    if (!nth_longest<ROWS, QB>(a, G, t, seq, block, &level, &top)) return false;
+    set_priority(level, top);
+    return true;
+  }
+  const int at = ROWS ? nt - 1 - t : t;
+  if (a.n <= 62) return any_tile<ROWS, QB>(a, G, at, seq, block);
+  const int s = ROWS ? find_tile<QB>(a.qoff, a.n, a.Tq, G, at, block)
+                     : find_tile<QB>(a.koff, a.n, a.Tk, 1, at, block);
+  const bool in = s > 0 && s <= a.n;  // the tokens outside of all sequences: no other side
+  const Span none = {0, 0};
+  const Span q = ROWS || in ? span_of(a.qoff, s, a.n, a.Tq) : none;
+  const Span k = !ROWS || in ? span_of(a.koff, s, a.n, a.Tk) : none;
+  *seq = {q.len, k.len, q.start, k.start};
+  return true;
+}
+
 // What a workgroup works on: QB rows from row0 of a sequence, for KV head j.
 struct Tile {
   int qstart, rows, row0, shift, kstart, klen, kmax;
   int t0, rem;  // the first row's token and head in the group
 };
-// ordered: longest first; else in the order of the tokens, from the end.
 template <int QB>
-__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, int ntiles, bool ordered,
-                                     Tile& x) {
-  int blk, s;
-  if (ordered) {
-    int level, top;
-    if (!nth_longest<true, QB>(a, gr.G, t, &s, &blk, &level, &top)) return false;
-    set_priority(level, top);
-  } else {
-    s = find_tile<QB>(a.qoff, a.n, a.Tq, gr.G, ntiles - 1 - t, &blk);
-  }
-  const Span qs = span_of(a.qoff, s, a.n, a.Tq);
-  Span ks = {0, 0};
-  if (s > 0 && s <= a.n) ks = span_of(a.koff, s, a.n, a.Tk);
-  x.qstart = qs.start;
-  x.rows = qs.len * gr.G;
+__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, int ntiles, Tile& x) {
+  int blk;
+  SeqLens s;
+  if (!pick_tile<true, QB>(a, gr.G, t, ntiles, &s, &blk)) return false;
+  x.qstart = s.qstart;
+  x.rows = s.ql * gr.G;
   if (blk < 0 || blk >= (x.rows + QB - 1) / QB) return false;
   x.row0 = blk * QB;
-  x.shift = ks.len - qs.len;
-  x.kstart = ks.start;
-  x.klen = ks.len;
+  x.shift = s.kl - s.ql;
+  x.kstart = s.kstart;
+  x.klen = s.kl;
   x.t0 = x.row0 / gr.G;
   x.rem = x.row0 - x.t0 * gr.G;
   const int last = x.t0 + gr.div(x.rem + min(QB, x.rows - x.row0) - 1);
@@ -429,11 +469,6 @@ int row_tiles(const PackArgs& a, int qb) {
   return (int)((long long)a.Tq * (a.nq / a.nkv) / qb) + a.n + 2;
 }
 int key_tiles(const PackArgs& a, int kb) { return a.Tk / kb + a.n + 2; }
-// Whether a launch of nt tiles a KV head goes longest first: where they do not
-// all run at once, and a wave can hold the sequences.
-bool ordered(const PackArgs& a, int nt) {
-  return a.n <= kOrdered && (long long)nt * a.nkv > 512;
-}
 
 }  // namespace
 

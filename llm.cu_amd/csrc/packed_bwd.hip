@@ -53,7 +53,7 @@ struct ColScale {
 // halves one after the other.
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowVecs rv) {
+void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   typedef typename E::T T8 __attribute__((ext_vector_type(8)));
@@ -64,7 +64,7 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkb = (x.kmax + BLK - 1) / BLK;
@@ -210,7 +210,7 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, bool ordered, RowV
 // past the end are not stored.
 template <class E, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dkdv_kernel(const PackArgs a, Group gr, bool ordered, RowVecs rv) {
+void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   constexpr int KB = NW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   constexpr int BUF = 2 * TILE + 2 * BLK * 2;
@@ -220,18 +220,11 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, bool ordered, RowVecs rv) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
-  int blk, s;
-  if (ordered) {
-    int level, top;
-    if (!nth_longest<false, KB>(a, gr.G, blockIdx.x / a.nkv, &s, &blk, &level, &top)) return;
-    set_priority(level, top);
-  } else {
-    s = find_tile<KB>(a.koff, a.n, a.Tk, 1, blockIdx.x / a.nkv, &blk);
-  }
-  const Span ks = span_of(a.koff, s, a.n, a.Tk);
+  int blk;
+  SeqLens s;
+  if (!pick_tile<false, KB>(a, gr.G, blockIdx.x / a.nkv, ntiles, &s, &blk)) return;
+  const Span qs = {s.qstart, s.ql}, ks = {s.kstart, s.kl};
   if (blk < 0 || blk >= (ks.len + KB - 1) / KB) return;
-  Span qs = {0, 0};
-  if (s > 0 && s <= a.n) qs = span_of(a.qoff, s, a.n, a.Tq);
   const int shift = ks.len - qs.len;
   const int k0 = blk * KB, kw = k0 + w * 16;
   const int tokens = 64 / gr.G, tr = tokens * gr.G;   // of a tile
@@ -361,29 +354,309 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, bool ordered, RowVecs rv) {
   }
 }
 
+// ---------------------------------------------------------------- few tiles
+// Where the launches above would leave CUs idle, their chains of tiles, each
+// waiting for its own loads, are the time: blocks of 16 rows (16 keys) whose
+// four waves take the tiles of 32 in turn, each through LDS of its own, without
+// a barrier in the loop; the waves' sums meet in LDS and are added in order.
+template <class E, int HD>
+__global__ __launch_bounds__(256, 2)
+void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
+  constexpr int NW = 4, QB = 16, KT = 32, KS = HD / 32, DT = HD / 16;
+  constexpr bool F = std::is_same_v<E, F16>;
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  __shared__ __attribute__((aligned(1024))) short smem[NW * 2 * KT * HD];
+  __shared__ float scale[NW][16];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  Tile x;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
+  const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
+  const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
+  const int nkt = (x.kmax + KT - 1) / KT;
+  short* const Ks = smem + w * 2 * KT * HD;
+  short* const Vs = Ks + KT * HD;
+  KeyDma<HD, 1, KT> dk, dv;
+  dk.init(a.k.token, 0);
+  dv.init(a.v.token, 0);
+  auto issue = [&](int kt) LLMT_INLINE {
+    dk.issue(kbase, a.k.token, kt * KT, x.klen, Ks, 0);
+    dv.issue(vbase, a.v.token, kt * KT, x.klen, Vs, 0);
+  };
+  if (w < nkt) issue(w);
+  const int left = x.rows - x.row0;
+  const int t = gr.div(x.rem + min(c, left - 1)), h = x.rem + min(c, left - 1) - t * gr.G;
+  const int lim = c < left ? x.t0 + t + x.shift : -1, at = x.qstart + x.t0 + t, hq = j * gr.G + h;
+  short8v qf[KS], df[KS];
+  float del = 0.f;
+  {
+    const short* row = (const short*)a.q.p + at * a.q.token + hq * a.q.head;
+    const short* dor = (const short*)a.dout.p + at * a.dout.token + hq * a.dout.head;
+    const short* orow = (const short*)a.o.p + at * a.o.token + hq * a.o.head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
+      df[ks] = *reinterpret_cast<const short8v*>(dor + 32 * ks + 8 * g);
+      const T8 d8 = __builtin_bit_cast(T8, df[ks]);
+      const T8 o8 = *reinterpret_cast<const T8*>(orow + 32 * ks + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) del = fmaf((float)d8[e], (float)o8[e], del);
+    }
+  }
+  del = xg_sum(del);
+  const float e = a.lse[(long long)at * a.nq + hq];
+  const float lse2 = e == -INFINITY ? INFINITY : e * LOG2E;
+  if (w == 0 && c < left && g == 0) {
+    const long long vi = vec_at(a, gr.G, j, at) + h;
+    rv.lse2[vi] = lse2;
+    rv.delta[vi] = del;
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 dqT[DT];
+  ColScale cs;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) dqT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int kt = w; kt < nkt; kt += NW) {
+    wait_vm<0>();  // the wave's own tile
+    asm volatile("" ::: "memory");
+    floatx4 p[2], dp[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      p[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+      dp[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        p[u] = E::mfma(frag_rm<HD>(Ks, u * 16, ks, lane), qf[ks], p[u]);
+        dp[u] = E::mfma(frag_rm<HD>(Vs, u * 16, ks, lane), df[ks], dp[u]);
+      }
+    }
+    float am = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float pv = __builtin_amdgcn_exp2f(fmaf(p[u][v], sl2, -lse2));
+        pv = kt * KT + u * 16 + 4 * g + v <= lim ? pv : 0.f;
+        dp[u][v] = pv * (dp[u][v] - del);
+        if (F) am = fmaxf(am, fabsf(dp[u][v]));
+      }
+    if constexpr (F) {
+      const float f = cs.follow(xg_max(am));
+#pragma unroll
+      for (int i = 0; i < DT; ++i) dqT[i] *= f;
+      dp[0] *= cs.s;
+      dp[1] *= cs.s;
+    }
+    const short8v db = pair_frag<E>(dp[0], dp[1]);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dqT[d] = E::mfma(frag_tr<HD>(Ks, d * 16, 0, lane), db, dqT[d]);
+    if (kt + NW < nkt) {  // refill once this tile's reads have returned
+      wait_lds();
+      asm volatile("" ::: "memory");
+      issue(kt + NW);
+    }
+  }
+  // the waves' sums, each in its own column scale, go where its tiles were
+  floatx4* const mine = reinterpret_cast<floatx4*>(smem + w * 2 * KT * HD);
+  static_assert(DT * 64 * 16 <= 2 * KT * HD * 2, "a wave's sums fit its tiles");
+  wait_lds();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int d = 0; d < DT; ++d) mine[d * 64 + lane] = dqT[d];
+  if (g == 0) scale[w][c] = F ? cs.s : 1.f;
+  __syncthreads();
+  // wave w takes a quarter of the dims
+#pragma unroll
+  for (int d0 = 0; d0 < DT / NW; ++d0) {
+    const int d = w * (DT / NW) + d0;
+    floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      const floatx4 y = reinterpret_cast<const floatx4*>(smem + u * 2 * KT * HD)[d * 64 + lane];
+      s += y * (a.scale / scale[u][c]);
+    }
+    if (c < left)
+      *reinterpret_cast<short4v*>((short*)a.dq.p + at * a.dq.token + hq * a.dq.head + d * 16 +
+                                  4 * g) = round4<E>(s);
+  }
+}
+
+template <class E, int HD>
+__global__ __launch_bounds__(256, 2)
+void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
+  constexpr int NW = 4, KB = 16, QT = 32, KS = HD / 32, DT = HD / 16, TILE = QT * HD;
+  constexpr int BUF = 2 * TILE + 2 * 64 * 2;  // a wave's Q and dO tile, lse and delta
+  constexpr bool F = std::is_same_v<E, F16>;
+  __shared__ __attribute__((aligned(1024))) short smem[NW * BUF];
+  __shared__ float scale[NW][16];
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int j = blockIdx.x % a.nkv;
+  int blk;
+  SeqLens s;
+  if (!pick_tile<false, KB>(a, gr.G, blockIdx.x / a.nkv, ntiles, &s, &blk)) return;
+  if (blk < 0 || blk >= (s.kl + KB - 1) / KB) return;
+  const int shift = s.kl - s.ql, key = blk * KB + c;
+  const int tokens = QT / gr.G, tr = tokens * gr.G;
+  const int t0 = min(max(blk * KB - shift, 0), s.ql);
+  const int niter = (s.ql - t0 + tokens - 1) / tokens, rows = (s.ql - t0) * gr.G;
+  const int rmin = (min(max(key - shift, 0), s.ql) - t0) * gr.G;
+  const short* qbase = (const short*)a.q.p + s.qstart * a.q.token + j * gr.G * a.q.head;
+  const short* dbase = (const short*)a.dout.p + s.qstart * a.dout.token + j * gr.G * a.dout.head;
+  const long long vbase = vec_at(a, gr.G, j, s.qstart + t0);
+  short* const Qs = smem + w * BUF;
+  short* const Ds = Qs + TILE;
+  float* const lse_s = reinterpret_cast<float*>(Qs + 2 * TILE);
+  float* const del_s = lse_s + 64;
+  RowDma<HD, 1, QT> dq_, dd_;
+  dq_.init(a.q.token, a.q.head, gr, tr, 0);
+  dd_.init(a.dout.token, a.dout.head, gr, tr, 0);
+  auto issue = [&](int it) LLMT_INLINE {
+    const int t = t0 + it * tokens;
+    dq_.issue(qbase, a.q.token, a.q.head, gr, t, s.ql, tokens, Qs, 0);
+    dd_.issue(dbase, a.dout.token, a.dout.head, gr, t, s.ql, tokens, Ds, 0);
+    dma_vec64(rv.lse2 + vbase, it * tr, min(rows, (it + 1) * tr), lse_s);
+    dma_vec64(rv.delta + vbase, it * tr, min(rows, (it + 1) * tr), del_s);
+  };
+  if (w < niter) issue(w);
+  const int tok = s.kstart + min(key, s.kl - 1);
+  short8v kf[KS], vf[KS];
+  {
+    const short* kr = (const short*)a.k.p + tok * a.k.token + j * a.k.head;
+    const short* vr = (const short*)a.v.p + tok * a.v.token + j * a.v.head;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      kf[i] = *reinterpret_cast<const short8v*>(kr + 32 * i + 8 * g);
+      vf[i] = *reinterpret_cast<const short8v*>(vr + 32 * i + 8 * g);
+    }
+  }
+  const float sl2 = a.scale * LOG2E;
+  floatx4 dkT[DT], dvT[DT];
+  ColScale cs;
+#pragma unroll
+  for (int i = 0; i < DT; ++i) {
+    dkT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    dvT[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int it = w; it < niter; it += NW) {
+    wait_vm<0>();  // the wave's own tile
+    asm volatile("" ::: "memory");
+    floatx4 p[2], ds[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      p[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+      ds[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        p[u] = E::mfma(frag_rm<HD>(Qs, u * 16, i, lane), kf[i], p[u]);
+        ds[u] = E::mfma(frag_rm<HD>(Ds, u * 16, i, lane), vf[i], ds[u]);
+      }
+    }
+    float am = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int i0 = u * 16 + 4 * g;
+      const floatx4 ls = *reinterpret_cast<const floatx4*>(lse_s + i0);
+      const floatx4 dl = *reinterpret_cast<const floatx4*>(del_s + i0);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        float pv = __builtin_amdgcn_exp2f(fmaf(p[u][v], sl2, -ls[v]));
+        pv = it * tr + i0 + v >= rmin ? pv : 0.f;
+        ds[u][v] = pv * (ds[u][v] - dl[v]);
+        p[u][v] = F ? pv * (float)(1 << E::PSH) : pv;
+        if (F) am = fmaxf(am, fabsf(ds[u][v]));
+      }
+    }
+    if constexpr (F) {
+      const float f = cs.follow(xg_max(am));
+#pragma unroll
+      for (int i = 0; i < DT; ++i) dkT[i] *= f;
+      ds[0] *= cs.s;
+      ds[1] *= cs.s;
+    }
+    const short8v pb = pair_frag<E>(p[0], p[1]), db = pair_frag<E>(ds[0], ds[1]);
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      dvT[i] = E::mfma(frag_tr<HD>(Ds, i * 16, 0, lane), pb, dvT[i]);
+      dkT[i] = E::mfma(frag_tr<HD>(Qs, i * 16, 0, lane), db, dkT[i]);
+    }
+    if (it + NW < niter) {
+      wait_lds();
+      asm volatile("" ::: "memory");
+      issue(it + NW);
+    }
+  }
+  floatx4* const mine = reinterpret_cast<floatx4*>(smem + w * BUF);
+  static_assert(2 * DT * 64 * 16 <= BUF * 2, "a wave's sums fit its tiles");
+  wait_lds();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < DT; ++i) {
+    mine[i * 64 + lane] = dkT[i];
+    mine[(DT + i) * 64 + lane] = dvT[i];
+  }
+  if (g == 0) scale[w][c] = F ? cs.s : 1.f;
+  __syncthreads();
+  const float fv = 1.0f / (float)(1 << E::PSH);
+#pragma unroll
+  for (int d0 = 0; d0 < DT / NW; ++d0) {
+    const int d = w * (DT / NW) + d0;
+    floatx4 sk = {0.f, 0.f, 0.f, 0.f}, sv = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      const floatx4* y = reinterpret_cast<const floatx4*>(smem + u * BUF);
+      sk += y[d * 64 + lane] * (a.scale / scale[u][c]);
+      sv += y[(DT + d) * 64 + lane];
+    }
+    if (key < s.kl) {
+      *reinterpret_cast<short4v*>((short*)a.dk.p + tok * a.dk.token + j * a.dk.head + d * 16 +
+                                  4 * g) = round4<E>(sk);
+      *reinterpret_cast<short4v*>((short*)a.dv.p + tok * a.dv.token + j * a.dv.head + d * 16 +
+                                  4 * g) = round4<E>(sv * fv);
+    }
+  }
+}
+
 template <class E, int HD>
 hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   const Group gr = group_of(a);
   const long long R = (long long)a.Tq * a.nq;
   RowVecs rv = {(float*)ws, (float*)ws + R};
   if (a.Tq) {
+    const long long rows = (long long)a.Tq * gr.G;
     // 32 rows a wave feed two matrix instructions a fragment; 16 while that
-    // leaves CUs without a workgroup
-    const bool wide = R / a.nkv / 128 * a.nkv >= 256;
-    const int nt = row_tiles(a, wide ? 128 : 64);
+    // leaves CUs without a workgroup; the keys over a workgroup's waves while all
+    // blocks of 16 rows run at once (us of a backward, without -> with: one head, 1
+    // x 2000 78 -> 62; 4 heads, 2 x 500 30 -> 26; 16 / 8 heads, 512 39 -> 39, above
+    // 8 x 77 23 -> 30)
+    const bool split = rows / 16 * a.nkv <= 512, wide = rows / 128 * a.nkv >= 256;
+    const int nt = row_tiles(a, split ? 16 : wide ? 128 : 64);
     const dim3 grid((unsigned)nt * a.nkv);
-    if (wide)
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt,
-                         ordered(a, nt), rv);
+    if (split)
+      hipLaunchKernelGGL((packed_dq_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
+    else if (wide)
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
     else
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt,
-                         ordered(a, nt), rv);
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
     LLMT_LAUNCH_CHECK();
   }
   if (a.Tk) {
-    const int nt = key_tiles(a, 64);
-    hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), dim3((unsigned)nt * a.nkv), dim3(256), 0, st,
-                       a, gr, ordered(a, nt), rv);
+    // the rows over a workgroup's waves up to 1280 blocks of 16 keys (us of a
+    // backward, 16 / 8 heads of 128, without -> with: 1 x 512 40 -> 27, 8 x 77 23 ->
+    // 19, 6 x 250 44 -> 38, 6 x 417 74 -> 72; above, 4 x 1000 136 -> 147), and up to
+    // 2048 where the chains are long (32 / 8 heads of 64, 4 x 1000 149 -> 129)
+    const long long blocks = (long long)a.Tk / 16 * a.nkv;
+    const bool split = gr.G <= 32 && (blocks <= 1280 || (blocks <= 2048 && gr.G >= 4 &&
+                                                         a.Tq / a.n * gr.G >= 64 * 48));
+    const int nt = key_tiles(a, split ? 16 : 64);
+    const dim3 grid((unsigned)nt * a.nkv);
+    if (split)
+      hipLaunchKernelGGL((packed_dkdv_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
+    else
+      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), grid, dim3(256), 0, st, a, gr, nt, rv);
     LLMT_LAUNCH_CHECK();
   }
   return hipSuccess;

@@ -89,7 +89,7 @@ constexpr float GROW = 7.f;
 
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles, bool ordered) {
+void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
   constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   __shared__ __attribute__((aligned(1024))) short kbuf0[TILE];
   __shared__ __attribute__((aligned(1024))) short kbuf1[TILE];
@@ -100,7 +100,7 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles, bool ordered) {
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
 
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
@@ -300,8 +300,7 @@ struct Parts {
 
 template <class E, int HD, int RW>
 __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs a, Group gr,
-                                                                  int ntiles, bool ordered,
-                                                                  Parts parts) {
+                                                                  int ntiles, Parts parts) {
   constexpr int NW = 4, QB = RW * 16, KS = HD / 32, DT = HD / 16, FT = FS_KEYS * HD;
   // a wave's K and V tile; later its output, 16 rows x HD fp32 each
   __shared__ __attribute__((aligned(1024))) short kbuf[NW * FT];
@@ -313,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
   const int j = blockIdx.x % a.nkv;
   const int part = blockIdx.y;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ordered, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkt_all = (x.kmax + FS_KEYS - 1) / FS_KEYS;
@@ -461,10 +460,12 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackArgs a, Part
   if (row >= R) return;
   const int d = (threadIdx.x % LR) * 4;
   float M = -INFINITY;
+#pragma unroll 8
   for (int s = 0; s < parts.nsplit; ++s) M = fmaxf(M, parts.ml[s * R + row].x);
   const float mu = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (int s = 0; s < parts.nsplit; ++s) {
     const float2 p = parts.ml[s * R + row];
     const float f = __builtin_amdgcn_exp2f(p.x - mu);
@@ -488,11 +489,12 @@ FwdPlan fwd_plan(const PackArgs& a) {
   const long long n = std::min(a.n, a.Tq);
   if (rows / 128 * a.nkv >= 512) return {4, 2, 1};
   if (rows / 64 * a.nkv >= 256) return {4, 1, 1};
-  // tiles of 16 rows: at least one a sequence that has queries
-  const long long wgs = std::max<long long>(1, std::max(rows / 16, n) * a.nkv);
+  // tiles of 16 rows, or of 32 where that many workgroups would not run at once
+  const int rw = rows / 16 * a.nkv > 512 ? 2 : 1;
+  const long long wgs = std::max<long long>(1, std::max(rows / (16 * rw), n) * a.nkv);
   const long long keys = a.Tk / std::max<long long>(1, n);
   const long long most = std::min<long long>(64, std::max<long long>(1, keys / 128));
-  return {0, 1, (int)std::min(most, std::max<long long>(1, 768 / wgs))};
+  return {0, rw, (int)std::min(most, std::max<long long>(1, 768 / wgs))};
 }
 
 template <class E, int HD>
@@ -503,11 +505,9 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     const int nt = row_tiles(a, p.nw * p.rw * 16);
     const dim3 grid((unsigned)nt * a.nkv);
     if (p.rw == 2)
-      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt,
-                         ordered(a, nt));
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt);
     else
-      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt,
-                         ordered(a, nt));
+      hipLaunchKernelGGL((packed_fwd_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt);
     LLMT_LAUNCH_CHECK();
     return hipSuccess;
   }
@@ -518,8 +518,11 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     parts.ml = (float2*)(parts.o + p.nsplit * R * HD);
   }
   const int nt = row_tiles(a, 16 * p.rw);
-  hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1>), dim3((unsigned)nt * a.nkv, p.nsplit),
-                     dim3(256), 0, st, a, gr, nt, ordered(a, nt), parts);
+  const dim3 grid((unsigned)nt * a.nkv, p.nsplit);
+  if (p.rw == 2)
+    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, parts);
+  else
+    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, parts);
   LLMT_LAUNCH_CHECK();
   if (p.nsplit > 1) {
     constexpr int RB = 256 / (HD / 4);

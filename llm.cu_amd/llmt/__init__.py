@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 from pathlib import Path
 from typing import NamedTuple
 
@@ -105,12 +106,11 @@ _PROTOS = {
     "llmt_muon_update": (i32, [vp, vp, vp, i32, i32, C.POINTER(i32), C.POINTER(i32),
                                C.POINTER(MuonParams), vp, sz, vp]),
     "llmt_muon": (i32, [vp, C.POINTER(MuonParams)]),
-    "llmt_packed_attention_workspace": (sz, [C.POINTER(PackedDims)]),
-    "llmt_packed_attention": (i32, [C.POINTER(PackedDims)] + [C.POINTER(Heads)] * 4 +
-                              [vp, vp, sz, vp]),
-    "llmt_packed_attention_bwd_workspace": (sz, [C.POINTER(PackedDims)]),
-    "llmt_packed_attention_bwd": (i32, [C.POINTER(PackedDims)] + [C.POINTER(Heads)] * 4 + [vp] +
-                                  [C.POINTER(Heads)] * 4 + [vp, sz, vp]),
+    # dims and views: addresses of PackedDims and Heads, or their bytes
+    "llmt_packed_attention_workspace": (sz, [vp]),
+    "llmt_packed_attention": (i32, [vp] * 7 + [sz, vp]),
+    "llmt_packed_attention_bwd_workspace": (sz, [vp]),
+    "llmt_packed_attention_bwd": (i32, [vp] * 11 + [sz, vp]),
     "llmt_embedding": (i32, [vp, i32, vp, i32, i64, i32, i32, f32, vp, i32, i64, vp]),
     "llmt_embedding_bwd_workspace": (sz, [i32, i32, i32]),
     "llmt_embedding_bwd": (i32, [vp, i32, vp, i32, i64, f32, vp, i32, i64, i32, i32, i32, vp, sz,
@@ -555,44 +555,53 @@ def muon_update(p, g, m, shapes, hp: MuonParams, stream=None):
 
 # ------------------------------------------------------------------ packed sequences
 
-def _heads(name, t, like=None):
-    """A [T, heads, d] tensor as llmt_heads (the stride of one token or one head is of no
-    account)."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+_HEADS = struct.Struct("Pqq")      # a Heads
+_PACKED = struct.Struct("7if2P")   # a PackedDims
+_HALVES = {}                       # torch.float16 and bfloat16 to the library's codes
+
+
+def _heads(name, t, shape=None, dtype=None):
+    """The bytes of the Heads of a [T, heads, d] tensor (the stride of one token or one head is
+    of no account)."""
+    at = t.shape
+    if shape is not None and (at != shape or t.dtype is not dtype):
+        raise LlmtError(f"{name} must be {list(shape)} {dtype} (got {list(at)} {t.dtype})")
+    T, heads, d = at
+    token, head, one = t.stride()
+    if one != 1 and d > 1:
         raise LlmtError(f"{name} must be [T, heads, head_dim] with a last stride of 1")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype):
-        raise LlmtError(f"{name} must be {list(like.shape)} {like.dtype} "
-                        f"(got {list(t.shape)} {t.dtype})")
-    T, heads, d = t.shape
-    token, head = t.stride(0), t.stride(1)
     if heads < 2:
         head = d
     if T < 2:
         token = (d + 7) // 8 * 8
-    return Heads(t.data_ptr(), token, head)
+    return _HEADS.pack(t.data_ptr(), token, head)
 
 
 def _packed_dims(q, k, v, q_offsets, k_offsets, scale):
+    """(the bytes of PackedDims, q's shape and type, k's shape)."""
     import torch
-    dt = {torch.float16: 1, torch.bfloat16: 2}.get(q.dtype)
-    if dt is None or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise LlmtError(f"q, k and v must be float16 or bfloat16 (got {q.dtype}, {k.dtype}, "
-                        f"{v.dtype})")
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+    if not _HALVES:
+        _HALVES.update({torch.float16: 1, torch.bfloat16: 2})
+    dtype, qs, ks = q.dtype, q.shape, k.shape
+    code = _HALVES.get(dtype)
+    if code is None or k.dtype is not dtype or v.dtype is not dtype:
+        raise LlmtError(f"q, k and v must be float16 or bfloat16 (got {dtype}, {k.dtype}, {v.dtype})")
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or ks[2] != qs[2]:
         raise LlmtError("q must be [Tq, nq, head_dim], k and v [Tk, nkv, head_dim]")
     _expect("q_offsets", q_offsets, torch.int32, None)
     n = q_offsets.shape[0] - 1
-    _expect("k_offsets", k_offsets, torch.int32, n + 1)
     if n < 1:
         raise LlmtError("offsets must be [n + 1] with n >= 1")
-    if k_offsets is None and k.shape[0] != q.shape[0]:
-        raise LlmtError(f"without k_offsets q and k are the same tokens (got {q.shape[0]} and "
-                        f"{k.shape[0]})")
-    d = q.shape[2]
-    _sizes("tokens, heads", n + 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], d)
-    return PackedDims(dt, q.shape[1], k.shape[1], d, n, q.shape[0], k.shape[0],
-                      d ** -0.5 if scale is None else scale, q_offsets.data_ptr(),
-                      (q_offsets if k_offsets is None else k_offsets).data_ptr())
+    if k_offsets is None:
+        k_offsets = q_offsets
+        if ks[0] != qs[0]:
+            raise LlmtError(f"without k_offsets q and k are the same tokens (got {qs[0]} and {ks[0]})")
+    else:
+        _expect("k_offsets", k_offsets, torch.int32, n + 1)
+    _sizes("tokens, heads", n + 1, *qs, *ks)
+    return _PACKED.pack(code, qs[1], ks[1], qs[2], n, qs[0], ks[0],
+                        qs[2] ** -0.5 if scale is None else scale, q_offsets.data_ptr(),
+                        k_offsets.data_ptr()), qs, ks, dtype
 
 
 def packed_attention(q, k, v, q_offsets, k_offsets=None, scale=None, out=None, stream=None):
@@ -603,14 +612,15 @@ def packed_attention(q, k, v, q_offsets, k_offsets=None, scale=None, out=None, s
     sqrt(d).  Returns (o like q, lse fp32 [Tq, nq]); 0 and -inf where a query has no keys."""
     import torch
     with _On("q k v q_offsets k_offsets out", (q, k, v, q_offsets, k_offsets, out), stream) as on:
-        dims = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
-        o = q.new_empty(q.shape) if out is None else out
-        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+        dims, qs, ks, dtype = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
+        o = q.new_empty(qs) if out is None else out
+        lse = q.new_empty(qs[:2], dtype=torch.float32)
         L = lib()
         need = L.llmt_packed_attention_workspace(dims)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         check(L.llmt_packed_attention(dims, _heads("q", q), _heads("k", k), _heads("v", v),
-                                      _heads("out", o, q), lse.data_ptr(), _at(ws), need, on.raw))
+                                      _heads("out", o, qs, dtype), lse.data_ptr(), _at(ws), need,
+                                      on.raw))
     return o, lse
 
 
@@ -623,18 +633,17 @@ def packed_attention_bwd(q, k, v, o, lse, dout, q_offsets, k_offsets=None, scale
     dq, dk, dv = (None, None, None) if out is None else out
     with _On("q k v o lse dout q_offsets k_offsets dq dk dv",
              (q, k, v, o, lse, dout, q_offsets, k_offsets, dq, dk, dv), stream) as on:
-        dims = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
-        _expect("lse", lse, torch.float32, q.shape[0], q.shape[1])
-        dq = q.new_empty(q.shape) if dq is None else dq
-        dk = k.new_empty(k.shape) if dk is None else dk
-        dv = v.new_empty(v.shape) if dv is None else dv
+        dims, qs, ks, dtype = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
+        _expect("lse", lse, torch.float32, qs[0], qs[1])
+        if out is None:
+            dq, dk, dv = q.new_empty(qs), k.new_empty(ks), v.new_empty(ks)
         L = lib()
         need = L.llmt_packed_attention_bwd_workspace(dims)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         check(L.llmt_packed_attention_bwd(
-            dims, _heads("q", q), _heads("k", k), _heads("v", v), _heads("o", o, q), lse.data_ptr(),
-            _heads("dout", dout, q), _heads("dq", dq, q), _heads("dk", dk, k), _heads("dv", dv, v),
-            _at(ws), need, on.raw))
+            dims, _heads("q", q), _heads("k", k), _heads("v", v), _heads("o", o, qs, dtype),
+            lse.data_ptr(), _heads("dout", dout, qs, dtype), _heads("dq", dq, qs, dtype),
+            _heads("dk", dk, ks, dtype), _heads("dv", dv, ks, dtype), _at(ws), need, on.raw))
     return dq, dk, dv
 
 

@@ -1,6 +1,7 @@
 """GPU: llmt.packed_attention and its gradients against float64 (packed_ref.py, which derives
 the bounds): lengths from none to several tiles, every kernel, layouts, offsets, masks that leave
 rows empty, tokens of no sequence, streams and graphs."""
+import ctypes as C
 import math
 
 import pytest
@@ -112,7 +113,7 @@ def test_keys_are_split_over_workgroups():
     for tq, tk, n, nq, nkv, d in ((1, 5000, 1, 16, 8, 128), (8, 14000, 8, 16, 8, 128),
                                   (1, 5000, 1, 6, 2, 64)):
         dims = llmt.PackedDims(2, nq, nkv, d, n, tq, tk, 1.0, 16, 16)
-        assert llmt.lib().llmt_packed_attention_workspace(dims) > 0
+        assert llmt.lib().llmt_packed_attention_workspace(C.byref(dims)) > 0
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])

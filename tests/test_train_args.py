@@ -30,6 +30,8 @@ def packed(dims=None, ws=A(9), need=1 << 30, backward=False, lse=A(8), **views):
              o=heads(A(6), 256, 64), dout=heads(A(10), 256, 64), dq=heads(A(11), 256, 64),
              dk=heads(A(12), 128, 64), dv=heads(A(13), 128, 64))
     h.update(views)
+    h = {k: None if x is None else C.byref(x) for k, x in h.items()}
+    d = None if d is None else C.byref(d)
     L = llmt.lib()
     if backward:
         return L.llmt_packed_attention_bwd(d, h["q"], h["k"], h["v"], h["o"], lse, h["dout"], h["dq"],
@@ -71,16 +73,23 @@ def test_packed_attention_output_refusals(backward, bad):
     assert message().startswith("llmt_packed_attention")
 
 
+def test_the_bindings_bytes_are_the_structs():
+    assert llmt._HEADS.size == C.sizeof(llmt.Heads) and llmt._PACKED.size == C.sizeof(llmt.PackedDims)
+    a = llmt.PackedDims(1, 2, 3, 4, 5, 6, 7, 0.5, 8, 9)
+    assert bytes(a) == llmt._PACKED.pack(1, 2, 3, 4, 5, 6, 7, 0.5, 8, 9)
+    assert bytes(llmt.Heads(1, 2, 3)) == llmt._HEADS.pack(1, 2, 3)
+
+
 def test_workspaces_of_bad_sizes_are_none():
     L = llmt.lib()
     for bad in (dict(head_dim=32), dict(Tq=-1), dict(nq=3)):
-        d = llmt.PackedDims(**{**DIMS, **bad})
+        d = C.byref(llmt.PackedDims(**{**DIMS, **bad}))
         assert L.llmt_packed_attention_workspace(d) == 0 == L.llmt_packed_attention_bwd_workspace(d)
     assert L.llmt_packed_attention_workspace(None) == 0
     assert L.llmt_embedding_bwd_workspace(0, 5, 5) == 0 == L.llmt_embedding_bwd_workspace(5, 0, 5)
 
 
-def embed(backward=False, tok=A(1), T=10, w=A(2), wt=0, ldw=64, V=50, H=64, scale=1.0, x=A(3), xt=0,
+def embed(backward=False, tok=A(1), T=2000, w=A(2), wt=0, ldw=64, V=50, H=64, scale=1.0, x=A(3), xt=0,
           ldx=64, ws=A(4), need=1 << 30):
     L = llmt.lib()
     if backward:
@@ -90,11 +99,11 @@ def embed(backward=False, tok=A(1), T=10, w=A(2), wt=0, ldw=64, V=50, H=64, scal
 
 @pytest.mark.parametrize("backward", [False, True])
 @pytest.mark.parametrize("bad", [
-    dict(T=-1), dict(T=2 ** 30 + 1), dict(V=0), dict(V=2 ** 30 + 1, ldw=64), dict(H=0),
-    dict(H=2 ** 30 + 1, ldw=2 ** 31, ldx=2 ** 31), dict(wt=3), dict(xt=-1), dict(ldw=63), dict(ldx=63),
+    dict(T=-1), dict(T=2 ** 23 + 1), dict(V=0), dict(V=2 ** 30 + 1, ldw=64), dict(H=0),
+    dict(H=2 ** 20 + 1, ldw=2 ** 31, ldx=2 ** 31), dict(wt=3), dict(xt=-1), dict(ldw=63), dict(ldx=63),
     dict(ldw=2 ** 41), dict(ldx=2 ** 41), dict(scale=math.nan), dict(scale=math.inf), dict(tok=None),
     dict(w=None), dict(x=None), dict(w=A(2) + 2), dict(x=A(3) + 1, xt=1), dict(tok=A(1) + 2),
-    dict(x=A(2)), dict(x=A(2) + 50 * 256 - 4), dict(x=A(2) - 10 * 256 + 4)])
+    dict(x=A(2)), dict(x=A(2) + 50 * 256 - 4), dict(x=A(2) - 2000 * 256 + 4)])
 def test_embedding_refusals(bad, backward):
     assert embed(backward, **bad) == ARG
     assert message().startswith("llmt_embedding_bwd:" if backward else "llmt_embedding:")
