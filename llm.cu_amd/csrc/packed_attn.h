@@ -198,6 +198,21 @@ __device__ __forceinline__ short8v pair_frag(const floatx4& a, const floatx4& b)
   }
   return __builtin_bit_cast(short8v, r);
 }
+// The same in two parts, the rounded value and what it left out: twice the bits.
+template <class E>
+__device__ __forceinline__ void pair_split(const floatx4& a, const floatx4& b, short8v& hi,
+                                           short8v& lo) {
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  T8 h, l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = i < 4 ? a[i & 3] : b[i & 3];
+    h[i] = (typename E::T)x;
+    l[i] = (typename E::T)(x - (float)h[i]);
+  }
+  hi = __builtin_bit_cast(short8v, h);
+  lo = __builtin_bit_cast(short8v, l);
+}
 template <class E>
 __device__ __forceinline__ short4v round4(const floatx4& a) {
   typedef typename E::T T4 __attribute__((ext_vector_type(4)));

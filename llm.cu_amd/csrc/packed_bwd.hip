@@ -49,12 +49,13 @@ struct ColScale {
 };
 
 // ---------------------------------------------------------------- dQ
-// 16 NW RW rows a workgroup, 16 RW a wave, against keys in tiles of 64, two
-// halves one after the other.
-template <class E, int HD, int NW, int RW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+// Four waves of 16 RW rows, against keys in tiles of 64, two halves one after
+// the other.  (Two waves for each of two halves, as in dK/dV below, were slower
+// at every size: 16 sequences of 8192 tokens 215 us against 201.)
+template <class E, int HD, int RW>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+  constexpr int NW = 4, QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   typedef typename E::T T8 __attribute__((ext_vector_type(8)));
   __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
@@ -62,6 +63,7 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
+  const int row = w * RW * 16;
   const int j = blockIdx.x % a.nkv;
   Tile x;
   if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
@@ -76,13 +78,13 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
     dk.issue(kbase, a.k.token, 0, x.klen, buf0, w);
     dv.issue(vbase, a.v.token, 0, x.klen, buf0 + TILE, w);
   }
-  const int left = x.rows - x.row0 - w * RW * 16;  // rows from the wave's first on
+  const int left = x.rows - x.row0 - row;  // rows from the wave's first on
   short8v qf[RW][KS], df[RW][KS];
   int lim[RW], at[RW], hq[RW];
   float lse2[RW], del[RW];
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
-    const int i = min(w * RW * 16 + 16 * r + c, x.rows - 1 - x.row0);
+    const int i = min(row + 16 * r + c, x.rows - 1 - x.row0);
     const int t = gr.div(x.rem + i), h = x.rem + i - t * gr.G;
     lim[r] = 16 * r + c < left ? x.t0 + t + x.shift : -1;
     at[r] = x.qstart + x.t0 + t;
@@ -203,15 +205,16 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
 }
 
 // ---------------------------------------------------------------- dK, dV
-// 16 NW keys a workgroup, 16 a wave, in registers; the rows that see them pass
-// through LDS in tiles with their lse and delta.  Row r sees key k where
+// Four waves: 4 / JG groups of 16 keys, in registers; the rows that see them pass
+// through LDS in tiles with their lse and delta, two halves one after the other
+// (JG = 2: a wave takes one half, and the two groups' sums meet in LDS).  Row r sees key k where
 // r >= (k - shift) G: only the first tiles take a mask.  Rows of zeros (past the
 // end, or past the tile's whole tokens) add nothing by themselves, and keys
 // past the end are not stored.
-template <class E, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+template <class E, int HD, int JG>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int KB = NW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+  constexpr int NW = 4, WG = NW / JG, KB = WG * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
   constexpr int BUF = 2 * TILE + 2 * BLK * 2;
   __shared__ __attribute__((aligned(1024))) short buf0[BUF];
@@ -219,6 +222,7 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
+  const int jg = JG == 1 ? 0 : w / WG, wk = w - jg * WG;  // row group, key group
   const int j = blockIdx.x % a.nkv;
   int blk;
   SeqLens s;
@@ -226,7 +230,7 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   const Span qs = {s.qstart, s.ql}, ks = {s.kstart, s.kl};
   if (blk < 0 || blk >= (ks.len + KB - 1) / KB) return;
   const int shift = ks.len - qs.len;
-  const int k0 = blk * KB, kw = k0 + w * 16;
+  const int k0 = blk * KB, kw = k0 + wk * 16;
   const int tokens = 64 / gr.G, tr = tokens * gr.G;   // of a tile
   const int t0 = min(max(k0 - shift, 0), qs.len);     // the first token that sees a key
   const int niter = (qs.len - t0 + tokens - 1) / tokens;
@@ -279,7 +283,8 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
     const float* lse_s = reinterpret_cast<const float*>(Qs + 2 * TILE);
     const float* del_s = lse_s + BLK;
 #pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
+    for (int h = 0; h < 2 / JG; ++h) {
+      const int jj = JG == 1 ? h : jg;
       floatx4 p[2], ds[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -341,6 +346,28 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
     tile_step(it, std::false_type{}, buf0, buf1);
     if (it + 1 < niter) tile_step(it + 1, std::false_type{}, buf1, buf0);
   }
+  if constexpr (JG == 2) {  // [register][lane], where the tiles were
+    auto room = [&](int i) LLMT_INLINE { return reinterpret_cast<floatx4*>(i ? buf1 : buf0); };
+    static_assert(2 * DT * 64 * 16 <= BUF * 2, "a wave's sums fit a buffer");
+    __shared__ float scale[WG][16];
+    __syncthreads();
+    if (jg == 1) {
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        room(wk)[i * 64 + lane] = dkT[i];
+        room(wk)[(DT + i) * 64 + lane] = dvT[i];
+      }
+      if (g == 0) scale[wk][c] = F ? cs.s : 1.f;
+    }
+    __syncthreads();
+    if (jg == 1) return;
+    const float f = F ? cs.s / scale[wk][c] : 1.f;  // a power of two
+#pragma unroll
+    for (int i = 0; i < DT; ++i) {
+      dkT[i] += room(wk)[i * 64 + lane] * f;
+      dvT[i] += room(wk)[(DT + i) * 64 + lane];
+    }
+  }
   if (key < ks.len) {
     const float fk = F ? a.scale / cs.s : a.scale;
     const float fv = 1.0f / (float)(1 << E::PSH);
@@ -359,6 +386,8 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
 // waiting for its own loads, are the time: blocks of 16 rows (16 keys) whose
 // four waves take the tiles of 32 in turn, each through LDS of its own, without
 // a barrier in the loop; the waves' sums meet in LDS and are added in order.
+// They wait for loads, not for the matrix units, so P and dS enter in two parts
+// (pair_split), and nothing but the result is rounded to the type.
 template <class E, int HD>
 __global__ __launch_bounds__(256, 2)
 void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
@@ -449,9 +478,13 @@ void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) 
       dp[0] *= cs.s;
       dp[1] *= cs.s;
     }
-    const short8v db = pair_frag<E>(dp[0], dp[1]);
+    short8v db, dl;
+    pair_split<E>(dp[0], dp[1], db, dl);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) dqT[d] = E::mfma(frag_tr<HD>(Ks, d * 16, 0, lane), db, dqT[d]);
+    for (int d = 0; d < DT; ++d) {
+      const short8v kt = frag_tr<HD>(Ks, d * 16, 0, lane);
+      dqT[d] = E::mfma(kt, db, E::mfma(kt, dl, dqT[d]));
+    }
     if (kt + NW < nkt) {  // refill once this tile's reads have returned
       wait_lds();
       asm volatile("" ::: "memory");
@@ -577,11 +610,14 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
       ds[0] *= cs.s;
       ds[1] *= cs.s;
     }
-    const short8v pb = pair_frag<E>(p[0], p[1]), db = pair_frag<E>(ds[0], ds[1]);
+    short8v pb, pl, db, dl;
+    pair_split<E>(p[0], p[1], pb, pl);
+    pair_split<E>(ds[0], ds[1], db, dl);
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
-      dvT[i] = E::mfma(frag_tr<HD>(Ds, i * 16, 0, lane), pb, dvT[i]);
-      dkT[i] = E::mfma(frag_tr<HD>(Qs, i * 16, 0, lane), db, dkT[i]);
+      const short8v x = frag_tr<HD>(Ds, i * 16, 0, lane), y = frag_tr<HD>(Qs, i * 16, 0, lane);
+      dvT[i] = E::mfma(x, pb, E::mfma(x, pl, dvT[i]));
+      dkT[i] = E::mfma(y, db, E::mfma(y, dl, dkT[i]));
     }
     if (it + NW < niter) {
       wait_lds();
@@ -638,25 +674,29 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     if (split)
       hipLaunchKernelGGL((packed_dq_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
     else if (wide)
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
     else
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 4, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
+      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
     LLMT_LAUNCH_CHECK();
   }
   if (a.Tk) {
-    // the rows over a workgroup's waves up to 1280 blocks of 16 keys (us of a
-    // backward, 16 / 8 heads of 128, without -> with: 1 x 512 40 -> 27, 8 x 77 23 ->
-    // 19, 6 x 250 44 -> 38, 6 x 417 74 -> 72; above, 4 x 1000 136 -> 147), and up to
-    // 2048 where the chains are long (32 / 8 heads of 64, 4 x 1000 149 -> 129)
+    // By blocks of 16 keys: up to 768 the rows over a workgroup's waves, up to 3072
+    // (of half the width 1024, 6144) over two halves of it.  us of a backward in a graph,
+    // 16 / 8 heads of 128, waves / halves / whole: 1 x 512 26 / 31 / 38, 8 x 77 19 /
+    // 19 / 23, 6 x 250 38 / 38 / 44, 6 x 417 73 / 66 / 74, 4 x 1000 - / 127 / 137, 16 x
+    // 512 - / 167 / 155; 32 / 8 heads of 64: 4 x 500 55 / 62 / 75, 4 x 1000 129 / 127 /
+    // 150, 8 x 1024 - / 256 / 276
     const long long blocks = (long long)a.Tk / 16 * a.nkv;
-    const bool split = gr.G <= 32 && (blocks <= 1280 || (blocks <= 2048 && gr.G >= 4 &&
-                                                         a.Tq / a.n * gr.G >= 64 * 48));
-    const int nt = key_tiles(a, split ? 16 : 64);
+    const bool split = blocks <= (HD == 64 ? 1024 : 768) && gr.G <= 32;
+    const bool halves = blocks <= (HD == 64 ? 6144 : 3072);
+    const int nt = key_tiles(a, split ? 16 : halves ? 32 : 64);
     const dim3 grid((unsigned)nt * a.nkv);
     if (split)
       hipLaunchKernelGGL((packed_dkdv_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
+    else if (halves)
+      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
     else
-      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 4>), grid, dim3(256), 0, st, a, gr, nt, rv);
+      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
     LLMT_LAUNCH_CHECK();
   }
   return hipSuccess;

@@ -288,7 +288,9 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
 
 // Few rows: a workgroup takes 16 RW rows and one of nsplit parts of their keys,
 // in 32-key tiles that its four waves take in turn, each through LDS of its own
-// and without a barrier in the loop; the waves' results meet in LDS.  With
+// and without a barrier in the loop; the waves' results meet in LDS.  It waits
+// for loads, not for the matrix units, so probabilities enter the product in two
+// parts (pair_split), and nothing but the result is rounded to the type.  With
 // several parts the result goes to the workspace as (max, sum) and the
 // unnormalised output, for packed_join_kernel.
 constexpr int FS_KEYS = 32;
@@ -377,9 +379,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
       softmax_tile<E, RW, DT, false, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
     else
       softmax_tile<E, RW, DT, true, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
-    short8v pb[RW];
+    short8v pb[RW], pl[RW];
 #pragma unroll
-    for (int r = 0; r < RW; ++r) pb[r] = pair_frag<E>(st[r][0], st[r][1]);
+    for (int r = 0; r < RW; ++r) pair_split<E>(st[r][0], st[r][1], pb[r], pl[r]);
     if (next) wait_vm<Dma::CH>();  // this V tile (the next K tile may be in flight)
     else wait_vm<0>();
     asm volatile("" ::: "memory");
@@ -387,7 +389,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
     for (int dt = 0; dt < DT; ++dt) {
       const short8v vf = frag_tr<HD>(Vs, dt * 16, 0, lane);
 #pragma unroll
-      for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r], ot[r][dt]);
+      for (int r = 0; r < RW; ++r) ot[r][dt] = E::mfma(vf, pb[r], E::mfma(vf, pl[r], ot[r][dt]));
     }
     wait_lds();
     asm volatile("" ::: "memory");
