@@ -539,7 +539,9 @@ typedef struct {
  * A query without keys, and tokens of no sequence, have o 0 and lse -inf.  dtype
  * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
  * fp32, probabilities are rounded to dtype before the second product.
- * head_dim 64 or 128; nq at most 64 nkv; Tq nq / nkv and Tk at most 2^30. */
+ * head_dim 64 or 128; nq at most 64 nkv; and, the launches' limit, the larger of
+ * Tq nq / nkv and Tk at most 64 (2^23 / nkv - n - 2).  The scores of a query must
+ * be finite: a NaN or an infinity stays in its sequence. */
 typedef struct {
     int dtype, nq, nkv, head_dim;
     int n, Tq, Tk;
@@ -569,7 +571,8 @@ int llmt_embedding(const int* tokens, int T, const void* weight, int wdtype, lon
                    int H, float scale, void* out, int odtype, long long ldo, void* stream);
 /* Its gradient: dweight[v] = scale sum of dout[i] over tokens[i] = v, or that
  * added to what dweight holds (accumulate; rows of no token are then not
- * touched).  Sums are fp32 in the order of the positions, rounded once. */
+ * touched).  Sums are fp32, in an order that the positions alone decide, rounded
+ * once. */
 size_t llmt_embedding_bwd_workspace(int T, int V, int H);
 int llmt_embedding_bwd(const int* tokens, int T, const void* dout, int ddtype, long long ldd,
                        float scale, void* dweight, int wdtype, long long ldw, int V, int H,
@@ -590,7 +593,8 @@ int llmt_embedding_bwd(const int* tokens, int T, const void* dout, int ddtype, l
  * remainder, from a generator's draws of (seed, step, the tensor's place in the
  * list, element), a v above 0 to at least its smallest code; p is updated from
  * the moments before that rounding.  A block with a NaN or an infinity (or
- * beyond 2^127) becomes NaN.  No two written arrays may overlap, nor a written
+ * beyond 2^127) becomes NaN.  Betas in [0, 1), eps at least 2^-126, count at most
+ * 2^20, n 2^35.  No two written arrays may overlap, nor a written
  * one a gradient.  hp, step and seed are the call's: a captured call repeats
  * them. */
 typedef struct {

@@ -211,8 +211,11 @@ __global__ __launch_bounds__(NTH) void adamw_list_kernel(const AdamBatch<BITS> b
     for (int e = 0; e < 4; ++e) {
       const float gg = k.gscale ? g[e] * gs : g[e];
       moments(k, gg, m[e], v[e]);
-      const float denom = __builtin_amdgcn_sqrtf(v[e] * k.ib2) + k.eps;
-      p[e] = p[e] * k.decay - k.lr * (m[e] * k.ib1) * __builtin_amdgcn_rcpf(denom);
+      // the root's instruction takes a subnormal for 0: small v at 2^64 times their size
+      const bool low = v[e] < 0x1p-64f;
+      const float root = __builtin_amdgcn_sqrtf((low ? v[e] * 0x1p64f : v[e]) * k.ib2);
+      const float denom = (low ? root * 0x1p-32f : root) + k.eps;
+      p[e] = p[e] * k.decay - k.lr * (m[e] * k.ib1 * __builtin_amdgcn_rcpf(denom));
     }
     store4(t.p + at, vec, ok, p);
     if (t.ctype == kF16) store4((_Float16*)t.copy + at, vec, ok, p);

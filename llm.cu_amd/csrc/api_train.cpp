@@ -316,8 +316,9 @@ int llmt_adamw_update(const llmt_adam_tensor* t, int count, int state_bits, cons
   TRY_ARG(state_bits == 8 || state_bits == 32, "%s: moments of %d bits (8 or 32)", fn, state_bits);
   TRY_ARG(hp, "%s: NULL hp", fn);
   TRY_ARG(isfinite(hp->lr) && isfinite(hp->wd) && hp->beta1 >= 0.f && hp->beta1 < 1.f &&
-              hp->beta2 >= 0.f && hp->beta2 < 1.f && hp->eps > 0.f && isfinite(hp->eps) && step >= 1,
-          "%s: betas in [0, 1), eps positive, step from 1 on, finite lr and wd", fn);
+              hp->beta2 >= 0.f && hp->beta2 < 1.f && hp->eps >= 0x1p-126f && isfinite(hp->eps) &&
+              step >= 1,
+          "%s: betas in [0, 1), eps from 2^-126, step from 1 on, finite lr and wd", fn);
   TRY_ARG(aligned(grad_scale, 4), "%s: misaligned grad_scale", fn);
   for (int i = 0; i < count; ++i) {
     const llmt_adam_tensor& x = t[i];

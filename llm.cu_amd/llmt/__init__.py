@@ -630,7 +630,11 @@ def packed_attention_bwd(q, k, v, o, lse, dout, q_offsets, k_offsets=None, scale
     gradient of o.  out: the three tensors to write, of any strides (parts of a fused
     projection's gradient)."""
     import torch
-    dq, dk, dv = (None, None, None) if out is None else out
+    dq = dk = dv = None
+    if out is not None:
+        if len(out) != 3 or any(t is None for t in out):
+            raise LlmtError("out must be the three tensors dq, dk and dv")
+        dq, dk, dv = out
     with _On("q k v o lse dout q_offsets k_offsets dq dk dv",
              (q, k, v, o, lse, dout, q_offsets, k_offsets, dq, dk, dv), stream) as on:
         dims, qs, ks, dtype = _packed_dims(q, k, v, q_offsets, k_offsets, scale)
@@ -728,7 +732,9 @@ def adamw_state(p, bits=32) -> AdamState:
 class AdamTensors:
     """A list of tensors for adamw_update: parameters fp32, gradients of any type, states (of
     adamw_state, all of one width) and, where given, 16-bit working copies (or None for some);
-    contiguous, all on one device.  Holds the tensors: a program makes one and keeps it."""
+    contiguous, all on one device.  Keeps their memory: a program makes one list and updates it
+    every step.  A tensor that is given other memory later (``p.data = ..``, gradients set to None
+    and made anew) needs set_grads or a new list."""
 
     def __init__(self, params, grads, states, copies=None):
         import torch
@@ -759,7 +765,7 @@ class AdamTensors:
                 p.data_ptr(), g.data_ptr(), s[0].data_ptr(), s[1].data_ptr(), _at(s[2]), _at(s[3]),
                 _at(c), n, _type_code(f"grads[{i}]", g.dtype),
                 0 if c is None else _type_code("copies", c.dtype))
-            self.tensors.append([p, g, *s, c])
+            self.tensors.append([None if t is None else t.detach() for t in (p, g, *s, c)])
 
     def _check(self, name, t, dtype, size, bits, kind):
         import torch
@@ -788,14 +794,15 @@ class AdamTensors:
         for i, g in enumerate(grads):
             self.table[i].g = g.data_ptr()
             self.table[i].g_dtype = _type_code("grads", g.dtype)
-            self.tensors[i][1] = g
+            self.tensors[i][1] = g.detach()
 
 
 def adamw_update(tensors: AdamTensors, hp: HParams, step: int, grad_scale=None, seed=0,
                  stream=None):
     """One AdamW step in place over all tensors (llmt_adamw_update).  grad_scale fp32 [1] on the
     device: a factor of the gradients (clipping, a loss scale's inverse).  seed: of the 8-bit
-    moments' rounding; the step's number enters its draws too."""
+    moments' rounding; the step's number enters its draws too.  A captured call keeps its step and
+    its tensors."""
     import torch
     if not tensors.tensors:
         return

@@ -163,6 +163,38 @@ def test_small_moments_beside_large_ones(dev):
         assert (v > 0).all()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_smallest_gradients(dev, bits):
+    """Squares that are subnormal numbers, under an eps below them: the moments bit for bit, the
+    update as for any other size."""
+    n = 768
+    g = (10.0 ** torch.linspace(-20, -17, n)).to(dev)
+    hp = dict(HP, eps=1e-30)
+    p = torch.zeros(n, device=dev)
+    s = llmt.adamw_state(p, bits)
+    z = np.zeros(n, np.float32)
+    llmt.adamw_update(llmt.AdamTensors([p], [g], [s]), llmt.hparams(**hp), 1, seed=2)
+    want, up, m, v = numpy_step(z, g.cpu().numpy(), z, z, 1, hp=hp)
+    assert (v > 0).all() and v.min() < 2.0 ** -126 and up.min() > 0.9 * HP["lr"]
+    check_p(p, want, up)
+    if bits == 32:
+        assert np.array_equal(s.m.cpu().numpy(), m) and np.array_equal(s.v.cpu().numpy(), v)
+
+
+def test_a_list_keeps_its_memory(dev):
+    """A parameter that is given other memory afterwards: the list's own is updated, not freed."""
+    ps, gs = problem([4000], dev=dev)
+    first = ps[0]
+    old = first.detach()
+    lst = llmt.AdamTensors(ps, gs, [llmt.adamw_state(first)])
+    want = old.clone()
+    llmt.adamw_update(llmt.AdamTensors([want], gs, [llmt.adamw_state(want)]), llmt.hparams(**HP), 1)
+    other = torch.full_like(old, 5.0)
+    first.data = other
+    llmt.adamw_update(lst, llmt.hparams(**HP), 1)
+    assert torch.equal(old, want) and (other == 5).all()
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
 def test_values_beyond_range(dev, bad):
     ps, gs = problem([700], dev=dev)

@@ -43,6 +43,8 @@ def packed(dims=None, ws=A(9), need=1 << 30, backward=False, lse=A(8), **views):
 @pytest.mark.parametrize("bad", [
     dict(dims=False), dict(dims=dict(dtype=0)), dict(dims=dict(dtype=3)), dict(dims=dict(nq=5)),
     dict(dims=dict(nkv=0)), dict(dims=dict(nq=0)), dict(dims=dict(nq=8192, nkv=1)),
+    dict(dims=dict(nq=65, nkv=1)), dict(dims=dict(nq=130, nkv=2)),
+    dict(dims=dict(nq=16, nkv=16, n=2 ** 19)), dict(dims=dict(nq=32, nkv=32, Tk=2 ** 24)),
     dict(dims=dict(head_dim=96)), dict(dims=dict(n=0)), dict(dims=dict(n=2 ** 25)),
     dict(dims=dict(Tq=-1)), dict(dims=dict(Tk=-1)), dict(dims=dict(Tq=2 ** 30)),
     dict(dims=dict(Tk=2 ** 30 + 1)), dict(dims=dict(scale=0.0)), dict(dims=dict(scale=-1.0)),
@@ -127,7 +129,7 @@ def adam(tensors=None, count=None, bits=32, hp=(1e-3, 0.9, 0.99, 1e-8, 0.0), ste
 @pytest.mark.parametrize("bad", [
     dict(bits=16), dict(bits=0), dict(hp=None), dict(step=0), dict(step=-3), dict(count=-1),
     dict(count=2 ** 21), dict(hp=(math.nan, 0.9, 0.99, 1e-8, 0)), dict(hp=(1, 1.0, 0.99, 1e-8, 0)),
-    dict(hp=(1, 0.9, 1.0, 1e-8, 0)), dict(hp=(1, -0.1, 0.9, 1e-8, 0)), dict(hp=(1, 0.9, 0.9, 0.0, 0)),
+    dict(hp=(1, 0.9, 1.0, 1e-8, 0)), dict(hp=(1, -0.1, 0.9, 1e-8, 0)), dict(hp=(1, 0.9, 0.9, 0.0, 0)), dict(hp=(1, 0.9, 0.9, 1e-40, 0)),
     dict(hp=(1, 0.9, 0.9, 1e-8, math.inf)), dict(scale=A(8) + 2), dict(n=-1), dict(n=2 ** 41),
     dict(g_dtype=3), dict(copy_dtype=0), dict(p=None), dict(g=None), dict(m=None), dict(v=None),
     dict(bits=8, m_exp=None), dict(bits=8, v_exp=None), dict(p=A(1) + 2), dict(g=A(2) + 1),
@@ -182,6 +184,9 @@ def test_the_binding_refuses_host_tensors():
                  lambda: llmt.AdamTensors([x[0].float()], [x[0]], [llmt.adamw_state(x[0])])):
         with pytest.raises(llmt.LlmtError, match="must be a device tensor"):
             call()
+    for out in ((x, x), (x, None, x)):
+        with pytest.raises(llmt.LlmtError, match="three tensors"):
+            llmt.packed_attention_bwd(x, x, x, x, x, x, t, out=out)
     with pytest.raises(llmt.LlmtError, match="32 or 8"):
         llmt.adamw_state(x, 16)
     with pytest.raises(llmt.LlmtError, match="grads"):
