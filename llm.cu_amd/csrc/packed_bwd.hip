@@ -680,7 +680,7 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     LLMT_LAUNCH_CHECK();
   }
   if (a.Tk) {
-    // By blocks of 16 keys: up to 768 the rows over a workgroup's waves, up to 3072
+    // By blocks of 16 keys: up to 768 the rows over a workgroup's waves, up to 2560
     // (of half the width 1024, 6144) over two halves of it.  us of a backward in a graph,
     // 16 / 8 heads of 128, waves / halves / whole: 1 x 512 26 / 31 / 38, 8 x 77 19 /
     // 19 / 23, 6 x 250 38 / 38 / 44, 6 x 417 73 / 66 / 74, 4 x 1000 - / 127 / 137, 16 x
@@ -688,7 +688,7 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
     // 150, 8 x 1024 - / 256 / 276
     const long long blocks = (long long)a.Tk / 16 * a.nkv;
     const bool split = blocks <= (HD == 64 ? 1024 : 768) && gr.G <= 32;
-    const bool halves = blocks <= (HD == 64 ? 6144 : 3072);
+    const bool halves = blocks <= (HD == 64 ? 6144 : 2560);
     const int nt = key_tiles(a, split ? 16 : halves ? 32 : 64);
     const dim3 grid((unsigned)nt * a.nkv);
     if (split)

@@ -84,7 +84,10 @@ def test_keys_of_another_length(dev, dtype, nq, nkv, d, ql, kl):
 @pytest.mark.parametrize("dtype,nq,nkv,d,ql", [
     (BF, 16, 8, 128, [700, 1, 513, 64, 1000]), (HF, 16, 8, 128, [2049, 31, 900, 1200]),
     (BF, 32, 8, 64, [1300, 777]), (HF, 6, 2, 128, [3000]), (BF, 5, 1, 64, [4100, 3]),
-    (BF, 16, 8, 128, [4099, 130]), (HF, 32, 8, 64, [2100, 65, 7])])
+    (BF, 16, 8, 128, [4099, 130]), (HF, 32, 8, 64, [2100, 65, 7]),
+    # keys enough for workgroups of 64 in one piece
+    (BF, 16, 16, 128, [3300, 50]), (HF, 16, 16, 128, [1, 2700]), (HF, 32, 32, 64, [3310]),
+    (BF, 40, 40, 64, [2500, 131])])
 def test_many_rows(dev, dtype, nq, nkv, d, ql):
     check(*problem(dev, dtype, d, nq, nkv, ql, qkv=True), same=True)
 
@@ -98,6 +101,41 @@ def test_many_sequences(dev, dtype, n):
     kl = [a + b for a, b in zip(ql, torch.randint(0, 9, (n,), generator=g).tolist())]
     q, k, v, do, qo, ko = problem(dev, dtype, 64, 2, 1, ql, kl)
     check(q, k, v, do, qo, ko)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nq,nkv,d", [(33, 1, 64), (64, 1, 128), (128, 2, 64)])
+@pytest.mark.parametrize("ql,kl", [([1], [1]), ([2, 63, 17], None), ([300, 5], None), ([1, 3], [700, 2])])
+def test_large_groups(dev, dtype, nq, nkv, d, ql, kl):
+    """Up to 64 query heads share a KV head: a token is a whole tile."""
+    check(*problem(dev, dtype, d, nq, nkv, ql, kl))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n", [253, 254, 255])
+@pytest.mark.parametrize("most", [3, 70])
+def test_as_many_sequences_as_are_ordered(dev, dtype, n, most):
+    g = torch.Generator().manual_seed(n + most)
+    ql = torch.randint(0, most, (n,), generator=g).tolist()
+    check(*problem(dev, dtype, 64, 4, 4, ql, pad=5))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("ql,kl", [([40, 33, 70], None), ([700, 900, 1100], None), ([1, 1, 1], [90, 900, 2000])])
+def test_a_sequence_of_nan_stays_alone(dev, dtype, ql, kl):
+    """NaN and infinities in one sequence leave its neighbours' bits as they were, in tiles that
+    both have rows in."""
+    q, k, v, do, qo, ko = problem(dev, dtype, 128, 16, 8, ql, kl)
+    o, lse = llmt.packed_attention(q, k, v, qo, ko)
+    want = (o, lse, *llmt.packed_attention_bwd(q, k, v, o, lse, do, qo, ko))
+    a, b, c, e = int(qo[1]), int(qo[2]), int(ko[1]), int(ko[2])
+    for bad in (math.nan, INF):
+        q2, k2, v2, do2 = (t.clone() for t in (q, k, v, do))
+        q2[a:b], do2[a:b], k2[c:e], v2[c:e] = bad, bad, bad, bad
+        o, lse = llmt.packed_attention(q2, k2, v2, qo, ko)
+        got = (o, lse, *llmt.packed_attention_bwd(q2, k2, v2, o, lse, do2, qo, ko))
+        for x, y, i, j in zip(got, want, (a, a, a, c, c), (b, b, b, e, e)):
+            assert torch.equal(x[:i], y[:i]) and torch.equal(x[j:], y[j:])
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
