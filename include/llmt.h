@@ -540,8 +540,9 @@ typedef struct {
  * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
  * fp32, probabilities are rounded to dtype before the second product.
  * head_dim 64 or 128; nq at most 64 nkv; and, the launches' limit, the larger of
- * Tq nq / nkv and Tk at most 64 (2^23 / nkv - n - 2).  The scores of a query must
- * be finite: a NaN or an infinity stays in its sequence. */
+ * Tq nq / nkv and Tk at most 64 (2^23 / nkv - n - 2).  Scores (scale q k) up to
+ * 2^24 in magnitude; larger ones, and NaN or infinities in the inputs, spoil
+ * results of their own sequence only. */
 typedef struct {
     int dtype, nq, nkv, head_dim;
     int n, Tq, Tk;
@@ -554,7 +555,8 @@ int llmt_packed_attention(const llmt_packed_dims* dims, const llmt_heads* q, con
                           const llmt_heads* v, const llmt_heads* o, float* lse, void* workspace,
                           size_t workspace_bytes, void* stream);
 /* Its gradients, in dtype: dq of the queries, dk and dv of the keys (summed over
- * a group's query heads), from the forward's o and lse and dout = d o.  Queries
+ * a group's query heads), from the forward's o and lse and dout = d o.  (The
+ * rounding of lse to fp32 is 2^-23 of its magnitude in every probability.)  Queries
  * without keys, keys without queries and tokens of no sequence get zeros. */
 size_t llmt_packed_attention_bwd_workspace(const llmt_packed_dims* dims);
 int llmt_packed_attention_bwd(const llmt_packed_dims* dims, const llmt_heads* q,

@@ -260,6 +260,7 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
     // the rest, masked: i is even
     for (; i < nkb; ++i) {
       const bool odd = i & 1;
+      wait_lds();  // the reads of the tiles that the next ones replace have returned
       land(i, odd ? kbuf1 : kbuf0, odd ? vbuf0 : vbuf1);
       short8v pb[RW][2];
       probs(sa, pb);

@@ -599,9 +599,13 @@ def _packed_dims(q, k, v, q_offsets, k_offsets, scale):
     else:
         _expect("k_offsets", k_offsets, torch.int32, n + 1)
     _sizes("tokens, heads", n + 1, *qs, *ks)
-    return _PACKED.pack(code, qs[1], ks[1], qs[2], n, qs[0], ks[0],
-                        qs[2] ** -0.5 if scale is None else scale, q_offsets.data_ptr(),
-                        k_offsets.data_ptr()), qs, ks, dtype
+    if scale is None:
+        scale = (qs[2] or 1) ** -0.5
+    try:
+        return _PACKED.pack(code, qs[1], ks[1], qs[2], n, qs[0], ks[0], scale, q_offsets.data_ptr(),
+                            k_offsets.data_ptr()), qs, ks, dtype
+    except (OverflowError, struct.error):
+        raise LlmtError(f"scale must be positive and finite in fp32 (got {scale})") from None
 
 
 def packed_attention(q, k, v, q_offsets, k_offsets=None, scale=None, out=None, stream=None):

@@ -216,6 +216,29 @@ def test_scale_and_large_scores(dev, dtype):
     assert torch.isfinite(o).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("ql", [[200], [3000]])
+def test_scores_of_millions(dev, dtype, ql):
+    """Scores up to 2^24: one key has all of a row's weight.  A row of q is the row of a key that it
+    sees: their product is 2^23, those with the other keys (signs drawn apart) less than 2^22, and
+    what fp32 leaves out of a score is below 2.  o is then v's row: off by one rounding of P and its
+    own.  lse: five roundings and constants of 2^-24."""
+    g = torch.Generator().manual_seed(1)
+    T = ql[0]
+    k = torch.where(torch.rand(T, 1, 128, generator=g) < 0.5, -1.0, 1.0) * 256
+    pick = torch.tensor([int(torch.randint(0, t + 1, (1,), generator=g)) for t in range(T)])
+    q = k[pick].repeat(1, 2, 1)
+    v, do = torch.randn(T, 1, 128, generator=g), torch.randn(T, 2, 128, generator=g)
+    q, k, v, do = (t.to(dtype).to(dev) for t in (q, k, v, do))
+    off = offsets(ql).to(dev)
+    o, lse = llmt.packed_attention(q, k, v, off, scale=1.9)
+    want = v[pick.to(dev)].repeat(1, 2, 1).double()
+    assert ((o.double() - want).abs() <= 2.02 * ref.unit(dtype) * want.abs()).all()
+    assert torch.allclose(lse, torch.full_like(lse, 1.9 * 2 ** 23), rtol=2 ** -21, atol=0)
+    dq, dk, dv = llmt.packed_attention_bwd(q, k, v, o, lse, do, off, scale=1.9)
+    assert all(t.isfinite().all() for t in (dq, dk, dv))
+
+
 @pytest.mark.parametrize("dtype,small", [(HF, 2.0 ** -13), (BF, 2.0 ** -60)])
 @pytest.mark.parametrize("ql", [[300, 41], [1500, 900]])
 def test_small_gradients_keep_their_bits(dev, dtype, small, ql):

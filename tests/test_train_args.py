@@ -187,6 +187,9 @@ def test_the_binding_refuses_host_tensors():
     for out in ((x, x), (x, None, x)):
         with pytest.raises(llmt.LlmtError, match="three tensors"):
             llmt.packed_attention_bwd(x, x, x, x, x, x, t, out=out)
+    for scale in (1e39, -1e39, "1"):
+        with pytest.raises(llmt.LlmtError):
+            llmt.packed_attention(x, x, x, t, scale=scale)
     with pytest.raises(llmt.LlmtError, match="32 or 8"):
         llmt.adamw_state(x, 16)
     with pytest.raises(llmt.LlmtError, match="grads"):
