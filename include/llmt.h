@@ -540,7 +540,7 @@ typedef struct {
  * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
  * fp32, probabilities are rounded to dtype before the second product.
  * head_dim 64 or 128; nq at most 64 nkv; and, the launches' limit, the larger of
- * Tq nq / nkv and Tk at most 64 (2^23 / nkv - n - 2).  Scores (scale q k) up to
+ * Tq nq / nkv and Tk at most 64 ((2^23 - 2^12) / nkv - n - 2).  Scores (scale q k) up to
  * 2^24 in magnitude; larger ones, and NaN or infinities in the inputs, spoil
  * results of their own sequence only. */
 typedef struct {

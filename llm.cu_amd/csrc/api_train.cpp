@@ -44,10 +44,11 @@ static bool dims_ok(const llmt_packed_dims* d) {
     return false;
   if (d->n < 1 || d->n > (1 << 24) || d->Tq < 0 || d->Tk < 0 || d->Tk > kMost) return false;
   const long long rows = (long long)d->Tq * (d->nq / d->nkv);
-  // A launch has at most 2^24 workgroups: two each 64 rows or keys, and two a
-  // sequence, for each KV head (one each 16 rows only where those are few).
+  // A launch has less than 2^24 workgroups: one each 64 rows and each 64 keys, and
+  // two a sequence, for each KV head, and up to 2^13 more where rows or keys are so
+  // few that their blocks are smaller.
   return rows <= kMost &&
-         (std::max<long long>(rows, d->Tk) / 64 + d->n + 2) * d->nkv * 2 < (1 << 24) &&
+         (std::max<long long>(rows, d->Tk) / 64 + d->n + 2) * d->nkv * 2 < (1 << 24) - (1 << 13) &&
          (long long)d->Tq * d->nq <= 0x7fffffff;
 }
 

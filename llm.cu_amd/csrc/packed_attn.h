@@ -409,13 +409,13 @@ __device__ __forceinline__ bool any_tile(const PackArgs& a, int G, int t, SeqLen
   return true;
 }
 
-// Workgroup t of a launch of nt tiles a KV head: the spans of its sequence and
+// Tile t of nt in a launch of `all` a KV head: the spans of its sequence and
 // its block in it, which may lie behind the sequence's end (or, with malformed
 // offsets, before it).
 template <bool ROWS, int QB>
-__device__ __forceinline__ bool pick_tile(const PackArgs& a, int G, int t, int nt, SeqLens* seq,
-                                          int* block) {
-  if (nt * a.nkv > 512 && a.n <= kOrdered) {
+__device__ __forceinline__ bool pick_tile(const PackArgs& a, int G, int t, int nt, int all,
+                                          SeqLens* seq, int* block) {
+  if (all * a.nkv > 512 && a.n <= kOrdered) {
     int level, top;
     if (!nth_longest<ROWS, QB>(a, G, t, seq, block, &level, &top)) return false;
     set_priority(level, top);
@@ -439,10 +439,10 @@ struct Tile {
   int t0, rem;  // the first row's token and head in the group
 };
 template <int QB>
-__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, int ntiles, Tile& x) {
+__device__ __forceinline__ bool find(const PackArgs& a, Group gr, int t, int ntiles, int all, Tile& x) {
   int blk;
   SeqLens s;
-  if (!pick_tile<true, QB>(a, gr.G, t, ntiles, &s, &blk)) return false;
+  if (!pick_tile<true, QB>(a, gr.G, t, ntiles, all, &s, &blk)) return false;
   x.qstart = s.qstart;
   x.rows = s.ql * gr.G;
   if (blk < 0 || blk >= (x.rows + QB - 1) / QB) return false;

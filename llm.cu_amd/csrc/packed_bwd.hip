@@ -7,6 +7,16 @@
 // that see them: a sum over the whole group in registers, in a fixed order, no
 // atomics).  Rows, tiles and offsets: packed_attn.h.
 //
+// Both kinds are in one launch (Mix), behind one that writes each row's lse and
+// delta.  16 sequences of 8192 tokens together, 16 / 8 heads of 128 in bf16: 172
+// us, 195 with a launch for each kind, which both ended with the tiles of the
+// longest sequence; 1 x 512 tokens 21 and 28.  A long sequence is bound by issue:
+// a matrix instruction of 16 x 16 x 32 takes a SIMD 17 cycles, and the
+// exponentials and roundings of the other wave hardly run beside it (of the two
+// alone, 272 and 174 cycles, together 420).  1 x 8192 tokens take 872 us, 788
+// TFLOP/s of the five products, 1100 of the seven computed (S and dP twice); a
+// large library product reaches 1387.
+//
 // fp16.  dS spans many binades (a probability of one key in many times a small
 // gradient), so it enters its product times a power of two that belongs to the
 // accumulator's column (a row in dQ, a key in dK) and follows the largest value
@@ -21,9 +31,8 @@ namespace llmt {
 
 namespace {
 
-// Of each row in the order (KV head, token, head in the group), written by the dQ
-// blocks: the base-2 lse, +inf for a row without keys (its probabilities are
-// then 0), and delta.
+// Of each row in the order (KV head, token, head in the group): the base-2 lse,
+// +inf for a row without keys (its probabilities are then 0), and delta.
 struct RowVecs {
   float* lse2;
   float* delta;
@@ -48,25 +57,92 @@ struct ColScale {
   }
 };
 
+__device__ __forceinline__ float lse2_of(float lse) {
+  return lse == -INFINITY ? INFINITY : lse * LOG2E;
+}
+
+// Sum over a row's 8 or 16 lanes.
+template <int LR>
+__device__ __forceinline__ float row_lanes_sum(float x) {
+  x += dpp16<0xB1>(x);
+  x += dpp16<0x4E>(x);
+  x += dpp16<0x141>(x);
+  return LR == 16 ? x + dpp16<0x140>(x) : x;
+}
+
+// The rows' lse2 and delta: HD / 8 lanes a row.
+template <class E, int HD>
+__global__ __launch_bounds__(256) void packed_delta_kernel(const PackArgs a, int G, RowVecs rv) {
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  constexpr int LR = HD / 8;
+  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
+  if (row >= (long long)a.Tq * a.nq) return;
+  const long long t = row / a.nq;
+  const int h = (int)(row - t * a.nq), d = threadIdx.x % LR * 8;
+  const T8 x = *reinterpret_cast<const T8*>((const short*)a.dout.p + t * a.dout.token +
+                                            h * a.dout.head + d);
+  const T8 y = *reinterpret_cast<const T8*>((const short*)a.o.p + t * a.o.token + h * a.o.head + d);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
+  s = row_lanes_sum<LR>(s);
+  if (d) return;
+  const int j = h / G;
+  const long long at = vec_at(a, G, j, t) + h - j * G;
+  rv.lse2[at] = lse2_of(a.lse[row]);
+  rv.delta[at] = s;
+}
+
+// The workgroups of one launch are of keys (dK, dV) and of rows (dQ): a quarter of
+// those of keys, which take longest, then the others and those of rows in
+// turn, so that all end together.
+struct Mix {
+  int nrows, nkeys;           // tiles a KV head
+  unsigned long long share;  // of keys among what follows the quarter, times 2^32 (rounded up)
+  // The tiles of keys before tile t of the launch.
+  __device__ __forceinline__ int keys_before(int t) const {
+    const int k0 = nkeys >> 2;
+    return t < k0 ? t : k0 + (int)((t - k0) * share >> 32);
+  }
+};
+
+// LDS of a workgroup: two buffers, each two tiles of 64 with two vectors, or that
+// for two waves alone.
+constexpr int NW = 4;
+template <int HD>
+constexpr int kBuf = 2 * BLK * HD + 4 * BLK * 2;
+
+// Of one row's part in a lane (elements 32 ks + 8 g .. + 7 of df): its lse2 and
+// delta, from the forward's o and lse.
+template <class E, int KS>
+__device__ __forceinline__ float delta_of(const short8v (&df)[KS], const short* orow, int g) {
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  float s = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const T8 d8 = __builtin_bit_cast(T8, df[ks]);
+    const T8 o8 = *reinterpret_cast<const T8*>(orow + 32 * ks + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf((float)d8[e], (float)o8[e], s);
+  }
+  return xg_sum(s);
+}
+
 // ---------------------------------------------------------------- dQ
 // Four waves of 16 RW rows, against keys in tiles of 64, two halves one after
 // the other.  (Two waves for each of two halves, as in dK/dV below, were slower
-// at every size: 16 sequences of 8192 tokens 215 us against 201.)
-template <class E, int HD, int RW>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int NW = 4, QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+// at every size, 7% at 16 sequences of 8192 tokens.)
+template <class E, int HD, int RW, bool OWN>
+__device__ __forceinline__ void dq_block(const PackArgs& a, Group gr, int j, int tile, Mix mix,
+                                         RowVecs rv, short* buf0, short* buf1) {
+  constexpr int QB = NW * RW * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
-  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
-  __shared__ __attribute__((aligned(1024))) short buf0[2 * TILE];
-  __shared__ __attribute__((aligned(1024))) short buf1[2 * TILE];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int row = w * RW * 16;
-  const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
+  if (!find<QB>(a, gr, tile, mix.nrows, mix.nrows + mix.nkeys, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkb = (x.kmax + BLK - 1) / BLK;
@@ -91,24 +167,19 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
     hq[r] = j * gr.G + h;
     const short* row = (const short*)a.q.p + at[r] * a.q.token + hq[r] * a.q.head;
     const short* dor = (const short*)a.dout.p + at[r] * a.dout.token + hq[r] * a.dout.head;
-    const short* orow = (const short*)a.o.p + at[r] * a.o.token + hq[r] * a.o.head;
-    float s = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[r][ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
       df[r][ks] = *reinterpret_cast<const short8v*>(dor + 32 * ks + 8 * g);
-      const T8 d8 = __builtin_bit_cast(T8, df[r][ks]);
-      const T8 o8 = *reinterpret_cast<const T8*>(orow + 32 * ks + 8 * g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf((float)d8[e], (float)o8[e], s);
     }
-    del[r] = xg_sum(s);
-    const float e = a.lse[(long long)at[r] * a.nq + hq[r]];
-    lse2[r] = e == -INFINITY ? INFINITY : e * LOG2E;
-    if (16 * r + c < left && g == 0) {
+    if constexpr (OWN) {
+      const short* orow = (const short*)a.o.p + at[r] * a.o.token + hq[r] * a.o.head;
+      del[r] = delta_of<E, KS>(df[r], orow, g);
+      lse2[r] = lse2_of(a.lse[(long long)at[r] * a.nq + hq[r]]);
+    } else {
       const long long vi = vec_at(a, gr.G, j, at[r]) + h;
-      rv.lse2[vi] = lse2[r];
-      rv.delta[vi] = del[r];
+      lse2[r] = rv.lse2[vi];
+      del[r] = rv.delta[vi];
     }
   }
   const float sl2 = a.scale * LOG2E;
@@ -212,21 +283,18 @@ void packed_dq_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
 // end, or past the tile's whole tokens) add nothing by themselves, and keys
 // past the end are not stored.
 template <class E, int HD, int JG>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
-void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int NW = 4, WG = NW / JG, KB = WG * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
+__device__ __forceinline__ void dkdv_block(const PackArgs& a, Group gr, int j, int tile, Mix mix,
+                                           RowVecs rv, short* buf0, short* buf1,
+                                           float (*scale)[16]) {
+  constexpr int WG = NW / JG, KB = WG * 16, KS = HD / 32, DT = HD / 16, TILE = BLK * HD;
   constexpr bool F = std::is_same_v<E, F16>;
-  constexpr int BUF = 2 * TILE + 2 * BLK * 2;
-  __shared__ __attribute__((aligned(1024))) short buf0[BUF];
-  __shared__ __attribute__((aligned(1024))) short buf1[BUF];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int jg = JG == 1 ? 0 : w / WG, wk = w - jg * WG;  // row group, key group
-  const int j = blockIdx.x % a.nkv;
   int blk;
   SeqLens s;
-  if (!pick_tile<false, KB>(a, gr.G, blockIdx.x / a.nkv, ntiles, &s, &blk)) return;
+  if (!pick_tile<false, KB>(a, gr.G, tile, mix.nkeys, mix.nrows + mix.nkeys, &s, &blk)) return;
   const Span qs = {s.qstart, s.ql}, ks = {s.kstart, s.kl};
   if (blk < 0 || blk >= (ks.len + KB - 1) / KB) return;
   const int shift = ks.len - qs.len;
@@ -348,8 +416,7 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
   }
   if constexpr (JG == 2) {  // [register][lane], where the tiles were
     auto room = [&](int i) LLMT_INLINE { return reinterpret_cast<floatx4*>(i ? buf1 : buf0); };
-    static_assert(2 * DT * 64 * 16 <= BUF * 2, "a wave's sums fit a buffer");
-    __shared__ float scale[WG][16];
+    static_assert(2 * DT * 64 * 16 <= kBuf<HD> * 2, "a wave's sums fit a buffer");
     __syncthreads();
     if (jg == 1) {
 #pragma unroll
@@ -382,30 +449,28 @@ void packed_dkdv_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
 }
 
 // ---------------------------------------------------------------- few tiles
-// Where the launches above would leave CUs idle, their chains of tiles, each
+// Where the blocks above would leave CUs idle, their chains of tiles, each
 // waiting for its own loads, are the time: blocks of 16 rows (16 keys) whose
 // four waves take the tiles of 32 in turn, each through LDS of its own, without
 // a barrier in the loop; the waves' sums meet in LDS and are added in order.
 // They wait for loads, not for the matrix units, so P and dS enter in two parts
 // (pair_split), and nothing but the result is rounded to the type.
-template <class E, int HD>
-__global__ __launch_bounds__(256, 2)
-void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int NW = 4, QB = 16, KT = 32, KS = HD / 32, DT = HD / 16;
+template <class E, int HD, bool OWN>
+__device__ __forceinline__ void dq_split_block(const PackArgs& a, Group gr, int j, int tile,
+                                               Mix mix, RowVecs rv, short* buf0, short* buf1,
+                                               float (*scale)[16]) {
+  constexpr int QB = 16, KT = 32, KS = HD / 32, DT = HD / 16;
   constexpr bool F = std::is_same_v<E, F16>;
-  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
-  __shared__ __attribute__((aligned(1024))) short smem[NW * 2 * KT * HD];
-  __shared__ float scale[NW][16];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
+  if (!find<QB>(a, gr, tile, mix.nrows, mix.nrows + mix.nkeys, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkt = (x.kmax + KT - 1) / KT;
-  short* const Ks = smem + w * 2 * KT * HD;
+  auto room = [&](int u) LLMT_INLINE { return (u & 2 ? buf1 : buf0) + (u & 1) * 2 * KT * HD; };
+  short* const Ks = room(w);
   short* const Vs = Ks + KT * HD;
   KeyDma<HD, 1, KT> dk, dv;
   dk.init(a.k.token, 0);
@@ -419,28 +484,23 @@ void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) 
   const int t = gr.div(x.rem + min(c, left - 1)), h = x.rem + min(c, left - 1) - t * gr.G;
   const int lim = c < left ? x.t0 + t + x.shift : -1, at = x.qstart + x.t0 + t, hq = j * gr.G + h;
   short8v qf[KS], df[KS];
-  float del = 0.f;
   {
     const short* row = (const short*)a.q.p + at * a.q.token + hq * a.q.head;
     const short* dor = (const short*)a.dout.p + at * a.dout.token + hq * a.dout.head;
-    const short* orow = (const short*)a.o.p + at * a.o.token + hq * a.o.head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       qf[ks] = *reinterpret_cast<const short8v*>(row + 32 * ks + 8 * g);
       df[ks] = *reinterpret_cast<const short8v*>(dor + 32 * ks + 8 * g);
-      const T8 d8 = __builtin_bit_cast(T8, df[ks]);
-      const T8 o8 = *reinterpret_cast<const T8*>(orow + 32 * ks + 8 * g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) del = fmaf((float)d8[e], (float)o8[e], del);
     }
   }
-  del = xg_sum(del);
-  const float e = a.lse[(long long)at * a.nq + hq];
-  const float lse2 = e == -INFINITY ? INFINITY : e * LOG2E;
-  if (w == 0 && c < left && g == 0) {
+  float lse2, del;
+  if constexpr (OWN) {
+    del = delta_of<E, KS>(df, (const short*)a.o.p + at * a.o.token + hq * a.o.head, g);
+    lse2 = lse2_of(a.lse[(long long)at * a.nq + hq]);
+  } else {
     const long long vi = vec_at(a, gr.G, j, at) + h;
-    rv.lse2[vi] = lse2;
-    rv.delta[vi] = del;
+    lse2 = rv.lse2[vi];
+    del = rv.delta[vi];
   }
   const float sl2 = a.scale * LOG2E;
   floatx4 dqT[DT];
@@ -492,7 +552,7 @@ void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) 
     }
   }
   // the waves' sums, each in its own column scale, go where its tiles were
-  floatx4* const mine = reinterpret_cast<floatx4*>(smem + w * 2 * KT * HD);
+  floatx4* const mine = reinterpret_cast<floatx4*>(Ks);
   static_assert(DT * 64 * 16 <= 2 * KT * HD * 2, "a wave's sums fit its tiles");
   wait_lds();
   asm volatile("" ::: "memory");
@@ -507,7 +567,7 @@ void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) 
     floatx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NW; ++u) {
-      const floatx4 y = reinterpret_cast<const floatx4*>(smem + u * 2 * KT * HD)[d * 64 + lane];
+      const floatx4 y = reinterpret_cast<const floatx4*>(room(u))[d * 64 + lane];
       s += y * (a.scale / scale[u][c]);
     }
     if (c < left)
@@ -516,21 +576,19 @@ void packed_dq_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) 
   }
 }
 
-template <class E, int HD>
-__global__ __launch_bounds__(256, 2)
-void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv) {
-  constexpr int NW = 4, KB = 16, QT = 32, KS = HD / 32, DT = HD / 16, TILE = QT * HD;
+template <class E, int HD, bool OWN>
+__device__ __forceinline__ void dkdv_split_block(const PackArgs& a, Group gr, int j, int tile,
+                                                 Mix mix, RowVecs rv, short* buf0, short* buf1,
+                                                 float (*scale)[16]) {
+  constexpr int KB = 16, QT = 32, KS = HD / 32, DT = HD / 16, TILE = QT * HD;
   constexpr int BUF = 2 * TILE + 2 * 64 * 2;  // a wave's Q and dO tile, lse and delta
   constexpr bool F = std::is_same_v<E, F16>;
-  __shared__ __attribute__((aligned(1024))) short smem[NW * BUF];
-  __shared__ float scale[NW][16];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int j = blockIdx.x % a.nkv;
   int blk;
   SeqLens s;
-  if (!pick_tile<false, KB>(a, gr.G, blockIdx.x / a.nkv, ntiles, &s, &blk)) return;
+  if (!pick_tile<false, KB>(a, gr.G, tile, mix.nkeys, mix.nrows + mix.nkeys, &s, &blk)) return;
   if (blk < 0 || blk >= (s.kl + KB - 1) / KB) return;
   const int shift = s.kl - s.ql, key = blk * KB + c;
   const int tokens = QT / gr.G, tr = tokens * gr.G;
@@ -539,20 +597,40 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
   const int rmin = (min(max(key - shift, 0), s.ql) - t0) * gr.G;
   const short* qbase = (const short*)a.q.p + s.qstart * a.q.token + j * gr.G * a.q.head;
   const short* dbase = (const short*)a.dout.p + s.qstart * a.dout.token + j * gr.G * a.dout.head;
-  const long long vbase = vec_at(a, gr.G, j, s.qstart + t0);
-  short* const Qs = smem + w * BUF;
+  const short* obase = (const short*)a.o.p + s.qstart * a.o.token + j * gr.G * a.o.head;
+  auto room = [&](int u) LLMT_INLINE { return (u & 2 ? buf1 : buf0) + (u & 1) * BUF; };
+  static_assert(2 * BUF <= kBuf<HD>, "two waves a buffer");
+  short* const Qs = room(w);
   short* const Ds = Qs + TILE;
   float* const lse_s = reinterpret_cast<float*>(Qs + 2 * TILE);
   float* const del_s = lse_s + 64;
   RowDma<HD, 1, QT> dq_, dd_;
   dq_.init(a.q.token, a.q.head, gr, tr, 0);
   dd_.init(a.dout.token, a.dout.head, gr, tr, 0);
+  const long long vbase = vec_at(a, gr.G, j, s.qstart + t0);
+  // OWN: o's pieces of 8 of the tile's rows, HD / 8 lanes a row, and (lanes below QT) its lse
+  constexpr int LR = HD / 8, RL = 64 / LR, NO = QT / RL;
+  typedef typename E::T T8 __attribute__((ext_vector_type(8)));
+  T8 ov[NO];
+  float lv = 0.f;
   auto issue = [&](int it) LLMT_INLINE {
     const int t = t0 + it * tokens;
     dq_.issue(qbase, a.q.token, a.q.head, gr, t, s.ql, tokens, Qs, 0);
     dd_.issue(dbase, a.dout.token, a.dout.head, gr, t, s.ql, tokens, Ds, 0);
-    dma_vec64(rv.lse2 + vbase, it * tr, min(rows, (it + 1) * tr), lse_s);
-    dma_vec64(rv.delta + vbase, it * tr, min(rows, (it + 1) * tr), del_s);
+    if constexpr (OWN) {
+      const int here = min(tr, rows - it * tr);
+#pragma unroll
+      for (int i = 0; i < NO; ++i) {
+        const int r = min(RL * i + lane / LR, here - 1), u = gr.div(r);
+        ov[i] = *reinterpret_cast<const T8*>(obase + (t + u) * a.o.token +
+                                             (r - u * gr.G) * a.o.head + lane % LR * 8);
+      }
+      const int r = min(lane, here - 1), u = gr.div(r);
+      lv = a.lse[(long long)(s.qstart + t + u) * a.nq + j * gr.G + r - u * gr.G];
+    } else {
+      dma_vec64(rv.lse2 + vbase, it * tr, min(rows, (it + 1) * tr), lse_s);
+      dma_vec64(rv.delta + vbase, it * tr, min(rows, (it + 1) * tr), del_s);
+    }
   };
   if (w < niter) issue(w);
   const int tok = s.kstart + min(key, s.kl - 1);
@@ -577,6 +655,21 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
   for (int it = w; it < niter; it += NW) {
     wait_vm<0>();  // the wave's own tile
     asm volatile("" ::: "memory");
+    if constexpr (OWN) {
+      // rows of zeros (past the tile's tokens, or past the end) have no probabilities
+      const int here = rows - it * tr < tr ? rows - it * tr : tr;
+#pragma unroll
+      for (int i = 0; i < NO; ++i) {
+        const int r = RL * i + lane / LR;
+        const T8 d8 = *reinterpret_cast<const T8*>(Ds + toff<HD>(r, lane % LR));
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = fmaf((float)d8[e], (float)ov[i][e], x);
+        x = row_lanes_sum<LR>(x);
+        if (lane % LR == 0) del_s[r] = r < here ? x : 0.f;
+      }
+      if (lane < QT) lse_s[lane] = lane < here ? lse2_of(lv) : INFINITY;
+    }
     floatx4 p[2], ds[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -625,7 +718,7 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
       issue(it + NW);
     }
   }
-  floatx4* const mine = reinterpret_cast<floatx4*>(smem + w * BUF);
+  floatx4* const mine = reinterpret_cast<floatx4*>(Qs);
   static_assert(2 * DT * 64 * 16 <= BUF * 2, "a wave's sums fit its tiles");
   wait_lds();
   asm volatile("" ::: "memory");
@@ -643,7 +736,7 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
     floatx4 sk = {0.f, 0.f, 0.f, 0.f}, sv = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NW; ++u) {
-      const floatx4* y = reinterpret_cast<const floatx4*>(smem + u * BUF);
+      const floatx4* y = reinterpret_cast<const floatx4*>(room(u));
       sk += y[d * 64 + lane] * (a.scale / scale[u][c]);
       sv += y[(DT + d) * 64 + lane];
     }
@@ -656,55 +749,97 @@ void packed_dkdv_split_kernel(const PackArgs a, Group gr, int ntiles, RowVecs rv
   }
 }
 
+template <class E, int HD, int ROWS, int KEYS>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void packed_bwd_kernel(const PackArgs a, Group gr, Mix mix, RowVecs rv) {
+  __shared__ __attribute__((aligned(1024))) short buf0[kBuf<HD>];
+  __shared__ __attribute__((aligned(1024))) short buf1[kBuf<HD>];
+  __shared__ float scale[NW][16];
+  const int j = blockIdx.x % a.nkv, t = blockIdx.x / a.nkv;
+  const int kt = mix.keys_before(t);
+  if (mix.keys_before(t + 1) > kt) {
+    if constexpr (KEYS <= 1)
+      dkdv_split_block<E, HD, KEYS == 0>(a, gr, j, kt, mix, rv, buf0, buf1, scale);
+    else
+      dkdv_block<E, HD, KEYS == 2 ? 2 : 1>(a, gr, j, kt, mix, rv, buf0, buf1, scale);
+  } else {
+    if constexpr (ROWS == 0)
+      dq_split_block<E, HD, KEYS == 0>(a, gr, j, t - kt, mix, rv, buf0, buf1, scale);
+    else
+      dq_block<E, HD, ROWS, KEYS == 0>(a, gr, j, t - kt, mix, rv, buf0, buf1);
+  }
+}
+
+// The blocks' kinds.  rows: 0 keys over a workgroup's waves, else 16 times that a wave;
+// keys: 0 and 1 the rows over a workgroup's waves, 2 over its two halves, 3 not;
+// with 0 every block works out the rows' delta for itself.
+//
+// Fewer and longer chains of tiles against idle CUs, us of a call in a graph, bf16,
+// the kind of smaller blocks first:
+//   rows 0 and keys 1, or 1 and 2: one head of 128, 1 x 8000 126 / 179; 16 / 8 heads of
+//     128, 1 x 512 23.8 / 21.4, 6 x 250 37.5 / 31.7; 32 / 8 of 64, 4 x 250 24.6 / 28.2
+//   rows 1 or 2: 16 / 8 of 128, 6 x 417 58 / 55, 4 x 1000 130 / 121
+//   keys 2 or 3: 16 / 8 of 128, 6 x 417 55 / 58, 4 x 1000 121 / 110; 32 / 8 of 64,
+//     4 x 1000 115 / 128, 8 x 1024 257 / 238
+// keys 0 saves the launch before and is longer by tile: 16 / 8 of 128, 8 x 77 called
+// from a program 18.4 / 22.0 us, 4 / 4 heads of 128, 2 x 500 21.1 / 17.6, one head 1 x
+// 2000 45 / 28.
+struct BwdPlan {
+  int rows, keys;
+};
+BwdPlan bwd_plan(const PackArgs& a) {
+  const long long rows = (long long)a.Tq * (a.nq / a.nkv), blocks = (long long)a.Tk / 16 * a.nkv;
+  const bool far = a.Tk / a.n >= 1024, half = a.hd == 64;
+  BwdPlan p{};
+  p.rows = rows / 16 * a.nkv <= (far ? 512 : 256) ? 0 : rows / 128 * a.nkv >= 256 ? 2 : 1;
+  p.keys = blocks <= (far ? 768 : half ? 512 : 384) && a.nq / a.nkv <= 32
+               ? (rows / a.n <= 256 ? 0 : 1)
+               : (blocks <= (half ? 3000 : 1280) ? 2 : 3);
+  if (p.keys == 0 && p.rows == 2) p.rows = 1;
+  return p;
+}
+
 template <class E, int HD>
 hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   const Group gr = group_of(a);
   const long long R = (long long)a.Tq * a.nq;
   RowVecs rv = {(float*)ws, (float*)ws + R};
-  if (a.Tq) {
-    const long long rows = (long long)a.Tq * gr.G;
-    // 32 rows a wave feed two matrix instructions a fragment; 16 while that
-    // leaves CUs without a workgroup; the keys over a workgroup's waves while all
-    // blocks of 16 rows run at once (us of a backward, without -> with: one head, 1
-    // x 2000 78 -> 62; 4 heads, 2 x 500 30 -> 26; 16 / 8 heads, 512 39 -> 39, above
-    // 8 x 77 23 -> 30)
-    const bool split = rows / 16 * a.nkv <= 512, wide = rows / 128 * a.nkv >= 256;
-    const int nt = row_tiles(a, split ? 16 : wide ? 128 : 64);
-    const dim3 grid((unsigned)nt * a.nkv);
-    if (split)
-      hipLaunchKernelGGL((packed_dq_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
-    else if (wide)
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
-    else
-      hipLaunchKernelGGL((packed_dq_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
+  if (a.Tq == 0 && a.Tk == 0) return hipSuccess;
+  const BwdPlan p = bwd_plan(a);
+  const int kr = p.rows, kk = p.keys;
+  if (a.Tq && kk) {
+    constexpr int RB = 256 / (HD / 8);
+    hipLaunchKernelGGL((packed_delta_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)), dim3(256),
+                       0, st, a, gr.G, rv);
     LLMT_LAUNCH_CHECK();
   }
-  if (a.Tk) {
-    // By blocks of 16 keys: up to 768 the rows over a workgroup's waves, up to 2560
-    // (of half the width 1024, 6144) over two halves of it.  us of a backward in a graph,
-    // 16 / 8 heads of 128, waves / halves / whole: 1 x 512 26 / 31 / 38, 8 x 77 19 /
-    // 19 / 23, 6 x 250 38 / 38 / 44, 6 x 417 73 / 66 / 74, 4 x 1000 - / 127 / 137, 16 x
-    // 512 - / 167 / 155; 32 / 8 heads of 64: 4 x 500 55 / 62 / 75, 4 x 1000 129 / 127 /
-    // 150, 8 x 1024 - / 256 / 276
-    const long long blocks = (long long)a.Tk / 16 * a.nkv;
-    const bool split = blocks <= (HD == 64 ? 1024 : 768) && gr.G <= 32;
-    const bool halves = blocks <= (HD == 64 ? 6144 : 2560);
-    const int nt = key_tiles(a, split ? 16 : halves ? 32 : 64);
-    const dim3 grid((unsigned)nt * a.nkv);
-    if (split)
-      hipLaunchKernelGGL((packed_dkdv_split_kernel<E, HD>), grid, dim3(256), 0, st, a, gr, nt, rv);
-    else if (halves)
-      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, rv);
-    else
-      hipLaunchKernelGGL((packed_dkdv_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, rv);
-    LLMT_LAUNCH_CHECK();
-  }
+  Mix mix{};
+  if (a.Tq) mix.nrows = row_tiles(a, kr == 0 ? 16 : 64 * kr);
+  if (a.Tk) mix.nkeys = key_tiles(a, kk < 2 ? 16 : 16 << (kk - 1));
+  const int nt = mix.nrows + mix.nkeys, k0 = mix.nkeys >> 2;
+  mix.share = (((unsigned long long)(mix.nkeys - k0) << 32) + nt - k0 - 1) / (nt - k0);
+  const auto kernel =
+      kr == 0   ? (kk == 0   ? packed_bwd_kernel<E, HD, 0, 0>
+                   : kk == 1 ? packed_bwd_kernel<E, HD, 0, 1>
+                   : kk == 2 ? packed_bwd_kernel<E, HD, 0, 2>
+                             : packed_bwd_kernel<E, HD, 0, 3>)
+      : kr == 1 ? (kk == 0   ? packed_bwd_kernel<E, HD, 1, 0>
+                   : kk == 1 ? packed_bwd_kernel<E, HD, 1, 1>
+                   : kk == 2 ? packed_bwd_kernel<E, HD, 1, 2>
+                             : packed_bwd_kernel<E, HD, 1, 3>)
+                : (kk <= 1   ? packed_bwd_kernel<E, HD, 2, 1>
+                   : kk == 2 ? packed_bwd_kernel<E, HD, 2, 2>
+                             : packed_bwd_kernel<E, HD, 2, 3>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)nt * a.nkv), dim3(256), 0, st, a, gr, mix, rv);
+  LLMT_LAUNCH_CHECK();
   return hipSuccess;
 }
 
 }  // namespace
 
-size_t packed_bwd_workspace(const PackArgs& a) { return (size_t)a.Tq * a.nq * 8; }
+size_t packed_bwd_workspace(const PackArgs& a) {
+  return bwd_plan(a).keys ? (size_t)a.Tq * a.nq * 8 : 0;
+}
 
 hipError_t packed_bwd(const PackArgs& a, void* ws, hipStream_t st) {
   if (a.hd == 128) return a.bf16 ? launch<B16, 128>(a, ws, st) : launch<F16, 128>(a, ws, st);

@@ -100,7 +100,7 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
   const int c = lane & 15, g = lane >> 4;
   const int j = blockIdx.x % a.nkv;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ntiles, x)) return;
 
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
   const int j = blockIdx.x % a.nkv;
   const int part = blockIdx.y;
   Tile x;
-  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, x)) return;
+  if (!find<QB>(a, gr, blockIdx.x / a.nkv, ntiles, ntiles, x)) return;
   const short* kbase = (const short*)a.k.p + x.kstart * a.k.token + j * a.k.head;
   const short* vbase = (const short*)a.v.p + x.kstart * a.v.token + j * a.v.head;
   const int nkt_all = (x.kmax + FS_KEYS - 1) / FS_KEYS;

@@ -103,6 +103,18 @@ def test_many_sequences(dev, dtype, n):
     check(q, k, v, do, qo, ko)
 
 
+# few or many rows against few or many keys: the blocks of rows and of keys that the others do not
+# bring together
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nq,nkv,d,ql,kl", [
+    (16, 8, 128, [77] * 8, None), (32, 8, 64, [60] * 9, None), (32, 1, 128, [7] * 157, None),
+    (16, 8, 128, [300, 30, 250], [3000, 2350, 250]), (32, 8, 64, [300, 30, 250], [3000, 2900, 250]),
+    (32, 1, 128, [1100], None), (32, 1, 64, [600, 600], [500, 700]), (32, 8, 64, [1, 1, 1], [5000, 2000, 3001]),
+    (16, 8, 128, [600], [90])])
+def test_rows_and_keys_of_other_numbers(dev, dtype, nq, nkv, d, ql, kl):
+    check(*problem(dev, dtype, d, nq, nkv, ql, kl))
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("nq,nkv,d", [(33, 1, 64), (64, 1, 128), (128, 2, 64)])
 @pytest.mark.parametrize("ql,kl", [([1], [1]), ([2, 63, 17], None), ([300, 5], None), ([1, 3], [700, 2])])

@@ -20,6 +20,9 @@ DIMS = dict(dtype=2, nq=4, nkv=2, head_dim=64, n=3, Tq=100, Tk=200, scale=0.1, q
             k_offsets=A(2))
 
 
+MANY = dict(Tq=9000, Tk=9000)
+
+
 def heads(at, token, head):
     return llmt.Heads(at, token, head)
 
@@ -65,8 +68,8 @@ def test_packed_attention_refusals(bad, backward):
     (False, dict(o=heads(A(3) + 128 * 100, 256, 64))), (False, dict(o=heads(A(4) - 1600, 256, 64))),
     (False, dict(o=None)), (True, dict(dq=None)), (True, dict(dout=None)), (True, dict(dk=heads(A(12), 64, 64))),
     (True, dict(dk=heads(A(13), 128, 64))), (True, dict(dq=heads(A(10), 256, 64))),
-    (True, dict(dv=heads(A(5) + 256 * 199, 128, 64))), (True, dict(ws=None)), (True, dict(need=100)),
-    (True, dict(ws=A(9) + 8)), (False, dict(dims=dict(Tq=3, Tk=5000), ws=None)),
+    (True, dict(dv=heads(A(5) + 256 * 199, 128, 64))), (True, dict(dims=MANY, ws=None)), (True, dict(dims=MANY, need=100)),
+    (True, dict(dims=MANY, ws=A(9) + 8)), (False, dict(dims=dict(Tq=3, Tk=5000), ws=None)),
     # parts of one row that overlap by a head
     (True, dict(dq=heads(A(14), 512, 64), dk=heads(A(14) + 3 * 128, 512, 64))),
     (True, dict(dq=heads(A(14), 512, 64), dk=heads(A(14) + 4 * 128, 504, 64)))])
