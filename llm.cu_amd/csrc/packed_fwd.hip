@@ -6,6 +6,15 @@
 // (its own position where the two are equally long); below 0 it sees none, its
 // output is 0 and its lse -inf.  One pass over the keys with the running
 // maximum and sum; the scores never leave registers.
+//
+// Long sequences are bound by issue: a wave's tile of 64 keys and 32 rows takes
+// 64 matrix instructions of 17 cycles and some 250 vector ones, which hardly
+// overlap those of the other wave on the SIMD.  1 x 8192 tokens, 16 / 8 heads of
+// 128 in bf16: 270 us, 1015 TFLOP/s (a large library product reaches 1387); 1 x
+// 16384, 32 / 8 heads of 64 in fp16, twice the exponentials a product: 1250 us,
+// 880.  Many sequences end with the longest one's chain of tiles: 16 of 8192 tokens
+// together 58 us, 630.  Single tokens wait for their keys: 8 tokens of 9001 keys
+// 10.9 us and 3.9 for the join.
 #include <algorithm>
 #include <type_traits>
 
@@ -86,6 +95,9 @@ __device__ __forceinline__ void mask_tile(floatx4 (&st)[RW][MT], int key0, const
 // output is then a branch that few tiles take, and what it saves in range is
 // in the types (P stays below 2^GROW, times 2^PSH).
 constexpr float GROW = 7.f;
+
+// Slower: 16 rows a wave at 16 sequences of 8192 tokens (71 us, 62 with 32), 64
+// rows a wave, two groups of waves on halves of the keys, a third tile in flight.
 
 template <class E, int HD, int NW, int RW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2)))
@@ -490,6 +502,8 @@ struct FwdPlan {
 FwdPlan fwd_plan(const PackArgs& a) {
   const long long rows = (long long)a.Tq * (a.nq / a.nkv);
   const long long n = std::min(a.n, a.Tq);
+  // 32 rows a wave where that gives every CU two workgroups, 16 where those do
+  // (32 / 8 heads of 64, 4 x 1000 tokens 44 us and 43, 16 / 8 of 128, 16 x 512 49 and 60)
   if (rows / 128 * a.nkv >= 512) return {4, 2, 1};
   if (rows / 64 * a.nkv >= 256) return {4, 1, 1};
   // tiles of 16 rows, or of 32 where that many workgroups would not run at once
