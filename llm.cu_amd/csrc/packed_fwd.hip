@@ -300,7 +300,7 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
 }
 
 // Few rows: a workgroup takes 16 RW rows and one of nsplit parts of their keys,
-// in 32-key tiles that its four waves take in turn, each through LDS of its own
+// in 32-key tiles that its four or eight waves take in turn, each through LDS of its own
 // and without a barrier in the loop; the waves' results meet in LDS.  It waits
 // for loads, not for the matrix units, so probabilities enter the product in two
 // parts (pair_split), and nothing but the result is rounded to the type.  With
@@ -313,10 +313,10 @@ struct Parts {
   float2* ml;  // [nsplit][Tq nq]: base-2 maximum, sum
 };
 
-template <class E, int HD, int RW>
-__global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs a, Group gr,
-                                                                  int ntiles, Parts parts) {
-  constexpr int NW = 4, QB = RW * 16, KS = HD / 32, DT = HD / 16, FT = FS_KEYS * HD;
+template <class E, int HD, int RW, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void packed_fwd_split_kernel(const PackArgs a, Group gr,
+                                                                      int ntiles, Parts parts) {
+  constexpr int QB = RW * 16, KS = HD / 32, DT = HD / 16, FT = FS_KEYS * HD;
   // a wave's K and V tile; later its output, 16 rows x HD fp32 each
   __shared__ __attribute__((aligned(1024))) short kbuf[NW * FT];
   __shared__ __attribute__((aligned(1024))) short vbuf[NW * FT];
@@ -422,6 +422,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
     if (g == 0) ml[w][16 * r + c] = make_float2(m[r], lw);
   }
   __syncthreads();
+  if (w >= 4) return;
   constexpr int PC = HD / 64;  // 16-byte pieces a lane
 #pragma unroll
   for (int r = 0; r < RW; ++r) {
@@ -466,27 +467,52 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_split_kernel(const PackArgs
   }
 }
 
-// The parts of a row joined in their order: HD / 4 lanes a row.
-template <class E, int HD>
+// The parts of a row joined in their order: HD / 4 lanes a row; GR groups of so
+// many lanes take every GR-th part, and their sums meet in LDS.
+template <class E, int HD, int GR>
 __global__ __launch_bounds__(256) void packed_join_kernel(const PackArgs a, Parts parts) {
-  constexpr int LR = HD / 4;
+  constexpr int LR = HD / 4, RB = 256 / LR / GR;
+  __shared__ float ml[GR * RB][2];
+  __shared__ __attribute__((aligned(16))) float sums[GR > 1 ? GR * RB * HD : 1];
   const long long R = (long long)a.Tq * a.nq;
-  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
-  if (row >= R) return;
-  const int d = (threadIdx.x % LR) * 4;
-  float M = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < parts.nsplit; ++s) M = fmaxf(M, parts.ml[s * R + row].x);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
+  const int grp = threadIdx.x / LR, q = grp % GR, d = (threadIdx.x % LR) * 4;
+  const long long row = (long long)blockIdx.x * RB + grp / GR;
+  const bool on = row < R;
+  float M = -INFINITY, L = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  if (on) {
 #pragma unroll 8
-  for (int s = 0; s < parts.nsplit; ++s) {
-    const float2 p = parts.ml[s * R + row];
-    const float f = __builtin_amdgcn_exp2f(p.x - mu);
-    L = fmaf(p.y, f, L);
-    o += *reinterpret_cast<const floatx4*>(parts.o + (s * R + row) * HD + d) * f;
+    for (int s = q; s < parts.nsplit; s += GR) M = fmaxf(M, parts.ml[s * R + row].x);
+    const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll 8
+    for (int s = q; s < parts.nsplit; s += GR) {
+      const float2 p = parts.ml[s * R + row];
+      const float f = __builtin_amdgcn_exp2f(p.x - mu);
+      L = fmaf(p.y, f, L);
+      o += *reinterpret_cast<const floatx4*>(parts.o + (s * R + row) * HD + d) * f;
+    }
   }
+  if constexpr (GR > 1) {
+    if (d == 0) {
+      ml[grp][0] = M;
+      ml[grp][1] = L;
+    }
+    *reinterpret_cast<floatx4*>(sums + grp * HD + d) = o;
+    __syncthreads();
+    if (q > 0) return;
+#pragma unroll
+    for (int u = 0; u < GR; ++u) M = fmaxf(M, ml[grp + u][0]);
+    const float mu = M == -INFINITY ? 0.f : M;
+    L = 0.f;
+    o = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      const float f = __builtin_amdgcn_exp2f(ml[grp + u][0] - mu);
+      L = fmaf(ml[grp + u][1], f, L);
+      o += *reinterpret_cast<const floatx4*>(sums + (grp + u) * HD + d) * f;
+    }
+  }
+  if (!on) return;
   const long long t = row / a.nq, h = row - t * a.nq;
   const float inv = L > 0.f || L != L ? 1.0f / L : 0.f;
   *reinterpret_cast<short4v*>((short*)a.o.p + t * a.o.token + h * a.o.head + d) =
@@ -497,21 +523,27 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackArgs a, Part
 // The kernel and its split.
 struct FwdPlan {
   int nw, rw;  // nw 0: packed_fwd_split_kernel
-  int nsplit;
+  int nsplit, sw;  // its parts and waves
 };
 FwdPlan fwd_plan(const PackArgs& a) {
   const long long rows = (long long)a.Tq * (a.nq / a.nkv);
   const long long n = std::min(a.n, a.Tq);
   // 32 rows a wave where that gives every CU two workgroups, 16 where those do
   // (32 / 8 heads of 64, 4 x 1000 tokens 44 us and 43, 16 / 8 of 128, 16 x 512 49 and 60)
-  if (rows / 128 * a.nkv >= 512) return {4, 2, 1};
-  if (rows / 64 * a.nkv >= 256) return {4, 1, 1};
+  if (rows / 128 * a.nkv >= 512) return {4, 2, 1, 0};
+  if (rows / 64 * a.nkv >= 256) return {4, 1, 1, 0};
   // tiles of 16 rows, or of 32 where that many workgroups would not run at once
   const int rw = rows / 16 * a.nkv > 512 ? 2 : 1;
   const long long wgs = std::max<long long>(1, std::max(rows / (16 * rw), n) * a.nkv);
   const long long keys = a.Tk / std::max<long long>(1, n);
   const long long most = std::min<long long>(64, std::max<long long>(1, keys / 128));
-  return {0, rw, (int)std::min(most, std::max<long long>(1, 768 / wgs))};
+  // A CU for each workgroup and few keys: eight waves, no parts.  us in a graph, four
+  // waves in parts / eight: single tokens of 500 keys 8.6 / 7.0, of 1000 8.2 / 9.2, 32 of
+  // 1000 31 / 38; whole tiles, whose parts are larger: 4 heads, 2 x 500 15.1 / 7.7, one
+  // head, 1 x 4000 24.9 / 21.2, 16 / 8 heads, 128 tokens behind 900 18.2 / 9.7
+  const long long seen = keys - a.Tq / std::max<long long>(1, n) / 2;
+  if (rw == 1 && wgs <= 256 && seen <= (rows / 16 >= n ? 2048 : 768)) return {0, 1, 1, 8};
+  return {0, rw, (int)std::min(most, std::max<long long>(1, 768 / wgs)), 4};
 }
 
 template <class E, int HD>
@@ -537,14 +569,21 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   const int nt = row_tiles(a, 16 * p.rw);
   const dim3 grid((unsigned)nt * a.nkv, p.nsplit);
   if (p.rw == 2)
-    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 2>), grid, dim3(256), 0, st, a, gr, nt, parts);
+    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 2, 4>), grid, dim3(256), 0, st, a, gr, nt, parts);
+  else if (p.sw == 8)
+    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1, 8>), grid, dim3(512), 0, st, a, gr, nt, parts);
   else
-    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1>), grid, dim3(256), 0, st, a, gr, nt, parts);
+    hipLaunchKernelGGL((packed_fwd_split_kernel<E, HD, 1, 4>), grid, dim3(256), 0, st, a, gr, nt, parts);
   LLMT_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    constexpr int RB = 256 / (HD / 4);
-    hipLaunchKernelGGL((packed_join_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)), dim3(256),
-                       0, st, a, parts);
+    // few rows and many parts: a workgroup a row (one token of 8000 keys, 62 parts: 15.7
+    // us, 28.2 with a row's lanes walking all of them)
+    constexpr int G = 256 / (HD / 4);
+    if (p.nsplit >= 4)
+      hipLaunchKernelGGL((packed_join_kernel<E, HD, G>), dim3((unsigned)R), dim3(256), 0, st, a, parts);
+    else
+      hipLaunchKernelGGL((packed_join_kernel<E, HD, 1>), dim3((unsigned)((R + G - 1) / G)), dim3(256),
+                         0, st, a, parts);
     LLMT_LAUNCH_CHECK();
   }
   return hipSuccess;

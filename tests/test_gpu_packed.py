@@ -110,7 +110,9 @@ def test_many_sequences(dev, dtype, n):
     (16, 8, 128, [77] * 8, None), (32, 8, 64, [60] * 9, None), (32, 1, 128, [7] * 157, None),
     (16, 8, 128, [300, 30, 250], [3000, 2350, 250]), (32, 8, 64, [300, 30, 250], [3000, 2900, 250]),
     (32, 1, 128, [1100], None), (32, 1, 64, [600, 600], [500, 700]), (32, 8, 64, [1, 1, 1], [5000, 2000, 3001]),
-    (16, 8, 128, [600], [90])])
+    (16, 8, 128, [600], [90]), (4, 4, 128, [500, 500], None), (1, 1, 64, [1900], None), (1, 1, 128, [4000], None),
+    (16, 8, 128, [100, 28], [900, 1020]), (8, 1, 64, [64], [4000]), (2, 1, 128, [33, 0, 7], [2500, 10, 2]),
+    (1, 1, 64, [4090], None)])
 def test_rows_and_keys_of_other_numbers(dev, dtype, nq, nkv, d, ql, kl):
     check(*problem(dev, dtype, d, nq, nkv, ql, kl))
 
@@ -152,7 +154,8 @@ def test_a_sequence_of_nan_stays_alone(dev, dtype, ql, kl):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("nq,nkv,d", [(16, 8, 128), (6, 2, 64)])
-@pytest.mark.parametrize("kl", [[5000], [1, 3000, 64, 129], [2000] * 7 + [0]])
+@pytest.mark.parametrize("kl", [[5000], [1, 3000, 64, 129], [2000] * 7 + [0], [700], [300, 0, 33, 1000], [9000],
+                                [16000, 4, 300]])
 def test_single_tokens_of_long_keys(dev, dtype, nq, nkv, d, kl):
     """One new token a sequence: the keys are split over workgroups and joined."""
     check(*problem(dev, dtype, d, nq, nkv, [1] * len(kl), kl))
