@@ -1,20 +1,20 @@
 // embed.hip — embedding lookup with scaling, out[i] = scale w[tok[i]], and its
 // gradient, dw[v] (+)= scale sum over tok[i] = v of dout[i].
 //
-// The gradient adds every token's rows in the order of their positions,
-// whatever the launch: positions are sorted by token (stable), the sorted list
+// The gradient adds every token's rows in an order that the positions alone
+// decide: positions are sorted by token (stable), the sorted list
 // is cut into chunks, a group of lanes sums the runs of equal tokens of its
 // chunk in fp32, and a run that spans chunks is joined from their partial sums
-// in order.  No atomics, and a frequent token's rows are shared by as many
+// in an order of their number alone.  No atomics, and a frequent token's rows are shared by as many
 // groups as it has chunks.  Few positions need no sort: a workgroup for each
 // looks whether it is its token's first and gathers the others.  Where the
 // table is written whole, its zeros ride in the sorting launches, which leave
 // the memory idle.
 //
-// Memory-bound where large: the lookup of 16384 rows of 1037 fp32 in 23 us, 4.0 TB/s
+// Memory-bound where large: the lookup of 16384 rows of 1037 fp32 in 17.9 us, 5.1 TB/s
 // (the odd width takes single elements); the gradient of 32768 rows of 1024 bf16
-// into a table of 50257 fp32 rows in 90 us, of which the sorting launches with the
-// 206 MB of zeros take 49, the sums 32 (its 67 MB gathered, 41 written) and the join
+// into a table of 50257 fp32 rows in 77 us, of which the sorting launches with the
+// 206 MB of zeros take 46, the sums 24 (its 67 MB gathered, 41 written) and the join
 // 8; a copy would take 56 for all of it.  Few tokens cost a launch: 128 rows 2.6 us,
 // the gradient of 300 added to the table 5.0.
 #include <algorithm>
@@ -101,12 +101,23 @@ __global__ __launch_bounds__(NTH) void embed_kernel(const EmbedArgs a, int lpr) 
   const bool ok = (unsigned)t < (unsigned)a.V;
   const TW* w = (const TW*)a.w + (ok ? t : 0) * a.ldw;
   TX* x = (TX*)a.x + i * a.ldx;
-  for (int c = (threadIdx.x % lpr) * N; c < a.H; c += lpr * N) {
-    float v[N];
-    if (ok) load_n<TW, N>(w + c, v);
+  // U pieces in flight
+  constexpr int U = N == 1 ? 8 : 2;
+  for (int c0 = (threadIdx.x % lpr) * N; c0 < a.H; c0 += U * lpr * N) {
+    float v[U][N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = ok ? v[e] * a.scale : 0.f;
-    store_n<TX, N>(x + c, v);
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * lpr * N;
+      if (ok && c < a.H) load_n<TW, N>(w + c, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * lpr * N;
+      if (c >= a.H) break;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[u][e] = ok ? v[u][e] * a.scale : 0.f;
+      store_n<TX, N>(x + c, v[u]);
+    }
   }
 }
 
@@ -142,12 +153,12 @@ __device__ __forceinline__ int key_of(const int* tok, int i, int V) {
 }
 
 // Up to kRankMost positions: a position's place is the number of positions in
-// front of it, counted by LPI lanes over all of them (T^2 comparisons: at 4096
-// positions fewer than the launches of a radix sort would wait for).
-constexpr int kRankMost = 16384;
-template <int LPI>
+// front of it, counted by 16 lanes over all of them (T^2 comparisons: at 3500
+// positions 9 us less than the launches of a radix sort, at 5000 3 more, at 16000 120).
+constexpr int kRankMost = 4096;
 __global__ __launch_bounds__(NTH) void embed_rank_kernel(const int* tok, int T, int V, int* skey,
                                                          int* spos, const Zeros z) {
+  constexpr int LPI = 16;
   if (blockIdx.x >= z.first) return zero_rows(z);
   const int sub = threadIdx.x % LPI;
   const int i = blockIdx.x * (NTH / LPI) + threadIdx.x / LPI;
@@ -371,41 +382,52 @@ __global__ __launch_bounds__(NTH) void embed_sum_kernel(const SumArgs a, int lpr
     put_row<TW, N>(a, run, c, s);
 }
 
-// Runs that begin in chunk k and go on behind it.
+// Runs that begin in chunk k and go on behind it: a workgroup for each chunk and
+// 32 N columns, whose eight groups of lanes take every eighth partial sum.
+constexpr int JG = NTH / 32;
 template <class TW, int N>
-__global__ __launch_bounds__(NTH) void embed_join_kernel(const SumArgs a, int lpr) {
-  const int k = blockIdx.x * (NTH / lpr) + threadIdx.x / lpr;
-  const int c = (blockIdx.y * lpr + threadIdx.x % lpr) * N;
-  if (k >= a.nchunks - 1) return;
+__global__ __launch_bounds__(NTH) void embed_join_kernel(const SumArgs a) {
+  __shared__ float sums[JG][32 * N];
+  const int k = blockIdx.x, lane = threadIdx.x % 32, grp = threadIdx.x / 32;
+  const int c = (blockIdx.y * 32 + lane) * N;
   const int i0 = k * a.C, end = i0 + a.C;
   const int first = a.skey[i0], run = a.skey[end - 1], next = a.skey[end];
   const int before = i0 > 0 ? a.skey[i0 - 1] : -1;
   if (run >= a.V || next != run || (first == run && before == run)) return;  // or begins earlier
-  // the chunks that it fills from their start, 32 looked at a time
-  int m = k + 1;
+  int m = k + 1;  // behind the chunks that it fills from their start
   for (;;) {
-    const int at = m + (int)(threadIdx.x % 32);
-    const bool in = at < a.nchunks && a.skey[(long long)at * a.C] == run;
-    const unsigned long long b = __ballot(in);
-    const int cnt = __popc((unsigned)(threadIdx.x & 32 ? b >> 32 : b));
-    m += cnt;
-    if (cnt < 32) break;
+    const int at = m + (int)threadIdx.x;
+    const int n = __syncthreads_count(at < a.nchunks && a.skey[(long long)at * a.C] == run);
+    m += n;
+    if (n < NTH) break;
   }
-  if (c >= a.H) return;
+  const int total = m - k;
   float s[N];
-  load_n<float, N>(a.part + (long long)(2 * k + 1) * a.H + c, s);
-  for (int i = k + 1; i < m; i += 8) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) s[e] = 0.f;
+  for (int i = grp; i < total && c < a.H; i += 8 * JG) {
     float x[8][N];
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i + u < m) load_n<float, N>(a.part + (long long)(2 * (i + u)) * a.H + c, x[u]);
+    for (int u = 0; u < 8; ++u) {
+      const int p = i + u * JG;  // the first partial sum is of a run that goes on
+      if (p < total)
+        load_n<float, N>(a.part + (long long)(2 * (k + p) + (p ? 0 : 1)) * a.H + c, x[u]);
+    }
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (i + u < m) {
+      if (i + u * JG < total) {
 #pragma unroll
         for (int e = 0; e < N; ++e) s[e] += x[u][e];
       }
   }
+#pragma unroll
+  for (int e = 0; e < N; ++e) sums[grp][e * 32 + lane] = s[e];
+  __syncthreads();
+  if (grp || c >= a.H) return;
+#pragma unroll
+  for (int u = 1; u < JG; ++u)
+#pragma unroll
+    for (int e = 0; e < N; ++e) s[e] += sums[u][e * 32 + lane];
   put_row<TW, N>(a, run, c, s);
 }
 
@@ -487,7 +509,9 @@ bool pieces(const void* p, long long ld, int H, size_t es, int N) {
 
 size_t size_of(int type) { return type == kF32 ? 4 : 2; }
 
-int chunk_of(int T) { return T >= 16384 ? 32 : T >= 4096 ? 16 : 8; }
+// Entries of a chunk: more chunks feed more CUs and leave more partial sums (us of a
+// gradient of 1024 columns with 16 / 32: 32768 positions 87 / 94, 65536 137 / 127).
+int chunk_of(int T) { return T >= 65536 ? 32 : T >= 4096 ? 16 : 8; }
 
 // The workspace: sorted keys and positions (twice for the radix passes), the
 // passes' counts, the partial sums.
@@ -554,14 +578,11 @@ static hipError_t sort_tokens(const EmbedArgs& a, const Space& sp, void* ws, Zer
   if (a.T <= kRankMost) {
     *key = k0;
     *pos = k0 + n;
-    const int per = a.T <= 8192 ? NTH / 16 : NTH / 8;
+    constexpr int per = NTH / 16;
     z.first = (unsigned)((a.T + per - 1) / per);
     z.v1 = a.add ? 0 : V;
     const dim3 grid(z.first + (a.add ? 0 : 2048));
-    if (a.T <= 8192)
-      hipLaunchKernelGGL(embed_rank_kernel<16>, grid, dim3(NTH), 0, st, a.tok, a.T, V, *key, *pos, z);
-    else
-      hipLaunchKernelGGL(embed_rank_kernel<8>, grid, dim3(NTH), 0, st, a.tok, a.T, V, *key, *pos, z);
+    hipLaunchKernelGGL(embed_rank_kernel, grid, dim3(NTH), 0, st, a.tok, a.T, V, *key, *pos, z);
     LLMT_LAUNCH_CHECK();
     return hipSuccess;
   }
@@ -581,9 +602,10 @@ static hipError_t sort_tokens(const EmbedArgs& a, const Space& sp, void* ws, Zer
     s.shift = p * RB;
     s.key_out = buf[p & 1][0];
     s.pos_out = buf[p & 1][1];
-    for (int half = 0; half < 2; ++half) {  // a launch's share of the rows
-      z.v0 = (int)((long long)V * (2 * p + half) / (2 * passes));
-      z.v1 = (int)((long long)V * (2 * p + half + 1) / (2 * passes));
+    for (int half = 0; half < 2; ++half) {
+      // a launch's share of the rows: a quarter beside a count, the rest beside a placement
+      z.v0 = (int)((long long)V * (4 * p + half) / (4 * passes));
+      z.v1 = (int)((long long)V * (4 * p + (half ? 4 : 1)) / (4 * passes));
       if (half == 0)
         hipLaunchKernelGGL(embed_count_kernel, grid, dim3(NTH), 0, st, s, z);
       else
@@ -634,14 +656,18 @@ hipError_t embed_bwd(const EmbedArgs& a, void* ws, hipStream_t st) {
       const int lpr = std::max(32, lanes_for(a.H, vec ? N : 1)), gpb = NTH / lpr;
       const int cols = lpr * (vec ? N : 1);
       const dim3 grid((unsigned)((s.nchunks + gpb - 1) / gpb), (unsigned)((a.H + cols - 1) / cols));
+      const int jcols = 32 * (vec ? N : 1);
+      const dim3 join((unsigned)(s.nchunks - 1), (unsigned)((a.H + jcols - 1) / jcols));
       if (vec) {
         hipLaunchKernelGGL((embed_sum_kernel<TX, TW, N>), grid, dim3(NTH), 0, st, s, lpr);
         LLMT_LAUNCH_CHECK();
-        hipLaunchKernelGGL((embed_join_kernel<TW, N>), grid, dim3(NTH), 0, st, s, lpr);
+        if (s.nchunks > 1)
+          hipLaunchKernelGGL((embed_join_kernel<TW, N>), join, dim3(NTH), 0, st, s);
       } else {
         hipLaunchKernelGGL((embed_sum_kernel<TX, TW, 1>), grid, dim3(NTH), 0, st, s, lpr);
         LLMT_LAUNCH_CHECK();
-        hipLaunchKernelGGL((embed_join_kernel<TW, 1>), grid, dim3(NTH), 0, st, s, lpr);
+        if (s.nchunks > 1)
+          hipLaunchKernelGGL((embed_join_kernel<TW, 1>), join, dim3(NTH), 0, st, s);
       }
       LLMT_LAUNCH_CHECK();
       return hipSuccess;

@@ -1,5 +1,5 @@
 """GPU: llmt.embedding and its gradient against float64: types, odd widths, strides, padding, tokens
-that repeat, every sort (up to 16384 positions by rank, more by radix passes).
+that repeat, every sort (few positions by rank, more by radix passes).
 
 A gradient row is a sum of c products in fp32 in the positions' order: off by at most c 2^-24 of the
 sum of magnitudes, then scaled, added and rounded (2^-23 of the parts' magnitudes) and rounded to the
@@ -31,6 +31,26 @@ def test_lookup(dev, wt, ot, V, W):
         ok = (t >= 0) & (t < V)
         want = torch.where(ok[:, None], w[t.long().clamp(0, V - 1)].float() * scale, 0.0).to(ot)
         assert x.dtype == ot and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("T,V,W", [(4096, 900, 24), (4097, 900, 24), (9000, 70000, 33), (65535, 300, 8),
+                                   (65536, 300, 8), (65537, 600, 5)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_gradient_where_sort_and_chunks_change(dev, accumulate, T, V, W):
+    g = torch.Generator().manual_seed(T)
+    dout = torch.randn(T, W, generator=g).to(B).to(dev)
+    check_grad(dev, tokens(T, V).to(dev), dout, torch.randn(V, W, generator=g).to(dev), 0.5, accumulate)
+
+
+@pytest.mark.parametrize("T", [1025, 4096, 20000])
+@pytest.mark.parametrize("W", [4, 264, 1000])
+def test_one_token_at_all_positions(dev, T, W):
+    """A run over every chunk, more of them than a workgroup has threads."""
+    g = torch.Generator().manual_seed(T)
+    dout = torch.randn(T, W, generator=g).to(dev)
+    for at, V in ((0, 1), (2, 5)):
+        t = torch.full((T,), at, dtype=torch.int32, device=dev)
+        check_grad(dev, t, dout, torch.ones(V, W, device=dev), 2.0, False)
 
 
 def test_lookup_of_strided_rows_and_shapes(dev):
