@@ -14,7 +14,7 @@
 // 16384, 32 / 8 heads of 64 in fp16, twice the exponentials a product: 1250 us,
 // 880.  Many sequences end with the longest one's chain of tiles: 16 of 8192 tokens
 // together 58 us, 630.  Single tokens wait for their keys: 8 tokens of 9001 keys
-// 10.9 us and 3.9 for the join.
+// 13.5 us in a graph with the join, 32 of 32000 31, 4.2 TB/s.
 #include <algorithm>
 #include <type_traits>
 
