@@ -91,10 +91,14 @@ __device__ __forceinline__ void mask_tile(floatx4 (&st)[RW][MT], int key0, const
 // then its output beside the maxima of tile i + 1.
 //
 // The maximum that a row's exponentials refer to follows the running one only
-// when some row of the wave has left it by more than 2^GROW: rescaling the
+// when some row of the wave has left it by more than 2^kGrow: rescaling the
 // output is then a branch that few tiles take, and what it saves in range is
-// in the types (P stays below 2^GROW, times 2^PSH).
-constexpr float GROW = 7.f;
+// in the types.  Base-2 scores of 2^24 and more are even numbers in fp32, where
+// m + 7 is a tie that rounds up for every other m, so that a maximum of m + 8 would
+// not be followed; with the score's own rounding P times 2^PSH would reach 2^17,
+// beyond fp16.  m + 6 is exact up to 2^25, and fp16's P 2^PSH stays at or below 2^15.
+template <class E>
+constexpr float kGrow = E::PSH ? 6.f : 7.f;
 
 // Slower: 16 rows a wave at 16 sequences of 8192 tokens (71 us, 62 with 32), 64
 // rows a wave, two groups of waves on halves of the keys, a third tile in flight.
@@ -176,7 +180,7 @@ void packed_fwd_kernel(const PackArgs a, Group gr, int ntiles) {
   auto follow = [&](const float (&bm)[RW]) LLMT_INLINE {
     bool grow = false;
 #pragma unroll
-    for (int r = 0; r < RW; ++r) grow = grow || bm[r] > m[r] + GROW;
+    for (int r = 0; r < RW; ++r) grow = grow || bm[r] > m[r] + kGrow<E>;
     if (__ballot(grow)) {
 #pragma unroll
       for (int r = 0; r < RW; ++r) {

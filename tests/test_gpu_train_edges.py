@@ -1,0 +1,61 @@
+"""GPU: borders of the operators for training all weights on packed sequences: scores next to the
+documented bound in the attention's large tiles."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import llmt
+import packed_ref as ref
+from test_gpu_packed import offsets
+
+pytestmark = pytest.mark.gpu
+F, H, B = torch.float32, torch.float16, torch.bfloat16
+LN2 = float(np.float32(math.log(2)))
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("nq,nkv,d", [(16, 8, 128), (16, 8, 64), (32, 8, 64)])
+@pytest.mark.parametrize("T", [1100, 4200])
+def test_maxima_of_millions_that_grow_by_small_steps(dev, dtype, nq, nkv, d, T):
+    """Scores of 1.6e7 whose tiles' maxima rise by 2 to 14 steps of a base-2 score each, in the
+    workgroups of 64 and of 128 rows.  With scale ln 2 the base-2 scores are q k itself (ln 2 log2 e
+    is 1 in fp32): 4096 * 5632 + 2 r + s_j, even numbers below 2^25, which fp32 holds exactly in any
+    order of the sum.  So a score is exact, a weight 2^(s_j - max) too, and o is off by the rounding
+    of P (u), those of the sums and the exponential (2^-16) and its own (u).  lse: five roundings and
+    constants of 2^-24."""
+    assert np.float32(LN2) * np.float32(1.4426950408889634) == 1
+    g = torch.Generator().manual_seed(T + nq + d)
+    tiles = -(-T // 64)
+    # a tile's maximum: above the last one's by 2 .. 14, at most 500 in all: exact in both types
+    rise = 2 * torch.randint(1, 8, (tiles,), generator=g)
+    rise[1], rise[2] = 8, 8                       # the first two from an m that is 0 or 2 mod 4
+    top = rise.cumsum(0).clamp(max=500)
+    s = top.repeat_interleave(64)[:T] - 2 * torch.randint(0, 8, (T,), generator=g)
+    first = torch.arange(0, T, 64)
+    s[first + torch.randint(0, 64, (tiles,), generator=g).clamp(max=T - 1 - first)] = top
+    s = s - top[0]
+    q, k = torch.zeros(T, nq, d), torch.zeros(T, nkv, d)
+    r = torch.arange(T) // 64 % 2                 # by the token's block: a wave's rows alike
+    q[..., 0], q[..., 1], q[..., 2], k[..., 0], k[..., 2] = 4096, 1, r[:, None], 5632, 2
+    k[..., 1] = s[:, None]
+    v = torch.randn(T, nkv, d, generator=g).to(dtype).to(dev)
+    q, k = (x.to(dtype).to(dev) for x in (q, k))
+    assert (k[:, 0, 1].cpu() == s).all()
+    o, lse = llmt.packed_attention(q, k, v, offsets([T]).to(dev), scale=LN2)
+    w = s.double().to(dev)
+    see = torch.ones(T, T, dtype=torch.bool, device=dev).tril()
+    w = torch.where(see, w[None], -math.inf)
+    m = w.amax(1, keepdim=True)
+    p = torch.exp2(w - m)
+    total = p.sum(1, keepdim=True)
+    p = p / total
+    base = 4096.0 * 5632 + 2 * r.double().to(dev)
+    want = (base + (m + total.log2())[:, 0]) * math.log(2)
+    assert ((lse.double() - want[:, None]).abs() <= 5 * 2 ** -24 * want[:, None]).all()
+    u = ref.unit(dtype)
+    for h in range(nq):
+        x = v[:, h // (nq // nkv)].double()
+        y, mag = p @ x, p @ x.abs()
+        assert ((o[:, h].double() - y).abs() <= (u + 2 ** -16) * mag + u * y.abs() + 2 ** -25).all(), h
