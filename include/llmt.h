@@ -521,7 +521,10 @@ int llmt_muon(llmt_ctx* ctx, const llmt_muon_params* params);
  * a part of a fused projection's rows, [heads, T, d].  p is 16-byte aligned, the
  * strides are multiples of 8, token in [head_dim, 2^23], head in [0, 2^40], for
  * q, o, dout and dq (group - 1) head at most 2^28.  An output's elements must not
- * coincide with one another or with another argument's. */
+ * coincide with one another or with another argument's.  Parts of one buffer may lie
+ * between one another ([T, heads, 2, d]) where they have the same strides; where
+ * strides differ, they are taken as apart only if one lies behind the other, or
+ * every token's heads do. */
 typedef struct {
     void* p;
     long long token, head;

@@ -76,20 +76,41 @@ static int check_view(const char* fn, const llmt_packed_dims* d, const View& x) 
   return LLMT_OK;
 }
 
-// Whether two views have no element in common: apart from one another, or
-// columns of their own in rows of the same stride.
+// Pieces of `piece` bytes, n of them `stride` apart.
+struct Comb {
+  long long n, stride;
+  long long width(long long piece) const { return (n - 1) * stride + piece; }
+};
+// Whether combs that begin at 0 and at `at` have no byte in common: one behind the
+// other, or of one stride with pieces of the one between those of the other.
+static bool combs_apart(const Comb& a, const Comb& b, long long at, long long piece) {
+  if (at >= a.width(piece) || at + b.width(piece) <= 0) return true;
+  const long long s = a.n == 1 ? b.stride : a.stride;
+  if ((b.n > 1 && b.stride != s) || (a.n == 1 && b.n == 1) || s <= 0) return false;
+  const long long d = ((at % s) + s) % s;
+  return d >= piece && d + piece <= s;
+}
+
+// Whether two views have no element in common: apart from one another; or of the
+// same stride from token to token (from head to head), with each token's heads
+// (each head's tokens) inside one such stride and apart from the other view's
+// there.  Other layouts may be apart as well: they are refused.
 static bool views_apart(const View& a, const View& b, int hd) {
   if (a.T == 0 || b.T == 0) return true;
-  auto extent = [&](const View& x) {
-    return ((x.T - 1) * x.h->token + (x.heads - 1) * x.h->head + hd) * 2;
+  const long long piece = hd * 2;
+  const Comb ta = {a.T, a.h->token * 2}, ha = {a.heads, a.h->head * 2};
+  const Comb tb = {b.T, b.h->token * 2}, hb = {b.heads, b.h->head * 2};
+  const long long at = (intptr_t)b.h->p - (intptr_t)a.h->p;
+  if (at >= ta.width(ha.width(piece)) || at + tb.width(hb.width(piece)) <= 0) return true;
+  auto nested = [&](const Comb& oa, const Comb& ia, const Comb& ob, const Comb& ib) {
+    if (oa.n == 1 && ob.n == 1) return combs_apart(ia, ib, at, piece);
+    const long long s = oa.n == 1 ? ob.stride : oa.stride;
+    if ((ob.n > 1 && ob.stride != s) || ia.width(piece) > s || ib.width(piece) > s) return false;
+    // the row of b that begins in a's row at 0 ends in a's next one at the latest
+    const long long d = ((at % s) + s) % s;
+    return combs_apart(ia, ib, d, piece) && combs_apart(ia, ib, d - s, piece);
   };
-  const intptr_t pa = (intptr_t)a.h->p, pb = (intptr_t)b.h->p;
-  if (pa + extent(a) <= pb || pb + extent(b) <= pa) return true;
-  const long long t = a.h->token * 2;
-  const long long wa = ((a.heads - 1) * a.h->head + hd) * 2, wb = ((b.heads - 1) * b.h->head + hd) * 2;
-  if (b.h->token * 2 != t || wa > t || wb > t) return false;
-  const long long delta = (((pb - pa) % t) + t) % t;
-  return delta >= wa && delta + wb <= t;
+  return nested(ta, ha, tb, hb) || nested(ha, ta, hb, tb);
 }
 
 static int check_packed(const char* fn, const llmt_packed_dims* d, const View* v, int nv,

@@ -1,5 +1,5 @@
 """GPU: borders of the operators for training all weights on packed sequences: scores next to the
-documented bound in the attention's large tiles."""
+documented bound in the attention's large tiles, heads of one buffer that lie between one another."""
 import math
 
 import numpy as np
@@ -8,7 +8,7 @@ import torch
 
 import llmt
 import packed_ref as ref
-from test_gpu_packed import offsets
+from test_gpu_packed import offsets, problem
 
 pytestmark = pytest.mark.gpu
 F, H, B = torch.float32, torch.float16, torch.bfloat16
@@ -59,3 +59,31 @@ def test_maxima_of_millions_that_grow_by_small_steps(dev, dtype, nq, nkv, d, T):
         x = v[:, h // (nq // nkv)].double()
         y, mag = p @ x, p @ x.abs()
         assert ((o[:, h].double() - y).abs() <= (u + 2 ** -16) * mag + u * y.abs() + 2 ** -25).all(), h
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("ql", [[1], [9, 50], [700, 900]])
+@pytest.mark.parametrize("nq,nkv,d,parts,turned", [(6, 2, 64, 2, False), (16, 8, 128, 2, False), (8, 4, 128, 2, True),
+                                                   (4, 4, 64, 3, False), (4, 4, 128, 3, True)])
+def test_heads_between_one_another(dev, dtype, ql, nq, nkv, d, parts, turned):
+    """Projections whose rows are [heads, 2, d] (keys and values) or [heads, 3, d] (queries too),
+    tokens or heads outermost: the bits of separate tensors, and what lies beside stays."""
+    q, k, v, do, qo, _ = problem(dev, dtype, d, nq, nkv, ql)
+    T, heads = q.shape[0], (q, k, v)[3 - parts:]
+
+    def buffer():
+        x = torch.full((nkv, T, parts, d) if turned else (T, nkv, parts, d + 8), 7.0, dtype=dtype, device=dev)
+        return x, [(x.transpose(0, 1) if turned else x)[:, :, i, :d] for i in range(parts)]
+    _, inside = buffer()
+    for x, y in zip(inside, heads):
+        x.copy_(y)
+    inside = [q, k, v][:3 - parts] + inside
+    o, lse = llmt.packed_attention(q, k, v, qo)
+    o2, lse2 = llmt.packed_attention(*inside, qo)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    want = llmt.packed_attention_bwd(q, k, v, o, lse, do, qo)
+    buf, out = buffer()
+    out = [torch.empty_like(q)][:3 - parts] + out
+    got = llmt.packed_attention_bwd(*inside, o, lse, do, qo, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert turned or (buf[..., d:] == 7).all()
