@@ -70,27 +70,32 @@ __device__ __forceinline__ float row_lanes_sum(float x) {
   return LR == 16 ? x + dpp16<0x140>(x) : x;
 }
 
-// The rows' lse2 and delta: HD / 8 lanes a row.
+// The rows' lse2 and delta: HD / 8 lanes a row, in at most kDeltaWgs workgroups (a
+// launch has less than 2^32 threads; the rows of one may be up to 2^29).
+constexpr unsigned kDeltaWgs = 1 << 23;
 template <class E, int HD>
 __global__ __launch_bounds__(256) void packed_delta_kernel(const PackArgs a, int G, RowVecs rv) {
   typedef typename E::T T8 __attribute__((ext_vector_type(8)));
   constexpr int LR = HD / 8;
-  const long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR;
-  if (row >= (long long)a.Tq * a.nq) return;
-  const long long t = row / a.nq;
-  const int h = (int)(row - t * a.nq), d = threadIdx.x % LR * 8;
-  const T8 x = *reinterpret_cast<const T8*>((const short*)a.dout.p + t * a.dout.token +
-                                            h * a.dout.head + d);
-  const T8 y = *reinterpret_cast<const T8*>((const short*)a.o.p + t * a.o.token + h * a.o.head + d);
-  float s = 0.f;
+  const long long rows = (long long)a.Tq * a.nq;
+  for (long long row = (long long)blockIdx.x * (256 / LR) + threadIdx.x / LR; row < rows;
+       row += (long long)gridDim.x * (256 / LR)) {
+    const long long t = row / a.nq;
+    const int h = (int)(row - t * a.nq), d = threadIdx.x % LR * 8;
+    const T8 x = *reinterpret_cast<const T8*>((const short*)a.dout.p + t * a.dout.token +
+                                              h * a.dout.head + d);
+    const T8 y = *reinterpret_cast<const T8*>((const short*)a.o.p + t * a.o.token + h * a.o.head + d);
+    float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
-  s = row_lanes_sum<LR>(s);
-  if (d) return;
-  const int j = h / G;
-  const long long at = vec_at(a, G, j, t) + h - j * G;
-  rv.lse2[at] = lse2_of(a.lse[row]);
-  rv.delta[at] = s;
+    for (int e = 0; e < 8; ++e) s = fmaf((float)x[e], (float)y[e], s);
+    s = row_lanes_sum<LR>(s);
+    if (d == 0) {
+      const int j = h / G;
+      const long long at = vec_at(a, G, j, t) + h - j * G;
+      rv.lse2[at] = lse2_of(a.lse[row]);
+      rv.delta[at] = s;
+    }
+  }
 }
 
 // The workgroups of one launch are of keys (dK, dV) and of rows (dQ): a quarter of
@@ -809,8 +814,8 @@ hipError_t launch(const PackArgs& a, void* ws, hipStream_t st) {
   const int kr = p.rows, kk = p.keys;
   if (a.Tq && kk) {
     constexpr int RB = 256 / (HD / 8);
-    hipLaunchKernelGGL((packed_delta_kernel<E, HD>), dim3((unsigned)((R + RB - 1) / RB)), dim3(256),
-                       0, st, a, gr.G, rv);
+    const unsigned wgs = (unsigned)std::min<long long>((R + RB - 1) / RB, kDeltaWgs);
+    hipLaunchKernelGGL((packed_delta_kernel<E, HD>), dim3(wgs), dim3(256), 0, st, a, gr.G, rv);
     LLMT_LAUNCH_CHECK();
   }
   Mix mix{};

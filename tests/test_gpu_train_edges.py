@@ -1,5 +1,5 @@
 """GPU: borders of the operators for training all weights on packed sequences: scores next to the
-documented bound in the attention's large tiles, heads of one buffer that lie between one another."""
+documented bound in the attention's large tiles, heads of one buffer that lie between one another, rows beyond 2^28."""
 import math
 
 import numpy as np
@@ -87,3 +87,35 @@ def test_heads_between_one_another(dev, dtype, ql, nq, nkv, d, parts, turned):
     got = llmt.packed_attention_bwd(*inside, o, lse, do, qo, out=out)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert turned or (buf[..., d:] == 7).all()
+
+
+def test_gradients_of_more_than_2_28_rows(dev):
+    """16 heads of 2^24 tokens and some: 100 tokens with keys behind all the others, which have
+    none.  (One row of q, dout and o serves a token's heads; dq alone is 69 GB.)"""
+    nq, d, few, T = 16, 128, 100, (1 << 24) + 4096
+    if torch.cuda.mem_get_info()[0] < 90e9:
+        torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 90e9:
+        pytest.skip("90 GB of device memory are needed")
+    g = torch.Generator().manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(B).to(dev)
+    row = torch.zeros(T, d, dtype=B, device=dev)
+    row[-few:] = rnd(few, d)
+    x = row[:, None].expand(T, nq, d)
+    k, v = rnd(few, nq, d), rnd(few, nq, d)
+    qo = torch.tensor([0, T - few, T], dtype=torch.int32, device=dev)
+    ko = torch.tensor([0, 0, few], dtype=torch.int32, device=dev)
+    tail = x[-few:]
+    _, end = llmt.packed_attention(tail, k, v, ko[1:])
+    lse = torch.full((T, nq), -math.inf, device=dev)
+    lse[-few:] = end
+    dq = torch.empty(T, nq, d, dtype=B, device=dev).fill_(math.nan)
+    dk, dv = torch.empty_like(k), torch.empty_like(v)
+    llmt.packed_attention_bwd(x, k, v, x, lse, x, qo, ko, out=(dq, dk, dv))
+    want, bounds = ref.backward(tail, k, v, tail, end, tail, ko[1:], ko[1:], d ** -0.5)
+    for name, a, b, bound in zip(("dq", "dk", "dv"), (dq[-few:], dk, dv), want, bounds):
+        ref.within(name, a, b, bound)
+    for part in dq[:-few].split(1 << 20):
+        assert not (part != 0).any()
+    del dq, part
+    torch.cuda.empty_cache()
