@@ -368,7 +368,9 @@ int llmt_adamw_update(const llmt_adam_tensor* t, int count, int state_bits, cons
   k.c1 = 1.0f - hp->beta1;
   k.c2 = 1.0f - hp->beta2;
   k.ib1 = (float)(1.0 / (1.0 - pow((double)hp->beta1, step)));
-  k.ib2 = (float)(1.0 / (1.0 - pow((double)hp->beta2, step)));
+  const float ib2 = (float)(1.0 / (1.0 - pow((double)hp->beta2, step)));
+  k.ib2_up = ib2 * 0x1p64f;
+  k.ib2_down = ib2 * 0x1p-64f;
   k.decay = (float)(1.0 - (double)hp->lr * hp->wd);
   k.lr = hp->lr;
   k.eps = hp->eps;

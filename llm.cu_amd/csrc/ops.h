@@ -420,7 +420,8 @@ struct AdamTensor {
   int gtype, ctype;
 };
 struct AdamStep {
-  float b1, b2, c1, c2, ib1, ib2, decay, lr, eps;
+  float b1, b2, c1, c2, ib1, decay, lr, eps;
+  float ib2_up, ib2_down;  // 1 / (1 - b2^step), times 2^64 and 2^-64
   const float* gscale; // NULL, or one factor of the gradients on the device
   unsigned long long seed;  // mixed; of the tensors' draws
   int step;

@@ -1,5 +1,6 @@
 """GPU: borders of the operators for training all weights on packed sequences: scores next to the
-documented bound in the attention's large tiles, heads of one buffer that lie between one another, rows beyond 2^28."""
+documented bound in the attention's large tiles, heads of one buffer that lie between one another, rows beyond 2^28;
+AdamW's largest moments."""
 import math
 
 import numpy as np
@@ -8,6 +9,7 @@ import torch
 
 import llmt
 import packed_ref as ref
+from test_gpu_adamw_list import HP, check_p, numpy_step
 from test_gpu_packed import offsets, problem
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +121,32 @@ def test_gradients_of_more_than_2_28_rows(dev):
         assert not (part != 0).any()
     del dq, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("beta2", [0.9, 0.99, 0.999])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_the_largest_gradients(dev, bits, beta2, sign):
+    """Second moments in fp32's range whose quotient by 1 - beta2^step is not: the update as for any
+    other size, lr in the first step.  (8 bits: the largest block ends below 1.875 2^126.)"""
+    n, steps = 1024, 3
+    largest = math.sqrt(1.2e38 / (1 - beta2 ** steps))     # v to 1.2e38, codes an eighth more
+    g = (sign * largest * 2.0 ** -torch.linspace(0, 12, n)).to(dev)
+    hp = dict(HP, beta2=beta2)
+    p, s = torch.zeros(n, device=dev), llmt.adamw_state(torch.zeros(n, device=dev), bits)
+    lst = llmt.AdamTensors([p], [g], [s])
+    m = v = np.zeros(n, np.float32)
+    for step in range(1, steps + 1):
+        before = p.cpu().numpy()
+        llmt.adamw_update(lst, llmt.hparams(**hp), step, seed=4)
+        want, up, m, v = numpy_step(before, g.cpu().numpy(), m, v, step, hp=hp)
+        assert np.isfinite(v).all()
+        if step == 1:
+            hat = v.astype(np.float64) / (1 - float(np.float32(beta2)))
+            assert (hat > float(np.finfo(np.float32).max)).sum() > 10 and (up > 0.99 * HP["lr"]).all()
+        check_p(p, want, up)
+        if bits == 32:
+            assert np.array_equal(s.m.cpu().numpy(), m) and np.array_equal(s.v.cpu().numpy(), v)
+        else:
+            m, v = (x.cpu().numpy() for x in llmt.adamw_moments(s))
+            assert np.isfinite(v).all()
