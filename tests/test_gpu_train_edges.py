@@ -1,6 +1,7 @@
 """GPU: borders of the operators for training all weights on packed sequences: scores next to the
 documented bound in the attention's large tiles, heads of one buffer that lie between one another, rows beyond 2^28;
-AdamW's largest moments."""
+AdamW's largest moments, its lists of large tensors and of tensors unlike in size; small
+gradients with exact inputs; calls beside others."""
 import math
 
 import numpy as np
@@ -9,6 +10,7 @@ import torch
 
 import llmt
 import packed_ref as ref
+import test_gpu_adamw_list as adamw
 from test_gpu_adamw_list import HP, check_p, numpy_step
 from test_gpu_packed import offsets, problem
 
@@ -150,3 +152,75 @@ def test_the_largest_gradients(dev, bits, beta2, sign):
         else:
             m, v = (x.cpu().numpy() for x in llmt.adamw_moments(s))
             assert np.isfinite(v).all()
+
+
+@pytest.mark.parametrize("sizes", [
+    # above 2.1 M elements: pieces of 4096, a search in every launch, more descriptors than one holds
+    [1500001, 4095, 4096, 4097, 0, 1, 700003, 257] + [33, 4097] * 40,
+    [4096] * 60 + [2500000, 3],
+    # below: pieces of 1024, a search where the sizes are unlike
+    [3] * 60 + [200001] + [5] * 8, [200001] + [1025, 3] * 20, [1, 0, 1023, 150000, 1024, 0] + [700] * 20])
+@pytest.mark.parametrize("gt,ct", [(F, None), (B, B), (H, H)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_lists_whose_workgroups_search_their_tensor(dev, sizes, gt, ct, bits):
+    adamw.test_steps(dev, sizes, gt, ct, bits)
+
+
+@pytest.mark.parametrize("dtype,small", [(H, 2.0 ** -10), (B, 2.0 ** -60)])
+@pytest.mark.parametrize("ql", [[300, 41], [1500, 900]])
+def test_gradients_of_small_and_large_dout_have_the_same_bits(dev, dtype, small, ql):
+    """dout of random signs times [0.5, 4], exact in the type times `small` too, so every
+    intermediate value is (fp16's dS in part below its smallest normal number, were it not scaled).
+    Keys and queries of 2^-6 under a scale of 2^12 leave the weights as they are and raise dq and
+    dk, so that most outputs of the small run are normal numbers (of dv, whose late keys have few
+    rows, a third): those are compared from twice the smallest on, where the steps are the
+    type's."""
+    q, k, v, do, qo, ko = problem(dev, dtype, 128, 16, 8, ql)
+    g = torch.Generator().manual_seed(9)
+    do = torch.randn(do.shape, generator=g).sign() * (0.5 + 3.5 * torch.rand(do.shape, generator=g))
+    do = do.to(dtype).to(dev)
+    assert ((do * small).double() == do.double() * small).all()
+    q, k, scale = q / 64, k / 64, 128 ** -0.5 * 4096
+    o, lse = llmt.packed_attention(q, k, v, qo, scale=scale)
+    big = llmt.packed_attention_bwd(q, k, v, o, lse, do, qo, scale=scale)
+    low = llmt.packed_attention_bwd(q, k, v, o, lse, do * small, qo, scale=scale)
+    for a, b, share in zip(big, low, (0.9, 0.9, 1 / 3)):
+        normal = b.double().abs() >= 2 * torch.finfo(dtype).tiny
+        assert a.isfinite().all() and normal.double().mean() > share
+        assert torch.equal(a.double()[normal] * small, b.double()[normal])
+
+
+def test_beside_other_work_the_same_bits(dev):
+    """The operators on four streams at once, beside a stream of products, against the same calls
+    one after another."""
+    A = llmt.packed_attention
+    P = [problem(dev, *p) for p in (
+        (B, 128, 16, 8, [1500, 700, 33, 2000, 900, 1, 800, 1200, 1058]), (H, 128, 16, 8, [80, 77, 1, 90, 60, 305]),
+        (H, 64, 32, 8, [2100, 65, 7]), (B, 128, 16, 8, [1] * 8, [900, 1, 3000, 64, 700, 2000, 50, 9]))]
+    tok = torch.randint(-1, 3000, (20000,), dtype=torch.int32, device=dev)
+    dx = torch.randn(20000, 264, device=dev).to(B)
+    g = [torch.randn(n, device=dev) for n in (3000000, 70001)]
+
+    def calls(i):
+        q, k, v, do, qo, ko = P[i]
+        o, lse = A(q, k, v, qo, ko)
+        grads = llmt.packed_attention_bwd(q, k, v, o, lse, do, qo, ko)
+        dw = llmt.embedding_bwd(tok, dx, torch.zeros(3000, 264, device=dev))
+        p = [torch.ones_like(x) for x in g]
+        s = [llmt.adamw_state(x, 8) for x in p]
+        llmt.adamw_update(llmt.AdamTensors(p, g, s), llmt.hparams(**HP), 1, seed=i)
+        return [o, lse, *grads, dw, *p, *(t for x in s for t in x)]
+    want = [calls(i) for i in range(4)]
+    noise = torch.randn(4096, 4096, device=dev).to(B)
+    streams = [torch.cuda.Stream() for _ in range(5)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(streams[4]):
+            for _ in range(8):
+                noise @ noise
+        got = []
+        for i in range(4):
+            with torch.cuda.stream(streams[i]):
+                got.append(calls(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
