@@ -391,9 +391,9 @@ __device__ __forceinline__ void set_priority(int level, int top) {
 
 // The tiles of few rows run at once: any order.  Up to 62 sequences a wave holds
 // them all, and one load finds the t-th tile (numbered as in find_tile) and its
-// spans; false where it lies behind the sequence's end.
+// spans; its block may lie behind the sequence's end.
 template <bool ROWS, int QB>
-__device__ __forceinline__ bool any_tile(const PackArgs& a, int G, int t, SeqLens* seq, int* block) {
+__device__ __forceinline__ void any_tile(const PackArgs& a, int G, int t, SeqLens* seq, int* block) {
   const int i = threadIdx.x & 63, last = a.n + 1;
   const bool in = i > 0 && i < last;
   Span q = {0, 0}, k = {0, 0};
@@ -406,7 +406,6 @@ __device__ __forceinline__ bool any_tile(const PackArgs& a, int G, int t, SeqLen
   *seq = {__builtin_amdgcn_readlane(q.len, l), __builtin_amdgcn_readlane(k.len, l),
           __builtin_amdgcn_readlane(q.start, l), __builtin_amdgcn_readlane(k.start, l)};
   *block = t - __builtin_amdgcn_readlane(first, l);
-  return true;
 }
 
 // Tile t of nt in a launch of `all` a KV head: the spans of its sequence and
@@ -422,7 +421,10 @@ __device__ __forceinline__ bool pick_tile(const PackArgs& a, int G, int t, int n
     return true;
   }
   const int at = ROWS ? nt - 1 - t : t;
-  if (a.n <= 62) return any_tile<ROWS, QB>(a, G, at, seq, block);
+  if (a.n <= 62) {
+    any_tile<ROWS, QB>(a, G, at, seq, block);
+    return true;
+  }
   const int s = ROWS ? find_tile<QB>(a.qoff, a.n, a.Tq, G, at, block)
                      : find_tile<QB>(a.koff, a.n, a.Tk, 1, at, block);
   const bool in = s > 0 && s <= a.n;  // the tokens outside of all sequences: no other side

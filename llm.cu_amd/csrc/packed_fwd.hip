@@ -24,12 +24,12 @@ namespace llmt {
 
 namespace {
 
-// A tile of 16 MT keys of the running softmax for RW 16-row tiles of a wave:
+// A tile of 32 keys of the running softmax for RW 16-row tiles of a wave:
 // st holds raw scores (rows key, column row) and on return probabilities
 // relative to the running maximum, times 2^PSH.  lim: the last key a lane's
 // row sees.
-template <class E, int RW, int DT, bool MASK, int MT>
-__device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[RW], float (&l)[RW],
+template <class E, int RW, int DT, bool MASK>
+__device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][2], float (&m)[RW], float (&l)[RW],
                                              floatx4 (&ot)[RW][DT], float sl2, int key0,
                                              const int (&lim)[RW], int lane) {
   const int g = lane >> 4;
@@ -37,7 +37,7 @@ __device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[R
   for (int r = 0; r < RW; ++r) {
     float bm = -INFINITY;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         float s = st[r][mt][v];
@@ -54,18 +54,15 @@ __device__ __forceinline__ void softmax_tile(floatx4 (&st)[RW][MT], float (&m)[R
     m[r] = mn;
     const float shift = mu - E::PSH;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int v = 0; v < 4; ++v)
         st[r][mt][v] = __builtin_amdgcn_exp2f(fmaf(st[r][mt][v], sl2, -shift));
-    float ps[MT];
+    float ps[2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
       ps[mt] = (st[r][mt][0] + st[r][mt][1]) + (st[r][mt][2] + st[r][mt][3]);
-    if constexpr (MT == 4)
-      l[r] = l[r] * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-    else
-      l[r] = l[r] * alpha + (ps[0] + ps[1]);
+    l[r] = l[r] * alpha + (ps[0] + ps[1]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) ot[r][dt] *= alpha;
   }
@@ -393,9 +390,9 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_fwd_split_kernel(const Pack
     asm volatile("" ::: "memory");
     if (next) dk.issue(kbase, a.k.token, (kt + NW) * FS_KEYS, x.klen, Ks, 0);
     if (kt * FS_KEYS + FS_KEYS - 1 <= wfirst && left >= QB)
-      softmax_tile<E, RW, DT, false, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
+      softmax_tile<E, RW, DT, false>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
     else
-      softmax_tile<E, RW, DT, true, 2>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
+      softmax_tile<E, RW, DT, true>(st, m, l, ot, sl2, kt * FS_KEYS, lim, lane);
     short8v pb[RW], pl[RW];
 #pragma unroll
     for (int r = 0; r < RW; ++r) pair_split<E>(st[r][0], st[r][1], pb[r], pl[r]);
