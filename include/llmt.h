@@ -541,7 +541,8 @@ typedef struct {
  *   o = softmax(scale q k^T) v,  lse = ln sum exp(scale q k^T)  (fp32 [Tq, nq])
  * A query without keys, and tokens of no sequence, have o 0 and lse -inf.  dtype
  * (q, k, v, o, the gradients): LLMT_F16 or LLMT_BF16; products accumulate in
- * fp32, probabilities are rounded to dtype before the second product.
+ * fp32, probabilities are rounded to dtype before the second product (with few
+ * rows or keys they enter it with their remainder: the result alone is rounded).
  * head_dim 64 or 128; nq at most 64 nkv; and, the launches' limit, the larger of
  * Tq nq / nkv and Tk at most 64 ((2^23 - 2^12) / nkv - n - 2).  Scores (scale q k) up to
  * 2^24 in magnitude; larger ones, and NaN or infinities in the inputs, spoil
@@ -558,7 +559,9 @@ int llmt_packed_attention(const llmt_packed_dims* dims, const llmt_heads* q, con
                           const llmt_heads* v, const llmt_heads* o, float* lse, void* workspace,
                           size_t workspace_bytes, void* stream);
 /* Its gradients, in dtype: dq of the queries, dk and dv of the keys (summed over
- * a group's query heads), from the forward's o and lse and dout = d o.  (The
+ * a group's query heads), from the forward's o and lse and dout = d o.  P, and dS =
+ * P (dout v^T - rowsum(dout o)), are rounded to dtype before their products as the
+ * forward's probabilities are.  (The
  * rounding of lse to fp32 is 2^-23 of its magnitude in every probability.)  Queries
  * without keys, keys without queries and tokens of no sequence get zeros. */
 size_t llmt_packed_attention_bwd_workspace(const llmt_packed_dims* dims);
@@ -568,7 +571,8 @@ int llmt_packed_attention_bwd(const llmt_packed_dims* dims, const llmt_heads* q,
                               const llmt_heads* dk, const llmt_heads* dv, void* workspace,
                               size_t workspace_bytes, void* stream);
 
-/* Embedding: out[i] = scale weight[tokens[i]], rounded once; zeros where the
+/* Embedding: out[i] = scale weight[tokens[i]], the product in fp32, rounded to the
+ * output's type; zeros where the
  * token is outside [0, V) (padding).  weight [V, H], ldw elements from row to
  * row, out [T, H], ldo; LLMT_F32, LLMT_F16 or LLMT_BF16 each.  T at most 2^23, V
  * 2^30, H 2^20. */
@@ -598,7 +602,7 @@ int llmt_embedding_bwd(const int* tokens, int T, const void* dout, int ddtype, l
  * remainder, from a generator's draws of (seed, step, the tensor's place in the
  * list, element), a v above 0 to at least its smallest code; p is updated from
  * the moments before that rounding.  A block with a NaN or an infinity (or
- * beyond 2^127) becomes NaN.  Betas in [0, 1), eps at least 2^-126, count at most
+ * a magnitude beyond 1.875 2^126) becomes NaN.  Betas in [0, 1), eps at least 2^-126, count at most
  * 2^20, n 2^35.  No two written arrays may overlap, nor a written
  * one a gradient.  hp, step and seed are the call's: a captured call repeats
  * them. */

@@ -19,8 +19,8 @@
 //
 // Memory-bound: 26 bytes an element with fp32 moments, 14 with 8-bit ones (a
 // 16-bit gradient, plus 2 for a copy).  50.3 M parameters with copies: 266 us,
-// 5.3 TB/s; 100.7 M with 8-bit moments 325 us, 5.0 TB/s, and those in fp32 227,
-// 4.4.  200 tensors of up to 5000: three launches of 3.8 us.  A wave takes a
+// 5.3 TB/s; 100.7 M with 8-bit moments 325 us, 5.0 TB/s, and the decoding of those
+// moments into fp32 (adamw_moments_kernel) 227, 4.4.  200 tensors of up to 5000: three launches of 3.8 us.  A wave takes a
 // block of 256 elements at a time, a workgroup one piece of one tensor.  The
 // list is cut into launches of as many descriptors as travel in 4 KB of kernel
 // arguments.
@@ -135,8 +135,8 @@ __device__ __forceinline__ float decode(unsigned c, unsigned e) {
   return e == 255 ? __uint_as_float(0x7fc00000u) : s;
 }
 // The exponent byte of a block whose largest magnitude has these bits: the
-// largest stays at or below 1.875; 255 (infinite, NaN, or beyond) is a block
-// of NaN.
+// largest stays at or below 1.875; 255 (infinite, NaN, or beyond 1.875 2^126) is a
+// block of NaN.
 __device__ __forceinline__ unsigned block_exp(unsigned amax) {
   const unsigned e = (amax >> 23) + ((amax & 0x7FFFFF) > 0x700000 ? 1 : 0);
   return e >= 254 ? 255 : e < 1 ? 1 : e;

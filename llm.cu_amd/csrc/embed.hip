@@ -13,10 +13,10 @@
 //
 // Memory-bound where large: the lookup of 16384 rows of 1037 fp32 in 17.9 us, 5.1 TB/s
 // (the odd width takes single elements); the gradient of 32768 rows of 1024 bf16
-// into a table of 50257 fp32 rows in 77 us, of which the sorting launches with the
-// 206 MB of zeros take 46, the sums 24 (its 67 MB gathered, 41 written) and the join
-// 8; a copy would take 56 for all of it.  Few tokens cost a launch: 128 rows 2.6 us,
-// the gradient of 300 added to the table 5.0.
+// into a table of 50257 fp32 rows in 78 us of kernels (88 a call whose inputs change), of
+// which the sorting launches with the 206 MB of zeros take 46, the sums 24 (its 67 MB
+// gathered, 41 written) and the join 8; a copy would take 56 for all of it.  Few
+// tokens cost a launch: 128 rows 2.6 us, the gradient of 300 added to the table 5.0.
 #include <algorithm>
 
 #include "ops.h"
@@ -509,8 +509,9 @@ bool pieces(const void* p, long long ld, int H, size_t es, int N) {
 
 size_t size_of(int type) { return type == kF32 ? 4 : 2; }
 
-// Entries of a chunk: more chunks feed more CUs and leave more partial sums (us of a
-// gradient of 1024 columns with 16 / 32: 32768 positions 87 / 94, 65536 137 / 127).
+// Entries of a chunk: more chunks feed more CUs and leave more partial sums (us of a call
+// in a row, 50257 fp32 rows of 1024 written whole, with 16 / 32: 4096 positions 55 / 64,
+// 32768 79 / 84, 65536 133 / 122; added to the table 28 / 36, 58 / 64, 97 / 91).
 int chunk_of(int T) { return T >= 65536 ? 32 : T >= 4096 ? 16 : 8; }
 
 // The workspace: sorted keys and positions (twice for the radix passes), the

@@ -13,9 +13,9 @@
 // longest sequence; 1 x 512 tokens 21 and 28.  A long sequence is bound by issue:
 // a matrix instruction of 16 x 16 x 32 takes a SIMD 17 cycles, and the
 // exponentials and roundings of the other wave hardly run beside it (of the two
-// alone, 272 and 174 cycles, together 420).  1 x 8192 tokens take 872 us, 788
-// TFLOP/s of the five products, 1100 of the seven computed (S and dP twice); a
-// large library product reaches 1387.
+// alone, 272 and 174 cycles, together 420).  1 x 8192 tokens take 872 to
+// 910 us, 755 to 788 TFLOP/s of the five products, up to 1100 of the seven computed
+// (S and dP twice); a large library product reaches 1387.
 //
 // fp16.  dS spans many binades (a probability of one key in many times a small
 // gradient), so it enters its product times a power of two that belongs to the
@@ -136,7 +136,9 @@ __device__ __forceinline__ float delta_of(const short8v (&df)[KS], const short* 
 // ---------------------------------------------------------------- dQ
 // Four waves of 16 RW rows, against keys in tiles of 64, two halves one after
 // the other.  (Two waves for each of two halves, as in dK/dV below, were slower
-// at every size, 7% at 16 sequences of 8192 tokens.)
+// at every size, 7% at 16 sequences of 8192 tokens.)  dS is rounded to the type
+// once, here as P and dS in dK/dV: these blocks are bound by issue, and the remainder
+// as a second operand would be a third (dQ) or half (dK, dV) more products.
 template <class E, int HD, int RW, bool OWN>
 __device__ __forceinline__ void dq_block(const PackArgs& a, Group gr, int j, int tile, Mix mix,
                                          RowVecs rv, short* buf0, short* buf1) {
@@ -779,16 +781,18 @@ void packed_bwd_kernel(const PackArgs a, Group gr, Mix mix, RowVecs rv) {
 // keys: 0 and 1 the rows over a workgroup's waves, 2 over its two halves, 3 not;
 // with 0 every block works out the rows' delta for itself.
 //
-// Fewer and longer chains of tiles against idle CUs, us of a call in a graph, bf16,
-// the kind of smaller blocks first:
-//   rows 0 and keys 1, or 1 and 2: one head of 128, 1 x 8000 126 / 179; 16 / 8 heads of
-//     128, 1 x 512 23.8 / 21.4, 6 x 250 37.5 / 31.7; 32 / 8 of 64, 4 x 250 24.6 / 28.2
-//   rows 1 or 2: 16 / 8 of 128, 6 x 417 58 / 55, 4 x 1000 130 / 121
-//   keys 2 or 3: 16 / 8 of 128, 6 x 417 55 / 58, 4 x 1000 121 / 110; 32 / 8 of 64,
-//     4 x 1000 115 / 128, 8 x 1024 257 / 238
-// keys 0 saves the launch before and is longer by tile: 16 / 8 of 128, 8 x 77 called
-// from a program 18.4 / 22.0 us, 4 / 4 heads of 128, 2 x 500 21.1 / 17.6, one head 1 x
-// 2000 45 / 28.
+// Fewer and longer chains of tiles against idle CUs, us of a call in a graph with
+// changing inputs, bf16, the kind of smaller blocks first:
+//   rows 0 or 1, with keys 1: one head of 128, 1 x 8000 117 / 140; 16 / 8 heads of 128,
+//     1 x 512 25.1 / 22.2, 6 x 250 45 / 35; 32 / 8 of 64, 4 x 250 29.4 / 21.4
+//   keys 1 or 2, with rows 1: 16 / 8 of 128, 1 x 512 22.2 / 25.4, 6 x 250 34.9 / 29.2;
+//     32 / 8 of 64, 4 x 250 21.4 / 23.4
+//   rows 1 or 2: 16 / 8 of 128, 6 x 417 53 / 47, 4 x 1000 106 / 97
+//   keys 2 or 3, with rows 2: 16 / 8 of 128, 6 x 417, just below that border, 47 / 43, 4 x
+//     1000 97 / 89; 32 / 8 of 64, 4 x 1000 91 / 94, 8 x 1024 181 / 169
+// keys 0 saves the launch before and is longer by tile: with rows 1, 16 / 8 of 128, 8 x 77
+// 14.9 / 15.8, with rows 0, 4 / 4 heads of 128, 2 x 500 19.9 / 17.6, one head 1 x 2000
+// 45 / 28.
 struct BwdPlan {
   int rows, keys;
 };

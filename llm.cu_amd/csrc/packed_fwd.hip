@@ -10,9 +10,9 @@
 // Long sequences are bound by issue: a wave's tile of 64 keys and 32 rows takes
 // 64 matrix instructions of 17 cycles and some 250 vector ones, which hardly
 // overlap those of the other wave on the SIMD.  1 x 8192 tokens, 16 / 8 heads of
-// 128 in bf16: 270 us, 1015 TFLOP/s (a large library product reaches 1387); 1 x
-// 16384, 32 / 8 heads of 64 in fp16, twice the exponentials a product: 1250 us,
-// 880.  Many sequences end with the longest one's chain of tiles: 16 of 8192 tokens
+// 128 in bf16: 270 to 277 us, 990 to 1015 TFLOP/s (a large library product reaches
+// 1387); 1 x 16384, 32 / 8 heads of 64 in fp16, twice the exponentials a product: 1240
+// to 1265 us, 870 to 885.  Many sequences end with the longest one's chain of tiles: 16 of 8192 tokens
 // together 58 us, 630.  Single tokens wait for their keys: 8 tokens of 9001 keys
 // 13.5 us in a graph with the join, 32 of 32000 31, 4.2 TB/s.
 #include <algorithm>
@@ -529,8 +529,9 @@ struct FwdPlan {
 FwdPlan fwd_plan(const PackArgs& a) {
   const long long rows = (long long)a.Tq * (a.nq / a.nkv);
   const long long n = std::min(a.n, a.Tq);
-  // 32 rows a wave where that gives every CU two workgroups, 16 where those do
-  // (32 / 8 heads of 64, 4 x 1000 tokens 44 us and 43, 16 / 8 of 128, 16 x 512 49 and 60)
+  // 32 rows a wave where that gives every CU two workgroups, 16 where those do (us in a
+  // graph with changing inputs, 32 / 16: 32 / 8 heads of 64, 4 x 1000 tokens 39 / 38, 16 / 8
+  // of 128, 16 x 512 46 / 58, 4 x 1000, a little below that border, 33 / 37)
   if (rows / 128 * a.nkv >= 512) return {4, 2, 1, 0};
   if (rows / 64 * a.nkv >= 256) return {4, 1, 1, 0};
   // tiles of 16 rows, or of 32 where that many workgroups would not run at once
@@ -538,10 +539,12 @@ FwdPlan fwd_plan(const PackArgs& a) {
   const long long wgs = std::max<long long>(1, std::max(rows / (16 * rw), n) * a.nkv);
   const long long keys = a.Tk / std::max<long long>(1, n);
   const long long most = std::min<long long>(64, std::max<long long>(1, keys / 128));
-  // A CU for each workgroup and few keys: eight waves, no parts.  us in a graph, four
-  // waves in parts / eight: single tokens of 500 keys 8.6 / 7.0, of 1000 8.2 / 9.2, 32 of
-  // 1000 31 / 38; whole tiles, whose parts are larger: 4 heads, 2 x 500 15.1 / 7.7, one
-  // head, 1 x 4000 24.9 / 21.2, 16 / 8 heads, 128 tokens behind 900 18.2 / 9.7
+  // A CU for each workgroup and few keys: eight waves, no parts.  us in a graph with
+  // changing inputs, four waves in parts / eight: single tokens of 500 keys 9.1 / 7.8, of
+  // 1000 10.4 / 15.5, 8 of 1000 14.6 / 17.0 (32 of 1000, where every CU has a workgroup
+  // without parts, 34 / 25); whole tiles, whose parts are larger: 4 heads, 2 x 500 15.9 /
+  // 8.1, 16 / 8 heads, 128 tokens behind 900 19.6 / 12.1, one head, 1 x 4000 (the same
+  // inputs) 25.1 / 21.1
   const long long seen = keys - a.Tq / std::max<long long>(1, n) / 2;
   if (rw == 1 && wgs <= 256 && seen <= (rows / 16 >= n ? 2048 : 768)) return {0, 1, 1, 8};
   return {0, rw, (int)std::min(most, std::max<long long>(1, 768 / wgs)), 4};
